@@ -294,6 +294,78 @@ int vc_lstm_pointwise_fwd(const void* gates, const float* b_ih, const float* b_h
 int vc_lstm_pointwise_bwd(const float* dh, const float* dc_next, const float* saved, const float* c_prev, void* dgates,
                           float* dc_prev, float* db_ih, float* db_hh, int32_t N, int32_t H, void* stream);
 
+/* ---- AdamW (decoupled weight decay) over a list of tensors in one launch per 60 of them.  No counterpart in the reference
+ * (its create_optimizer, lib/utils/utils.py:13-36, builds SGD or Adam); torch.optim.AdamW's formula:
+ *   m' = b1 m + (1 - b1) g;  v' = b2 v + (1 - b2) g^2;  p' = (1 - lr wd) p - lr / (1 - b1^t) m' / (sqrt(v' / (1 - b2^t)) + eps)
+ * p and g are fp32 or bf16 (both the same).  state_bits 32: m, v fp32, m_scale / v_scale null.  state_bits 8: m, v hold OCP
+ * e4m3 codes, one fp32 scale for every 256 consecutive elements; m = code * scale, sqrt(v) = code * scale (the second moment
+ * is held by its root; what is not 0 there never rounds to 0).  The parameters move by the unrounded moments; a gradient that
+ * is not finite reaches all 256 elements of its block.  Every tensor is n consecutive elements in memory; tensors of one
+ * call must not overlap.  g is multiplied by grad_scale and, if given, by the device scalar *grad_scale_dev (a clipping
+ * factor that never visits the host).  `tensors` and `hyper` are host memory, read before the call returns. */
+typedef struct vc_adamw_tensor {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* m_scale;
+    float* v_scale;
+    int64_t n;
+} vc_adamw_tensor;
+typedef struct vc_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay, grad_scale;
+    int64_t step; /* 1 for the first call */
+} vc_adamw_hyper;
+int vc_adamw_step(const vc_adamw_tensor* tensors, int32_t count, int32_t is_bf16, int32_t state_bits, const vc_adamw_hyper* hyper,
+                  const float* grad_scale_dev /* nullable */, void* stream);
+
+/* ---- Gated linear recurrence over time: what a sequence of LSTM cells (reference lib/models/lstm.py:16,25-27) is used for,
+ * in a form that is computed over all steps at once.  gates[b][t] = (z | v), H values each, fp32 or bf16:
+ *   f = sigmoid(z);  h_t = f h_(t-1) + (1 - f) v
+ * Sequence b has lengths[b] steps (nullable: T; values outside [0, T] are clamped); h and dgates are 0 behind them, and what
+ * gates and dy hold there is not read.  reverse: the recurrence runs from the last step to the first.  h0 (nullable: zeros), last, dlast
+ * (nullable), dh0 (nullable) are fp32 [B][H]; last = the state behind the last step, h0 for a sequence without steps.  The
+ * state is fp32 throughout; h, dgates are of gates' type, contiguous [B][T][H] and [B][T][2H], as is dy (nullable) and all of
+ * them aligned to two elements.  gates has any strides over B and T.  states (fp32 [B][ceil(T / 64)][H]; forward: nullable)
+ * carries the forward's states to the backward.  workspace: vc_gated_scan_workspace_bytes(d, op), op 0 forward, 1 backward
+ * (0: none needed); its content is not kept.  Results do not depend on the order in which workgroups run. */
+#define VC_SCAN_STATE_STEPS 64
+typedef struct vc_scan_desc {
+    int32_t B, T, H;
+    int32_t is_bf16, reverse, pad_;
+    int64_t stride_b, stride_t; /* of gates, in elements */
+} vc_scan_desc;
+size_t vc_gated_scan_workspace_bytes(const vc_scan_desc* d, int32_t op);
+int vc_gated_scan_fwd(const vc_scan_desc* d, const void* gates, const float* h0, const int32_t* lengths, void* h, float* last,
+                      float* states, void* workspace, size_t ws_bytes, void* stream);
+int vc_gated_scan_bwd(const vc_scan_desc* d, const void* gates, const int32_t* lengths, const float* states, const void* dy,
+                      const float* dlast, void* dgates, float* dh0, void* workspace, size_t ws_bytes, void* stream);
+/* one step for each of B sequences (serving): state [B][H] fp32 is updated in place, h [B][H] is of gates' type; gates row b
+ * is at gates + b * stride_b */
+int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, float* state, void* h, int32_t B, int32_t H, void* stream);
+
+/* ---- Linear classifier + cross-entropy in one operator, the vocabulary in pieces: the reference's clf_haed and
+ * CrossEntropyLoss (lib/models/model.py:24,38, lib/core/loss.py:10,25) for class counts whose logits are not worth keeping.
+ *   z = x w^T + bias;  loss_n = logsumexp(z_n) - z[n][label_n]
+ * x [N][D], w [V][D], bias [V] (nullable): all fp32 or all bf16; ldx, ldw = row strides in elements.  Rows whose label is
+ * ignore_index take no part: loss 0, gradient 0, x not read.  Any other label outside [0, V) makes that row's loss NaN (as
+ * vc_softmax_ce does).  reduction: 0 none (loss_rows [N]), 1 mean over the rows that count (0 if none does), 2 sum (loss [1]).
+ * The forward writes lse [N] and rows (int32 [N + 4]: the rows that count, ascending; from the end those that do not; their
+ * number), which the backward takes.  dloss: fp32 on the device, [1], or [N] with reduction 0.  dx [N][D], dw [V][D], db [V]
+ * (each nullable) are contiguous and of x's type, and are written, not added to.  workspace (required):
+ * vc_linear_ce_workspace_bytes(d, op), op 0 forward, 1 backward; it does not grow with N * V. */
+typedef struct vc_linear_ce_desc {
+    int32_t N, D, V, is_bf16;
+    int32_t reduction, pad_;
+    int64_t ldx, ldw, ignore_index;
+} vc_linear_ce_desc;
+size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op);
+int vc_linear_ce_fwd(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels, float* loss,
+                     float* loss_rows, float* lse, int32_t* rows, void* workspace, size_t ws_bytes, void* stream);
+int vc_linear_ce_bwd(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels,
+                     const float* lse, const int32_t* rows, const float* dloss, void* dx, void* dw, void* db, void* workspace,
+                     size_t ws_bytes, void* stream);
+
 /* ---- Layout helpers at the API edge (NCTHW <-> NTHWC). */
 int vc_ncthw_to_nthwc(const void* in, int32_t in_is_bf16, void* out, int32_t N, int32_t C, int64_t S,
                       void* stream);

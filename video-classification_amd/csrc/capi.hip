@@ -1208,6 +1208,129 @@ int vc_lstm_pointwise_bwd(const float* dh, const float* dc_next, const float* sa
     return vc_ew_lstm_pointwise_bwd(dh, dc_next, saved, c_prev, dgates, dc_prev, db_ih, db_hh, N, H, S(stream));
 }
 
+/* ------------------------------------------------------------------ AdamW over a list of tensors */
+static_assert(sizeof(vc_adamw_tensor) == sizeof(VcAdamwTensor), "one layout on both sides of the boundary");
+int vc_adamw_step(const vc_adamw_tensor* tensors, int32_t count, int32_t is_bf16, int32_t state_bits, const vc_adamw_hyper* hyper,
+                  const float* grad_scale_dev, void* stream) {
+    VC_REQUIRE(hyper && count >= 0 && (tensors || count == 0), "adamw_step: bad arguments");
+    VC_REQUIRE(state_bits == 32 || state_bits == 8, "adamw_step: moments are held in 32 or 8 bits (got %d)", state_bits);
+    VC_REQUIRE(hyper->step >= 1, "adamw_step: step counts from 1 (got %lld)", (long long)hyper->step);
+    VC_REQUIRE(hyper->lr >= 0 && hyper->eps >= 0 && hyper->weight_decay >= 0 && hyper->beta1 >= 0 && hyper->beta1 < 1 &&
+                   hyper->beta2 >= 0 && hyper->beta2 < 1,
+               "adamw_step: lr, eps and weight_decay are at least 0, the betas in [0, 1)");
+    for (int32_t i = 0; i < count; ++i) {
+        const vc_adamw_tensor& t = tensors[i];
+        VC_REQUIRE(t.n >= 0 && t.n < (1ll << 42), "adamw_step: tensor %d has %lld elements", i, (long long)t.n);
+        if (t.n == 0) continue;
+        VC_REQUIRE(t.p && t.g && t.m && t.v, "adamw_step: null pointer in tensor %d", i);
+        VC_REQUIRE(state_bits == 32 || (t.m_scale && t.v_scale), "adamw_step: tensor %d has no scales for its 8-bit moments", i);
+    }
+    VcAdamwArgs a;
+    memset(&a, 0, sizeof(a));
+    a.c0 = (float)(1.0 - hyper->lr * hyper->weight_decay);
+    a.b1 = (float)hyper->beta1, a.one_b1 = (float)(1.0 - hyper->beta1);
+    a.b2 = (float)hyper->beta2, a.one_b2 = (float)(1.0 - hyper->beta2);
+    a.root2 = (float)(1.0 / std::sqrt(1.0 - std::pow(hyper->beta2, (double)hyper->step)));
+    a.step = (float)(hyper->lr / (1.0 - std::pow(hyper->beta1, (double)hyper->step)));
+    a.eps = (float)hyper->eps;
+    a.gscale = grad_scale_dev, a.gscale_host = (float)hyper->grad_scale;
+    return vc_adamw_launch((const VcAdamwTensor*)tensors, count, is_bf16 != 0, state_bits, a, S(stream));
+}
+
+/* ------------------------------------------------------------------ gated linear recurrence */
+static int scan_check(const vc_scan_desc* d) {
+    VC_REQUIRE(d != nullptr, "null descriptor");
+    VC_REQUIRE(d->B > 0 && d->T > 0 && d->H > 0, "gated_scan: bad sizes B=%d T=%d H=%d", d->B, d->T, d->H);
+    VC_REQUIRE(d->B <= 65535, "gated_scan: at most 65535 sequences (got %d)", d->B);
+    VC_REQUIRE(d->T <= (1 << 30) && d->H <= (1 << 24), "gated_scan: T=%d or H=%d too large", d->T, d->H);
+    return 0;
+}
+static VcScanParams scan_params(const vc_scan_desc* d, const void* gates, const int32_t* lengths) {
+    VcScanParams p;
+    memset(&p, 0, sizeof(p));
+    p.B = d->B, p.T = d->T, p.H = d->H, p.reverse = d->reverse != 0;
+    p.sb = d->stride_b, p.st = d->stride_t, p.gates = gates, p.lengths = lengths;
+    return p;
+}
+static bool pair_aligned(const void* q, int32_t is_bf16) { return ((uintptr_t)q & (is_bf16 ? 3 : 7)) == 0; }
+size_t vc_gated_scan_workspace_bytes(const vc_scan_desc* d, int32_t op) {
+    (void)op;
+    return d == nullptr ? 0 : 0;
+}
+int vc_gated_scan_fwd(const vc_scan_desc* d, const void* gates, const float* h0, const int32_t* lengths, void* h, float* last,
+                      float* states, void* workspace, size_t ws_bytes, void* stream) {
+    (void)workspace, (void)ws_bytes;
+    const int rc = scan_check(d);
+    if (rc) return rc;
+    VC_REQUIRE(gates && h && last, "gated_scan_fwd: null pointer");
+    VC_REQUIRE(pair_aligned(h, d->is_bf16), "gated_scan_fwd: h is not aligned to two elements");
+    VcScanParams p = scan_params(d, gates, lengths);
+    p.h0 = h0, p.h = h, p.last = last, p.states = states;
+    return vc_scan_launch_fwd(p, d->is_bf16 != 0, S(stream));
+}
+int vc_gated_scan_bwd(const vc_scan_desc* d, const void* gates, const int32_t* lengths, const float* states, const void* dy,
+                      const float* dlast, void* dgates, float* dh0, void* workspace, size_t ws_bytes, void* stream) {
+    (void)workspace, (void)ws_bytes;
+    const int rc = scan_check(d);
+    if (rc) return rc;
+    VC_REQUIRE(gates && states && dgates, "gated_scan_bwd: null pointer");
+    VC_REQUIRE(pair_aligned(dgates, d->is_bf16) && pair_aligned(dy, d->is_bf16), "gated_scan_bwd: dy or dgates is not aligned to two elements");
+    VcScanParams p = scan_params(d, gates, lengths);
+    p.states = (float*)states, p.dy = dy, p.dlast = dlast, p.dgates = dgates, p.dh0 = dh0;
+    return vc_scan_launch_bwd(p, d->is_bf16 != 0, S(stream));
+}
+int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, float* state, void* h, int32_t B, int32_t H, void* stream) {
+    VC_REQUIRE(gates && state && h && B > 0 && H > 0, "gated_scan_step: bad arguments");
+    return vc_scan_launch_step(gates, stride_b, state, h, B, H, is_bf16 != 0, S(stream));
+}
+
+/* ------------------------------------------------------------------ linear classifier + cross-entropy */
+static int lce_check(const vc_linear_ce_desc* d) {
+    VC_REQUIRE(d != nullptr, "null descriptor");
+    VC_REQUIRE(d->N > 0 && d->D > 0 && d->V > 0, "linear_ce: bad sizes N=%d D=%d V=%d", d->N, d->D, d->V);
+    VC_REQUIRE(d->N <= (1 << 23) && d->V <= (1 << 23) && d->D <= (1 << 20), "linear_ce: at most 2^23 rows and classes, 2^20 features");
+    VC_REQUIRE(d->ldx >= d->D && d->ldw >= d->D, "linear_ce: row strides %lld, %lld below D=%d", (long long)d->ldx, (long long)d->ldw, d->D);
+    VC_REQUIRE(d->reduction >= 0 && d->reduction <= 2, "linear_ce: reduction %d (0 none, 1 mean, 2 sum)", d->reduction);
+    return 0;
+}
+size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op) {
+    if (lce_check(d) != 0) return 0;
+    return vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, op);
+}
+static VcLceParams lce_params(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels, void* ws,
+                              size_t ws_bytes) {
+    VcLceParams p;
+    memset(&p, 0, sizeof(p));
+    p.N = d->N, p.D = d->D, p.V = d->V, p.ldx = d->ldx, p.ldw = d->ldw;
+    p.x = x, p.w = w, p.bias = bias, p.labels = (const long long*)labels, p.ignore_index = d->ignore_index, p.reduction = d->reduction;
+    p.ws = ws, p.ws_bytes = ws_bytes;
+    return p;
+}
+int vc_linear_ce_fwd(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels, float* loss,
+                     float* loss_rows, float* lse, int32_t* rows, void* workspace, size_t ws_bytes, void* stream) {
+    const int rc = lce_check(d);
+    if (rc) return rc;
+    VC_REQUIRE(x && w && labels && lse && rows && (d->reduction == 0 ? loss_rows != nullptr : loss != nullptr), "linear_ce_fwd: null pointer");
+    const size_t need = vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, 0);
+    VC_REQUIRE(workspace && ws_bytes >= need, "linear_ce_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    VcLceParams p = lce_params(d, x, w, bias, labels, workspace, ws_bytes);
+    p.loss = loss, p.loss_rows = loss_rows, p.lse = lse, p.rows = rows;
+    return vc_lce_launch_fwd(p, d->is_bf16 != 0, S(stream));
+}
+int vc_linear_ce_bwd(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels,
+                     const float* lse, const int32_t* rows, const float* dloss, void* dx, void* dw, void* db, void* workspace,
+                     size_t ws_bytes, void* stream) {
+    const int rc = lce_check(d);
+    if (rc) return rc;
+    VC_REQUIRE(x && w && labels && lse && rows && dloss, "linear_ce_bwd: null pointer");
+    VC_REQUIRE(db == nullptr || bias != nullptr, "linear_ce_bwd: a gradient of a bias that is not there");
+    const size_t need = vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, 1);
+    VC_REQUIRE(workspace && ws_bytes >= need, "linear_ce_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    VcLceParams p = lce_params(d, x, w, bias, labels, workspace, ws_bytes);
+    p.lse = (float*)lse, p.rows = (int*)rows, p.dloss = dloss, p.dx = dx, p.dw = dw, p.db = db;
+    return vc_lce_launch_bwd(p, d->is_bf16 != 0, S(stream));
+}
+
 /* ------------------------------------------------------------------ layout */
 int vc_ncthw_to_nthwc(const void* in, int32_t in_is_bf16, void* out, int32_t N, int32_t C, int64_t Sp, void* stream) {
     VC_REQUIRE(in && out && N > 0 && C > 0 && Sp > 0, "ncthw_to_nthwc: bad arguments");

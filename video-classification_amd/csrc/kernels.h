@@ -174,3 +174,74 @@ int vc_launch_wgrad(const VcWgradParams& p, int mode, hipStream_t stream);
 // split-K planning (shared by the workspace query and the launch)
 int vc_igemm_splits(int M, int Cn, int nchunks);
 int vc_wgrad_splits(int M, int Co, int nblk, int* rows_per_split);
+
+// adamw.hip: one AdamW step over a list of tensors (kernel arguments: at most 4 KB)
+#define VC_ADAMW_BLOCK 256
+#define VC_ADAMW_MAX_TENSORS 60
+struct VcAdamwTensor {  // = vc_adamw_tensor of include/vc3d.h
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* ms;  // scales of 8-bit moments, one per VC_ADAMW_BLOCK elements
+    float* vs;
+    long long n;
+};
+struct VcAdamwArgs {
+    VcAdamwTensor t[VC_ADAMW_MAX_TENSORS];
+    unsigned first[VC_ADAMW_MAX_TENSORS];  // first workgroup of each tensor
+    int count;
+    float c0, b1, one_b1, b2, one_b2, root2, eps, step, gscale_host;
+    const float* gscale;  // nullable: device scalar, multiplied in
+};
+static_assert(sizeof(VcAdamwArgs) <= 4096, "kernel argument limit");
+int vc_adamw_launch(const VcAdamwTensor* t, int count, bool is_bf16, int bits, VcAdamwArgs& a, hipStream_t s);
+
+// scan.hip: gated linear recurrence
+#define VC_SCAN_CHUNK 64  // steps between two saved states
+struct VcScanParams {
+    int B, T, H;
+    int reverse;
+    long long sb, st;    // strides of gates, in elements
+    const void* gates;   // [B][T][2H]: gate logits, values
+    const float* h0;     // nullable [B][H]
+    const int* lengths;  // nullable [B]
+    float* states;       // [B][ceil(T / VC_SCAN_CHUNK)][H]: state before each chunk (forward: nullable)
+    // forward
+    void* h;      // [B][T][H]
+    float* last;  // [B][H]
+    // backward
+    const void* dy;      // nullable [B][T][H]
+    const float* dlast;  // nullable [B][H]
+    void* dgates;        // [B][T][2H]
+    float* dh0;          // nullable [B][H]
+};
+int vc_scan_launch_fwd(const VcScanParams& p, bool is_bf16, hipStream_t s);
+int vc_scan_launch_bwd(const VcScanParams& p, bool is_bf16, hipStream_t s);
+int vc_scan_launch_step(const void* gates, long long sb, float* state, void* h, int B, int H, bool is_bf16, hipStream_t s);
+
+// linear_ce.hip: linear classifier + cross-entropy in pieces of the vocabulary
+struct VcLceParams {
+    int N, D, V;
+    long long ldx, ldw;  // row strides of x, w in elements
+    const void* x;       // [N][D]
+    const void* w;       // [V][D]
+    const void* bias;    // nullable [V]
+    const long long* labels;
+    long long ignore_index;
+    int reduction;  // 0 none, 1 mean, 2 sum
+    float* loss;       // forward: [1], nullable with reduction 0
+    float* loss_rows;  // forward: [N], nullable unless reduction is 0
+    float* lse;        // [N]
+    int* rows;         // [N + 4]: rows that count (in order), rows that do not, from the end; then their number
+    // backward
+    const float* dloss;  // [1], or [N] with reduction 0
+    void* dx;            // nullable
+    void* dw;            // nullable
+    void* db;            // nullable
+    void* ws;
+    size_t ws_bytes;
+};
+size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, int op);
+int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s);
+int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s);

@@ -68,10 +68,28 @@ class Cmd(C.Structure):
 
 CMD_CALL, CMD_EVENT_RECORD, CMD_STREAM_WAIT = 0, 1, 2
 
+
+class AdamwHyper(C.Structure):
+    """vc_adamw_hyper (include/vc3d.h)"""
+    _fields_ = [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "grad_scale")] + [("step", C.c_int64)]
+
+
+class ScanDesc(C.Structure):
+    """vc_scan_desc (include/vc3d.h)"""
+    _fields_ = [(n, C.c_int32) for n in ("B", "T", "H", "is_bf16", "reverse", "pad_")] + [("stride_b", C.c_int64), ("stride_t", C.c_int64)]
+
+
+class LinearCeDesc(C.Structure):
+    """vc_linear_ce_desc (include/vc3d.h)"""
+    _fields_ = [(n, C.c_int32) for n in ("N", "D", "V", "is_bf16", "reduction", "pad_")] + \
+               [(n, C.c_int64) for n in ("ldx", "ldw", "ignore_index")]
+
 _CD = C.POINTER(ConvDesc)
 _PD = C.POINTER(PoolDesc)
 _IP = C.POINTER(C.c_int32)
 _BF = C.POINTER(BnFin)
+_SD = C.POINTER(ScanDesc)
+_LD = C.POINTER(LinearCeDesc)
 
 # name -> argtypes (every function returns int unless listed in _RESTYPE)
 PROTOTYPES = {
@@ -126,6 +144,14 @@ PROTOTYPES = {
     "vc_linear_bwd": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P],
     "vc_lstm_pointwise_fwd": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P],
     "vc_lstm_pointwise_bwd": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P],
+    "vc_adamw_step": [_P, _I, _I, _I, C.POINTER(AdamwHyper), _P, _P],
+    "vc_gated_scan_workspace_bytes": [_SD, _I],
+    "vc_gated_scan_fwd": [_SD, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P],
+    "vc_gated_scan_bwd": [_SD, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P],
+    "vc_gated_scan_step": [_P, _L, _I, _P, _P, _I, _I, _P],
+    "vc_linear_ce_workspace_bytes": [_LD, _I],
+    "vc_linear_ce_fwd": [_LD] + [_P] * 9 + [C.c_size_t, _P],
+    "vc_linear_ce_bwd": [_LD] + [_P] * 11 + [C.c_size_t, _P],
     "vc_ncthw_to_nthwc": [_P, _I, _P, _I, _I, _L, _P],
     "vc_nthwc_to_ncthw": [_P, _P, _I, _I, _I, _L, _P],
     "vc_replay": [C.POINTER(Cmd), _I, C.POINTER(C.c_void_p), _I, _I, _P, _P, _IP],
@@ -136,7 +162,8 @@ PROTOTYPES = {
     "vc_incr_i64": [_P, _I, _P],
 }
 _RESTYPE = {"vc_last_error": C.c_char_p, "vc_stem_packed_input_elems": C.c_size_t, "vc_static_scratch_bytes": C.c_size_t,
-            "vc_conv3d_workspace_bytes": C.c_size_t, "vc_stem_wgrad_workspace_bytes": C.c_size_t}
+            "vc_conv3d_workspace_bytes": C.c_size_t, "vc_stem_wgrad_workspace_bytes": C.c_size_t,
+            "vc_gated_scan_workspace_bytes": C.c_size_t, "vc_linear_ce_workspace_bytes": C.c_size_t}
 
 
 def _load():

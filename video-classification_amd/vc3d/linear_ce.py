@@ -1,0 +1,48 @@
+"""Linear classifier and cross-entropy in one operator, for class counts whose logits are not worth keeping: the reference's
+clf_haed and nn.CrossEntropyLoss (lib/models/model.py:24,38, lib/core/loss.py:10,25), which linear_apply + cross_entropy compute
+with kept logits up to 1024 classes."""
+import torch
+
+from . import ops
+from .capi import Vc3dError
+
+_REDUCTION = {"none": 0, "mean": 1, "sum": 2}
+
+
+class _LinearCEFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, labels, bias, ignore_index, reduction):
+        loss, lse, rows = ops.linear_ce_fwd(x.detach(), weight.detach(), labels, None if bias is None else bias.detach(), ignore_index, reduction)
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(x, weight, labels, bias, lse, rows)
+            ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        return loss if reduction == 0 else loss.view(())
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, weight, labels, bias, lse, rows = ctx.saved_tensors
+        want = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
+        dx, dw, db = ops.linear_ce_bwd(x.detach(), weight.detach(), labels, None if bias is None else bias.detach(), lse, rows,
+                                       dloss.contiguous(), ctx.ignore_index, ctx.reduction, want)
+        return dx, dw, None, db, None, None
+
+
+def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduction="mean"):
+    """F.cross_entropy(x @ weight.T + bias, labels) without the logits: x [..., D], weight [V][D], bias [V] or None, all fp32 or
+    all bf16; labels int64 [...] on the GPU.  Logits, sums and the loss are fp32.  Rows whose label is ignore_index take no part
+    (their x is not read and its gradient is 0); "mean" is over the others, and 0 where there is none (torch: NaN).  Any other
+    label outside [0, V) gives a NaN.  reduction "none" returns labels' shape.  Differentiable in x, weight and bias; the
+    gradients are of the inputs' type."""
+    if not torch.is_tensor(x) or not x.is_cuda:
+        raise Vc3dError("linear_cross_entropy runs on the GPU only (no CPU fallback)")
+    if reduction not in _REDUCTION:
+        raise Vc3dError("linear_cross_entropy: reduction 'none', 'mean' or 'sum', got %r" % (reduction,))
+    if x.dim() < 1 or x.shape[-1] == 0 or weight.dim() != 2 or tuple(labels.shape) != tuple(x.shape[:-1]):
+        raise Vc3dError("linear_cross_entropy: x [..., D], weight [V][D] and labels [...] expected, got %s, %s, %s" %
+                        (tuple(x.shape), tuple(weight.shape), tuple(labels.shape)))
+    shape = labels.shape
+    x2 = ops._rows(x.reshape(-1, x.shape[-1]))
+    loss = _LinearCEFn.apply(x2, ops._rows(weight), labels.reshape(-1).contiguous(), None if bias is None else bias.contiguous(),
+                             int(ignore_index), _REDUCTION[reduction])
+    return loss.view(shape) if reduction == "none" else loss

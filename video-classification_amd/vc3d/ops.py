@@ -4,6 +4,8 @@ Every wrapper checks device, dtype, contiguity and element counts on the host be
 launch: a kernel that reads past a buffer can take the whole GPU down.  torch is used for
 device memory and the current stream only.
 """
+import ctypes
+
 import torch
 
 from . import capi
@@ -672,6 +674,262 @@ def linear_bwd(dlogits, feat, W, dW=None, db=None, want_dfeat=True):
     check(lib.vc_linear_bwd(ptr(dlogits), ptr(feat), ptr(W), ptr(dfeat), ptr(dW), ptr(db), N, Fd, K, cur_stream()),
           "vc_linear_bwd")
     return dfeat
+
+
+# ---- operators of long sequences and large vocabularies.  They take tensors on any GPU (the launch goes to that device's
+# current stream) and bring their own workspace from torch's allocator, per call: nothing is shared between calls, streams or
+# captured graphs.
+
+_E4M3 = torch.float8_e4m3fn
+ADAMW_BLOCK = 256  # elements that share a scale of an 8-bit moment
+SCAN_STATE_STEPS = 64  # steps between two saved states
+
+
+class _on:
+    """the current device set to a tensor's, where it is another one"""
+
+    def __init__(self, t):
+        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _float_kind(t, name):
+    """1 for bf16, 0 for fp32; anything else and tensors that are not on the GPU are refused"""
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise capi.Vc3dError("%s must be a CUDA/HIP tensor: the vc3d path has no CPU fallback" % name)
+    if t.dtype not in (F32, BF16):
+        raise capi.Vc3dError("%s: expected fp32 or bf16, got %s" % (name, t.dtype))
+    return 1 if t.dtype == BF16 else 0
+
+
+def _same_device(ref, **others):
+    for name, t in others.items():
+        if t is not None and t.device != ref.device:
+            raise capi.Vc3dError("%s is on %s, not on %s" % (name, t.device, ref.device))
+
+
+def _rows(t):
+    """a matrix whose last dimension is contiguous and whose rows do not overlap: as it is, or a copy"""
+    return t if (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _ld(t):
+    """row stride of such a matrix"""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction):
+    kind = _float_kind(x, "x")
+    if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1]:
+        raise capi.Vc3dError("linear_ce: x [N][D] and weight [V][D] expected, got %s and %s" % (tuple(x.shape), tuple(weight.shape)))
+    N, D, V = x.shape[0], x.shape[1], weight.shape[0]
+    if V == 0 or D == 0:
+        raise capi.Vc3dError("linear_ce: no classes or no features (weight %s)" % (tuple(weight.shape),))
+    _same_device(x, weight=weight, labels=labels, bias=bias)
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.dtype != x.dtype:
+            raise capi.Vc3dError("linear_ce: %s is %s, x is %s" % (name, t.dtype, x.dtype))
+    if labels.dtype != torch.int64 or labels.dim() != 1 or labels.shape[0] != N:
+        raise capi.Vc3dError("linear_ce: labels int64 [%d] expected, got %s %s" % (N, labels.dtype, tuple(labels.shape)))
+    if bias is not None and tuple(bias.shape) != (V,):
+        raise capi.Vc3dError("linear_ce: bias [%d] expected, got %s" % (V, tuple(bias.shape)))
+    return capi.LinearCeDesc(N, D, V, kind, reduction, 0, _ld(x), _ld(weight), ignore_index)
+
+
+def linear_ce_fwd(x, weight, labels, bias=None, ignore_index=-100, reduction=1):
+    """cross-entropy of x weight^T + bias against labels, the vocabulary in pieces (vc_linear_ce_fwd); reduction 0 none, 1 mean
+    over the rows that count, 2 sum -> (loss [1] or [N], lse [N], rows): lse and rows are what linear_ce_bwd takes.
+    x [N][D] and weight [V][D] have contiguous rows (_rows), bias and labels are contiguous."""
+    d = _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction)
+    with _on(x):
+        loss = torch.empty(x.shape[0] if reduction == 0 else 1, dtype=F32, device=x.device)
+        lse = torch.empty(x.shape[0], dtype=F32, device=x.device)
+        rows = torch.empty(x.shape[0] + 4, dtype=torch.int32, device=x.device)
+        if x.shape[0] == 0:
+            return loss.zero_(), lse, rows
+        need = lib.vc_linear_ce_workspace_bytes(d, 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        check(lib.vc_linear_ce_fwd(d, ptr(x), ptr(weight), ptr(bias), ptr(labels), ptr(loss) if reduction else None,
+                                   None if reduction else ptr(loss), ptr(lse), ptr(rows), ptr(ws), need, cur_stream()), "vc_linear_ce_fwd")
+    return loss, lse, rows
+
+
+def linear_ce_bwd(x, weight, labels, bias, lse, rows, dloss, ignore_index=-100, reduction=1, want=(True, True, True)):
+    """gradients of linear_ce_fwd's loss with respect to (x, weight, bias), those that `want` names -> contiguous tensors of
+    x's type, or None (vc_linear_ce_bwd)"""
+    d = _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction)
+    N = x.shape[0]
+    _chk(lse, F32, N, "lse")
+    _chk(rows, torch.int32, N + 4, "rows")
+    _chk(dloss, F32, N if reduction == 0 else 1, "dloss")
+    _same_device(x, lse=lse, rows=rows, dloss=dloss)
+    with _on(x):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
+        dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device) if want[1] else None
+        db = torch.empty(bias.shape, dtype=x.dtype, device=x.device) if want[2] and bias is not None else None
+        if N == 0:
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+        need = lib.vc_linear_ce_workspace_bytes(d, 1)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        check(lib.vc_linear_ce_bwd(d, ptr(x), ptr(weight), ptr(bias), ptr(labels), ptr(lse), ptr(rows), ptr(dloss), ptr(dx), ptr(dw),
+                                   ptr(db), ptr(ws), need, cur_stream()), "vc_linear_ce_bwd")
+    return dx, dw, db
+
+
+def _scan_desc(gates, lengths, reverse):
+    kind = _float_kind(gates, "gates")
+    if gates.dim() != 3 or gates.shape[2] == 0 or gates.shape[2] % 2:
+        raise capi.Vc3dError("gated_scan: gates [B][T][2H] expected, got %s" % (tuple(gates.shape),))
+    B, T, H = gates.shape[0], gates.shape[1], gates.shape[2] // 2
+    if gates.stride(2) != 1:
+        raise capi.Vc3dError("gated_scan: the last dimension of gates must be contiguous")
+    if lengths is not None:
+        _chk(lengths, torch.int32, B, "lengths")
+        _same_device(gates, lengths=lengths)
+    return capi.ScanDesc(B, T, H, kind, 1 if reverse else 0, 0, gates.stride(0), gates.stride(1))
+
+
+def _scan_workspace(d, op, device):
+    need = lib.vc_gated_scan_workspace_bytes(d, op)
+    return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
+
+
+def gated_scan_fwd(gates, h0=None, lengths=None, reverse=False, want_states=False):
+    """the recurrence h_t = f h_(t-1) + (1 - f) v over [B][T], gates packed [B][T][2H] = (logits of f | v), any strides over B
+    and T (vc_gated_scan_fwd) -> (h [B][T][H], last state [B][H] fp32, states for gated_scan_bwd or None)"""
+    d = _scan_desc(gates, lengths, reverse)
+    _chk(h0, F32, d.B * d.H, "h0")
+    _same_device(gates, h0=h0)
+    with _on(gates):
+        h = torch.empty(d.B, d.T, d.H, dtype=gates.dtype, device=gates.device)
+        n = (d.T + SCAN_STATE_STEPS - 1) // SCAN_STATE_STEPS
+        states = torch.empty(d.B, n, d.H, dtype=F32, device=gates.device) if want_states else None
+        if d.T == 0 or d.B == 0:
+            last = torch.zeros(d.B, d.H, dtype=F32, device=gates.device) if h0 is None else h0.clone()
+            return h, last, states
+        last = torch.empty(d.B, d.H, dtype=F32, device=gates.device)
+        ws, need = _scan_workspace(d, 0, gates.device)
+        check(lib.vc_gated_scan_fwd(d, ptr(gates), ptr(h0), ptr(lengths), ptr(h), ptr(last), ptr(states), ptr(ws), need, cur_stream()),
+              "vc_gated_scan_fwd")
+    return h, last, states
+
+
+def gated_scan_bwd(gates, lengths, states, dy, dlast, reverse=False, want_dh0=True):
+    """gradients of gated_scan_fwd from those of h (dy, nullable) and of the last state (dlast, nullable)
+    -> (dgates [B][T][2H], dh0 [B][H] fp32 or None)"""
+    d = _scan_desc(gates, lengths, reverse)
+    _chk(states, F32, d.B * ((d.T + SCAN_STATE_STEPS - 1) // SCAN_STATE_STEPS) * d.H, "states")
+    _chk(dy, gates.dtype, d.B * d.T * d.H, "dy")
+    _chk(dlast, F32, d.B * d.H, "dlast")
+    _same_device(gates, states=states, dy=dy, dlast=dlast)
+    with _on(gates):
+        dgates = torch.empty(d.B, d.T, 2 * d.H, dtype=gates.dtype, device=gates.device)
+        dh0 = torch.empty(d.B, d.H, dtype=F32, device=gates.device) if want_dh0 else None
+        if d.T == 0 or d.B == 0:
+            if dh0 is not None:
+                dh0.zero_() if dlast is None else dh0.copy_(dlast.view(d.B, d.H))
+            return dgates, dh0
+        ws, need = _scan_workspace(d, 1, gates.device)
+        check(lib.vc_gated_scan_bwd(d, ptr(gates), ptr(lengths), ptr(states), ptr(dy), ptr(dlast), ptr(dgates), ptr(dh0), ptr(ws), need,
+                                    cur_stream()), "vc_gated_scan_bwd")
+    return dgates, dh0
+
+
+def gated_scan_step(gates, state):
+    """one step for each of B sequences: gates [B][2H] (rows of any stride), state [B][H] fp32 updated in place -> h [B][H] of
+    gates' type (vc_gated_scan_step)"""
+    kind = _float_kind(gates, "gates")
+    if gates.dim() != 2 or gates.shape[1] == 0 or gates.shape[1] % 2 or gates.stride(1) != 1:
+        raise capi.Vc3dError("gated_scan_step: gates [B][2H] with contiguous rows expected, got %s" % (tuple(gates.shape),))
+    B, H = gates.shape[0], gates.shape[1] // 2
+    _chk(state, F32, B * H, "state")
+    _same_device(gates, state=state)
+    with _on(gates):
+        h = torch.empty(B, H, dtype=gates.dtype, device=gates.device)
+        if B:
+            check(lib.vc_gated_scan_step(ptr(gates), gates.stride(0), kind, ptr(state), ptr(h), B, H, cur_stream()), "vc_gated_scan_step")
+            torch.autograd.graph.increment_version(state)
+    return h
+
+
+def _dense(t):
+    """whether a tensor's elements fill one stretch of memory, each once, in whatever order of dimensions"""
+    if t.is_contiguous():
+        return True
+    at = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride != at:
+            return False
+        at *= size
+    return True
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, m_scale=None, v_scale=None, *, lr, beta1, beta2, eps, weight_decay, step,
+               grad_scale=None):
+    """one AdamW step, in place, over lists of tensors (vc_adamw_step).  params and grads are fp32 or bf16; exp_avg and
+    exp_avg_sq are fp32, or, with m_scale and v_scale, float8_e4m3fn codes with one fp32 scale per 256 elements
+    (ceil(numel / 256) of them; exp_avg_sq's codes then hold the ROOT of the second moment).  A parameter may lie in memory in any
+    dense order of its dimensions (channels_last ...); its gradient and moments lie in the same one.  `step` counts from 1.
+    grad_scale: a number, or a one-element fp32 tensor on the device, that gradients are multiplied by."""
+    n = len(params)
+    eight = m_scale is not None
+    if eight != (v_scale is not None):
+        raise capi.Vc3dError("adamw_step: 8-bit moments need m_scale and v_scale, 32-bit ones neither")
+    lists = (grads, exp_avg, exp_avg_sq) + ((m_scale, v_scale) if eight else ())
+    if any(len(x) != n for x in lists):
+        raise capi.Vc3dError("adamw_step: the lists have %s entries" % ([n] + [len(x) for x in lists],))
+    if n == 0:
+        return
+    kind, dev, dt = _float_kind(params[0], "params[0]"), params[0].device, params[0].dtype
+    held = _E4M3 if eight else F32
+    table = []
+    for i in range(n):
+        p, g, m, v = params[i], grads[i], exp_avg[i], exp_avg_sq[i]
+        size = p.numel()
+        if p.dtype != dt or g.dtype != dt or m.dtype != held or v.dtype != held:
+            raise capi.Vc3dError("adamw_step: tensor %d has types %s, %s, %s, %s; %s, %s, %s, %s expected" %
+                                 (i, p.dtype, g.dtype, m.dtype, v.dtype, dt, dt, held, held))
+        if p.device != dev or g.device != dev or m.device != dev or v.device != dev:
+            raise capi.Vc3dError("adamw_step: tensor %d is not all on %s" % (i, dev))
+        if p.shape != g.shape or p.shape != m.shape or p.shape != v.shape:
+            raise capi.Vc3dError("adamw_step: tensor %d has shapes %s, %s, %s, %s" %
+                                 (i, tuple(p.shape), tuple(g.shape), tuple(m.shape), tuple(v.shape)))
+        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+            order = p.stride()
+            if not _dense(p) or size > 1 and not (g.stride() == order and m.stride() == order and v.stride() == order):
+                raise capi.Vc3dError("adamw_step: tensor %d and its gradient and moments must lie in memory in one dense order" % i)
+        a = b = 0
+        if eight:
+            rows = (size + ADAMW_BLOCK - 1) // ADAMW_BLOCK
+            for s in (m_scale[i], v_scale[i]):
+                _chk(s, F32, rows, "scales of tensor %d" % i)
+                if s.device != dev:
+                    raise capi.Vc3dError("adamw_step: scales of tensor %d are not on %s" % (i, dev))
+            a, b = m_scale[i].data_ptr(), v_scale[i].data_ptr()
+        table += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), a, b, size)
+    starts = [table[k] for k in range(0, 7 * n, 7) if table[k + 6]]
+    if len(set(starts)) != len(starts):
+        raise capi.Vc3dError("adamw_step: a parameter is in the list twice")
+    scale, scale_dev = 1.0, None
+    if torch.is_tensor(grad_scale):
+        _chk(grad_scale, F32, 1, "grad_scale")
+        _same_device(params[0], grad_scale=grad_scale)
+        scale_dev = grad_scale
+    elif grad_scale is not None:
+        scale = float(grad_scale)
+    hyper = capi.AdamwHyper(lr, beta1, beta2, eps, weight_decay, scale, step)
+    with _on(params[0]):
+        check(lib.vc_adamw_step((ctypes.c_int64 * len(table))(*table), n, kind, 8 if eight else 32, hyper, ptr(scale_dev), cur_stream()),
+              "vc_adamw_step")
+    for ts in (params,) + lists[1:]:
+        torch.autograd.graph.increment_version(ts)
 
 
 def ncthw_to_nthwc(x):
