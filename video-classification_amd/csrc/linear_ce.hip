@@ -41,54 +41,73 @@ __global__ __launch_bounds__(1024) void rows_kernel(const long long* labels, lon
     if (tid == 0) rows[N] = base;
 }
 
-// ---------------------------------------------------------------- matrix product, any sizes and strides
-// out[s][r] = sum_k S(s, k) R(r, k), 128 x 128 per workgroup of four waves (64 x 64 each).  An operand is addressed by row
-// and k strides (one of them is 1) and optional gather lists of its rows or its k.
+// ---------------------------------------------------------------- matrix products
+// out[s][r] = sum_k S(s, k) R(r, k).  A workgroup of WR x WS waves makes a BR x BS tile, a wave BR/WR x BS/WS of it, in steps
+// of 128 bytes of k (64 bf16, 32 fp32).  Both operand tiles of a step come in by DMA (global_load_lds, 16 bytes a lane), into
+// one of two buffers while the other one is multiplied.  An operand lies in memory with k contiguous (rows of x, w; P for dx)
+// or with its rows contiguous and k across (w for dx; x and P for dw: nothing is transposed in memory):
+//   k contiguous: LDS rows of 128 bytes, the 16-byte chunk c of row r at slot c ^ (r / 2 % 8); a fragment is one ds_read_b128.
+//   k across: LDS rows of one k each.  bf16: fragments come through ds_read_b64_tr_b16, which hands lane i of 16 the i-th
+//     column of four rows; a lane group reads four rows x 32 bytes, so the 32-byte unit u of row k lies at u ^ f(k) with f
+//     different for the eight rows that half a wave reads at once.  fp32: one ds_read_b32 a value, units of 64 bytes at u ^ (k / 4 % 4).
+// The swizzles act on the DMA's source address: what a lane fetches, not where it lands.
+// Nothing is read outside the operands: rows and columns behind the end are read from a row or column inside (what they make
+// is not stored), k behind the end from a page of zeros (k contiguous) or, with k across, from a k inside, where the other
+// operand, P, is 0 (EPI_PROB writes whole tiles of P, zeros behind the last row and the last word).
 struct Operand {
-    const void* p;
-    long long row, k;  // strides in elements
-    const int* rows;   // nullable: row i is at rows[i]
-    const int* ks;     // nullable: k is at ks[k]
+    const char* p;
+    long long ld;     // bytes from row to row (k contiguous) or from k to k (k across)
+    const int* list;  // nullable: the index of row i (k contiguous) or of k i (k across)
 };
 
 enum { EPI_STATS, EPI_PROB, EPI_DX, EPI_DW };
 
 struct Gemm {
     Operand R, S;
-    int nr, ns, K;
+    int nr, ns, K;      // K: where k is contiguous in an operand, a multiple of its 16-byte chunk
     const int* ns_dev;  // nullable: ns is *ns_dev
     const int* k_dev;   // nullable: K is *k_dev
+    int rtiles, stiles;
+    int k_split;  // k of one split (a multiple of the step), gridDim.y splits
     // EPI_STATS / EPI_PROB: r = word v0 + r, s = listed row
     const void* bias;
     const long long* labels;
     const int* rows;
     int v0;
-    float2* part;  // [s][tiles]
-    int tiles;
+    float2* part;  // [s][part_ld], this launch's tiles from part0 on
+    int part_ld, part0;
     float* zlab;   // [s]: logit of the row's label
     const float* lse;
     const float* scale;  // nullable: [N], each row's own factor
     void* P;
     long long ldp;
-    float* dbpart;  // [s tiles][nr]
-    float* acc;     // EPI_DX: [s][nr]
+    float* dbpart;   // nullable: [s tile][ldp]
+    float* acc;      // EPI_DX: [split][s][nr]
+    long long acc_split;
     int add;
     void* out;       // EPI_DW: [s][nr]
     const float* g;  // EPI_DW: the factor common to all rows
 };
 
+typedef __attribute__((address_space(1))) const void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+typedef __attribute__((address_space(3))) s16x4* ltr_t;
+
+__device__ __attribute__((aligned(128))) unsigned int vc_lce_zero_page[32];
+
 template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16> {
-    static constexpr int KSTEP = 32, PER = 8;  // k of an instruction, of a lane
+    static constexpr int STEP = 64, PER = 8;  // k of a step, of a 16-byte chunk
     typedef bf16x8 frag;
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Mma<float> {
-    static constexpr int KSTEP = 16, PER = 4;  // four instructions of k = 4; k is dealt to the lanes in fours, alike for both operands
+    static constexpr int STEP = 32, PER = 4;
     typedef f32x4 frag;
+    // four instructions of k = 4; k is dealt to the lane groups in fours, alike for both operands
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -96,148 +115,292 @@ struct Mma<float> {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ T fetch(const Operand& o, int row, int nrows, int k, int K) {
-    if (row >= nrows || k >= K) return (T)0.f;
-    const long long i = o.rows != nullptr ? o.rows[row] : row, j = o.ks != nullptr ? o.ks[k] : k;
-    return ((const T*)o.p)[i * o.row + j * o.k];
-}
+// one operand of a tile: ROWS rows, KACROSS = k across
+template <typename T, int ROWS, int NTHR, bool KACROSS>
+struct Tile {
+    static constexpr int STEP = Mma<T>::STEP, PER = Mma<T>::PER, BYTES = ROWS * 128;
+    static constexpr int PIECES = ROWS * 8 / NTHR;  // 16-byte pieces of a thread
+    static constexpr int CPR = ROWS / PER;          // k across: chunks of an LDS row
+    static constexpr int KPP = KACROSS ? NTHR / CPR : 1;  // k across: k of one pass of the workgroup
+    const char* p[PIECES];  // k contiguous: the piece at k = 0; k across: p[0] = its column
+    int tid;
+    // what a piece's chunk of a row of one k is moved by
+    static __device__ __forceinline__ int swz(int k) { return sizeof(T) == 2 ? ((k & 3) | ((k >> 3) & 1) << 2) << 1 : ((k >> 2) & 3) << 2; }
 
-template <typename T, int EPI>
-__global__ __launch_bounds__(256) void lce_gemm_any(const Gemm g) {
-    constexpr int BK = Mma<T>::KSTEP, PITCH = BK + Mma<T>::PER;
-    __shared__ __attribute__((aligned(16))) T sR[128][PITCH], sS[128][PITCH];
+    __device__ __forceinline__ void init(const Operand& o, int row0, int nrows) {
+        tid = threadIdx.x;
+        if (!KACROSS) {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                int row = row0 + j * (NTHR / 8) + (tid >> 3);
+                row = row < nrows ? row : nrows - 1;
+                const long long i = o.list != nullptr ? o.list[row] : row;
+                p[j] = o.p + i * o.ld + chunk() * 16;
+            }
+        } else
+            p[0] = o.p;
+    }
+    __device__ __forceinline__ int chunk() const { return (tid & 7) ^ ((tid >> 4) & 7); }  // k contiguous: of every piece (rows differ by 16s)
+    // k across: the k that piece j of the step at k0 reads, clamped and looked up
+    __device__ __forceinline__ int at(const Operand& o, int k0, int K, int j) const {
+        int k = k0 + j * KPP + tid / CPR;
+        k = k < K ? k : K - 1;
+        return o.list != nullptr ? o.list[k] : k;
+    }
+    __device__ __forceinline__ void issue(const Operand& o, char* lds, int k0, int K, int row0, int nrows, const int* ks) const {
+        char* const base = lds + (tid >> 6) * 1024;
+        if (!KACROSS) {
+            const bool out = k0 + STEP > K && k0 + chunk() * PER >= K;
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                const gptr_t src = out ? (gptr_t)vc_lce_zero_page : (gptr_t)(p[j] + (long long)k0 * (int)sizeof(T));
+                __builtin_amdgcn_global_load_lds(src, (lptr_t)(base + j * NTHR * 16), 16, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                int c = row0 + ((tid % CPR) ^ swz(j * KPP + tid / CPR)) * PER;
+                c = c < nrows ? c : 0;
+                __builtin_amdgcn_global_load_lds((gptr_t)(p[0] + (long long)ks[j] * o.ld + c * (int)sizeof(T)), (lptr_t)(base + j * NTHR * 16), 16, 0, 0);
+            }
+        }
+    }
+    // the fragment of rows [row, row + 16), half ks of the step
+    static __device__ __forceinline__ typename Mma<T>::frag frag(const char* lds, int row, int ks, int l15, int lg) {
+        if (!KACROSS) {
+            const int r = row + l15;
+            return *(const typename Mma<T>::frag*)(lds + r * 128 + ((((ks << 2) + lg) ^ ((r >> 1) & 7)) << 4));
+        }
+        const int u = row / 16;
+        typename Mma<T>::frag f;
+        if constexpr (sizeof(T) == 2) {
+            const int k = ks * 32 + lg * 8 + (l15 >> 2);
+            const char* q = lds + k * (ROWS * 2) + ((u ^ (swz(k) >> 1)) << 5) + (l15 & 3) * 8;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)(q + 4 * ROWS * 2));
+            f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = *(const float*)(lds + (ks * 16 + lg * 4 + i) * (ROWS * 4) + ((u ^ lg) << 6) + l15 * 4);
+        }
+        return f;
+    }
+};
+
+template <typename T, int EPI, int BR, int BS, int WR, int WS>
+__global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
+    constexpr int NTHR = WR * WS * 64, STEP = Mma<T>::STEP;
+    constexpr int NA = BR / WR / 16, NB = BS / WS / 16;
+    constexpr bool RK = EPI == EPI_DX || EPI == EPI_DW, SK = EPI == EPI_DW;
+    typedef Tile<T, BR, NTHR, RK> TR;
+    typedef Tile<T, BS, NTHR, SK> TS;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int BUF = TR::BYTES + TS::BYTES;
     const int ns = g.ns_dev != nullptr ? *g.ns_dev : g.ns, K = g.k_dev != nullptr ? *g.k_dev : g.K;
-    const int r0 = blockIdx.x * 128, s0 = blockIdx.y * 128;
+    // tile order: XCD x (workgroups go round the 8 XCDs) takes the x-th share of an order in which 4 tiles of s by all tiles of r
+    // follow each other, so that the 32 workgroups of an XCD share 4 + 8 operand panels in its L2
+    int r0, s0, st;
+    {
+        const unsigned total = gridDim.x, lin = blockIdx.x, x = lin & 7u, base = total >> 3, rem = total & 7u;
+        const unsigned t = x * base + (x < rem ? x : rem) + (lin >> 3);
+        const unsigned per = 4u * g.rtiles, grp = t / per, in = t - grp * per;
+        const unsigned left = g.stiles - grp * 4u, w = left < 4u ? left : 4u;
+        r0 = (int)(in / w) * BR, st = (int)(grp * 4u + in % w), s0 = st * BS;
+    }
     if (s0 >= ns) return;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
-    const int wr = (wave & 1) * 64, wsx = (wave >> 1) * 64;
-    f32x4 acc[4][4];
+    const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = (wave % WR) * (BR / WR), wsx = (wave / WR) * (BS / WS);
+    f32x4 acc[NA][NB];
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) acc[a][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < K; k0 += BK) {
-        // neighbouring threads take neighbouring addresses: along k where k is contiguous, along the rows otherwise
-        for (int i = tid; i < 128 * BK; i += 256) {
-            const int rr = g.R.k == 1 ? i / BK : i % 128, rk = g.R.k == 1 ? i % BK : i / 128;
-            sR[rr][rk] = fetch<T>(g.R, r0 + rr, g.nr, k0 + rk, K);
-            const int sr = g.S.k == 1 ? i / BK : i % 128, sk = g.S.k == 1 ? i % BK : i / 128;
-            sS[sr][sk] = fetch<T>(g.S, s0 + sr, ns, k0 + sk, K);
+        for (int b = 0; b < NB; ++b) acc[a][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int kb = blockIdx.y * g.k_split, ke = K < kb + g.k_split ? K : kb + g.k_split;
+    if (kb < ke) {
+        TR tr;
+        TS ts;
+        tr.init(g.R, r0, g.nr);
+        ts.init(g.S, s0, ns);
+        int kr[RK ? TR::PIECES : 1], kt[SK ? TS::PIECES : 1];
+        auto look = [&](int k0) {
+            if (RK)
+#pragma unroll
+                for (int j = 0; j < TR::PIECES; ++j) kr[j] = tr.at(g.R, k0, K, j);
+            if (SK)
+#pragma unroll
+                for (int j = 0; j < TS::PIECES; ++j) kt[j] = ts.at(g.S, k0, (K + STEP - 1) / STEP * STEP, j);  // (P: zeros up to there)
+        };
+        auto issue = [&](int k0, char* buf) {
+            tr.issue(g.R, buf, k0, K, r0, g.nr, kr);
+            ts.issue(g.S, buf + TR::BYTES, k0, K, s0, (int)(g.S.ld / (int)sizeof(T)), kt);
+        };
+        look(kb);
+        issue(kb, smem);
+        look(kb + STEP);
+        int cur = 0;
+        for (int k0 = kb; k0 < ke; k0 += STEP, cur ^= 1) {
+            __syncthreads();  // this step's tiles have landed; the other buffer has been read
+            if (k0 + STEP < ke) {
+                issue(k0 + STEP, smem + (cur ^ 1) * BUF);
+                look(k0 + 2 * STEP);
+            }
+            const char* const lr = smem + cur * BUF;
+            const char* const ls = lr + TR::BYTES;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                typename Mma<T>::frag fs[NB];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) fs[b] = TS::frag(ls, wsx + b * 16, ks, l15, lg);
+#pragma unroll
+                for (int a = 0; a < NA; ++a) {
+                    const typename Mma<T>::frag fr = TR::frag(lr, wr + a * 16, ks, l15, lg);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) acc[a][b] = Mma<T>::run(fr, fs[b], acc[a][b]);
+                }
+            }
         }
-        __syncthreads();
-        typename Mma<T>::frag fs[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) fs[b] = *(const typename Mma<T>::frag*)&sS[wsx + b * 16 + l15][lg * Mma<T>::PER];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const typename Mma<T>::frag fr = *(const typename Mma<T>::frag*)&sR[wr + a * 16 + l15][lg * Mma<T>::PER];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) acc[a][b] = Mma<T>::run(fr, fs[b], acc[a][b]);
-        }
-        __syncthreads();
     }
     // acc[a][b][j] = out[s = s0 + wsx + 16 b + l15][r = r0 + wr + 16 a + 4 lg + j]
-    if (EPI == EPI_STATS || EPI == EPI_PROB) {
+    if constexpr (EPI == EPI_STATS || EPI == EPI_PROB) {
+        const bool edge = r0 + BR > g.nr;
+        if (g.bias != nullptr || edge)
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
+            for (int a = 0; a < NA; ++a)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = r0 + wr + a * 16 + lg * 4 + j;
-                const float bias = g.bias != nullptr && r < g.nr ? (float)((const T*)g.bias)[g.v0 + r] : 0.f;
+                for (int j = 0; j < 4; ++j) {
+                    const int r = r0 + wr + a * 16 + lg * 4 + j;
+                    const float bias = g.bias != nullptr && r < g.nr ? (float)((const T*)g.bias)[g.v0 + r] : 0.f;
 #pragma unroll
-                for (int b = 0; b < 4; ++b) acc[a][b][j] = r < g.nr ? acc[a][b][j] + bias : -INFINITY;
-            }
+                    for (int b = 0; b < NB; ++b) acc[a][b][j] = r < g.nr ? acc[a][b][j] + bias : -INFINITY;
+                }
     }
-    if (EPI == EPI_STATS) {
-        __shared__ float2 join[2][128];
+    constexpr float LOG2E = 1.44269504088896340736f;
+    if constexpr (EPI == EPI_STATS) {
+        __syncthreads();
+        float2* const join = (float2*)smem;  // [WR][BS]
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < NB; ++b) {
             const int s = s0 + wsx + b * 16 + l15;
-            const long long label = s < ns ? g.labels[g.rows[s]] - g.v0 : -1;
+            const long long label = s < ns ? g.labels[g.rows[s]] - g.v0 - r0 - wr - lg * 4 : -1;
             float m = -INFINITY, e = 0.f;
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
+            for (int a = 0; a < NA; ++a)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     m = fmaxf(m, acc[a][b][j]);
-                    if (r0 + wr + a * 16 + lg * 4 + j == label && label < g.nr) g.zlab[s] = acc[a][b][j];
+                    if (label == a * 16 + j) g.zlab[s] = acc[a][b][j];
                 }
             m = fmaxf(m, __shfl_xor(m, 16, 64));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
             const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
+            for (int a = 0; a < NA; ++a)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) e += __expf(acc[a][b][j] - ref);
+                for (int j = 0; j < 4; ++j) e += __builtin_amdgcn_exp2f((acc[a][b][j] - ref) * LOG2E);
             e += __shfl_xor(e, 16, 64);
             e += __shfl_xor(e, 32, 64);
-            if (lg == 0) join[wave & 1][wsx + b * 16 + l15] = make_float2(m, e);
+            if (lg == 0) join[(wave % WR) * BS + wsx + b * 16 + l15] = make_float2(m, e);
         }
         __syncthreads();
-        if (tid < 128 && s0 + tid < ns) {
-            const float2 p = join[0][tid], q = join[1][tid];
-            const float m = fmaxf(p.x, q.x), ref = m == -INFINITY ? 0.f : m;
-            g.part[(size_t)(s0 + tid) * g.tiles + blockIdx.x] = make_float2(m, p.y * __expf(p.x - ref) + q.y * __expf(q.x - ref));
+        if (tid < BS && s0 + tid < ns) {
+            float m = -INFINITY, e = 0.f;
+#pragma unroll
+            for (int w = 0; w < WR; ++w) m = fmaxf(m, join[w * BS + tid].x);
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int w = 0; w < WR; ++w) e += join[w * BS + tid].y * __builtin_amdgcn_exp2f((join[w * BS + tid].x - ref) * LOG2E);
+            g.part[(long long)(s0 + tid) * g.part_ld + g.part0 + r0 / BR] = make_float2(m, e);
         }
-        return;
     }
-    if (EPI == EPI_PROB) {
-        __shared__ float colsum[2][128];
-        f32x4 cs[4];
+    if constexpr (EPI == EPI_PROB) {
+        f32x4 cs[NA];
 #pragma unroll
-        for (int a = 0; a < 4; ++a) cs[a] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int a = 0; a < NA; ++a) cs[a] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < NB; ++b) {
             const int s = s0 + wsx + b * 16 + l15;
-            if (s < ns) {
-                const int n = g.rows[s];
-                const long long label = g.labels[n] - g.v0;
-                const float lse = g.lse[n], sc = g.scale != nullptr ? g.scale[n] : 1.f;
+            const bool in = s < ns;
+            const int n = in ? g.rows[s] : 0;
+            const long long label = in ? g.labels[n] - g.v0 - r0 - wr - lg * 4 : -1;
+            const float lse = in ? g.lse[n] : 0.f, sc = !in ? 0.f : g.scale != nullptr ? g.scale[n] : 1.f;
+            T* const row = (T*)g.P + (long long)s * g.ldp + r0 + wr + lg * 4;
 #pragma unroll
-                for (int a = 0; a < 4; ++a)
+            for (int a = 0; a < NA; ++a) {
+                f32x4 v;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = r0 + wr + a * 16 + lg * 4 + j;
-                        const float v = (__expf(acc[a][b][j] - lse) - (r == label ? 1.f : 0.f)) * sc;
-                        if (r < g.nr) {
-                            cs[a][j] += v;
-                            ((T*)g.P)[(size_t)s * g.ldp + r] = (T)v;
-                        }
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = __builtin_amdgcn_exp2f((acc[a][b][j] - lse) * LOG2E) - (label == a * 16 + j ? 1.f : 0.f);
+                    v[j] = in ? v[j] * sc : 0.f;
+                }
+                if (r0 + BR > g.nr)  // (behind the last word: 0, also in a row whose lse is no number)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = r0 + wr + a * 16 + lg * 4 + j < g.nr ? v[j] : 0.f;
+                cs[a] += v;
+                if constexpr (sizeof(T) == 2) *(bf16x4*)(row + a * 16) = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
+                else *(f32x4*)(row + a * 16) = v;
             }
         }
         if (g.dbpart != nullptr) {
+            __syncthreads();
+            float* const colsum = (float*)smem;  // [WS][BR]
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
+            for (int a = 0; a < NA; ++a)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     float v = cs[a][j];
 #pragma unroll
                     for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o, 64);
-                    if (l15 == 0) colsum[wave >> 1][wr + a * 16 + lg * 4 + j] = v;
+                    if (l15 == 0) colsum[(wave / WR) * BR + wr + a * 16 + lg * 4 + j] = v;
                 }
             __syncthreads();
-            if (tid < 128 && r0 + tid < g.nr) g.dbpart[(size_t)blockIdx.y * g.nr + r0 + tid] = colsum[0][tid] + colsum[1][tid];
-        }
-        return;
-    }
+            if (tid < BR) {
+                float v = 0.f;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const int s = s0 + wsx + b * 16 + l15;
-        if (s >= ns) continue;
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = r0 + wr + a * 16 + lg * 4 + j;
-                if (r >= g.nr) continue;
-                if (EPI == EPI_DX) {
-                    float* q = g.acc + (size_t)s * g.nr + r;
-                    *q = acc[a][b][j] + (g.add ? *q : 0.f);
-                } else
-                    ((T*)g.out)[(size_t)s * g.nr + r] = (T)(acc[a][b][j] * *g.g);
+                for (int w = 0; w < WS; ++w) v += colsum[w * BR + tid];
+                g.dbpart[(long long)st * g.ldp + r0 + tid] = v;
             }
+        }
+    }
+    if constexpr (EPI == EPI_DX || EPI == EPI_DW) {
+        const float f = EPI == EPI_DW ? *g.g : 1.f;
+        const bool vec = (g.nr & 3) == 0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int s = s0 + wsx + b * 16 + l15;
+            if (s >= ns) continue;
+#pragma unroll
+            for (int a = 0; a < NA; ++a) {
+                const int r = r0 + wr + a * 16 + lg * 4;
+                if constexpr (EPI == EPI_DX) {
+                    float* const q = g.acc + blockIdx.y * g.acc_split + (long long)s * g.nr + r;
+                    if (vec && r < g.nr) *(f32x4*)q = g.add ? acc[a][b] + *(const f32x4*)q : acc[a][b];
+                    else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (r + j < g.nr) q[j] = acc[a][b][j] + (g.add ? q[j] : 0.f);
+                } else {
+                    T* const q = (T*)g.out + (long long)s * g.nr + r;
+                    const f32x4 v = acc[a][b] * f;
+                    if (vec && r < g.nr) {
+                        if constexpr (sizeof(T) == 2) *(bf16x4*)q = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
+                        else *(f32x4*)q = v;
+                    } else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (r + j < g.nr) q[j] = (T)v[j];
+                }
+            }
+        }
+    }
+}
+
+// rows whose bytes are no whole 16-byte chunks, or begin at none, are copied: [n][D] -> [n][dp], zeros behind D
+template <typename T>
+__global__ __launch_bounds__(256) void lce_pack_kernel(const T* in, long long ld, long long n, int D, int dp, T* out) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n * dp; i += (long long)gridDim.x * 256) {
+        const long long r = i / dp;
+        const int d = (int)(i - r * dp);
+        out[i] = d < D ? in[r * ld + d] : (T)0.f;
     }
 }
 
@@ -296,52 +459,71 @@ __global__ void lce_factor_kernel(const float* dloss, const int* rows, int N, in
 }
 // dx of the rows that count from their sums, zeros for the others
 template <typename T>
-__global__ __launch_bounds__(256) void lce_dx_kernel(const float* acc, const int* rows, const float* g, int N, int D, T* dx) {
+__global__ __launch_bounds__(256) void lce_dx_kernel(const float* acc, int splits, long long split, const int* rows, const float* g, int N, int D,
+                                                     T* dx) {
     const int i = blockIdx.x, n = rows[i];
     const bool keep = i < rows[N];
-    for (int d = threadIdx.x; d < D; d += 256) dx[(size_t)n * D + d] = keep ? (T)(acc[(size_t)i * D + d] * *g) : (T)0.f;
+    for (int d = threadIdx.x; d < D; d += 256) {
+        float v = 0.f;
+        for (int k = 0; k < splits && keep; ++k) v += acc[k * split + (long long)i * D + d];
+        dx[(long long)n * D + d] = keep ? (T)(v * *g) : (T)0.f;
+    }
 }
 template <typename T>
-__global__ __launch_bounds__(256) void lce_db_kernel(const float* part, const int* count, const float* g, int nr, T* db) {
+__global__ __launch_bounds__(256) void lce_db_kernel(const float* part, long long ld, int bs, const int* count, const float* g, int nr, T* db) {
     const int r = blockIdx.x * 256 + threadIdx.x;
     if (r >= nr) return;
-    const int tiles = (*count + 127) / 128;
+    const int tiles = (*count + bs - 1) / bs;
     float s = 0.f;
-    for (int t = 0; t < tiles; ++t) s += part[(size_t)t * nr + r];
+    for (int t = 0; t < tiles; ++t) s += part[t * ld + r];
     db[r] = (T)(s * *g);
 }
 
-// ---------------------------------------------------------------- workspace
-struct Layout {
+// ---------------------------------------------------------------- plan and workspace
+struct Plan {
     size_t bytes = 0;
+    int tile;        // side of a tile
+    int piece;       // words of a piece, a multiple of the tile
+    int tiles;       // tiles of the vocabulary
+    int splits;      // of k in the product for dx
+    int dp;          // row length of x, w as the products read them
+    bool pack;       // x, w have to be copied for that
+    size_t g, acc, P, dbpart, part, zlab, loss_rows, xp, wp;
     size_t take(size_t n) {
         const size_t at = bytes;
         bytes += (n + 255) & ~(size_t)255;
         return at;
     }
-};
-struct FwdLayout : Layout {
-    size_t part, zlab, loss_rows;
-    int tiles;
-    FwdLayout(int N, int V) {
-        tiles = (V + 127) / 128;
-        part = take((size_t)N * tiles * sizeof(float2));
-        zlab = take((size_t)N * 4);
-        loss_rows = take((size_t)N * 4);
-    }
-};
-struct BwdLayout : Layout {
-    size_t g, acc, P, dbpart;
-    int piece;
-    BwdLayout(int N, int D, int V, int elem) {
-        // a piece's P takes up to 256 MB (what stays near the chip between its writer and its two readers), in whole tiles
-        const long long fit = (256ll << 20) / elem / N / 128 * 128;
-        const long long all = (V + 127ll) / 128 * 128;
-        piece = (int)(fit < 128 ? 128 : fit < all ? fit : all);
+    // what the sizes alone decide; `aligned`: both operands' rows begin at 16-byte chunks (if not known: the larger need)
+    Plan(int N, int D, int V, int elem, int op, bool aligned) {
+        const int per = 16 / elem;
+        pack = !aligned || D % per != 0;
+        dp = (D + per - 1) / per * per;
+        tile = N > 128 && (long long)N * V >= (1ll << 22) ? 256 : 128;
+        const long long np = ((long long)N + tile - 1) / tile * tile, all = ((long long)V + tile - 1) / tile * tile;
+        long long fit = (512ll << 20) / elem / np / tile * tile;
+        if (pack && op == 0) fit = (512ll << 20) / elem / dp / tile * tile;  // (the forward holds a piece of w only)
+        fit = fit < tile ? tile : fit;
+        piece = (int)(op == 0 && !pack ? all : fit < all ? fit : all);
+        tiles = (int)(all / tile);
+        if (pack) {
+            xp = take((size_t)N * dp * elem);
+            wp = take((size_t)(piece < V ? piece : V) * dp * elem);
+        }
+        if (op == 0) {
+            part = take((size_t)N * tiles * sizeof(float2));
+            zlab = take((size_t)N * 4);
+            loss_rows = take((size_t)N * 4);
+            return;
+        }
+        const long long t = np / tile * ((D + tile - 1) / tile), most = piece / 512 > 1 ? piece / 512 : 1;
+        long long z = 512 / t;
+        z = z < 1 ? 1 : z > most ? most : z;
+        splits = (int)(z > 16 ? 16 : z);
         g = take(4);
-        acc = take((size_t)N * D * 4);
-        P = take((size_t)N * piece * elem);
-        dbpart = take((size_t)((N + 127) / 128) * piece * 4);
+        acc = take((size_t)splits * N * D * 4);
+        P = take((size_t)np * piece * elem);
+        dbpart = take((size_t)(np / tile) * piece * 4);
     }
 };
 
@@ -354,21 +536,70 @@ int launched(const char* what) {
     return 0;
 }
 
+template <typename T, int EPI, int B>
+void gemm_tile(const Gemm& g, int splits, hipStream_t s) {
+    constexpr int WR = 2, WS = B == 256 ? 4 : 2, LDS = 2 * 2 * B * 128;
+    const auto kernel = lce_gemm<T, EPI, B, B, WR, WS>;
+    static VcPerDeviceOnce once;
+    once.run([&] { (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
+    hipLaunchKernelGGL((lce_gemm<T, EPI, B, B, WR, WS>), dim3(g.rtiles * g.stiles, splits), dim3(WR * WS * 64), LDS, s, g);
+}
+template <typename T, int EPI>
+void gemm(Gemm& g, int tile, int ns_most, int splits, hipStream_t s) {
+    g.rtiles = (g.nr + tile - 1) / tile, g.stiles = (ns_most + tile - 1) / tile;
+    if (tile == 256) gemm_tile<T, EPI, 256>(g, splits, s);
+    else gemm_tile<T, EPI, 128>(g, splits, s);
+}
+
+template <typename T>
+void pack(const void* in, long long ld, long long n, int D, int dp, void* out, hipStream_t s) {
+    const long long blocks = (n * dp + 255) / 256;
+    hipLaunchKernelGGL((lce_pack_kernel<T>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, (const T*)in, ld, n, D, dp, (T*)out);
+}
+
+bool chunks(const VcLceParams& p, int elem) {
+    return (((uintptr_t)p.x | (uintptr_t)p.w | (uintptr_t)(p.ldx * elem) | (uintptr_t)(p.ldw * elem)) & 15) == 0;
+}
+
+// x as the products read it, and w from word v0 on
+template <typename T>
+struct Source {
+    const VcLceParams& p;
+    const Plan& L;
+    hipStream_t s;
+    Operand x;
+    Source(const VcLceParams& p, const Plan& L, hipStream_t s) : p(p), L(L), s(s) {
+        x = {(const char*)p.x, p.ldx * (long long)sizeof(T), p.rows};
+        if (L.pack) {
+            pack<T>(p.x, p.ldx, p.N, p.D, L.dp, (char*)p.ws + L.xp, s);
+            x = {(const char*)p.ws + L.xp, L.dp * (long long)sizeof(T), p.rows};
+        }
+    }
+    Operand w(int v0, int nv) const {
+        const T* at = (const T*)p.w + v0 * p.ldw;
+        if (!L.pack) return {(const char*)at, p.ldw * (long long)sizeof(T), nullptr};
+        pack<T>(at, p.ldw, nv, p.D, L.dp, (char*)p.ws + L.wp, s);
+        return {(const char*)p.ws + L.wp, L.dp * (long long)sizeof(T), nullptr};
+    }
+};
+
 template <typename T>
 int fwd(const VcLceParams& p, hipStream_t s) {
-    const FwdLayout L(p.N, p.V);
+    const Plan L(p.N, p.D, p.V, sizeof(T), 0, chunks(p, sizeof(T)));
     char* ws = (char*)p.ws;
     float2* part = (float2*)(ws + L.part);
     float* zlab = (float*)(ws + L.zlab);
     float* loss_rows = p.loss_rows != nullptr ? p.loss_rows : (float*)(ws + L.loss_rows);
     (void)hipGetLastError();
     hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, s, p.labels, p.ignore_index, p.N, p.rows);
-    Gemm g = {};
-    g.R = {p.w, p.ldw, 1, nullptr, nullptr};
-    g.S = {p.x, p.ldx, 1, p.rows, nullptr};
-    g.nr = p.V, g.ns_dev = p.rows + p.N, g.K = p.D;
-    g.bias = p.bias, g.labels = p.labels, g.rows = p.rows, g.part = part, g.tiles = L.tiles, g.zlab = zlab;
-    hipLaunchKernelGGL((lce_gemm_any<T, EPI_STATS>), dim3(L.tiles, (p.N + 127) / 128), dim3(256), 0, s, g);
+    const Source<T> src(p, L, s);
+    for (int v0 = 0; v0 < p.V; v0 += L.piece) {
+        Gemm g = {};
+        g.nr = p.V - v0 < L.piece ? p.V - v0 : L.piece, g.ns_dev = p.rows + p.N, g.K = g.k_split = L.dp;
+        g.R = src.w(v0, g.nr), g.S = src.x;
+        g.bias = p.bias, g.labels = p.labels, g.rows = p.rows, g.v0 = v0, g.part = part, g.part_ld = L.tiles, g.part0 = v0 / L.tile, g.zlab = zlab;
+        gemm<T, EPI_STATS>(g, L.tile, p.N, 1, s);
+    }
     hipLaunchKernelGGL(lce_rows_kernel, dim3((p.N + 3) / 4), dim3(256), 0, s, part, L.tiles, zlab, p.labels, p.rows, p.N, p.V, p.lse,
                        loss_rows);
     if (p.reduction != 0)
@@ -378,48 +609,51 @@ int fwd(const VcLceParams& p, hipStream_t s) {
 
 template <typename T>
 int bwd(const VcLceParams& p, hipStream_t s) {
-    const BwdLayout L(p.N, p.D, p.V, sizeof(T));
+    const Plan L(p.N, p.D, p.V, sizeof(T), 1, chunks(p, sizeof(T)));
     char* ws = (char*)p.ws;
     float *factor = (float*)(ws + L.g), *acc = (float*)(ws + L.acc), *dbpart = (float*)(ws + L.dbpart);
     const int* count = p.rows + p.N;
-    const int st = (p.N + 127) / 128, dt = (p.D + 127) / 128;
+    const long long ldp = (long long)L.piece * (int)sizeof(T);
     (void)hipGetLastError();
     hipLaunchKernelGGL(lce_factor_kernel, dim3(1), dim3(1), 0, s, p.dloss, p.rows, p.N, p.reduction, factor);
+    const Source<T> src(p, L, s);
     for (int v0 = 0; v0 < p.V; v0 += L.piece) {
-        const int nv = p.V - v0 < L.piece ? p.V - v0 : L.piece, vt = (nv + 127) / 128;
-        const T* w = (const T*)p.w + (long long)v0 * p.ldw;
+        const int nv = p.V - v0 < L.piece ? p.V - v0 : L.piece;
+        const Operand w = src.w(v0, nv);
         Gemm g = {};
-        g.R = {w, p.ldw, 1, nullptr, nullptr};
-        g.S = {p.x, p.ldx, 1, p.rows, nullptr};
-        g.nr = nv, g.ns_dev = count, g.K = p.D;
+        g.R = w, g.S = src.x;
+        g.nr = nv, g.ns_dev = count, g.K = g.k_split = L.dp;
         g.bias = p.bias, g.labels = p.labels, g.rows = p.rows, g.v0 = v0;
         g.lse = p.lse, g.scale = p.reduction == 0 ? p.dloss : nullptr, g.P = ws + L.P, g.ldp = L.piece, g.dbpart = p.db != nullptr ? dbpart : nullptr;
-        hipLaunchKernelGGL((lce_gemm_any<T, EPI_PROB>), dim3(vt, st), dim3(256), 0, s, g);
+        gemm<T, EPI_PROB>(g, L.tile, p.N, 1, s);
         if (p.db != nullptr)
-            hipLaunchKernelGGL((lce_db_kernel<T>), dim3((nv + 255) / 256), dim3(256), 0, s, dbpart, count, factor, nv, (T*)p.db + v0);
+            hipLaunchKernelGGL((lce_db_kernel<T>), dim3((nv + 255) / 256), dim3(256), 0, s, dbpart, (long long)L.piece, L.tile, count, factor, nv,
+                               (T*)p.db + v0);
         if (p.dx != nullptr) {
             Gemm x = {};
-            x.R = {w, 1, p.ldw, nullptr, nullptr};
-            x.S = {ws + L.P, L.piece, 1, nullptr, nullptr};
-            x.nr = p.D, x.ns_dev = count, x.K = nv, x.acc = acc, x.add = v0 > 0;
-            hipLaunchKernelGGL((lce_gemm_any<T, EPI_DX>), dim3(dt, st), dim3(256), 0, s, x);
+            x.R = w, x.S = {ws + L.P, ldp, nullptr};
+            x.nr = p.D, x.ns_dev = count, x.K = nv, x.acc = acc, x.add = v0 > 0, x.acc_split = (long long)p.N * p.D;
+            x.k_split = ((nv + L.splits - 1) / L.splits + 127) / 128 * 128;
+            gemm<T, EPI_DX>(x, L.tile, p.N, L.splits, s);
         }
         if (p.dw != nullptr) {
             Gemm d = {};
-            d.R = {p.x, 1, p.ldx, nullptr, p.rows};
-            d.S = {ws + L.P, 1, L.piece, nullptr, nullptr};
-            d.nr = p.D, d.ns = nv, d.k_dev = count, d.out = (T*)p.dw + (size_t)v0 * p.D, d.g = factor;
-            hipLaunchKernelGGL((lce_gemm_any<T, EPI_DW>), dim3(dt, vt), dim3(256), 0, s, d);
+            d.R = src.x, d.S = {ws + L.P, ldp, nullptr};
+            d.nr = p.D, d.ns = nv, d.k_dev = count, d.k_split = 0x7fffffc0, d.out = (T*)p.dw + (long long)v0 * p.D, d.g = factor;
+            gemm<T, EPI_DW>(d, L.tile, nv, 1, s);
         }
     }
-    if (p.dx != nullptr) hipLaunchKernelGGL((lce_dx_kernel<T>), dim3(p.N), dim3(256), 0, s, acc, p.rows, factor, p.N, p.D, (T*)p.dx);
+    if (p.dx != nullptr)
+        hipLaunchKernelGGL((lce_dx_kernel<T>), dim3(p.N), dim3(256), 0, s, acc, L.splits, (long long)p.N * p.D, p.rows, factor, p.N, p.D, (T*)p.dx);
     return launched("linear_ce_bwd");
 }
 
 }  // namespace
 
 size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, int op) {
-    return op == 0 ? FwdLayout(N, V).bytes : BwdLayout(N, D, V, is_bf16 ? 2 : 4).bytes;
+    const int elem = is_bf16 ? 2 : 4;
+    const size_t a = Plan(N, D, V, elem, op, true).bytes, b = Plan(N, D, V, elem, op, false).bytes;
+    return a > b ? a : b;
 }
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? fwd<bf16>(p, s) : fwd<float>(p, s); }
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? bwd<bf16>(p, s) : bwd<float>(p, s); }
