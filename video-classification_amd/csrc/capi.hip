@@ -1243,6 +1243,8 @@ static int scan_check(const vc_scan_desc* d) {
     VC_REQUIRE(d->B > 0 && d->T > 0 && d->H > 0, "gated_scan: bad sizes B=%d T=%d H=%d", d->B, d->T, d->H);
     VC_REQUIRE(d->B <= 65535, "gated_scan: at most 65535 sequences (got %d)", d->B);
     VC_REQUIRE(d->T <= (1 << 30) && d->H <= (1 << 24), "gated_scan: T=%d or H=%d too large", d->T, d->H);
+    VC_REQUIRE(((long long)d->T + 63) / 64 * d->B * ((d->H + 127) / 128) < (1ll << 31), "gated_scan: B=%d T=%d H=%d are too many tiles", d->B,
+               d->T, d->H);
     return 0;
 }
 static VcScanParams scan_params(const vc_scan_desc* d, const void* gates, const int32_t* lengths) {
@@ -1254,29 +1256,33 @@ static VcScanParams scan_params(const vc_scan_desc* d, const void* gates, const 
 }
 static bool pair_aligned(const void* q, int32_t is_bf16) { return ((uintptr_t)q & (is_bf16 ? 3 : 7)) == 0; }
 size_t vc_gated_scan_workspace_bytes(const vc_scan_desc* d, int32_t op) {
-    (void)op;
-    return d == nullptr ? 0 : 0;
+    return scan_check(d) != 0 ? 0 : vc_scan_workspace(d->B, d->T, d->H, op);
 }
 int vc_gated_scan_fwd(const vc_scan_desc* d, const void* gates, const float* h0, const int32_t* lengths, void* h, float* last,
                       float* states, void* workspace, size_t ws_bytes, void* stream) {
-    (void)workspace, (void)ws_bytes;
     const int rc = scan_check(d);
     if (rc) return rc;
     VC_REQUIRE(gates && h && last, "gated_scan_fwd: null pointer");
     VC_REQUIRE(pair_aligned(h, d->is_bf16), "gated_scan_fwd: h is not aligned to two elements");
+    const size_t need = vc_scan_workspace(d->B, d->T, d->H, 0);
+    VC_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+               "gated_scan_fwd: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, need);
     VcScanParams p = scan_params(d, gates, lengths);
-    p.h0 = h0, p.h = h, p.last = last, p.states = states;
+    p.h0 = h0, p.h = h, p.last = last, p.states = states, p.ws = (char*)workspace;
     return vc_scan_launch_fwd(p, d->is_bf16 != 0, S(stream));
 }
 int vc_gated_scan_bwd(const vc_scan_desc* d, const void* gates, const int32_t* lengths, const float* states, const void* dy,
                       const float* dlast, void* dgates, float* dh0, void* workspace, size_t ws_bytes, void* stream) {
-    (void)workspace, (void)ws_bytes;
     const int rc = scan_check(d);
     if (rc) return rc;
     VC_REQUIRE(gates && states && dgates, "gated_scan_bwd: null pointer");
     VC_REQUIRE(pair_aligned(dgates, d->is_bf16) && pair_aligned(dy, d->is_bf16), "gated_scan_bwd: dy or dgates is not aligned to two elements");
+    const size_t need = vc_scan_workspace(d->B, d->T, d->H, 1);
+    VC_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+               "gated_scan_bwd: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, need);
     VcScanParams p = scan_params(d, gates, lengths);
     p.states = (float*)states, p.dy = dy, p.dlast = dlast, p.dgates = dgates, p.dh0 = dh0;
+    p.ws = (char*)workspace;
     return vc_scan_launch_bwd(p, d->is_bf16 != 0, S(stream));
 }
 int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, float* state, void* h, int32_t B, int32_t H, void* stream) {

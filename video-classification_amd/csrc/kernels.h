@@ -215,7 +215,9 @@ struct VcScanParams {
     const float* dlast;  // nullable [B][H]
     void* dgates;        // [B][T][2H]
     float* dh0;          // nullable [B][H]
+    char* ws;
 };
+size_t vc_scan_workspace(int B, int T, int H, int op);
 int vc_scan_launch_fwd(const VcScanParams& p, bool is_bf16, hipStream_t s);
 int vc_scan_launch_bwd(const VcScanParams& p, bool is_bf16, hipStream_t s);
 int vc_scan_launch_step(const void* gates, long long sb, float* state, void* h, int B, int H, bool is_bf16, hipStream_t s);
