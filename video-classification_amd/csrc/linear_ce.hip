@@ -12,6 +12,8 @@
 //
 // Rows whose label is ignore_index take no part: the rows that count are listed first (rows_kernel) and all products run
 // over that list, so that an ignored row costs nothing and whatever it holds (NaN included) reaches nothing.
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -43,10 +45,12 @@ __global__ __launch_bounds__(1024) void rows_kernel(const long long* labels, lon
 
 // ---------------------------------------------------------------- matrix products
 // out[s][r] = sum_k S(s, k) R(r, k).  A workgroup of WR x WS waves makes a BR x BS tile, a wave BR/WR x BS/WS of it, in steps
-// of 128 bytes of k (64 bf16, 32 fp32).  Both operand tiles of a step come in by DMA (global_load_lds, 16 bytes a lane), into
-// one of two buffers while the other one is multiplied.  An operand lies in memory with k contiguous (rows of x, w; P for dx)
-// or with its rows contiguous and k across (w for dx; x and P for dw: nothing is transposed in memory):
-//   k contiguous: LDS rows of 128 bytes, the 16-byte chunk c of row r at slot c ^ (r / 2 % 8); a fragment is one ds_read_b128.
+// of 64 bytes of k (32 bf16, 16 fp32: one fragment).  The operands' tiles come in by DMA (global_load_lds, 16 bytes a lane)
+// into a ring of four buffers, three steps ahead of their use.  An operand lies in memory with k contiguous (rows of x, w; P
+// for dx) or with its rows contiguous and k across (w for dx; x and P for dw: nothing is transposed in memory):
+//   k contiguous: LDS rows of 64 bytes; a fragment is one ds_read_b128.  The 16-byte chunk c of row r lies at slot
+//     c ^ turn(r / 4 % 4), turn = 0 2 3 1: of the sixteen lanes that one cycle pair serves, whether they are rows 0-15 of one
+//     chunk or rows 0-3, 12-15 of one and 4-11 of the next, no two meet in a bank (measured: 0 conflicts).
 //   k across: LDS rows of one k each.  bf16: fragments come through ds_read_b64_tr_b16, which hands lane i of 16 the i-th
 //     column of four rows; a lane group reads four rows x 32 bytes, so the 32-byte unit u of row k lies at u ^ f(k) with f
 //     different for the eight rows that half a wave reads at once.  fp32: one ds_read_b32 a value, units of 64 bytes at u ^ (k / 4 % 4).
@@ -56,8 +60,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(const long long* labels, lon
 // operand, P, is 0 (EPI_PROB writes whole tiles of P, zeros behind the last row and the last word).
 struct Operand {
     const char* p;
-    long long ld;     // bytes from row to row (k contiguous) or from k to k (k across)
-    const int* list;  // nullable: the index of row i (k contiguous) or of k i (k across)
+    long long ld;  // bytes from row to row (k contiguous) or from k to k (k across), below 2^32
 };
 
 enum { EPI_STATS, EPI_PROB, EPI_DX, EPI_DW };
@@ -89,7 +92,6 @@ struct Gemm {
     const float* g;  // EPI_DW: the factor common to all rows
 };
 
-typedef __attribute__((address_space(1))) const void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 typedef __attribute__((address_space(3))) s16x4* ltr_t;
 
@@ -99,13 +101,13 @@ template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16> {
-    static constexpr int STEP = 64, PER = 8;  // k of a step, of a 16-byte chunk
+    static constexpr int STEP = 32, PER = 8;  // k of a step, of a 16-byte chunk
     typedef bf16x8 frag;
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Mma<float> {
-    static constexpr int STEP = 32, PER = 4;
+    static constexpr int STEP = 16, PER = 4;
     typedef f32x4 frag;
     // four instructions of k = 4; k is dealt to the lane groups in fours, alike for both operands
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) {
@@ -115,72 +117,67 @@ struct Mma<float> {
     }
 };
 
+// 16 bytes per lane from `src` to LDS at the wave-uniform `lds` + 16 * lane.  Written out, not the builtin: the compiler knows
+// which LDS the builtin writes only as "some", and waits for every such load before any transposed read (measured: the products
+// with k across 1.9x slower); here the waits at the end of a step are all there are.  It has no result register; the address
+// registers are read when it issues.
+__device__ __forceinline__ void dma(unsigned lds, const char* src) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "m0");
+}
+
 // one operand of a tile: ROWS rows, KACROSS = k across
 template <typename T, int ROWS, int NTHR, bool KACROSS>
 struct Tile {
-    static constexpr int STEP = Mma<T>::STEP, PER = Mma<T>::PER, BYTES = ROWS * 128;
-    static constexpr int PIECES = ROWS * 8 / NTHR;  // 16-byte pieces of a thread
-    static constexpr int CPR = ROWS / PER;          // k across: chunks of an LDS row
+    static constexpr int STEP = Mma<T>::STEP, PER = Mma<T>::PER, BYTES = ROWS * 64;
+    static constexpr int PIECES = ROWS * 4 / NTHR;        // 16-byte pieces of a thread
+    static constexpr int CPR = ROWS / PER;                // k across: chunks of an LDS row
     static constexpr int KPP = KACROSS ? NTHR / CPR : 1;  // k across: k of one pass of the workgroup
-    const char* p[PIECES];  // k contiguous: the piece at k = 0; k across: p[0] = its column
+    const char* p[PIECES];  // k contiguous: a piece at k = 0; k across: its column at k = 0
     int tid;
-    // what a piece's chunk of a row of one k is moved by
+    // k across: what a piece's chunk of a row of one k is moved by
     static __device__ __forceinline__ int swz(int k) { return sizeof(T) == 2 ? ((k & 3) | ((k >> 3) & 1) << 2) << 1 : ((k >> 2) & 3) << 2; }
+    // k contiguous: 0 2 3 1
+    static __device__ __forceinline__ int turn(int h) { return (h >> 1) | ((h ^ (h >> 1)) & 1) << 1; }
+    __device__ __forceinline__ int chunk() const { return (tid & 3) ^ turn((tid >> 4) & 3); }  // of every piece (rows differ by 16s)
 
     __device__ __forceinline__ void init(const Operand& o, int row0, int nrows) {
         tid = threadIdx.x;
-        if (!KACROSS) {
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) {
-                int row = row0 + j * (NTHR / 8) + (tid >> 3);
-                row = row < nrows ? row : nrows - 1;
-                const long long i = o.list != nullptr ? o.list[row] : row;
-                p[j] = o.p + i * o.ld + chunk() * 16;
+        for (int j = 0; j < PIECES; ++j) {
+            if (!KACROSS) {
+                const int row = row0 + j * (NTHR / 4) + (tid >> 2);
+                p[j] = o.p + (row < nrows ? row : nrows - 1) * o.ld + chunk() * 16;
+            } else {
+                const int c = row0 + ((tid % CPR) ^ swz(j * KPP + tid / CPR)) * PER;
+                p[j] = o.p + (c < nrows ? c : 0) * (int)sizeof(T);
             }
-        } else
-            p[0] = o.p;
+        }
     }
-    __device__ __forceinline__ int chunk() const { return (tid & 7) ^ ((tid >> 4) & 7); }  // k contiguous: of every piece (rows differ by 16s)
-    // k across: the k that piece j of the step at k0 reads, clamped and looked up
-    __device__ __forceinline__ int at(const Operand& o, int k0, int K, int j) const {
-        int k = k0 + j * KPP + tid / CPR;
-        k = k < K ? k : K - 1;
-        return o.list != nullptr ? o.list[k] : k;
-    }
-    __device__ __forceinline__ void issue(const Operand& o, char* lds, int k0, int K, int row0, int nrows, const int* ks) const {
-        char* const base = lds + (tid >> 6) * 1024;
+    // piece j of the step at k0
+    __device__ __forceinline__ void issue(const Operand& o, unsigned lds, int k0, int K, int j) const {
+        const char* src;
         if (!KACROSS) {
-            const bool out = k0 + STEP > K && k0 + chunk() * PER >= K;
-#pragma unroll
-            for (int j = 0; j < PIECES; ++j) {
-                const gptr_t src = out ? (gptr_t)vc_lce_zero_page : (gptr_t)(p[j] + (long long)k0 * (int)sizeof(T));
-                __builtin_amdgcn_global_load_lds(src, (lptr_t)(base + j * NTHR * 16), 16, 0, 0);
-            }
+            src = p[j] + (long long)k0 * (int)sizeof(T);
+            if (k0 + STEP > K) src = k0 + chunk() * PER >= K ? (const char*)vc_lce_zero_page : src;
         } else {
-#pragma unroll
-            for (int j = 0; j < PIECES; ++j) {
-                int c = row0 + ((tid % CPR) ^ swz(j * KPP + tid / CPR)) * PER;
-                c = c < nrows ? c : 0;
-                __builtin_amdgcn_global_load_lds((gptr_t)(p[0] + (long long)ks[j] * o.ld + c * (int)sizeof(T)), (lptr_t)(base + j * NTHR * 16), 16, 0, 0);
-            }
+            const int k = k0 + j * KPP + tid / CPR;
+            src = p[j] + (unsigned long long)(unsigned)(k < K ? k : K - 1) * (unsigned)o.ld;
         }
+        dma(lds + j * NTHR * 16, src);
     }
-    // the fragment of rows [row, row + 16), half ks of the step
-    static __device__ __forceinline__ typename Mma<T>::frag frag(const char* lds, int row, int ks, int l15, int lg) {
-        if (!KACROSS) {
-            const int r = row + l15;
-            return *(const typename Mma<T>::frag*)(lds + r * 128 + ((((ks << 2) + lg) ^ ((r >> 1) & 7)) << 4));
-        }
+    // the fragment of rows [row, row + 16)
+    static __device__ __forceinline__ typename Mma<T>::frag frag(const char* lds, int row, int l15, int lg) {
+        if (!KACROSS) return *(const typename Mma<T>::frag*)(lds + row * 64 + l15 * 64 + ((lg ^ turn(l15 >> 2)) << 4));
         const int u = row / 16;
         typename Mma<T>::frag f;
         if constexpr (sizeof(T) == 2) {
-            const int k = ks * 32 + lg * 8 + (l15 >> 2);
+            const int k = lg * 8 + (l15 >> 2);
             const char* q = lds + k * (ROWS * 2) + ((u ^ (swz(k) >> 1)) << 5) + (l15 & 3) * 8;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)(q + 4 * ROWS * 2));
             f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = *(const float*)(lds + (ks * 16 + lg * 4 + i) * (ROWS * 4) + ((u ^ lg) << 6) + l15 * 4);
+            for (int i = 0; i < 4; ++i) f[i] = *(const float*)(lds + (lg * 4 + i) * (ROWS * 4) + ((u ^ lg) << 6) + l15 * 4);
         }
         return f;
     }
@@ -194,7 +191,7 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     typedef Tile<T, BR, NTHR, RK> TR;
     typedef Tile<T, BS, NTHR, SK> TS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int BUF = TR::BYTES + TS::BYTES;
+    constexpr int BUF = TR::BYTES + TS::BYTES, RING = 4;
     const int ns = g.ns_dev != nullptr ? *g.ns_dev : g.ns, K = g.k_dev != nullptr ? *g.k_dev : g.K;
     // tile order: XCD x (workgroups go round the 8 XCDs) takes the x-th share of an order in which 4 tiles of s by all tiles of r
     // follow each other, so that the 32 workgroups of an XCD share 4 + 8 operand panels in its L2
@@ -220,44 +217,67 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
         TR tr;
         TS ts;
         tr.init(g.R, r0, g.nr);
-        ts.init(g.S, s0, ns);
-        int kr[RK ? TR::PIECES : 1], kt[SK ? TS::PIECES : 1];
-        auto look = [&](int k0) {
-            if (RK)
-#pragma unroll
-                for (int j = 0; j < TR::PIECES; ++j) kr[j] = tr.at(g.R, k0, K, j);
-            if (SK)
-#pragma unroll
-                for (int j = 0; j < TS::PIECES; ++j) kt[j] = ts.at(g.S, k0, (K + STEP - 1) / STEP * STEP, j);  // (P: zeros up to there)
+        ts.init(g.S, s0, SK ? (int)(g.S.ld / (int)sizeof(T)) : ns);  // (P has whole tiles)
+        constexpr int PIECES = TR::PIECES + TS::PIECES;
+        static_assert(PIECES == 4, "the waits below count two steps of four pieces");
+        const int ks = SK ? (K + STEP - 1) / STEP * STEP : K;  // (P has zeros up to there)
+        const unsigned dst = (unsigned)(uintptr_t)(lptr_t)smem + wave * 1024;
+        auto issue = [&](int t, int j) {
+            const unsigned to = dst + (t & (RING - 1)) * BUF;
+            if (j < TR::PIECES) tr.issue(g.R, to, kb + t * STEP, K, j);
+            else ts.issue(g.S, to + TR::BYTES, kb + t * STEP, ks, j - TR::PIECES);
         };
-        auto issue = [&](int k0, char* buf) {
-            tr.issue(g.R, buf, k0, K, r0, g.nr, kr);
-            ts.issue(g.S, buf + TR::BYTES, k0, K, s0, (int)(g.S.ld / (int)sizeof(T)), kt);
-        };
-        look(kb);
-        issue(kb, smem);
-        look(kb + STEP);
-        int cur = 0;
-        for (int k0 = kb; k0 < ke; k0 += STEP, cur ^= 1) {
-            __syncthreads();  // this step's tiles have landed; the other buffer has been read
-            if (k0 + STEP < ke) {
-                issue(k0 + STEP, smem + (cur ^ 1) * BUF);
-                look(k0 + 2 * STEP);
-            }
-            const char* const lr = smem + cur * BUF;
-            const char* const ls = lr + TR::BYTES;
+        // A step is NA slots: one fragment of R and NB matrix instructions each.  Fragments are read two slots ahead of their
+        // use.  Two slots before its end a wave has read all of the step's tiles: there it waits for the next step's tiles
+        // (those of the two steps after it may be under way) and meets the others; the last two slots run while the first
+        // fragments of the next step are read.  The tiles of the third step from here go to the buffer that the step before
+        // read, a piece a slot: asked for all at once, they keep the wave from issuing anything else.
+        const int steps = (ke - kb + STEP - 1) / STEP;
+        typename Mma<T>::frag fr[4], fs[2][NB];
+        for (int t = 0; t < 3 && t < steps; ++t)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                typename Mma<T>::frag fs[NB];
+            for (int j = 0; j < PIECES; ++j) issue(t, j);
+        if (steps > 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
 #pragma unroll
-                for (int b = 0; b < NB; ++b) fs[b] = TS::frag(ls, wsx + b * 16, ks, l15, lg);
+        for (int b = 0; b < NB; ++b) fs[0][b] = TS::frag(smem + TR::BYTES, wsx + b * 16, l15, lg);
 #pragma unroll
-                for (int a = 0; a < NA; ++a) {
-                    const typename Mma<T>::frag fr = TR::frag(lr, wr + a * 16, ks, l15, lg);
+        for (int i = 0; i < 2; ++i) fr[i] = TR::frag(smem, wr + i * 16, l15, lg);
+        auto step = [&](int t, auto parity) {
+            constexpr int Q = decltype(parity)::value;
+            const char* const lr = smem + (t & (RING - 1)) * BUF;
+            const char* const nr = smem + ((t + 1) & (RING - 1)) * BUF;
+            const bool more = t + 3 < steps;
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) acc[a][b] = Mma<T>::run(fr, fs[b], acc[a][b]);
+            for (int i = 0; i < NA; ++i) {
+                constexpr int PER_SLOT = 2 * PIECES / NA;
+                if (i < NA / 2 && more)
+#pragma unroll
+                    for (int j = 0; j < PER_SLOT; ++j) issue(t + 3, i * PER_SLOT + j);
+                if (i == NA - 2) {
+                    if (more) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+                    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
                 }
+                // (behind the last step what is read here is not used)
+                fr[(i + 2) & 3] = TR::frag(i + 2 < NA ? lr : nr, wr + (i + 2) % NA * 16, l15, lg);
+                if (i >= NA - 2)
+#pragma unroll
+                    for (int b = 0; b < NB / 2; ++b) {
+                        const int c = (i - (NA - 2)) * (NB / 2) + b;
+                        fs[Q ^ 1][c] = TS::frag(nr + TR::BYTES, wsx + c * 16, l15, lg);
+                    }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) acc[i][b] = Mma<T>::run(fr[i & 3], fs[Q][b], acc[i][b]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        for (int t = 0; t < steps; t += 2) {
+            step(t, std::integral_constant<int, 0>());
+            if (t + 1 < steps) step(t + 1, std::integral_constant<int, 1>());
         }
     }
     // acc[a][b][j] = out[s = s0 + wsx + 16 b + l15][r = r0 + wr + 16 a + 4 lg + j]
@@ -276,7 +296,7 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     }
     constexpr float LOG2E = 1.44269504088896340736f;
     if constexpr (EPI == EPI_STATS) {
-        __syncthreads();
+        __syncthreads();  // (the tiles have been read)
         float2* const join = (float2*)smem;  // [WR][BS]
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -394,7 +414,7 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     }
 }
 
-// rows whose bytes are no whole 16-byte chunks, or begin at none, are copied: [n][D] -> [n][dp], zeros behind D
+// [n][D] -> [n][dp], zeros behind D: rows whose bytes are no whole 16-byte chunks, or begin at none
 template <typename T>
 __global__ __launch_bounds__(256) void lce_pack_kernel(const T* in, long long ld, long long n, int D, int dp, T* out) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n * dp; i += (long long)gridDim.x * 256) {
@@ -402,6 +422,19 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(const T* in, long long ld
         const int d = (int)(i - r * dp);
         out[i] = d < D ? in[r * ld + d] : (T)0.f;
     }
+}
+// the rows of x that count, one after the other (13 us of the 7 ms of 8192 x 2048 x 65536; the products then read x in order,
+// with k across too, and never a row that does not count).  VEC: whole 16-byte chunks
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long long ld, const int* rows, int N, int D, int dp, T* out) {
+    const int i = blockIdx.x;
+    if (i >= rows[N]) return;
+    const T* const from = x + rows[i] * ld;
+    T* const to = out + (long long)i * dp;
+    if (VEC)
+        for (int d = threadIdx.x; d < dp * (int)sizeof(T) / 16; d += 256) ((uint4*)to)[d] = ((const uint4*)from)[d];
+    else
+        for (int d = threadIdx.x; d < dp; d += 256) to[d] = d < D ? from[d] : (T)0.f;
 }
 
 // ---------------------------------------------------------------- the small launches around it
@@ -506,10 +539,8 @@ struct Plan {
         fit = fit < tile ? tile : fit;
         piece = (int)(op == 0 && !pack ? all : fit < all ? fit : all);
         tiles = (int)(all / tile);
-        if (pack) {
-            xp = take((size_t)N * dp * elem);
-            wp = take((size_t)(piece < V ? piece : V) * dp * elem);
-        }
+        xp = take((size_t)N * dp * elem);
+        if (pack) wp = take((size_t)(piece < V ? piece : V) * dp * elem);
         if (op == 0) {
             part = take((size_t)N * tiles * sizeof(float2));
             zlab = take((size_t)N * 4);
@@ -538,7 +569,7 @@ int launched(const char* what) {
 
 template <typename T, int EPI, int B>
 void gemm_tile(const Gemm& g, int splits, hipStream_t s) {
-    constexpr int WR = 2, WS = B == 256 ? 4 : 2, LDS = 2 * 2 * B * 128;
+    constexpr int WR = 2, WS = B == 256 ? 4 : 2, LDS = 4 * 2 * B * 64;
     const auto kernel = lce_gemm<T, EPI, B, B, WR, WS>;
     static VcPerDeviceOnce once;
     once.run([&] { (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
@@ -551,14 +582,8 @@ void gemm(Gemm& g, int tile, int ns_most, int splits, hipStream_t s) {
     else gemm_tile<T, EPI, 128>(g, splits, s);
 }
 
-template <typename T>
-void pack(const void* in, long long ld, long long n, int D, int dp, void* out, hipStream_t s) {
-    const long long blocks = (n * dp + 255) / 256;
-    hipLaunchKernelGGL((lce_pack_kernel<T>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, (const T*)in, ld, n, D, dp, (T*)out);
-}
-
 bool chunks(const VcLceParams& p, int elem) {
-    return (((uintptr_t)p.x | (uintptr_t)p.w | (uintptr_t)(p.ldx * elem) | (uintptr_t)(p.ldw * elem)) & 15) == 0;
+    return (((uintptr_t)p.x | (uintptr_t)p.w | (uintptr_t)(p.ldx * elem) | (uintptr_t)(p.ldw * elem)) & 15) == 0 && p.ldw * elem < (1ll << 32);
 }
 
 // x as the products read it, and w from word v0 on
@@ -569,17 +594,18 @@ struct Source {
     hipStream_t s;
     Operand x;
     Source(const VcLceParams& p, const Plan& L, hipStream_t s) : p(p), L(L), s(s) {
-        x = {(const char*)p.x, p.ldx * (long long)sizeof(T), p.rows};
-        if (L.pack) {
-            pack<T>(p.x, p.ldx, p.N, p.D, L.dp, (char*)p.ws + L.xp, s);
-            x = {(const char*)p.ws + L.xp, L.dp * (long long)sizeof(T), p.rows};
-        }
+        T* const to = (T*)((char*)p.ws + L.xp);
+        if (L.pack) hipLaunchKernelGGL((lce_rows_of_x_kernel<T, false>), dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, p.rows, p.N, p.D, L.dp, to);
+        else hipLaunchKernelGGL((lce_rows_of_x_kernel<T, true>), dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, p.rows, p.N, p.D, L.dp, to);
+        x = {(const char*)to, L.dp * (long long)sizeof(T)};
     }
     Operand w(int v0, int nv) const {
         const T* at = (const T*)p.w + v0 * p.ldw;
-        if (!L.pack) return {(const char*)at, p.ldw * (long long)sizeof(T), nullptr};
-        pack<T>(at, p.ldw, nv, p.D, L.dp, (char*)p.ws + L.wp, s);
-        return {(const char*)p.ws + L.wp, L.dp * (long long)sizeof(T), nullptr};
+        if (!L.pack) return {(const char*)at, p.ldw * (long long)sizeof(T)};
+        const long long n = (long long)nv * L.dp, blocks = (n + 255) / 256;
+        T* const to = (T*)((char*)p.ws + L.wp);
+        hipLaunchKernelGGL((lce_pack_kernel<T>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, at, p.ldw, (long long)nv, p.D, L.dp, to);
+        return {(const char*)to, L.dp * (long long)sizeof(T)};
     }
 };
 
@@ -631,14 +657,14 @@ int bwd(const VcLceParams& p, hipStream_t s) {
                                (T*)p.db + v0);
         if (p.dx != nullptr) {
             Gemm x = {};
-            x.R = w, x.S = {ws + L.P, ldp, nullptr};
+            x.R = w, x.S = {ws + L.P, ldp};
             x.nr = p.D, x.ns_dev = count, x.K = nv, x.acc = acc, x.add = v0 > 0, x.acc_split = (long long)p.N * p.D;
             x.k_split = ((nv + L.splits - 1) / L.splits + 127) / 128 * 128;
             gemm<T, EPI_DX>(x, L.tile, p.N, L.splits, s);
         }
         if (p.dw != nullptr) {
             Gemm d = {};
-            d.R = src.x, d.S = {ws + L.P, ldp, nullptr};
+            d.R = src.x, d.S = {ws + L.P, ldp};
             d.nr = p.D, d.ns = nv, d.k_dev = count, d.k_split = 0x7fffffc0, d.out = (T*)p.dw + (long long)v0 * p.D, d.g = factor;
             gemm<T, EPI_DW>(d, L.tile, nv, 1, s);
         }
