@@ -17,6 +17,16 @@
 #include "common.h"
 #include "kernels.h"
 
+#ifndef LCE_PER_SLOT
+#define LCE_PER_SLOT 4
+#endif
+#ifndef LCE_DIST
+#define LCE_DIST 2
+#endif
+#ifndef LCE_PRIO
+#define LCE_PRIO 0
+#endif
+
 namespace {
 
 // ---------------------------------------------------------------- the list of rows
@@ -101,13 +111,13 @@ template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16> {
-    static constexpr int STEP = 32, PER = 8;  // k of a step, of a 16-byte chunk
+    static constexpr int KF = 32, PER = 8;  // k of a fragment, of a 16-byte chunk
     typedef bf16x8 frag;
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Mma<float> {
-    static constexpr int STEP = 16, PER = 4;
+    static constexpr int KF = 16, PER = 4;
     typedef f32x4 frag;
     // four instructions of k = 4; k is dealt to the lane groups in fours, alike for both operands
     static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) {
@@ -125,30 +135,34 @@ __device__ __forceinline__ void dma(unsigned lds, const char* src) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "m0");
 }
 
-// one operand of a tile: ROWS rows, KACROSS = k across
-template <typename T, int ROWS, int NTHR, bool KACROSS>
+// one operand of a tile: ROWS rows by the k of SUBS fragments, KACROSS = k across
+template <typename T, int ROWS, int SUBS, int NTHR, bool KACROSS>
 struct Tile {
-    static constexpr int STEP = Mma<T>::STEP, PER = Mma<T>::PER, BYTES = ROWS * 64;
-    static constexpr int PIECES = ROWS * 4 / NTHR;        // 16-byte pieces of a thread
-    static constexpr int CPR = ROWS / PER;                // k across: chunks of an LDS row
-    static constexpr int KPP = KACROSS ? NTHR / CPR : 1;  // k across: k of one pass of the workgroup
+    static constexpr int STEP = Mma<T>::KF * SUBS, PER = Mma<T>::PER, ROWB = 64 * SUBS, BYTES = ROWS * ROWB;
+    static constexpr int PIECES = BYTES / 16 / NTHR;      // 16-byte pieces of a thread
+    static constexpr int CPR = KACROSS ? ROWS / PER : 4 * SUBS;  // chunks of an LDS row
+    static constexpr int RPP = NTHR / CPR;                // LDS rows of one pass of the workgroup
     const char* p[PIECES];  // k contiguous: a piece at k = 0; k across: its column at k = 0
     int tid;
     // k across: what a piece's chunk of a row of one k is moved by
     static __device__ __forceinline__ int swz(int k) { return sizeof(T) == 2 ? ((k & 3) | ((k >> 3) & 1) << 2) << 1 : ((k >> 2) & 3) << 2; }
-    // k contiguous: 0 2 3 1
-    static __device__ __forceinline__ int turn(int h) { return (h >> 1) | ((h ^ (h >> 1)) & 1) << 1; }
-    __device__ __forceinline__ int chunk() const { return (tid & 3) ^ turn((tid >> 4) & 3); }  // of every piece (rows differ by 16s)
+    // k contiguous: what a chunk of row r is moved by
+    static __device__ __forceinline__ int turn(int r) {
+        const int h = (r >> 2) & 3;
+        return SUBS == 2 ? (r >> 1) & 7 : (h >> 1) | ((h ^ (h >> 1)) & 1) << 1;
+    }
+    __device__ __forceinline__ int chunk() const { return (tid % CPR) ^ turn(tid / CPR); }  // k contiguous: of every piece (rows differ by 16s)
 
     __device__ __forceinline__ void init(const Operand& o, int row0, int nrows) {
+        static_assert(KACROSS || RPP % 16 == 0, "");
         tid = threadIdx.x;
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
             if (!KACROSS) {
-                const int row = row0 + j * (NTHR / 4) + (tid >> 2);
+                const int row = row0 + j * RPP + tid / CPR;
                 p[j] = o.p + (row < nrows ? row : nrows - 1) * o.ld + chunk() * 16;
             } else {
-                const int c = row0 + ((tid % CPR) ^ swz(j * KPP + tid / CPR)) * PER;
+                const int c = row0 + ((tid % CPR) ^ swz(j * RPP + tid / CPR)) * PER;
                 p[j] = o.p + (c < nrows ? c : 0) * (int)sizeof(T);
             }
         }
@@ -160,38 +174,45 @@ struct Tile {
             src = p[j] + (long long)k0 * (int)sizeof(T);
             if (k0 + STEP > K) src = k0 + chunk() * PER >= K ? (const char*)vc_lce_zero_page : src;
         } else {
-            const int k = k0 + j * KPP + tid / CPR;
+            const int k = k0 + j * RPP + tid / CPR;
             src = p[j] + (unsigned long long)(unsigned)(k < K ? k : K - 1) * (unsigned)o.ld;
         }
         dma(lds + j * NTHR * 16, src);
     }
-    // the fragment of rows [row, row + 16)
-    static __device__ __forceinline__ typename Mma<T>::frag frag(const char* lds, int row, int l15, int lg) {
-        if (!KACROSS) return *(const typename Mma<T>::frag*)(lds + row * 64 + l15 * 64 + ((lg ^ turn(l15 >> 2)) << 4));
+    // the fragment of rows [row, row + 16), k of fragment `sub`
+    static __device__ __forceinline__ typename Mma<T>::frag frag(const char* lds, int row, int sub, int l15, int lg) {
+        if (!KACROSS) return *(const typename Mma<T>::frag*)(lds + row * ROWB + l15 * ROWB + (((sub * 4 + lg) ^ turn(l15)) << 4));
         const int u = row / 16;
         typename Mma<T>::frag f;
         if constexpr (sizeof(T) == 2) {
             const int k = lg * 8 + (l15 >> 2);
-            const char* q = lds + k * (ROWS * 2) + ((u ^ (swz(k) >> 1)) << 5) + (l15 & 3) * 8;
+            const char* q = lds + (sub * 32 + k) * (ROWS * 2) + ((u ^ (swz(k) >> 1)) << 5) + (l15 & 3) * 8;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)(q + 4 * ROWS * 2));
             f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = *(const float*)(lds + (lg * 4 + i) * (ROWS * 4) + ((u ^ lg) << 6) + l15 * 4);
+            for (int i = 0; i < 4; ++i) f[i] = *(const float*)(lds + (sub * 16 + lg * 4 + i) * (ROWS * 4) + ((u ^ lg) << 6) + l15 * 4);
         }
         return f;
     }
 };
 
+// how a product's tiles come in: fragments of k a step, buffers of the ring
+template <int EPI>
+struct Feed {
+    static constexpr bool ROWS_OF_K = EPI == EPI_STATS || EPI == EPI_PROB;
+    static constexpr int SUBS = ROWS_OF_K ? 2 : 1, RING = ROWS_OF_K ? 2 : 4;
+};
+
 template <typename T, int EPI, int BR, int BS, int WR, int WS>
 __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
-    constexpr int NTHR = WR * WS * 64, STEP = Mma<T>::STEP;
+    constexpr int NTHR = WR * WS * 64, SUBS = Feed<EPI>::SUBS, RING = Feed<EPI>::RING, STEP = Mma<T>::KF * SUBS;
     constexpr int NA = BR / WR / 16, NB = BS / WS / 16;
     constexpr bool RK = EPI == EPI_DX || EPI == EPI_DW, SK = EPI == EPI_DW;
-    typedef Tile<T, BR, NTHR, RK> TR;
-    typedef Tile<T, BS, NTHR, SK> TS;
+    typedef Tile<T, BR, SUBS, NTHR, RK> TR;
+    typedef Tile<T, BS, SUBS, NTHR, SK> TS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int BUF = TR::BYTES + TS::BYTES, RING = 4;
+    constexpr int BUF = TR::BYTES + TS::BYTES;
     const int ns = g.ns_dev != nullptr ? *g.ns_dev : g.ns, K = g.k_dev != nullptr ? *g.k_dev : g.K;
     // tile order: XCD x (workgroups go round the 8 XCDs) takes the x-th share of an order in which 4 tiles of s by all tiles of r
     // follow each other, so that the 32 workgroups of an XCD share 4 + 8 operand panels in its L2
@@ -218,67 +239,81 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
         TS ts;
         tr.init(g.R, r0, g.nr);
         ts.init(g.S, s0, SK ? (int)(g.S.ld / (int)sizeof(T)) : ns);  // (P has whole tiles)
-        constexpr int PIECES = TR::PIECES + TS::PIECES;
-        static_assert(PIECES == 4, "the waits below count two steps of four pieces");
+        constexpr int PIECES = TR::PIECES + TS::PIECES, SL = SUBS * NA;
+        static_assert((RING - 2) * PIECES == 8 || RING == 2, "the waits below");
         const int ks = SK ? (K + STEP - 1) / STEP * STEP : K;  // (P has zeros up to there)
         const unsigned dst = (unsigned)(uintptr_t)(lptr_t)smem + wave * 1024;
+        const int steps = (ke - kb + STEP - 1) / STEP;
         auto issue = [&](int t, int j) {
             const unsigned to = dst + (t & (RING - 1)) * BUF;
             if (j < TR::PIECES) tr.issue(g.R, to, kb + t * STEP, K, j);
             else ts.issue(g.S, to + TR::BYTES, kb + t * STEP, ks, j - TR::PIECES);
         };
-        // A step is NA slots: one fragment of R and NB matrix instructions each.  Fragments are read two slots ahead of their
+        // A step is SL slots: one fragment of R and NB matrix instructions each.  Fragments are read two slots ahead of their
         // use.  Two slots before its end a wave has read all of the step's tiles: there it waits for the next step's tiles
-        // (those of the two steps after it may be under way) and meets the others; the last two slots run while the first
-        // fragments of the next step are read.  The tiles of the third step from here go to the buffer that the step before
-        // read, a piece a slot: asked for all at once, they keep the wave from issuing anything else.
-        const int steps = (ke - kb + STEP - 1) / STEP;
-        typename Mma<T>::frag fr[4], fs[2][NB];
-        for (int t = 0; t < 3 && t < steps; ++t)
+        // (those of later steps may be under way) and meets the others; the last two slots run while the first fragments of
+        // the next step are read.  The tiles of the step RING - 1 from here go to the buffer that the step before read, a
+        // few pieces a slot: asked for all at once, they keep the wave from issuing anything else.
+        constexpr int D = NA >= 8 ? LCE_DIST : 2;  // slots
+        typename Mma<T>::frag fr[2 * D], fs[2][NB];
+        for (int t = 0; t < RING - 1 && t < steps; ++t)
 #pragma unroll
             for (int j = 0; j < PIECES; ++j) issue(t, j);
-        if (steps > 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        if (RING > 2 && steps > RING - 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int b = 0; b < NB; ++b) fs[0][b] = TS::frag(smem + TR::BYTES, wsx + b * 16, l15, lg);
+        for (int b = 0; b < NB; ++b) fs[0][b] = TS::frag(smem + TR::BYTES, wsx + b * 16, 0, l15, lg);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) fr[i] = TR::frag(smem, wr + i * 16, l15, lg);
+        for (int i = 0; i < D; ++i) fr[i] = TR::frag(smem, wr + i * 16, 0, l15, lg);
         auto step = [&](int t, auto parity) {
             constexpr int Q = decltype(parity)::value;
             const char* const lr = smem + (t & (RING - 1)) * BUF;
             const char* const nr = smem + ((t + 1) & (RING - 1)) * BUF;
-            const bool more = t + 3 < steps;
+            const bool more = t + RING - 1 < steps;
 #pragma unroll
-            for (int i = 0; i < NA; ++i) {
-                constexpr int PER_SLOT = 2 * PIECES / NA;
-                if (i < NA / 2 && more)
+            for (int i = 0; i < SL; ++i) {
+                constexpr int PER_SLOT = LCE_PER_SLOT;
+                if (i * PER_SLOT < PIECES && more)
 #pragma unroll
-                    for (int j = 0; j < PER_SLOT; ++j) issue(t + 3, i * PER_SLOT + j);
-                if (i == NA - 2) {
-                    if (more) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+                    for (int j = 0; j < PER_SLOT; ++j) issue(t + RING - 1, i * PER_SLOT + j);
+                if (i == SL - D) {
+                    if (RING > 2 && more) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
                     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
                 }
                 // (behind the last step what is read here is not used)
-                fr[(i + 2) & 3] = TR::frag(i + 2 < NA ? lr : nr, wr + (i + 2) % NA * 16, l15, lg);
-                if (i >= NA - 2)
+                const int n = (i + D) % SL;
+                fr[(i + D) % (2 * D)] = TR::frag(i + D < SL ? lr : nr, wr + n % NA * 16, n / NA, l15, lg);
+                // S: the fragments of the step's second half, of the next step's first
+                if (SUBS == 2 && i >= NA - D && i < NA)
 #pragma unroll
-                    for (int b = 0; b < NB / 2; ++b) {
-                        const int c = (i - (NA - 2)) * (NB / 2) + b;
-                        fs[Q ^ 1][c] = TS::frag(nr + TR::BYTES, wsx + c * 16, l15, lg);
+                    for (int b = 0; b < NB / D; ++b) {
+                        const int c = (i - (NA - D)) * (NB / D) + b;
+                        fs[1][c] = TS::frag(lr + TR::BYTES, wsx + c * 16, 1, l15, lg);
                     }
+                if (i >= SL - D)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) acc[i][b] = Mma<T>::run(fr[i & 3], fs[Q][b], acc[i][b]);
+                    for (int b = 0; b < NB / D; ++b) {
+                        const int c = (i - (SL - D)) * (NB / D) + b;
+                        fs[SUBS == 2 ? 0 : Q ^ 1][c] = TS::frag(nr + TR::BYTES, wsx + c * 16, 0, l15, lg);
+                    }
+                if (LCE_PRIO) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) acc[i % NA][b] = Mma<T>::run(fr[i % (2 * D)], fs[SUBS == 2 ? i / NA : Q][b], acc[i % NA][b]);
+                if (LCE_PRIO) __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        for (int t = 0; t < steps; t += 2) {
-            step(t, std::integral_constant<int, 0>());
-            if (t + 1 < steps) step(t + 1, std::integral_constant<int, 1>());
-        }
+        if constexpr (SUBS == 2) {
+            for (int t = 0; t < steps; ++t) step(t, std::integral_constant<int, 0>());
+        } else
+            for (int t = 0; t < steps; t += 2) {
+                step(t, std::integral_constant<int, 0>());
+                if (t + 1 < steps) step(t + 1, std::integral_constant<int, 1>());
+            }
     }
     // acc[a][b][j] = out[s = s0 + wsx + 16 b + l15][r = r0 + wr + 16 a + 4 lg + j]
     if constexpr (EPI == EPI_STATS || EPI == EPI_PROB) {
