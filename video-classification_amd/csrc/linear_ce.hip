@@ -17,15 +17,6 @@
 #include "common.h"
 #include "kernels.h"
 
-#ifndef LCE_PER_SLOT
-#define LCE_PER_SLOT 4
-#endif
-#ifndef LCE_DIST
-#define LCE_DIST 2
-#endif
-#ifndef LCE_PRIO
-#define LCE_PRIO 0
-#endif
 
 namespace {
 
@@ -50,7 +41,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(const long long* labels, lon
         __syncthreads();
         base = base_sh;
     }
-    if (tid == 0) rows[N] = base;
+    if (tid == 0) rows[N] = base, rows[N + 1] = 0;  // (their number; workgroups of lce_rows_kernel that are done)
 }
 
 // ---------------------------------------------------------------- matrix products
@@ -74,6 +65,18 @@ struct Operand {
 };
 
 enum { EPI_STATS, EPI_PROB, EPI_DX, EPI_DW };
+
+// the factor common to all rows
+struct Factor {
+    const float* dloss;
+    const int* count;
+    int reduction;
+    __device__ __forceinline__ float get() const {
+        if (reduction == 0) return 1.f;
+        const int n = *count;
+        return reduction == 1 ? dloss[0] / (float)(n > 0 ? n : 1) : dloss[0];
+    }
+};
 
 struct Gemm {
     Operand R, S;
@@ -99,7 +102,7 @@ struct Gemm {
     long long acc_split;
     int add;
     void* out;       // EPI_DW: [s][nr]
-    const float* g;  // EPI_DW: the factor common to all rows
+    Factor factor;   // EPI_DW
 };
 
 typedef __attribute__((address_space(3))) void* lptr_t;
@@ -145,7 +148,8 @@ struct Tile {
     const char* p[PIECES];  // k contiguous: a piece at k = 0; k across: its column at k = 0
     int tid;
     // k across: what a piece's chunk of a row of one k is moved by
-    static __device__ __forceinline__ int swz(int k) { return sizeof(T) == 2 ? ((k & 3) | ((k >> 3) & 1) << 2) << 1 : ((k >> 2) & 3) << 2; }
+    // (64 columns of bf16 are four units only: two rows then share a bank)
+    static __device__ __forceinline__ int swz(int k) { return sizeof(T) == 2 ? ((k & 3) | (ROWS > 64 ? (k >> 3) & 1 : 0) << 2) << 1 : ((k >> 2) & 3) << 2; }
     // k contiguous: what a chunk of row r is moved by
     static __device__ __forceinline__ int turn(int r) {
         const int h = (r >> 2) & 3;
@@ -198,15 +202,17 @@ struct Tile {
 };
 
 // how a product's tiles come in: fragments of k a step, buffers of the ring
-template <int EPI>
+// Large tiles: where rows of k are read, 128 bytes of them (half a line a row costs the forward 15 %) and two buffers, all that
+// fits; with k across four buffers of one fragment.
+template <int EPI, int B>
 struct Feed {
     static constexpr bool ROWS_OF_K = EPI == EPI_STATS || EPI == EPI_PROB;
-    static constexpr int SUBS = ROWS_OF_K ? 2 : 1, RING = ROWS_OF_K ? 2 : 4;
+    static constexpr int SUBS = ROWS_OF_K || B == 64 ? 2 : 1, RING = ROWS_OF_K && B > 64 ? 2 : 4;
 };
 
 template <typename T, int EPI, int BR, int BS, int WR, int WS>
 __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
-    constexpr int NTHR = WR * WS * 64, SUBS = Feed<EPI>::SUBS, RING = Feed<EPI>::RING, STEP = Mma<T>::KF * SUBS;
+    constexpr int NTHR = WR * WS * 64, SUBS = Feed<EPI, BR>::SUBS, RING = Feed<EPI, BR>::RING, STEP = Mma<T>::KF * SUBS;
     constexpr int NA = BR / WR / 16, NB = BS / WS / 16;
     constexpr bool RK = EPI == EPI_DX || EPI == EPI_DW, SK = EPI == EPI_DW;
     typedef Tile<T, BR, SUBS, NTHR, RK> TR;
@@ -254,7 +260,8 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
         // (those of later steps may be under way) and meets the others; the last two slots run while the first fragments of
         // the next step are read.  The tiles of the step RING - 1 from here go to the buffer that the step before read, a
         // few pieces a slot: asked for all at once, they keep the wave from issuing anything else.
-        constexpr int D = NA >= 8 ? LCE_DIST : 2;  // slots
+        constexpr int D = 2;  // slots from a fragment's read to its use
+        static_assert(SL % (2 * D) == 0 && NB % D == 0, "");
         typename Mma<T>::frag fr[2 * D], fs[2][NB];
         for (int t = 0; t < RING - 1 && t < steps; ++t)
 #pragma unroll
@@ -274,7 +281,7 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
             const bool more = t + RING - 1 < steps;
 #pragma unroll
             for (int i = 0; i < SL; ++i) {
-                constexpr int PER_SLOT = LCE_PER_SLOT;
+                constexpr int PER_SLOT = 4;
                 if (i * PER_SLOT < PIECES && more)
 #pragma unroll
                     for (int j = 0; j < PER_SLOT; ++j) issue(t + RING - 1, i * PER_SLOT + j);
@@ -300,10 +307,8 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
                         const int c = (i - (SL - D)) * (NB / D) + b;
                         fs[SUBS == 2 ? 0 : Q ^ 1][c] = TS::frag(nr + TR::BYTES, wsx + c * 16, 0, l15, lg);
                     }
-                if (LCE_PRIO) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) acc[i % NA][b] = Mma<T>::run(fr[i % (2 * D)], fs[SUBS == 2 ? i / NA : Q][b], acc[i % NA][b]);
-                if (LCE_PRIO) __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
@@ -417,7 +422,7 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
         }
     }
     if constexpr (EPI == EPI_DX || EPI == EPI_DW) {
-        const float f = EPI == EPI_DW ? *g.g : 1.f;
+        const float f = EPI == EPI_DW ? g.factor.get() : 1.f;
         const bool vec = (g.nr & 3) == 0;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -473,90 +478,99 @@ __global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long lon
 }
 
 // ---------------------------------------------------------------- the small launches around it
-// a wave joins the pairs of one row: lse, loss
+// A wave joins the pairs of one row: lse, loss.  With `loss` the workgroup that is done last sums the rows up, in their order.
+// (It reads what the others wrote: their stores are device-scope atomics, complete before the workgroup counts itself done.)
 __global__ __launch_bounds__(256) void lce_rows_kernel(const float2* part, int tiles, const float* zlab, const long long* labels,
-                                                       const int* rows, int N, int V, float* lse, float* loss_rows) {
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (i >= N) return;
-    const int n = rows[i];
-    if (i >= rows[N]) {  // does not count
-        if (lane == 0) lse[n] = 0.f, loss_rows[n] = 0.f;
-        return;
-    }
-    float m = -INFINITY, e = 0.f;
-    for (int t = lane; t < tiles; t += 64) {
-        const float2 p = part[(size_t)i * tiles + t];
-        const float k = fmaxf(m, p.x), ref = k == -INFINITY ? 0.f : k;
-        e = e * __expf(m - ref) + p.y * __expf(p.x - ref);
-        m = k;
-    }
+                                                       int* rows, int N, int V, float* lse, float* loss_rows, int mean, float* loss) {
+    __shared__ double sums[4];
+    __shared__ int last;
+    const int wave = threadIdx.x >> 6, i = blockIdx.x * 4 + wave, lane = threadIdx.x & 63, count = rows[N];
+    if (i < N) {
+        const int n = rows[i];
+        float m = -INFINITY, e = 0.f, l = 0.f, loss_n = 0.f;
+        if (i < count) {
+            for (int t = lane; t < tiles; t += 64) {
+                const float2 p = part[(size_t)i * tiles + t];
+                const float k = fmaxf(m, p.x), ref = k == -INFINITY ? 0.f : k;
+                e = e * __expf(m - ref) + p.y * __expf(p.x - ref);
+                m = k;
+            }
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const float m2 = __shfl_xor(m, o, 64), e2 = __shfl_xor(e, o, 64);
-        const float k = fmaxf(m, m2), ref = k == -INFINITY ? 0.f : k;
-        e = e * __expf(m - ref) + e2 * __expf(m2 - ref);
-        m = k;
+            for (int o = 32; o >= 1; o >>= 1) {
+                const float m2 = __shfl_xor(m, o, 64), e2 = __shfl_xor(e, o, 64);
+                const float k = fmaxf(m, m2), ref = k == -INFINITY ? 0.f : k;
+                e = e * __expf(m - ref) + e2 * __expf(m2 - ref);
+                m = k;
+            }
+            const long long y = labels[n];
+            const bool ok = y >= 0 && y < V;
+            l = ok ? m + logf(e) : NAN;  // (a label that is no word: NaN, as with vc_softmax_ce)
+            loss_n = ok ? l - zlab[i] : NAN;
+        }
+        if (lane == 0) {
+            lse[n] = l;
+            __hip_atomic_store(loss_rows + n, loss_n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
     }
-    if (lane == 0) {
-        const long long y = labels[n];
-        const bool ok = y >= 0 && y < V;
-        const float l = ok ? m + logf(e) : NAN;  // (a label that is no word: NaN, as with vc_softmax_ce)
-        lse[n] = l;
-        loss_rows[n] = ok ? l - zlab[i] : NAN;
-    }
-}
-__global__ __launch_bounds__(1024) void lce_mean_kernel(const float* loss_rows, const int* rows, int N, int mean, float* loss) {
-    __shared__ double part[16];
+    if (loss == nullptr) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(rows + N + 1, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
     double s = 0.0;
-    for (int n = threadIdx.x; n < N; n += 1024) s += (double)loss_rows[n];
+    for (int n = threadIdx.x; n < N; n += 256) s += (double)__hip_atomic_load(loss_rows + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    if (lane == 0) sums[wave] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
-        s = 0.0;
-        for (int w = 0; w < 16; ++w) s += part[w];
-        const int count = rows[N];
+        s = ((sums[0] + sums[1]) + sums[2]) + sums[3];
         loss[0] = (float)(mean ? s / (double)(count > 0 ? count : 1) : s);
     }
 }
-// the factor common to all rows
-__global__ void lce_factor_kernel(const float* dloss, const int* rows, int N, int reduction, float* g) {
-    const int count = rows[N];
-    g[0] = reduction == 0 ? 1.f : reduction == 1 ? dloss[0] / (float)(count > 0 ? count : 1) : dloss[0];
-}
 // dx of the rows that count from their sums, zeros for the others
 template <typename T>
-__global__ __launch_bounds__(256) void lce_dx_kernel(const float* acc, int splits, long long split, const int* rows, const float* g, int N, int D,
+__global__ __launch_bounds__(256) void lce_dx_kernel(const float* acc, int splits, long long split, const int* rows, Factor factor, int N, int D,
                                                      T* dx) {
+    const float g = factor.get();
     const int i = blockIdx.x, n = rows[i];
     const bool keep = i < rows[N];
     for (int d = threadIdx.x; d < D; d += 256) {
         float v = 0.f;
         for (int k = 0; k < splits && keep; ++k) v += acc[k * split + (long long)i * D + d];
-        dx[(long long)n * D + d] = keep ? (T)(v * *g) : (T)0.f;
+        dx[(long long)n * D + d] = keep ? (T)(v * g) : (T)0.f;
     }
 }
 template <typename T>
-__global__ __launch_bounds__(256) void lce_db_kernel(const float* part, long long ld, int bs, const int* count, const float* g, int nr, T* db) {
+__global__ __launch_bounds__(256) void lce_db_kernel(const float* part, long long ld, int bs, Factor factor, int nr, T* db) {
     const int r = blockIdx.x * 256 + threadIdx.x;
     if (r >= nr) return;
-    const int tiles = (*count + bs - 1) / bs;
+    const int tiles = (*factor.count + bs - 1) / bs;
     float s = 0.f;
     for (int t = 0; t < tiles; ++t) s += part[t * ld + r];
-    db[r] = (T)(s * *g);
+    db[r] = (T)(s * factor.get());
 }
 
 // ---------------------------------------------------------------- plan and workspace
+// side of the tiles of an ns x nr product: the largest that makes work for most of the 256 CUs (96, 192 and 384 tiles as the
+// border measured alike within 2 %; 256 against 128 wide tiles where both fill the chip: 0.88 x the time)
+int pick_tile(long long ns, long long nr) {
+    for (int b = 256; b > 64; b /= 2)
+        if (ns > b / 2 && nr > b / 2 && ((ns + b - 1) / b) * ((nr + b - 1) / b) >= 192) return b;
+    return 64;
+}
+
 struct Plan {
     size_t bytes = 0;
-    int tile;        // side of a tile
-    int piece;       // words of a piece, a multiple of the tile
-    int tiles;       // tiles of the vocabulary
-    int splits;      // of k in the product for dx
-    int dp;          // row length of x, w as the products read them
-    bool pack;       // x, w have to be copied for that
-    size_t g, acc, P, dbpart, part, zlab, loss_rows, xp, wp;
+    int tile, tile_dx, tile_dw;  // sides of the tiles of N x V, N x D, piece x D
+    int piece;                   // words of a piece, a multiple of 256
+    int tiles;                   // tiles of the vocabulary
+    int splits;                  // of k in the product for dx
+    int dp;                      // row length of x, w as the products read them
+    bool pack;                   // w has to be copied for that
+    size_t acc, P, dbpart, part, zlab, loss_rows, xp, wp;
     size_t take(size_t n) {
         const size_t at = bytes;
         bytes += (n + 255) & ~(size_t)255;
@@ -567,13 +581,13 @@ struct Plan {
         const int per = 16 / elem;
         pack = !aligned || D % per != 0;
         dp = (D + per - 1) / per * per;
-        tile = N > 128 && (long long)N * V >= (1ll << 22) ? 256 : 128;
-        const long long np = ((long long)N + tile - 1) / tile * tile, all = ((long long)V + tile - 1) / tile * tile;
-        long long fit = (512ll << 20) / elem / np / tile * tile;
-        if (pack && op == 0) fit = (512ll << 20) / elem / dp / tile * tile;  // (the forward holds a piece of w only)
-        fit = fit < tile ? tile : fit;
+        const long long np = ((long long)N + 255) / 256 * 256, all = ((long long)V + 255) / 256 * 256;
+        long long fit = (512ll << 20) / elem / np / 256 * 256;
+        if (pack && op == 0) fit = (512ll << 20) / elem / dp / 256 * 256;  // (the forward holds a piece of w only)
+        fit = fit < 256 ? 256 : fit;
         piece = (int)(op == 0 && !pack ? all : fit < all ? fit : all);
-        tiles = (int)(all / tile);
+        tile = pick_tile(N, piece < V ? piece : V);
+        tiles = (int)(((long long)V + tile - 1) / tile);
         xp = take((size_t)N * dp * elem);
         if (pack) wp = take((size_t)(piece < V ? piece : V) * dp * elem);
         if (op == 0) {
@@ -582,14 +596,18 @@ struct Plan {
             loss_rows = take((size_t)N * 4);
             return;
         }
-        const long long t = np / tile * ((D + tile - 1) / tile), most = piece / 512 > 1 ? piece / 512 : 1;
+        // dx has few tiles and a long k: k is split until the tiles fill the chip, into no less than 512 words.  Smaller tiles
+        // need fewer splits, i.e. fewer sums to write and join (4000 x 256 of 2000 words: 182, 183 us; 500 x 256 of 100000: 349
+        // us with 256, 286 with 128; 8192 x 2048 of 65536, 256 tiles of 256: 6.96 against 7.73 ms)
+        tile_dx = N > 128 && D > 128 && (N + 255ll) / 256 * ((D + 255) / 256) >= 128 ? 256 : N > 64 && D > 64 ? 128 : 64;
+        tile_dw = pick_tile(piece < V ? piece : V, D);
+        const long long t = ((N + tile_dx - 1) / tile_dx) * (long long)((D + tile_dx - 1) / tile_dx), most = piece / 512 > 1 ? piece / 512 : 1;
         long long z = 512 / t;
         z = z < 1 ? 1 : z > most ? most : z;
         splits = (int)(z > 16 ? 16 : z);
-        g = take(4);
         acc = take((size_t)splits * N * D * 4);
         P = take((size_t)np * piece * elem);
-        dbpart = take((size_t)(np / tile) * piece * 4);
+        dbpart = take((size_t)(np / 64) * piece * 4);
     }
 };
 
@@ -604,7 +622,7 @@ int launched(const char* what) {
 
 template <typename T, int EPI, int B>
 void gemm_tile(const Gemm& g, int splits, hipStream_t s) {
-    constexpr int WR = 2, WS = B == 256 ? 4 : 2, LDS = 4 * 2 * B * 64;
+    constexpr int WR = 2, WS = B == 256 ? 4 : 2, LDS = Feed<EPI, B>::RING * Feed<EPI, B>::SUBS * 2 * B * 64;
     const auto kernel = lce_gemm<T, EPI, B, B, WR, WS>;
     static VcPerDeviceOnce once;
     once.run([&] { (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
@@ -614,7 +632,8 @@ template <typename T, int EPI>
 void gemm(Gemm& g, int tile, int ns_most, int splits, hipStream_t s) {
     g.rtiles = (g.nr + tile - 1) / tile, g.stiles = (ns_most + tile - 1) / tile;
     if (tile == 256) gemm_tile<T, EPI, 256>(g, splits, s);
-    else gemm_tile<T, EPI, 128>(g, splits, s);
+    else if (tile == 128) gemm_tile<T, EPI, 128>(g, splits, s);
+    else gemm_tile<T, EPI, 64>(g, splits, s);
 }
 
 bool chunks(const VcLceParams& p, int elem) {
@@ -662,9 +681,7 @@ int fwd(const VcLceParams& p, hipStream_t s) {
         gemm<T, EPI_STATS>(g, L.tile, p.N, 1, s);
     }
     hipLaunchKernelGGL(lce_rows_kernel, dim3((p.N + 3) / 4), dim3(256), 0, s, part, L.tiles, zlab, p.labels, p.rows, p.N, p.V, p.lse,
-                       loss_rows);
-    if (p.reduction != 0)
-        hipLaunchKernelGGL(lce_mean_kernel, dim3(1), dim3(1024), 0, s, loss_rows, p.rows, p.N, p.reduction == 1, p.loss);
+                       loss_rows, p.reduction == 1, p.reduction != 0 ? p.loss : nullptr);
     return launched("linear_ce_fwd");
 }
 
@@ -672,11 +689,11 @@ template <typename T>
 int bwd(const VcLceParams& p, hipStream_t s) {
     const Plan L(p.N, p.D, p.V, sizeof(T), 1, chunks(p, sizeof(T)));
     char* ws = (char*)p.ws;
-    float *factor = (float*)(ws + L.g), *acc = (float*)(ws + L.acc), *dbpart = (float*)(ws + L.dbpart);
+    float *acc = (float*)(ws + L.acc), *dbpart = (float*)(ws + L.dbpart);
     const int* count = p.rows + p.N;
+    const Factor factor = {p.dloss, count, p.reduction};
     const long long ldp = (long long)L.piece * (int)sizeof(T);
     (void)hipGetLastError();
-    hipLaunchKernelGGL(lce_factor_kernel, dim3(1), dim3(1), 0, s, p.dloss, p.rows, p.N, p.reduction, factor);
     const Source<T> src(p, L, s);
     for (int v0 = 0; v0 < p.V; v0 += L.piece) {
         const int nv = p.V - v0 < L.piece ? p.V - v0 : L.piece;
@@ -688,20 +705,20 @@ int bwd(const VcLceParams& p, hipStream_t s) {
         g.lse = p.lse, g.scale = p.reduction == 0 ? p.dloss : nullptr, g.P = ws + L.P, g.ldp = L.piece, g.dbpart = p.db != nullptr ? dbpart : nullptr;
         gemm<T, EPI_PROB>(g, L.tile, p.N, 1, s);
         if (p.db != nullptr)
-            hipLaunchKernelGGL((lce_db_kernel<T>), dim3((nv + 255) / 256), dim3(256), 0, s, dbpart, (long long)L.piece, L.tile, count, factor, nv,
+            hipLaunchKernelGGL((lce_db_kernel<T>), dim3((nv + 255) / 256), dim3(256), 0, s, dbpart, (long long)L.piece, L.tile, factor, nv,
                                (T*)p.db + v0);
         if (p.dx != nullptr) {
             Gemm x = {};
             x.R = w, x.S = {ws + L.P, ldp};
             x.nr = p.D, x.ns_dev = count, x.K = nv, x.acc = acc, x.add = v0 > 0, x.acc_split = (long long)p.N * p.D;
             x.k_split = ((nv + L.splits - 1) / L.splits + 127) / 128 * 128;
-            gemm<T, EPI_DX>(x, L.tile, p.N, L.splits, s);
+            gemm<T, EPI_DX>(x, L.tile_dx, p.N, L.splits, s);
         }
         if (p.dw != nullptr) {
             Gemm d = {};
             d.R = src.x, d.S = {ws + L.P, ldp};
-            d.nr = p.D, d.ns = nv, d.k_dev = count, d.k_split = 0x7fffffc0, d.out = (T*)p.dw + (long long)v0 * p.D, d.g = factor;
-            gemm<T, EPI_DW>(d, L.tile, nv, 1, s);
+            d.nr = p.D, d.ns = nv, d.k_dev = count, d.k_split = 0x7fffffc0, d.out = (T*)p.dw + (long long)v0 * p.D, d.factor = factor;
+            gemm<T, EPI_DW>(d, L.tile_dw, nv, 1, s);
         }
     }
     if (p.dx != nullptr)

@@ -12,19 +12,19 @@ _REDUCTION = {"none": 0, "mean": 1, "sum": 2}
 class _LinearCEFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, labels, bias, ignore_index, reduction):
-        loss, lse, rows = ops.linear_ce_fwd(x.detach(), weight.detach(), labels, None if bias is None else bias.detach(), ignore_index, reduction)
+        d = ops._linear_ce_desc(x, weight, labels, bias, ignore_index, reduction)
+        loss, lse, rows = ops._linear_ce_fwd(d, x, weight, labels, bias)
         if any(ctx.needs_input_grad):
             ctx.save_for_backward(x, weight, labels, bias, lse, rows)
-            ctx.ignore_index, ctx.reduction = ignore_index, reduction
+            ctx.desc = d
         return loss if reduction == 0 else loss.view(())
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         x, weight, labels, bias, lse, rows = ctx.saved_tensors
-        want = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
-        dx, dw, db = ops.linear_ce_bwd(x.detach(), weight.detach(), labels, None if bias is None else bias.detach(), lse, rows,
-                                       dloss.contiguous(), ctx.ignore_index, ctx.reduction, want)
+        want = ctx.needs_input_grad
+        dx, dw, db = ops._linear_ce_bwd(ctx.desc, x, weight, labels, bias, lse, rows, dloss.contiguous(), (want[0], want[1], want[3]))
         return dx, dw, None, db, None, None
 
 

@@ -747,17 +747,22 @@ def linear_ce_fwd(x, weight, labels, bias=None, ignore_index=-100, reduction=1):
     """cross-entropy of x weight^T + bias against labels, the vocabulary in pieces (vc_linear_ce_fwd); reduction 0 none, 1 mean
     over the rows that count, 2 sum -> (loss [1] or [N], lse [N], rows): lse and rows are what linear_ce_bwd takes.
     x [N][D] and weight [V][D] have contiguous rows (_rows), bias and labels are contiguous."""
-    d = _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction)
+    return _linear_ce_fwd(_linear_ce_desc(x, weight, labels, bias, ignore_index, reduction), x, weight, labels, bias)
+
+
+def _linear_ce_fwd(d, x, weight, labels, bias):
+    N, red, dev = d.N, d.reduction, x.device
     with _on(x):
-        loss = torch.empty(x.shape[0] if reduction == 0 else 1, dtype=F32, device=x.device)
-        lse = torch.empty(x.shape[0], dtype=F32, device=x.device)
-        rows = torch.empty(x.shape[0] + 4, dtype=torch.int32, device=x.device)
-        if x.shape[0] == 0:
+        loss = torch.empty(1 if red else N, dtype=F32, device=dev)
+        lse = torch.empty(N, dtype=F32, device=dev)
+        rows = torch.empty(N + 4, dtype=torch.int32, device=dev)
+        if N == 0:
             return loss.zero_(), lse, rows
         need = lib.vc_linear_ce_workspace_bytes(d, 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        check(lib.vc_linear_ce_fwd(d, ptr(x), ptr(weight), ptr(bias), ptr(labels), ptr(loss) if reduction else None,
-                                   None if reduction else ptr(loss), ptr(lse), ptr(rows), ptr(ws), need, cur_stream()), "vc_linear_ce_fwd")
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        at = loss.data_ptr()
+        check(lib.vc_linear_ce_fwd(d, x.data_ptr(), weight.data_ptr(), ptr(bias), labels.data_ptr(), at if red else None, None if red else at,
+                                   lse.data_ptr(), rows.data_ptr(), ws.data_ptr(), need, cur_stream()), "vc_linear_ce_fwd")
     return loss, lse, rows
 
 
@@ -770,16 +775,21 @@ def linear_ce_bwd(x, weight, labels, bias, lse, rows, dloss, ignore_index=-100, 
     _chk(rows, torch.int32, N + 4, "rows")
     _chk(dloss, F32, N if reduction == 0 else 1, "dloss")
     _same_device(x, lse=lse, rows=rows, dloss=dloss)
+    return _linear_ce_bwd(d, x, weight, labels, bias, lse, rows, dloss, want)
+
+
+def _linear_ce_bwd(d, x, weight, labels, bias, lse, rows, dloss, want):
+    dt, dev = x.dtype, x.device
     with _on(x):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
-        dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device) if want[1] else None
-        db = torch.empty(bias.shape, dtype=x.dtype, device=x.device) if want[2] and bias is not None else None
-        if N == 0:
+        dx = torch.empty((d.N, d.D), dtype=dt, device=dev) if want[0] else None
+        dw = torch.empty((d.V, d.D), dtype=dt, device=dev) if want[1] else None
+        db = torch.empty(d.V, dtype=dt, device=dev) if want[2] and bias is not None else None
+        if d.N == 0:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
         need = lib.vc_linear_ce_workspace_bytes(d, 1)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        check(lib.vc_linear_ce_bwd(d, ptr(x), ptr(weight), ptr(bias), ptr(labels), ptr(lse), ptr(rows), ptr(dloss), ptr(dx), ptr(dw),
-                                   ptr(db), ptr(ws), need, cur_stream()), "vc_linear_ce_bwd")
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        check(lib.vc_linear_ce_bwd(d, x.data_ptr(), weight.data_ptr(), ptr(bias), labels.data_ptr(), lse.data_ptr(), rows.data_ptr(),
+                                   dloss.data_ptr(), ptr(dx), ptr(dw), ptr(db), ws.data_ptr(), need, cur_stream()), "vc_linear_ce_bwd")
     return dx, dw, db
 
 
@@ -796,28 +806,27 @@ def _scan_desc(gates, lengths, reverse):
     return capi.ScanDesc(B, T, H, kind, 1 if reverse else 0, 0, gates.stride(0), gates.stride(1))
 
 
-def _scan_workspace(d, op, device):
-    need = lib.vc_gated_scan_workspace_bytes(d, op)
-    return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
-
-
 def gated_scan_fwd(gates, h0=None, lengths=None, reverse=False, want_states=False):
     """the recurrence h_t = f h_(t-1) + (1 - f) v over [B][T], gates packed [B][T][2H] = (logits of f | v), any strides over B
     and T (vc_gated_scan_fwd) -> (h [B][T][H], last state [B][H] fp32, states for gated_scan_bwd or None)"""
     d = _scan_desc(gates, lengths, reverse)
     _chk(h0, F32, d.B * d.H, "h0")
     _same_device(gates, h0=h0)
+    return _gated_scan_fwd(d, gates, h0, lengths, want_states)
+
+
+def _gated_scan_fwd(d, gates, h0, lengths, want_states):
+    B, T, H, dev = d.B, d.T, d.H, gates.device
     with _on(gates):
-        h = torch.empty(d.B, d.T, d.H, dtype=gates.dtype, device=gates.device)
-        n = (d.T + SCAN_STATE_STEPS - 1) // SCAN_STATE_STEPS
-        states = torch.empty(d.B, n, d.H, dtype=F32, device=gates.device) if want_states else None
-        if d.T == 0 or d.B == 0:
-            last = torch.zeros(d.B, d.H, dtype=F32, device=gates.device) if h0 is None else h0.clone()
-            return h, last, states
-        last = torch.empty(d.B, d.H, dtype=F32, device=gates.device)
-        ws, need = _scan_workspace(d, 0, gates.device)
-        check(lib.vc_gated_scan_fwd(d, ptr(gates), ptr(h0), ptr(lengths), ptr(h), ptr(last), ptr(states), ptr(ws), need, cur_stream()),
-              "vc_gated_scan_fwd")
+        h = torch.empty((B, T, H), dtype=gates.dtype, device=dev)
+        states = torch.empty((B, (T + SCAN_STATE_STEPS - 1) // SCAN_STATE_STEPS, H), dtype=F32, device=dev) if want_states else None
+        if T == 0 or B == 0:
+            return h, torch.zeros(B, H, dtype=F32, device=dev) if h0 is None else h0.clone(), states
+        last = torch.empty((B, H), dtype=F32, device=dev)
+        need = lib.vc_gated_scan_workspace_bytes(d, 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        check(lib.vc_gated_scan_fwd(d, gates.data_ptr(), ptr(h0), ptr(lengths), h.data_ptr(), last.data_ptr(), ptr(states), ptr(ws), need,
+                                    cur_stream()), "vc_gated_scan_fwd")
     return h, last, states
 
 
@@ -829,16 +838,22 @@ def gated_scan_bwd(gates, lengths, states, dy, dlast, reverse=False, want_dh0=Tr
     _chk(dy, gates.dtype, d.B * d.T * d.H, "dy")
     _chk(dlast, F32, d.B * d.H, "dlast")
     _same_device(gates, states=states, dy=dy, dlast=dlast)
+    return _gated_scan_bwd(d, gates, lengths, states, dy, dlast, want_dh0)
+
+
+def _gated_scan_bwd(d, gates, lengths, states, dy, dlast, want_dh0):
+    dev = gates.device
     with _on(gates):
-        dgates = torch.empty(d.B, d.T, 2 * d.H, dtype=gates.dtype, device=gates.device)
-        dh0 = torch.empty(d.B, d.H, dtype=F32, device=gates.device) if want_dh0 else None
+        dgates = torch.empty((d.B, d.T, 2 * d.H), dtype=gates.dtype, device=dev)
+        dh0 = torch.empty((d.B, d.H), dtype=F32, device=dev) if want_dh0 else None
         if d.T == 0 or d.B == 0:
             if dh0 is not None:
                 dh0.zero_() if dlast is None else dh0.copy_(dlast.view(d.B, d.H))
             return dgates, dh0
-        ws, need = _scan_workspace(d, 1, gates.device)
-        check(lib.vc_gated_scan_bwd(d, ptr(gates), ptr(lengths), ptr(states), ptr(dy), ptr(dlast), ptr(dgates), ptr(dh0), ptr(ws), need,
-                                    cur_stream()), "vc_gated_scan_bwd")
+        need = lib.vc_gated_scan_workspace_bytes(d, 1)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        check(lib.vc_gated_scan_bwd(d, gates.data_ptr(), ptr(lengths), states.data_ptr(), ptr(dy), ptr(dlast), dgates.data_ptr(), ptr(dh0),
+                                    ptr(ws), need, cur_stream()), "vc_gated_scan_bwd")
     return dgates, dh0
 
 

@@ -15,10 +15,13 @@ class _GatedScanFn(torch.autograd.Function):
     def forward(ctx, gates, h0, lengths, reverse):
         ctx.set_materialize_grads(False)
         grad = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        h, last, states = ops.gated_scan_fwd(gates.detach(), None if h0 is None else h0.detach(), lengths, reverse, want_states=grad)
+        d = ops._scan_desc(gates, lengths, reverse)
+        if h0 is not None:
+            ops._same_device(gates, h0=h0)
+        h, last, states = ops._gated_scan_fwd(d, gates, h0, lengths, grad)
         if grad:
             ctx.save_for_backward(gates, lengths, states)
-            ctx.reverse = reverse
+            ctx.desc = d
         return h, last
 
     @staticmethod
@@ -27,9 +30,9 @@ class _GatedScanFn(torch.autograd.Function):
         if dy is None and dlast is None:
             return None, None, None, None
         gates, lengths, states = ctx.saved_tensors
-        dgates, dh0 = ops.gated_scan_bwd(gates.detach(), lengths, states, _aligned(dy), None if dlast is None else dlast.contiguous(), ctx.reverse,
-                                         want_dh0=ctx.needs_input_grad[1])
-        return dgates if ctx.needs_input_grad[0] else None, dh0, None, None
+        want = ctx.needs_input_grad
+        dgates, dh0 = ops._gated_scan_bwd(ctx.desc, gates, lengths, states, _aligned(dy), None if dlast is None else dlast.contiguous(), want[1])
+        return dgates if want[0] else None, dh0, None, None
 
 
 def _aligned(t):
