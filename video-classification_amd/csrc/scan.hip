@@ -20,8 +20,13 @@
 // ready mark (words are 0 before), written and read by relaxed device-scope atomics: no fence, no L2 write-back.  Tiles take
 // their number from a counter, earlier steps first, so a tile only ever waits for tiles that run already, and every wait ends.
 //
+// Measured (copies on this card reach 5.14 TB/s): 8 x 2048 x 2048 bf16 forward 44 us = 4.6 TB/s, backward 82 us = 4.1; one
+// sequence of 131072 x 1024 193 us = 4.2 TB/s.
+//
 // All arithmetic and the state are fp32; h and dgates round once, to their type.  1 - f is computed as its own quotient
 // (sigmoid(-z)), so that a gate near 1 keeps its relative precision.
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -67,9 +72,26 @@ struct Raw<float> {
     }
     __device__ __forceinline__ f2 get() const { return {a, b}; }
 };
+// two neighbouring values as they lie in memory
+template <typename T>
+struct Pair;
+template <>
+struct Pair<float> {
+    typedef float2 type;
+    static __device__ __forceinline__ type make(f2 v) { return make_float2(v.x, v.y); }
+};
+template <>
+struct Pair<bf16> {
+    typedef __attribute__((ext_vector_type(2))) __bf16 type;
+    static __device__ __forceinline__ type make(f2 v) { return (type){f2bf(v.x), f2bf(v.y)}; }
+};
+template <typename T>
+__device__ __forceinline__ typename Pair<T>::type pair(f2 v) {
+    return Pair<T>::make(v);
+}
 template <bool VEC>
 __device__ __forceinline__ void store2(float* p, f2 v, int n) {
-    if (VEC && n == 2) *(float2*)p = make_float2(v.x, v.y);
+    if (VEC && n == 2) *(float2*)p = pair<float>(v);
     else {
         if (n > 0) p[0] = v.x;
         if (n > 1) p[1] = v.y;
@@ -77,8 +99,7 @@ __device__ __forceinline__ void store2(float* p, f2 v, int n) {
 }
 template <bool VEC>
 __device__ __forceinline__ void store2(bf16* p, f2 v, int n) {
-    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-    if (VEC && n == 2) *(bf16x2*)p = (bf16x2){f2bf(v.x), f2bf(v.y)};
+    if (VEC && n == 2) *(Pair<bf16>::type*)p = pair<bf16>(v);
     else {
         if (n > 0) p[0] = f2bf(v.x);
         if (n > 1) p[1] = f2bf(v.y);
@@ -101,7 +122,7 @@ struct Between {
 
     // the state in front of tile `tile` > 0
     __device__ __forceinline__ f2 before(int tile) const {
-        constexpr int W = 4;
+        constexpr int W = 4;  // (2: the same within 1 %; 8: 30 % slower, its registers spill)
         // the nearest tile whose state is there for all lanes, the latest W tiles first; the first tile's always comes
         int from = -1;
         while (from < 0) {
@@ -195,6 +216,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_fwd_kernel(const VcScanPar
     __shared__ f2 carry[64];
     __shared__ int shared;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    typedef typename Pair<T>::type P2;
     const Place<T> L(p, TILE, lane, &shared);
     T* const out = (T*)p.h + (long long)L.b * p.T * p.H + L.c;
     const int w0 = L.tile * TILE + wave * SUB;  // the wave's first step
@@ -224,19 +246,23 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_fwd_kernel(const VcScanPar
             }
         }
         f2 f[SUB], u[SUB], a = {1.f, 1.f}, b = {0.f, 0.f};
+        auto compose = [&](auto whole) {  // (a wave whose steps are all there tests none of them)
 #pragma unroll
-        for (int j = 0; j < SUB; ++j) {
-            f[j] = {1.f, 1.f}, u[j] = {0.f, 0.f};
-            if (j < left) {
-                const f2 zz = z[j].get(), vv = v[j].get();
-                f2 q;
-                gate(zz.x, f[j].x, q.x);
-                gate(zz.y, f[j].y, q.y);
-                u[j] = {q.x * vv.x, q.y * vv.y};
+            for (int j = 0; j < SUB; ++j) {
+                f[j] = {1.f, 1.f}, u[j] = {0.f, 0.f};
+                if (decltype(whole)::value || j < left) {
+                    const f2 zz = z[j].get(), vv = v[j].get();
+                    f2 q;
+                    gate(zz.x, f[j].x, q.x);
+                    gate(zz.y, f[j].y, q.y);
+                    u[j] = {q.x * vv.x, q.y * vv.y};
+                }
+                a = {a.x * f[j].x, a.y * f[j].y};
+                b = {f[j].x * b.x + u[j].x, f[j].y * b.y + u[j].y};
             }
-            a = {a.x * f[j].x, a.y * f[j].y};
-            b = {f[j].x * b.x + u[j].x, f[j].y * b.y + u[j].y};
-        }
+        };
+        if (left >= SUB) compose(std::true_type());
+        else compose(std::false_type());
         agg[wave][lane] = make_float4(a.x, a.y, b.x, b.y);
         __syncthreads();
         if (wave == 0) {
@@ -271,11 +297,16 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_fwd_kernel(const VcScanPar
         }
         T* const o = out + t0 * p.H;
         const long long so = (long long)p.H * dt;
+        auto write = [&](auto whole) {
 #pragma unroll
-        for (int j = 0; j < SUB; ++j) {
-            h = {f[j].x * h.x + u[j].x, f[j].y * h.y + u[j].y};
-            if (j < left) store2<VEC>(o + j * so, h, L.n);
-        }
+            for (int j = 0; j < SUB; ++j) {
+                h = {f[j].x * h.x + u[j].x, f[j].y * h.y + u[j].y};
+                if (decltype(whole)::value) *(P2*)(o + j * so) = pair<T>(h);
+                else if (j < left) store2<VEC>(o + j * so, h, L.n);
+            }
+        };
+        if (VEC && left >= SUB && __all(L.n == 2)) write(std::true_type());
+        else write(std::false_type());
     } else if (L.len == 0 && L.tile == 0 && wave == 0)
         store2<false>(p.last + sc, p.h0 != nullptr ? f2{p.h0[sc], p.h0[sc + L.d]} : f2{0.f, 0.f}, L.n);
     if (left < SUB)  // behind the end: zeros
@@ -291,6 +322,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_bwd_kernel(const VcScanPar
     __shared__ f2 carry[64];
     __shared__ int shared;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    typedef typename Pair<T>::type P2;
     const Place<T> L(p, TILE, lane, &shared);
     const int tile = L.ntiles - 1 - L.tile;                  // the last steps come first
     const int first = (L.len + TILE - 1) / TILE - 1 - tile;  // tiles of this sequence that come before
@@ -318,24 +350,29 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_bwd_kernel(const VcScanPar
             }
         }
         f2 f[SUB], q[SUB], a = {1.f, 1.f}, b = {0.f, 0.f}, c = {0.f, 0.f};
+        const bool has_dy = p.dy != nullptr;
+        auto dy = [&](int j, auto whole) { return decltype(whole)::value || has_dy && j < left ? d[j].get() : f2{0.f, 0.f}; };
+        auto compose = [&](auto whole) {  // (a wave whose steps are all there tests none of them)
 #pragma unroll
-        for (int j = 0; j < SUB; ++j) {
-            f[j] = {1.f, 1.f}, q[j] = {0.f, 0.f};
-            if (j < left) {
-                const f2 zz = z[j].get();
-                gate(zz.x, f[j].x, q[j].x);
-                gate(zz.y, f[j].y, q[j].y);
-                const f2 vv = v[j].get();
-                b = {f[j].x * b.x + q[j].x * vv.x, f[j].y * b.y + q[j].y * vv.y};
+            for (int j = 0; j < SUB; ++j) {
+                f[j] = {1.f, 1.f}, q[j] = {0.f, 0.f};
+                if (decltype(whole)::value || j < left) {
+                    const f2 zz = z[j].get();
+                    gate(zz.x, f[j].x, q[j].x);
+                    gate(zz.y, f[j].y, q[j].y);
+                    const f2 vv = v[j].get();
+                    b = {f[j].x * b.x + q[j].x * vv.x, f[j].y * b.y + q[j].y * vv.y};
+                }
+                a = {a.x * f[j].x, a.y * f[j].y};
             }
-            a = {a.x * f[j].x, a.y * f[j].y};
-        }
-        auto dy = [&](int j) { return p.dy != nullptr && j < left ? d[j].get() : f2{0.f, 0.f}; };
 #pragma unroll
-        for (int j = SUB - 1; j >= 0; --j) {
-            const f2 e = dy(j);
-            c = {f[j].x * (e.x + c.x), f[j].y * (e.y + c.y)};
-        }
+            for (int j = SUB - 1; j >= 0; --j) {
+                const f2 e = dy(j, whole);
+                c = {f[j].x * (e.x + c.x), f[j].y * (e.y + c.y)};
+            }
+        };
+        if (left >= SUB && has_dy) compose(std::true_type());
+        else compose(std::false_type());
         agg[wave][lane] = make_float4(a.x, a.y, b.x, b.y);
         back[wave][lane] = c;
         __syncthreads();
@@ -374,24 +411,32 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_bwd_kernel(const VcScanPar
             mu = {m.x * mu.x + n.x, m.y * mu.y + n.y};
         }
         f2 before[SUB];
-#pragma unroll
-        for (int j = 0; j < SUB; ++j) {
-            const f2 vv = v[j].get();
-            before[j] = h;
-            if (j < left) h = {f[j].x * h.x + q[j].x * vv.x, f[j].y * h.y + q[j].y * vv.y};
-        }
         T* const o = out + t0 * 2 * p.H;
         const long long so = 2ll * p.H * dt;
+        auto write = [&](auto whole) {
 #pragma unroll
-        for (int j = SUB - 1; j >= 0; --j) {
-            const f2 e = dy(j), lam = {e.x + mu.x, e.y + mu.y};
-            mu = {f[j].x * lam.x, f[j].y * lam.y};
-            if (j < left) {
+            for (int j = 0; j < SUB; ++j) {
                 const f2 vv = v[j].get();
-                store2<VEC>(o + j * so, {mu.x * q[j].x * (before[j].x - vv.x), mu.y * q[j].y * (before[j].y - vv.y)}, L.n);
-                store2<VEC>(o + j * so + p.H, {q[j].x * lam.x, q[j].y * lam.y}, L.n);
+                before[j] = h;
+                if (decltype(whole)::value || j < left) h = {f[j].x * h.x + q[j].x * vv.x, f[j].y * h.y + q[j].y * vv.y};
             }
-        }
+#pragma unroll
+            for (int j = SUB - 1; j >= 0; --j) {
+                const f2 e = dy(j, whole), lam = {e.x + mu.x, e.y + mu.y}, vv = v[j].get();
+                mu = {f[j].x * lam.x, f[j].y * lam.y};
+                const f2 dv = {q[j].x * lam.x, q[j].y * lam.y};
+                const f2 dz = {mu.x * q[j].x * (before[j].x - vv.x), mu.y * q[j].y * (before[j].y - vv.y)};
+                if (decltype(whole)::value) {
+                    *(P2*)(o + j * so) = pair<T>(dz);
+                    *(P2*)(o + j * so + p.H) = pair<T>(dv);
+                } else if (j < left) {
+                    store2<VEC>(o + j * so, dz, L.n);
+                    store2<VEC>(o + j * so + p.H, dv, L.n);
+                }
+            }
+        };
+        if (VEC && has_dy && left >= SUB && __all(L.n == 2)) write(std::true_type());
+        else write(std::false_type());
     } else if (L.len == 0 && tile == 0 && wave == 0 && p.dh0 != nullptr)
         store2<false>(p.dh0 + sc, p.dlast != nullptr ? f2{p.dlast[sc], p.dlast[sc + L.d]} : f2{0.f, 0.f}, L.n);
     if (left < SUB)  // behind the end: zeros
@@ -430,17 +475,22 @@ int launched(const char* what) {
 
 namespace {
 
-constexpr int FWD_WAVES = 8, FWD_SUB = 16, BWD_WAVES = 8, BWD_SUB = 8;
+// Forward: 16 waves of 16 steps, one workgroup a CU.  Half as many waves or steps: 8 .. 30 % slower (a sequence is more tiles,
+// whose states wait for each other, and a wave has fewer loads in flight); 32 steps spill.  Backward: its three inputs and h
+// in registers leave room for 8 steps; 16 waves against 8: one sequence of 131072 x 512 320 against 433 us, 32 sequences
+// of 2048 x 1024 262 against 258.  Workgroups that stay and ask for their next tile's gates while they finish one measured 20 %
+// slower in both directions (more registers, fewer loads in flight).
+constexpr int FWD_WAVES = 16, FWD_SUB = 16, BWD_WAVES = 16, BWD_SUB = 8;
 
 // whether every pair of channels begins at a multiple of two elements
 bool pairs(const VcScanParams& p, int elem) {
     return ((p.H | p.sb | p.st) & 1) == 0 && ((uintptr_t)p.gates & (2 * elem - 1)) == 0;
 }
 // the workgroups of a launch; clears what they exchange their states through
-unsigned begin(const VcScanParams& p, int steps, hipStream_t s) {
-    const long long tiles = (p.T + steps - 1) / steps, bytes = (long long)vc_scan_workspace(p.B, p.T, p.H, steps == BWD_WAVES * BWD_SUB);
+unsigned begin(const VcScanParams& p, int steps, size_t bytes, hipStream_t s) {
+    const long long tiles = (p.T + steps - 1) / steps;
     if (bytes > 0) {
-        const long long n = bytes / 16, blocks = (n + 255) / 256;
+        const long long n = (long long)bytes / 16, blocks = (n + 255) / 256;
         hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)p.ws, n);
     }
     return (unsigned)(tiles * ((p.H + 127) / 128) * p.B);
@@ -449,7 +499,7 @@ unsigned begin(const VcScanParams& p, int steps, hipStream_t s) {
 template <typename T>
 int fwd(const VcScanParams& p, hipStream_t s) {
     (void)hipGetLastError();
-    const dim3 grid(begin(p, FWD_WAVES * FWD_SUB, s)), block(FWD_WAVES * 64);
+    const dim3 grid(begin(p, FWD_WAVES * FWD_SUB, vc_scan_workspace(p.B, p.T, p.H, 0), s)), block(FWD_WAVES * 64);
     if (pairs(p, sizeof(T))) hipLaunchKernelGGL((scan_fwd_kernel<T, FWD_WAVES, FWD_SUB, true>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((scan_fwd_kernel<T, FWD_WAVES, FWD_SUB, false>), grid, block, 0, s, p);
     return launched("gated_scan_fwd");
@@ -457,7 +507,7 @@ int fwd(const VcScanParams& p, hipStream_t s) {
 template <typename T>
 int bwd(const VcScanParams& p, hipStream_t s) {
     (void)hipGetLastError();
-    const dim3 grid(begin(p, BWD_WAVES * BWD_SUB, s)), block(BWD_WAVES * 64);
+    const dim3 grid(begin(p, BWD_WAVES * BWD_SUB, vc_scan_workspace(p.B, p.T, p.H, 1), s)), block(BWD_WAVES * 64);
     if (pairs(p, sizeof(T))) hipLaunchKernelGGL((scan_bwd_kernel<T, BWD_WAVES, BWD_SUB, true>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((scan_bwd_kernel<T, BWD_WAVES, BWD_SUB, false>), grid, block, 0, s, p);
     return launched("gated_scan_bwd");
