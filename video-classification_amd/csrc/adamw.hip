@@ -15,10 +15,19 @@
 // Every product, sum, root and quotient rounds by itself (no contraction): the codes then do not depend on how a compiler
 // fuses, and a step is reproducible bit for bit by elementary operations.
 //
-// Bound by HBM: 28 bytes per element (fp32, 32-bit moments), 16.06 (fp32, 8-bit), 10.06 (bf16, 8-bit).  One wave owns
-// whole blocks of 256 elements, four per lane, so that a block's maximum is a butterfly over the wave and its codes are one
-// dword per lane; UNROLL blocks per wave keep their loads in flight together.  The tensors' addresses travel as kernel
-// arguments (64 per launch): nothing on the device has to be written before the launch, so a captured step replays.
+// Bound by HBM: 28 bytes per element (fp32, 32-bit moments), 16.06 (fp32, 8-bit), 10.06 (bf16, 8-bit); with 8-bit moments
+// nearly as much by the VALU, so what is done once per block is shared by few lanes: a block belongs to 16 lanes of 16
+// elements (its maximum is four DPP steps, its scales and reciprocals are 1/16 of a lane's work each), a wave has four.  A
+// lane's elements lie in pieces of 16 bytes of p and g, neighbouring lanes' pieces beside each other.
+// With 32-bit moments a lane has four elements of each of UNROLL stretches.
+// The tensors' addresses travel as kernel arguments (60 per launch): nothing on the device has to be written before the
+// launch, so a captured step replays.
+//
+// Root and quotient are correctly rounded.  The compiler's sequences for that (33 issue slots together) cover every input; a
+// wave whose values all lie in the middle of the range (v and |m'| in [2^-90, 2^20]) uses shorter ones (20): with y = the
+// reciprocal (root) from the hardware's estimate by one Newton step, q' = q + (a - b q) y is correctly rounded (P. Markstein,
+// Computation of elementary functions on the IBM RISC System/6000 processor, 1990); tests/test_adamw_gpu.py compares the
+// root's for all mantissas.
 #include "common.h"
 #include "kernels.h"
 
@@ -71,144 +80,234 @@ __device__ __forceinline__ void store4(bf16* p, f32x4 v, bool vec, int left) {
     for (int i = 0; i < 4; ++i)
         if (i < left) p[i] = f2bf(v[i]);
 }
-// four e4m3 codes as one dword
-__device__ __forceinline__ unsigned load_codes(const uint8_t* p, bool vec, int left) {
-    if (vec && left >= 4) return *(const unsigned*)p;
-    unsigned w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < left) w |= (unsigned)p[i] << (8 * i);
-    return w;
+__device__ __forceinline__ float root(float v) { return sqrtf(v); }
+__device__ __forceinline__ float quotient(float a, float b) { return a / b; }
+// v in [2^-90, 2^20]: s ~ sqrt v and h ~ 1 / (2 sqrt v) sharpened once, then the residual
+__device__ __forceinline__ float root_mid(float v) {
+    const float y = __builtin_amdgcn_rsqf(v);
+    float s = v * y, h = 0.5f * y;
+    const float e = __builtin_fmaf(-h, s, 0.5f);
+    s = __builtin_fmaf(s, e, s);
+    h = __builtin_fmaf(h, e, h);
+    return __builtin_fmaf(__builtin_fmaf(-s, s, v), h, s);
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, unsigned w, bool vec, int left) {
-    if (vec && left >= 4) {
-        *(unsigned*)p = w;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < left) p[i] = (uint8_t)(w >> (8 * i));
-}
-__device__ __forceinline__ f32x4 decode(unsigned w, float scale) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-    return (f32x4){lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
-}
-// largest magnitude of the wave's 256 values; compared as integers, where a NaN is above everything and so is kept
-__device__ __forceinline__ float wave_top(f32x4 v) {
-    unsigned t = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const unsigned b = __float_as_uint(v[i]) & 0x7fffffffu;
-        t = b > t ? b : t;
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const unsigned b = (unsigned)__shfl_xor((int)t, o, 64);
-        t = b > t ? b : t;
-    }
-    return __uint_as_float(t);
-}
-template <bool ROOT>
-__device__ __forceinline__ unsigned encode(f32x4 v, float& scale) {
-    const float top = wave_top(v);
-    const bool some = !(top < 0x1p-100f);  // (a NaN counts)
-    const float inv = some ? (1.f / top) * 448.f : 0.f;
-    scale = some ? top * (1.f / 448.f) : 0.f;
-    f32x4 c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        c[i] = v[i] * inv;
-        if (ROOT && some && v[i] > 0.f) c[i] = c[i] < 0x1p-9f ? 0x1p-9f : c[i];
-    }
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], w, true);
+// |a| in [2^-90, 2^20], b in [2^-45, 2^21]: nothing on the way leaves the normal numbers
+__device__ __forceinline__ float quotient_mid(float a, float b) {
+    float y = __builtin_amdgcn_rcpf(b);
+    y = __builtin_fmaf(__builtin_fmaf(-b, y, 1.f), y, y);
+    const float q = a * y;
+    return __builtin_fmaf(__builtin_fmaf(-b, q, a), y, q);
 }
 
-template <typename PT, int BITS>
-__global__ __launch_bounds__(WAVES * 64) void adamw_kernel(const VcAdamwArgs a) {
-    // the tensor whose range of workgroups this one is in
+// the tensor whose range of workgroups this one is in
+__device__ __forceinline__ int tensor_of(const VcAdamwArgs& a) {
     int lo = 0, hi = a.count;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (a.first[mid] <= blockIdx.x) lo = mid;
         else hi = mid;
     }
-    const VcAdamwTensor t = a.t[lo];
+    return lo;
+}
+
+// ---------------------------------------------------------------- moments in 8 bits
+// largest of 16 lanes' values, as integers: of magnitudes' bits a NaN is above everything and so is kept
+__device__ __forceinline__ unsigned top16(unsigned t) {
+    auto step = [&](unsigned u) { t = u > t ? u : t; };
+    step((unsigned)__builtin_amdgcn_update_dpp(0, (int)t, 0xB1, 0xF, 0xF, false));   // quad_perm 1 0 3 2
+    step((unsigned)__builtin_amdgcn_update_dpp(0, (int)t, 0x4E, 0xF, 0xF, false));   // quad_perm 2 3 0 1
+    step((unsigned)__builtin_amdgcn_update_dpp(0, (int)t, 0x141, 0xF, 0xF, false));  // row_half_mirror
+    step((unsigned)__builtin_amdgcn_update_dpp(0, (int)t, 0x140, 0xF, 0xF, false));  // row_mirror
+    return t;
+}
+// what a block's values are multiplied by for their codes, and what the codes are multiplied by
+__device__ __forceinline__ float inverse(float top, float& scale) {
+    const bool some = !(top < 0x1p-100f);  // (a NaN counts)
+    scale = some ? top * (1.f / 448.f) : 0.f;
+    return some ? (1.f / top) * 448.f : 0.f;
+}
+__device__ __forceinline__ unsigned encode(const float* c) {
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], w, true);
+}
+__device__ __forceinline__ void decode(unsigned w, float scale, float* v) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    v[0] = lo[0] * scale, v[1] = lo[1] * scale, v[2] = hi[0] * scale, v[3] = hi[1] * scale;
+}
+
+template <typename PT>
+__global__ __launch_bounds__(WAVES * 64) void adamw8_kernel(const VcAdamwArgs a) {
+    constexpr int E = 16, VE = 16 / sizeof(PT), PIECES = E / VE;  // elements of a lane, of a piece; pieces
+    const int t_ = tensor_of(a);
+    const VcAdamwTensor t = a.t[t_];
+    const int lane = threadIdx.x & 63, l16 = lane & 15;
+    const long long blk = (long long)(blockIdx.x - a.first[t_]) * (CHUNK / BLK) + (threadIdx.x >> 4);
+    if (blk * BLK >= t.n) return;
+    const long long base = blk * BLK + l16 * VE;  // the lane's first element; piece k is k * 16 * VE further on
+    const long long rest = t.n - blk * BLK;
+    PT* const P = (PT*)t.p + base;
+    const PT* const G = (const PT*)t.g + base;
+    uint8_t* const M = (uint8_t*)t.m + base;
+    uint8_t* const V = (uint8_t*)t.v + base;
+    const bool vec = rest >= BLK && (((uintptr_t)t.p | (uintptr_t)t.g) & 15) == 0 && (((uintptr_t)t.m | (uintptr_t)t.v) & (VE - 1)) == 0;
+    const float gs = a.gscale != nullptr ? a.gscale_host * *a.gscale : a.gscale_host;
+    float p[E], g[E], m[E], r[E];
+    unsigned qm[E / 4], qv[E / 4];
+    const float sm = t.ms[blk], sv = t.vs[blk];
+    auto there = [&](int i) { return l16 * VE + i / VE * (16 * VE) + i % VE < rest; };
+    if (vec) {
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int at = k * 16 * VE;
+            if constexpr (sizeof(PT) == 2) {
+                const bf16x8 x = *(const bf16x8*)(P + at), y = *(const bf16x8*)(G + at);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p[k * 8 + i] = bf2f(x[i]), g[k * 8 + i] = bf2f(y[i]);
+                const uint2 x8 = *(const uint2*)(M + at), y8 = *(const uint2*)(V + at);
+                qm[k * 2] = x8.x, qm[k * 2 + 1] = x8.y, qv[k * 2] = y8.x, qv[k * 2 + 1] = y8.y;
+            } else {
+                const f32x4 x = *(const f32x4*)(P + at), y = *(const f32x4*)(G + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[k * 4 + i] = x[i], g[k * 4 + i] = y[i];
+                qm[k] = *(const unsigned*)(M + at), qv[k] = *(const unsigned*)(V + at);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) qm[i] = qv[i] = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int at = i / VE * (16 * VE) + i % VE;
+            p[i] = g[i] = 0.f;
+            if (there(i)) {
+                p[i] = (float)P[at], g[i] = (float)G[at];
+                qm[i / 4] |= (unsigned)M[at] << (i % 4 * 8), qv[i / 4] |= (unsigned)V[at] << (i % 4 * 8);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < E; i += 4) decode(qm[i / 4], sm, m + i), decode(qv[i / 4], sv, r + i);
+    // r becomes v' and then its root
+    constexpr unsigned LO = (127 - 90) << 23, HI = (127 + 20) << 23;
+    unsigned out = 0;  // above HI - LO: some value is not in the middle of the range
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float gi = g[i] * gs;
+        m[i] = m[i] * a.b1 + gi * a.one_b1;
+        r[i] = (r[i] * r[i]) * a.b2 + (gi * a.one_b2) * gi;
+        const unsigned x = (__float_as_uint(m[i]) & 0x7fffffffu) - LO, y = __float_as_uint(r[i]) - LO;
+        out = out > x ? out : x;
+        out = out > y ? out : y;
+    }
+    if (a.mid && __all(out <= HI - LO)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            r[i] = root_mid(r[i]);
+            p[i] = p[i] * a.c0 - quotient_mid(m[i], r[i] * a.root2 + a.eps) * a.step;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            r[i] = root(r[i]);
+            p[i] = p[i] * a.c0 - quotient(m[i], r[i] * a.root2 + a.eps) * a.step;
+        }
+    }
+    unsigned tm = 0, tr = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (!vec && !there(i)) m[i] = r[i] = 0.f;  // (behind the end: 0 whatever eps and a scale of no number made of it)
+        const unsigned x = __float_as_uint(m[i]) & 0x7fffffffu, y = __float_as_uint(r[i]) & 0x7fffffffu;
+        tm = tm > x ? tm : x;
+        tr = tr > y ? tr : y;
+    }
+    float nm, nv;
+    const float im = inverse(__uint_as_float(top16(tm)), nm), iv = inverse(__uint_as_float(top16(tr)), nv);
+    const float least = iv > 0.f ? 0x1p-9f : 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        m[i] *= im;
+        const float c = r[i] * iv;
+        r[i] = c < least && r[i] > 0.f ? least : c;
+    }
+    if (vec) {
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int at = k * 16 * VE;
+            if constexpr (sizeof(PT) == 2) {
+                bf16x8 x;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = f2bf(p[k * 8 + i]);
+                *(bf16x8*)(P + at) = x;
+                *(uint2*)(M + at) = make_uint2(encode(m + k * 8), encode(m + k * 8 + 4));
+                *(uint2*)(V + at) = make_uint2(encode(r + k * 8), encode(r + k * 8 + 4));
+            } else {
+                *(f32x4*)(P + at) = (f32x4){p[k * 4], p[k * 4 + 1], p[k * 4 + 2], p[k * 4 + 3]};
+                *(unsigned*)(M + at) = encode(m + k * 4);
+                *(unsigned*)(V + at) = encode(r + k * 4);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+            const unsigned wm = encode(m + i), wv = encode(r + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int at = (i + j) / VE * (16 * VE) + (i + j) % VE;
+                if (there(i + j)) {
+                    P[at] = (PT)p[i + j];
+                    M[at] = (uint8_t)(wm >> (8 * j)), V[at] = (uint8_t)(wv >> (8 * j));
+                }
+            }
+        }
+    }
+    if (l16 == 0) t.ms[blk] = nm, t.vs[blk] = nv;
+}
+
+// ---------------------------------------------------------------- moments in 32 bits
+template <typename PT>
+__global__ __launch_bounds__(WAVES * 64) void adamw_kernel(const VcAdamwArgs a) {
+    const int t_ = tensor_of(a);
+    const VcAdamwTensor t = a.t[t_];
     PT* const P = (PT*)t.p;
     const PT* const G = (const PT*)t.g;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const long long base = (long long)(blockIdx.x - a.first[lo]) * CHUNK + wave * (UNROLL * BLK);
-    const bool vec = ((((uintptr_t)P | (uintptr_t)G) & (4 * sizeof(PT) - 1)) | (((uintptr_t)t.m | (uintptr_t)t.v) & (BITS == 8 ? 3 : 15))) == 0;
+    float* const M = (float*)t.m;
+    float* const V = (float*)t.v;
+    const long long base = (long long)(blockIdx.x - a.first[t_]) * CHUNK + (threadIdx.x >> 6) * (UNROLL * BLK) + (threadIdx.x & 63) * 4;
+    const bool vec = ((((uintptr_t)P | (uintptr_t)G) & (4 * sizeof(PT) - 1)) | (((uintptr_t)M | (uintptr_t)V) & 15)) == 0;
     const float gs = a.gscale != nullptr ? a.gscale_host * *a.gscale : a.gscale_host;
-
     f32x4 p[UNROLL], g[UNROLL], m[UNROLL], v[UNROLL];
-    unsigned qm[UNROLL], qv[UNROLL];
-    float sm[UNROLL], sv[UNROLL];
     int left[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-        const long long e = base + u * BLK + lane * 4;
-        const long long rest = t.n - e;
+        const long long e = base + u * BLK, rest = t.n - e;
         left[u] = rest <= 0 ? 0 : rest < 4 ? (int)rest : 4;
         const long long at = left[u] > 0 ? e : 0;
         p[u] = load4(P + at, vec, left[u]);
         g[u] = load4(G + at, vec, left[u]);
-        if (BITS == 8) {
-            const bool any = base + u * BLK < t.n;
-            const long long blk = any ? (base + u * BLK) / BLK : 0;
-            qm[u] = load_codes((const uint8_t*)t.m + at, vec, left[u]);
-            qv[u] = load_codes((const uint8_t*)t.v + at, vec, left[u]);
-            sm[u] = t.ms[blk], sv[u] = t.vs[blk];
-        } else {
-            m[u] = load4((const float*)t.m + at, vec, left[u]);
-            v[u] = load4((const float*)t.v + at, vec, left[u]);
-        }
+        m[u] = load4(M + at, vec, left[u]);
+        v[u] = load4(V + at, vec, left[u]);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-        const long long e = base + u * BLK + lane * 4;
-        if (base + u * BLK >= t.n) break;  // (uniform over the wave)
-        if (BITS == 8) {
-            m[u] = decode(qm[u], sm[u]);
-            const f32x4 r = decode(qv[u], sv[u]);
-            v[u] = r * r;
-        }
-        f32x4 r;
+        if (left[u] <= 0) break;
+        const long long e = base + u * BLK;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float gi = g[u][i] * gs;
-            const float mi = m[u][i] * a.b1 + gi * a.one_b1;
-            const float vi = v[u][i] * a.b2 + (gi * a.one_b2) * gi;
-            const float ri = sqrtf(vi);
-            const float move = (mi / (ri * a.root2 + a.eps)) * a.step;
-            p[u][i] = p[u][i] * a.c0 - move;
-            m[u][i] = mi, v[u][i] = vi, r[i] = ri;
+            m[u][i] = m[u][i] * a.b1 + gi * a.one_b1;
+            v[u][i] = v[u][i] * a.b2 + (gi * a.one_b2) * gi;
+            p[u][i] = p[u][i] * a.c0 - quotient(m[u][i], root(v[u][i]) * a.root2 + a.eps) * a.step;
         }
-        if (left[u] > 0) store4(P + e, p[u], vec, left[u]);
-        if (BITS == 8) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)  // (0 0 / eps = NaN with eps = 0: lanes behind the end must not reach the maximum)
-                if (i >= left[u]) m[u][i] = 0.f, r[i] = 0.f;
-            float nm, nv;
-            const unsigned wm = encode<false>(m[u], nm), wv = encode<true>(r, nv);
-            if (left[u] > 0) {
-                store_codes((uint8_t*)t.m + e, wm, vec, left[u]);
-                store_codes((uint8_t*)t.v + e, wv, vec, left[u]);
-            }
-            if (lane == 0) {
-                const long long blk = (base + u * BLK) / BLK;
-                t.ms[blk] = nm, t.vs[blk] = nv;
-            }
-        } else if (left[u] > 0) {
-            store4((float*)t.m + e, m[u], vec, left[u]);
-            store4((float*)t.v + e, v[u], vec, left[u]);
-        }
+        store4(P + e, p[u], vec, left[u]);
+        store4(M + e, m[u], vec, left[u]);
+        store4(V + e, v[u], vec, left[u]);
     }
 }
 
 }  // namespace
 
 int vc_adamw_launch(const VcAdamwTensor* t, int count, bool is_bf16, int bits, VcAdamwArgs& a, hipStream_t s) {
+    a.mid = a.root2 <= 0x1p10f && a.eps <= 0x1p10f;
     for (int i = 0; i < count;) {
         a.count = 0;
         unsigned blocks = 0;
@@ -224,10 +323,10 @@ int vc_adamw_launch(const VcAdamwTensor* t, int count, bool is_bf16, int bits, V
         if (a.count == 0) continue;
         (void)hipGetLastError();
         const dim3 grid(blocks), block(WAVES * 64);
-        if (is_bf16 && bits == 8) hipLaunchKernelGGL((adamw_kernel<bf16, 8>), grid, block, 0, s, a);
-        else if (is_bf16) hipLaunchKernelGGL((adamw_kernel<bf16, 32>), grid, block, 0, s, a);
-        else if (bits == 8) hipLaunchKernelGGL((adamw_kernel<float, 8>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((adamw_kernel<float, 32>), grid, block, 0, s, a);
+        if (is_bf16 && bits == 8) hipLaunchKernelGGL((adamw8_kernel<bf16>), grid, block, 0, s, a);
+        else if (is_bf16) hipLaunchKernelGGL((adamw_kernel<bf16>), grid, block, 0, s, a);
+        else if (bits == 8) hipLaunchKernelGGL((adamw8_kernel<float>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((adamw_kernel<float>), grid, block, 0, s, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) {
             vc_set_error("adamw launch failed: %s", hipGetErrorString(e));

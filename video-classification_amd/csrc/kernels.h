@@ -191,6 +191,7 @@ struct VcAdamwArgs {
     VcAdamwTensor t[VC_ADAMW_MAX_TENSORS];
     unsigned first[VC_ADAMW_MAX_TENSORS];  // first workgroup of each tensor
     int count;
+    int mid;  // root2 and eps leave the denominator of ordinary moments in the middle of the range
     float c0, b1, one_b1, b2, one_b2, root2, eps, step, gscale_host;
     const float* gscale;  // nullable: device scalar, multiplied in
 };

@@ -4,7 +4,7 @@ Every wrapper checks device, dtype, contiguity and element counts on the host be
 launch: a kernel that reads past a buffer can take the whole GPU down.  torch is used for
 device memory and the current stream only.
 """
-import ctypes
+import array
 
 import torch
 
@@ -681,6 +681,7 @@ def linear_bwd(dlogits, feat, W, dW=None, db=None, want_dfeat=True):
 # captured graphs.
 
 _E4M3 = torch.float8_e4m3fn
+_get_device, _numel, _data_ptr, _is_contiguous = (torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous)
 ADAMW_BLOCK = 256  # elements that share a scale of an 8-bit moment
 SCAN_STATE_STEPS = 64  # steps between two saved states
 
@@ -897,39 +898,39 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, m_scale=None, v_scale=None, *
     eight = m_scale is not None
     if eight != (v_scale is not None):
         raise capi.Vc3dError("adamw_step: 8-bit moments need m_scale and v_scale, 32-bit ones neither")
-    lists = (grads, exp_avg, exp_avg_sq) + ((m_scale, v_scale) if eight else ())
+    lists = (params, grads, exp_avg, exp_avg_sq) + ((m_scale, v_scale) if eight else ())
     if any(len(x) != n for x in lists):
-        raise capi.Vc3dError("adamw_step: the lists have %s entries" % ([n] + [len(x) for x in lists],))
+        raise capi.Vc3dError("adamw_step: the lists have %s entries" % ([len(x) for x in lists],))
     if n == 0:
         return
-    kind, dev, dt = _float_kind(params[0], "params[0]"), params[0].device, params[0].dtype
-    held = _E4M3 if eight else F32
-    table = []
-    for i in range(n):
-        p, g, m, v = params[i], grads[i], exp_avg[i], exp_avg_sq[i]
-        size = p.numel()
-        if p.dtype != dt or g.dtype != dt or m.dtype != held or v.dtype != held:
-            raise capi.Vc3dError("adamw_step: tensor %d has types %s, %s, %s, %s; %s, %s, %s, %s expected" %
-                                 (i, p.dtype, g.dtype, m.dtype, v.dtype, dt, dt, held, held))
-        if p.device != dev or g.device != dev or m.device != dev or v.device != dev:
-            raise capi.Vc3dError("adamw_step: tensor %d is not all on %s" % (i, dev))
-        if p.shape != g.shape or p.shape != m.shape or p.shape != v.shape:
-            raise capi.Vc3dError("adamw_step: tensor %d has shapes %s, %s, %s, %s" %
-                                 (i, tuple(p.shape), tuple(g.shape), tuple(m.shape), tuple(v.shape)))
-        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
-            order = p.stride()
-            if not _dense(p) or size > 1 and not (g.stride() == order and m.stride() == order and v.stride() == order):
+    kind, dt = _float_kind(params[0], "params[0]"), params[0].dtype
+    # list by list: hundreds of small tensors are a step whose time is this
+    types = (dt, dt, _E4M3 if eight else F32, _E4M3 if eight else F32, F32, F32)
+    names = ("params", "grads", "exp_avg", "exp_avg_sq", "m_scale", "v_scale")
+    for name, want, ts in zip(names, types, lists):
+        if {t.dtype for t in ts} != {want}:
+            raise capi.Vc3dError("adamw_step: %s are %s; %s expected" % (name, {t.dtype for t in ts}, want))
+        if set(map(_get_device, ts)) != {params[0].get_device()}:
+            raise capi.Vc3dError("adamw_step: %s are not all on %s" % (name, params[0].device))
+    sizes = list(map(_numel, params))
+    if eight:
+        rows = [(k + ADAMW_BLOCK - 1) // ADAMW_BLOCK for k in sizes]
+        for name, ts in zip(names[4:], lists[4:]):
+            if list(map(_numel, ts)) != rows or not all(map(_is_contiguous, ts)):
+                raise capi.Vc3dError("adamw_step: %s hold ceil(numel / %d) contiguous values each" % (name, ADAMW_BLOCK))
+    shapes = [t.shape for t in params]
+    for name, ts in zip(names[1:4], lists[1:4]):
+        if [t.shape for t in ts] != shapes:
+            raise capi.Vc3dError("adamw_step: %s and params differ in shape" % name)
+    if not all(all(map(_is_contiguous, ts)) for ts in lists[:4]):
+        for i, (p, g, m, v) in enumerate(zip(*lists[:4])):
+            if not _dense(p) or sizes[i] > 1 and not g.stride() == m.stride() == v.stride() == p.stride():
                 raise capi.Vc3dError("adamw_step: tensor %d and its gradient and moments must lie in memory in one dense order" % i)
-        a = b = 0
-        if eight:
-            rows = (size + ADAMW_BLOCK - 1) // ADAMW_BLOCK
-            for s in (m_scale[i], v_scale[i]):
-                _chk(s, F32, rows, "scales of tensor %d" % i)
-                if s.device != dev:
-                    raise capi.Vc3dError("adamw_step: scales of tensor %d are not on %s" % (i, dev))
-            a, b = m_scale[i].data_ptr(), v_scale[i].data_ptr()
-        table += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), a, b, size)
-    starts = [table[k] for k in range(0, 7 * n, 7) if table[k + 6]]
+    table = array.array("q", bytes(56 * n))
+    for k, ts in enumerate(lists):
+        table[k::7] = array.array("q", map(_data_ptr, ts))
+    table[6::7] = array.array("q", sizes)
+    starts = [q for q, k in zip(table[::7], sizes) if k]
     if len(set(starts)) != len(starts):
         raise capi.Vc3dError("adamw_step: a parameter is in the list twice")
     scale, scale_dev = 1.0, None
@@ -941,10 +942,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, m_scale=None, v_scale=None, *
         scale = float(grad_scale)
     hyper = capi.AdamwHyper(lr, beta1, beta2, eps, weight_decay, scale, step)
     with _on(params[0]):
-        check(lib.vc_adamw_step((ctypes.c_int64 * len(table))(*table), n, kind, 8 if eight else 32, hyper, ptr(scale_dev), cur_stream()),
-              "vc_adamw_step")
-    for ts in (params,) + lists[1:]:
-        torch.autograd.graph.increment_version(ts)
+        check(lib.vc_adamw_step(table.buffer_info()[0], n, kind, 8 if eight else 32, hyper, ptr(scale_dev), cur_stream()), "vc_adamw_step")
+    for ts in lists:
+        if ts is not grads:
+            torch.autograd.graph.increment_version(ts)
 
 
 def ncthw_to_nthwc(x):
