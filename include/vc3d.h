@@ -356,7 +356,7 @@ int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, flo
  * vc_linear_ce_workspace_bytes(d, op), op 0 forward, 1 backward; it does not grow with N * V. */
 typedef struct vc_linear_ce_desc {
     int32_t N, D, V, is_bf16;
-    int32_t reduction, pad_;
+    int32_t reduction, w_align; /* w's address modulo 16: rows that are no whole 16-byte chunks are copied, piece by piece */
     int64_t ldx, ldw, ignore_index;
 } vc_linear_ce_desc;
 size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op);

@@ -1296,12 +1296,14 @@ static int lce_check(const vc_linear_ce_desc* d) {
     VC_REQUIRE(d->N > 0 && d->D > 0 && d->V > 0, "linear_ce: bad sizes N=%d D=%d V=%d", d->N, d->D, d->V);
     VC_REQUIRE(d->N <= (1 << 23) && d->V <= (1 << 23) && d->D <= (1 << 20), "linear_ce: at most 2^23 rows and classes, 2^20 features");
     VC_REQUIRE(d->ldx >= d->D && d->ldw >= d->D, "linear_ce: row strides %lld, %lld below D=%d", (long long)d->ldx, (long long)d->ldw, d->D);
+    VC_REQUIRE(d->w_align >= 0 && d->w_align < 16, "linear_ce: w_align %d is no address modulo 16", d->w_align);
     VC_REQUIRE(d->reduction >= 0 && d->reduction <= 2, "linear_ce: reduction %d (0 none, 1 mean, 2 sum)", d->reduction);
     return 0;
 }
+static bool lce_pack(const vc_linear_ce_desc* d) { return vc_lce_pack(d->D, d->ldw, d->w_align, d->is_bf16 != 0); }
 size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op) {
     if (lce_check(d) != 0) return 0;
-    return vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, op);
+    return vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, lce_pack(d), op);
 }
 static VcLceParams lce_params(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels, void* ws,
                               size_t ws_bytes) {
@@ -1309,6 +1311,7 @@ static VcLceParams lce_params(const vc_linear_ce_desc* d, const void* x, const v
     memset(&p, 0, sizeof(p));
     p.N = d->N, p.D = d->D, p.V = d->V, p.ldx = d->ldx, p.ldw = d->ldw;
     p.x = x, p.w = w, p.bias = bias, p.labels = (const long long*)labels, p.ignore_index = d->ignore_index, p.reduction = d->reduction;
+    p.pack = lce_pack(d);
     p.ws = ws, p.ws_bytes = ws_bytes;
     return p;
 }
@@ -1317,7 +1320,9 @@ int vc_linear_ce_fwd(const vc_linear_ce_desc* d, const void* x, const void* w, c
     const int rc = lce_check(d);
     if (rc) return rc;
     VC_REQUIRE(x && w && labels && lse && rows && (d->reduction == 0 ? loss_rows != nullptr : loss != nullptr), "linear_ce_fwd: null pointer");
-    const size_t need = vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, 0);
+    VC_REQUIRE(((uintptr_t)w & 15) == (uintptr_t)d->w_align, "linear_ce_fwd: w is at %d modulo 16, w_align says %d", (int)((uintptr_t)w & 15),
+               d->w_align);
+    const size_t need = vc_linear_ce_workspace_bytes(d, 0);
     VC_REQUIRE(workspace && ws_bytes >= need, "linear_ce_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
     VcLceParams p = lce_params(d, x, w, bias, labels, workspace, ws_bytes);
     p.loss = loss, p.loss_rows = loss_rows, p.lse = lse, p.rows = rows;
@@ -1330,7 +1335,9 @@ int vc_linear_ce_bwd(const vc_linear_ce_desc* d, const void* x, const void* w, c
     if (rc) return rc;
     VC_REQUIRE(x && w && labels && lse && rows && dloss, "linear_ce_bwd: null pointer");
     VC_REQUIRE(db == nullptr || bias != nullptr, "linear_ce_bwd: a gradient of a bias that is not there");
-    const size_t need = vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, 1);
+    VC_REQUIRE(((uintptr_t)w & 15) == (uintptr_t)d->w_align, "linear_ce_bwd: w is at %d modulo 16, w_align says %d", (int)((uintptr_t)w & 15),
+               d->w_align);
+    const size_t need = vc_linear_ce_workspace_bytes(d, 1);
     VC_REQUIRE(workspace && ws_bytes >= need, "linear_ce_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
     VcLceParams p = lce_params(d, x, w, bias, labels, workspace, ws_bytes);
     p.lse = (float*)lse, p.rows = (int*)rows, p.dloss = dloss, p.dx = dx, p.dw = dw, p.db = db;

@@ -233,6 +233,7 @@ struct VcLceParams {
     const long long* labels;
     long long ignore_index;
     int reduction;  // 0 none, 1 mean, 2 sum
+    bool pack;      // the products read a copy of w
     float* loss;       // forward: [1], nullable with reduction 0
     float* loss_rows;  // forward: [N], nullable unless reduction is 0
     float* lse;        // [N]
@@ -245,6 +246,7 @@ struct VcLceParams {
     void* ws;
     size_t ws_bytes;
 };
-size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, int op);
+bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16);
+size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int op);
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s);
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s);

@@ -78,13 +78,24 @@ struct Factor {
     }
 };
 
+// The product for dx has few tiles and a long k: k is split, each split into sums of its own, so that all tiles make one round on
+// the chip (`slots` workgroups at once).  The tiles that there are decide, not those that the launch allows for (1777 rows of
+// which 1244 count: 4 splits by the former, 6 by the latter, 232 against LCE_Z us).
+struct Splits {
+    int slots, most, rtiles, bs;
+    __device__ __forceinline__ int of(int ns) const {
+        const int t = rtiles * ((ns + bs - 1) / bs), z = t > 0 ? slots / t : 1;
+        return z < 1 ? 1 : z > most ? most : z;
+    }
+};
+
 struct Gemm {
     Operand R, S;
     int nr, ns, K;      // K: where k is contiguous in an operand, a multiple of its 16-byte chunk
     const int* ns_dev;  // nullable: ns is *ns_dev
     const int* k_dev;   // nullable: K is *k_dev
-    int rtiles, stiles;
-    int k_split;  // k of one split (a multiple of the step), gridDim.y splits
+    int rtiles;
+    Splits splits;  // EPI_DX
     // EPI_STATS / EPI_PROB: r = word v0 + r, s = listed row
     const void* bias;
     const long long* labels;
@@ -221,16 +232,19 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     constexpr int BUF = TR::BYTES + TS::BYTES;
     const int ns = g.ns_dev != nullptr ? *g.ns_dev : g.ns, K = g.k_dev != nullptr ? *g.k_dev : g.K;
     // tile order: XCD x (workgroups go round the 8 XCDs) takes the x-th share of an order in which 4 tiles of s by all tiles of r
-    // follow each other, so that the 32 workgroups of an XCD share 4 + 8 operand panels in its L2
+    // follow each other, so that the 32 workgroups of an XCD share 4 + 8 operand panels in its L2.  The shares are of the tiles
+    // that there are: ns may be far below what the launch had to allow for (shares of all tiles of the launch: the XCDs with the
+    // last tiles of s idle, 1777 rows of which 1244 count 221 us instead of 155).
+    const int stiles = (ns + BS - 1) / BS;
     int r0, s0, st;
     {
-        const unsigned total = gridDim.x, lin = blockIdx.x, x = lin & 7u, base = total >> 3, rem = total & 7u;
+        const unsigned total = (unsigned)g.rtiles * stiles, lin = blockIdx.x, x = lin & 7u, base = total >> 3, rem = total & 7u;
+        if (lin >= total) return;
         const unsigned t = x * base + (x < rem ? x : rem) + (lin >> 3);
         const unsigned per = 4u * g.rtiles, grp = t / per, in = t - grp * per;
-        const unsigned left = g.stiles - grp * 4u, w = left < 4u ? left : 4u;
+        const unsigned left = stiles - grp * 4u, w = left < 4u ? left : 4u;
         r0 = (int)(in / w) * BR, st = (int)(grp * 4u + in % w), s0 = st * BS;
     }
-    if (s0 >= ns) return;
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = (wave % WR) * (BR / WR), wsx = (wave / WR) * (BS / WS);
@@ -239,7 +253,12 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     for (int a = 0; a < NA; ++a)
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[a][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const int kb = blockIdx.y * g.k_split, ke = K < kb + g.k_split ? K : kb + g.k_split;
+    int kb = 0, ke = K;
+    if constexpr (EPI == EPI_DX) {
+        const int z = g.splits.of(ns), each = ((K + z - 1) / z + 127) / 128 * 128;
+        if ((int)blockIdx.y >= z) return;
+        kb = blockIdx.y * each, ke = K < kb + each ? K : kb + each;
+    }
     if (kb < ke) {
         TR tr;
         TS ts;
@@ -335,28 +354,44 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
                 }
     }
     constexpr float LOG2E = 1.44269504088896340736f;
+    // exp(z - ref): with bf16 operands in one multiply-add and one exp2 (ref log2(e) rounds once for the row, 2^-24 |ref| of every
+    // term alike: far below what P is rounded by); with fp32 the difference first, which is exact near the largest terms
+    // (and with references whose multiple could overflow: words masked by the lowest value)
+    auto ex = [&](float z, float ref, float ref2, bool direct) {
+        return __builtin_amdgcn_exp2f(direct ? __builtin_fmaf(z, LOG2E, -ref2) : (z - ref) * LOG2E);
+    };
+    auto direct = [&](float ref) { return sizeof(T) == 2 && __all(!(fabsf(ref) > 1e30f)); };
     if constexpr (EPI == EPI_STATS) {
         __syncthreads();  // (the tiles have been read)
         float2* const join = (float2*)smem;  // [WR][BS]
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const int s = s0 + wsx + b * 16 + l15;
-            const long long label = s < ns ? g.labels[g.rows[s]] - g.v0 - r0 - wr - lg * 4 : -1;
-            float m = -INFINITY, e = 0.f;
+            const long long label = s < ns ? g.labels[g.rows[s]] - g.v0 - r0 - wr : -1;
+            float m = acc[0][b][0], e = 0.f;
 #pragma unroll
             for (int a = 0; a < NA; ++a)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    m = fmaxf(m, acc[a][b][j]);
-                    if (label == a * 16 + j) g.zlab[s] = acc[a][b][j];
-                }
+                for (int j = 0; j < 4; ++j) m = fmaxf(m, acc[a][b][j]);
+            if (__any(label >= 0 && label < BR / WR))  // (a wave in V / 128 has a row's label)
+#pragma unroll
+                for (int a = 0; a < NA; ++a)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (label == a * 16 + lg * 4 + j) g.zlab[s] = acc[a][b][j];
             m = fmaxf(m, __shfl_xor(m, 16, 64));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
-            const float ref = m == -INFINITY ? 0.f : m;
+            const float ref = m == -INFINITY ? 0.f : m, ref2 = ref * LOG2E;
+            if (direct(ref))
 #pragma unroll
-            for (int a = 0; a < NA; ++a)
+                for (int a = 0; a < NA; ++a)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) e += __builtin_amdgcn_exp2f((acc[a][b][j] - ref) * LOG2E);
+                    for (int j = 0; j < 4; ++j) e += ex(acc[a][b][j], ref, ref2, true);
+            else
+#pragma unroll
+                for (int a = 0; a < NA; ++a)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e += ex(acc[a][b][j], ref, ref2, false);
             e += __shfl_xor(e, 16, 64);
             e += __shfl_xor(e, 32, 64);
             if (lg == 0) join[(wave % WR) * BS + wsx + b * 16 + l15] = make_float2(m, e);
@@ -381,20 +416,37 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
             const int s = s0 + wsx + b * 16 + l15;
             const bool in = s < ns;
             const int n = in ? g.rows[s] : 0;
-            const long long label = in ? g.labels[n] - g.v0 - r0 - wr - lg * 4 : -1;
-            const float lse = in ? g.lse[n] : 0.f, sc = !in ? 0.f : g.scale != nullptr ? g.scale[n] : 1.f;
+            const long long label = in ? g.labels[n] - g.v0 - r0 - wr : -1;
+            const float lse = in ? g.lse[n] : 0.f, lse2 = lse * LOG2E;
+            if (direct(lse))
+#pragma unroll
+                for (int a = 0; a < NA; ++a)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[a][b][j] = ex(acc[a][b][j], lse, lse2, true);
+            else
+#pragma unroll
+                for (int a = 0; a < NA; ++a)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[a][b][j] = ex(acc[a][b][j], lse, lse2, false);
+            if (__any(label >= 0 && label < BR / WR))
+#pragma unroll
+                for (int a = 0; a < NA; ++a)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[a][b][j] -= label == a * 16 + lg * 4 + j ? 1.f : 0.f;
+            if (g.scale != nullptr) {
+                const float sc = in ? g.scale[n] : 0.f;
+#pragma unroll
+                for (int a = 0; a < NA; ++a) acc[a][b] *= sc;
+            }
+            if (s0 + BS > ns || r0 + BR > g.nr)  // behind the last row and the last word: 0, whatever lse is
+#pragma unroll
+                for (int a = 0; a < NA; ++a)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[a][b][j] = in && r0 + wr + a * 16 + lg * 4 + j < g.nr ? acc[a][b][j] : 0.f;
             T* const row = (T*)g.P + (long long)s * g.ldp + r0 + wr + lg * 4;
 #pragma unroll
             for (int a = 0; a < NA; ++a) {
-                f32x4 v;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[j] = __builtin_amdgcn_exp2f((acc[a][b][j] - lse) * LOG2E) - (label == a * 16 + j ? 1.f : 0.f);
-                    v[j] = in ? v[j] * sc : 0.f;
-                }
-                if (r0 + BR > g.nr)  // (behind the last word: 0, also in a row whose lse is no number)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = r0 + wr + a * 16 + lg * 4 + j < g.nr ? v[j] : 0.f;
+                const f32x4 v = acc[a][b];
                 cs[a] += v;
                 if constexpr (sizeof(T) == 2) *(bf16x4*)(row + a * 16) = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
                 else *(f32x4*)(row + a * 16) = v;
@@ -454,37 +506,38 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     }
 }
 
-// [n][D] -> [n][dp], zeros behind D: rows whose bytes are no whole 16-byte chunks, or begin at none
-template <typename T>
-__global__ __launch_bounds__(256) void lce_pack_kernel(const T* in, long long ld, long long n, int D, int dp, T* out) {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n * dp; i += (long long)gridDim.x * 256) {
-        const long long r = i / dp;
-        const int d = (int)(i - r * dp);
-        out[i] = d < D ? in[r * ld + d] : (T)0.f;
-    }
+// a row of D elements to one of ld, zeros behind D; VEC: both begin at 16-byte chunks and D is whole ones
+template <typename T, bool VEC>
+__device__ __forceinline__ void copy_row(const T* from, T* to, int D, int ld, int i, int n) {
+    if (VEC) {
+        const int c = D * (int)sizeof(T) / 16;
+        for (int d = i; d < ld * (int)sizeof(T) / 16; d += n) ((uint4*)to)[d] = d < c ? ((const uint4*)from)[d] : make_uint4(0, 0, 0, 0);
+    } else
+        for (int d = i; d < ld; d += n) to[d] = d < D ? from[d] : (T)0.f;
+}
+// words of w (a wave each), for the reasons that Plan gives
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void lce_words_of_w_kernel(const T* w, long long ldw, int n, int D, int ld, T* out) {
+    for (int v = blockIdx.x * 4 + (threadIdx.x >> 6); v < n; v += gridDim.x * 4)
+        copy_row<T, VEC>(w + v * ldw, out + (long long)v * ld, D, ld, threadIdx.x & 63, 64);
 }
 // the rows of x that count, one after the other (13 us of the 7 ms of 8192 x 2048 x 65536; the products then read x in order,
-// with k across too, and never a row that does not count).  VEC: whole 16-byte chunks
+// with k across too, and never a row that does not count)
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long long ld, const int* rows, int N, int D, int dp, T* out) {
+__global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long long ldx, const int* rows, int N, int D, int ld, T* out) {
     const int i = blockIdx.x;
-    if (i >= rows[N]) return;
-    const T* const from = x + rows[i] * ld;
-    T* const to = out + (long long)i * dp;
-    if (VEC)
-        for (int d = threadIdx.x; d < dp * (int)sizeof(T) / 16; d += 256) ((uint4*)to)[d] = ((const uint4*)from)[d];
-    else
-        for (int d = threadIdx.x; d < dp; d += 256) to[d] = d < D ? from[d] : (T)0.f;
+    if (i < rows[N]) copy_row<T, VEC>(x + rows[i] * ldx, out + (long long)i * ld, D, ld, threadIdx.x, 256);
 }
 
 // ---------------------------------------------------------------- the small launches around it
 // A wave joins the pairs of one row: lse, loss.  With `loss` the workgroup that is done last sums the rows up, in their order.
 // (It reads what the others wrote: their stores are device-scope atomics, complete before the workgroup counts itself done.)
-__global__ __launch_bounds__(256) void lce_rows_kernel(const float2* part, int tiles, const float* zlab, const long long* labels,
+// 16 rows a workgroup: workgroups count themselves on one word, 15 ns each (4 rows: 34 us for 8192 rows, 16: 14 us)
+__global__ __launch_bounds__(1024) void lce_rows_kernel(const float2* part, int tiles, const float* zlab, const long long* labels,
                                                        int* rows, int N, int V, float* lse, float* loss_rows, int mean, float* loss) {
-    __shared__ double sums[4];
+    __shared__ double sums[16];
     __shared__ int last;
-    const int wave = threadIdx.x >> 6, i = blockIdx.x * 4 + wave, lane = threadIdx.x & 63, count = rows[N];
+    const int wave = threadIdx.x >> 6, i = blockIdx.x * 16 + wave, lane = threadIdx.x & 63, count = rows[N];
     if (i < N) {
         const int n = rows[i];
         float m = -INFINITY, e = 0.f, l = 0.f, loss_n = 0.f;
@@ -520,23 +573,42 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(const float2* part, int t
     __syncthreads();
     if (!last) return;
     double s = 0.0;
-    for (int n = threadIdx.x; n < N; n += 256) s += (double)__hip_atomic_load(loss_rows + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int n0 = threadIdx.x; n0 < N; n0 += 8192) {  // (eight loads under way)
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            v[k] = n0 + k * 1024 < N ? __hip_atomic_load(loss_rows + n0 + k * 1024, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += (double)v[k];
+    }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
     if (lane == 0) sums[wave] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
-        s = ((sums[0] + sums[1]) + sums[2]) + sums[3];
+        s = 0.0;
+        for (int w = 0; w < 16; ++w) s += sums[w];
         loss[0] = (float)(mean ? s / (double)(count > 0 ? count : 1) : s);
     }
 }
 // dx of the rows that count from their sums, zeros for the others
 template <typename T>
-__global__ __launch_bounds__(256) void lce_dx_kernel(const float* acc, int splits, long long split, const int* rows, Factor factor, int N, int D,
+__global__ __launch_bounds__(256) void lce_dx_kernel(const float* acc, Splits splits_, long long split, const int* rows, Factor factor, int N, int D,
                                                      T* dx) {
     const float g = factor.get();
-    const int i = blockIdx.x, n = rows[i];
-    const bool keep = i < rows[N];
+    const int i = blockIdx.x, n = rows[i], count = rows[N], splits = splits_.of(count);
+    const bool keep = i < count;
+    if ((D & 3) == 0) {
+        for (int d = threadIdx.x * 4; d < D; d += 1024) {
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < splits && keep; ++k) v += *(const f32x4*)(acc + k * split + (long long)i * D + d);
+            v = keep ? v * g : (f32x4){0.f, 0.f, 0.f, 0.f};
+            T* const q = dx + (long long)n * D + d;
+            if constexpr (sizeof(T) == 2) *(bf16x4*)q = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
+            else *(f32x4*)q = v;
+        }
+        return;
+    }
     for (int d = threadIdx.x; d < D; d += 256) {
         float v = 0.f;
         for (int k = 0; k < splits && keep; ++k) v += acc[k * split + (long long)i * D + d];
@@ -567,45 +639,45 @@ struct Plan {
     int tile, tile_dx, tile_dw;  // sides of the tiles of N x V, N x D, piece x D
     int piece;                   // words of a piece, a multiple of 256
     int tiles;                   // tiles of the vocabulary
-    int splits;                  // of k in the product for dx
-    int dp;                      // row length of x, w as the products read them
-    bool pack;                   // w has to be copied for that
+    Splits dx;
+    int kd;                      // features, in whole 16-byte chunks
+    int ld;                      // row length of copies of x, w: whole 128-byte lines
     size_t acc, P, dbpart, part, zlab, loss_rows, xp, wp;
     size_t take(size_t n) {
         const size_t at = bytes;
         bytes += (n + 255) & ~(size_t)255;
         return at;
     }
-    // what the sizes alone decide; `aligned`: both operands' rows begin at 16-byte chunks (if not known: the larger need)
-    Plan(int N, int D, int V, int elem, int op, bool aligned) {
+    Plan(int N, int D, int V, int elem, int op, bool pack) {
         const int per = 16 / elem;
-        pack = !aligned || D % per != 0;
-        dp = (D + per - 1) / per * per;
+        kd = (D + per - 1) / per * per;
+        ld = (D + 8 * per - 1) / (8 * per) * 8 * per;
         const long long np = ((long long)N + 255) / 256 * 256, all = ((long long)V + 255) / 256 * 256;
         long long fit = (512ll << 20) / elem / np / 256 * 256;
-        if (pack && op == 0) fit = (512ll << 20) / elem / dp / 256 * 256;  // (the forward holds a piece of w only)
+        if (pack && op == 0) fit = (512ll << 20) / elem / ld / 256 * 256;  // (the forward holds a piece of w only)
         fit = fit < 256 ? 256 : fit;
         piece = (int)(op == 0 && !pack ? all : fit < all ? fit : all);
         tile = pick_tile(N, piece < V ? piece : V);
         tiles = (int)(((long long)V + tile - 1) / tile);
-        xp = take((size_t)N * dp * elem);
-        if (pack) wp = take((size_t)(piece < V ? piece : V) * dp * elem);
+        xp = take((size_t)N * ld * elem);
+        if (pack) wp = take((size_t)(piece < V ? piece : V) * ld * elem);
         if (op == 0) {
             part = take((size_t)N * tiles * sizeof(float2));
             zlab = take((size_t)N * 4);
             loss_rows = take((size_t)N * 4);
             return;
         }
-        // dx has few tiles and a long k: k is split until the tiles fill the chip, into no less than 512 words.  Smaller tiles
-        // need fewer splits, i.e. fewer sums to write and join (4000 x 256 of 2000 words: 182, 183 us; 500 x 256 of 100000: 349
+        // dx: smaller tiles need fewer splits of k, i.e. fewer sums to write and join (4000 x 256 of 2000 words: 182, 183 us; 500 x 256 of 100000: 349
         // us with 256, 286 with 128; 8192 x 2048 of 65536, 256 tiles of 256: 6.96 against 7.73 ms)
         tile_dx = N > 128 && D > 128 && (N + 255ll) / 256 * ((D + 255) / 256) >= 128 ? 256 : N > 64 && D > 64 ? 128 : 64;
         tile_dw = pick_tile(piece < V ? piece : V, D);
-        const long long t = ((N + tile_dx - 1) / tile_dx) * (long long)((D + tile_dx - 1) / tile_dx), most = piece / 512 > 1 ? piece / 512 : 1;
-        long long z = 512 / t;
-        z = z < 1 ? 1 : z > most ? most : z;
-        splits = (int)(z > 16 ? 16 : z);
-        acc = take((size_t)splits * N * D * 4);
+        // up to 16 splits, 256 MB of sums
+        dx = {tile_dx == 256 ? 256 : 512, 16, (D + tile_dx - 1) / tile_dx, tile_dx};
+        const long long room = (256ll << 20) / ((long long)N * D * 4), least = piece / 512;
+        dx.most = (int)(dx.most > room ? room : dx.most);
+        dx.most = (int)(dx.most > least ? least : dx.most);
+        dx.most = dx.most < 1 ? 1 : dx.most;
+        acc = take((size_t)dx.most * N * D * 4);
         P = take((size_t)np * piece * elem);
         dbpart = take((size_t)(np / 64) * piece * 4);
     }
@@ -621,23 +693,20 @@ int launched(const char* what) {
 }
 
 template <typename T, int EPI, int B>
-void gemm_tile(const Gemm& g, int splits, hipStream_t s) {
+void gemm_tile(const Gemm& g, int tiles, int splits, hipStream_t s) {
     constexpr int WR = 2, WS = B == 256 ? 4 : 2, LDS = Feed<EPI, B>::RING * Feed<EPI, B>::SUBS * 2 * B * 64;
     const auto kernel = lce_gemm<T, EPI, B, B, WR, WS>;
     static VcPerDeviceOnce once;
     once.run([&] { (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
-    hipLaunchKernelGGL((lce_gemm<T, EPI, B, B, WR, WS>), dim3(g.rtiles * g.stiles, splits), dim3(WR * WS * 64), LDS, s, g);
+    hipLaunchKernelGGL((lce_gemm<T, EPI, B, B, WR, WS>), dim3(tiles, splits), dim3(WR * WS * 64), LDS, s, g);
 }
 template <typename T, int EPI>
 void gemm(Gemm& g, int tile, int ns_most, int splits, hipStream_t s) {
-    g.rtiles = (g.nr + tile - 1) / tile, g.stiles = (ns_most + tile - 1) / tile;
-    if (tile == 256) gemm_tile<T, EPI, 256>(g, splits, s);
-    else if (tile == 128) gemm_tile<T, EPI, 128>(g, splits, s);
-    else gemm_tile<T, EPI, 64>(g, splits, s);
-}
-
-bool chunks(const VcLceParams& p, int elem) {
-    return (((uintptr_t)p.x | (uintptr_t)p.w | (uintptr_t)(p.ldx * elem) | (uintptr_t)(p.ldw * elem)) & 15) == 0 && p.ldw * elem < (1ll << 32);
+    g.rtiles = (g.nr + tile - 1) / tile;
+    const int tiles = g.rtiles * ((ns_most + tile - 1) / tile);
+    if (tile == 256) gemm_tile<T, EPI, 256>(g, tiles, splits, s);
+    else if (tile == 128) gemm_tile<T, EPI, 128>(g, tiles, splits, s);
+    else gemm_tile<T, EPI, 64>(g, tiles, splits, s);
 }
 
 // x as the products read it, and w from word v0 on
@@ -647,25 +716,26 @@ struct Source {
     const Plan& L;
     hipStream_t s;
     Operand x;
+    static bool chunks(const void* q, long long ld, int D) { return (((uintptr_t)q | (uintptr_t)(ld * sizeof(T)) | (uintptr_t)(D * sizeof(T))) & 15) == 0; }
     Source(const VcLceParams& p, const Plan& L, hipStream_t s) : p(p), L(L), s(s) {
         T* const to = (T*)((char*)p.ws + L.xp);
-        if (L.pack) hipLaunchKernelGGL((lce_rows_of_x_kernel<T, false>), dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, p.rows, p.N, p.D, L.dp, to);
-        else hipLaunchKernelGGL((lce_rows_of_x_kernel<T, true>), dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, p.rows, p.N, p.D, L.dp, to);
-        x = {(const char*)to, L.dp * (long long)sizeof(T)};
+        const auto kernel = chunks(p.x, p.ldx, p.D) ? lce_rows_of_x_kernel<T, true> : lce_rows_of_x_kernel<T, false>;
+        hipLaunchKernelGGL(kernel, dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, p.rows, p.N, p.D, L.ld, to);
+        x = {(const char*)to, L.ld * (long long)sizeof(T)};
     }
     Operand w(int v0, int nv) const {
         const T* at = (const T*)p.w + v0 * p.ldw;
-        if (!L.pack) return {(const char*)at, p.ldw * (long long)sizeof(T)};
-        const long long n = (long long)nv * L.dp, blocks = (n + 255) / 256;
+        if (!p.pack) return {(const char*)at, p.ldw * (long long)sizeof(T)};
         T* const to = (T*)((char*)p.ws + L.wp);
-        hipLaunchKernelGGL((lce_pack_kernel<T>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, at, p.ldw, (long long)nv, p.D, L.dp, to);
-        return {(const char*)to, L.dp * (long long)sizeof(T)};
+        const auto kernel = chunks(at, p.ldw, p.D) ? lce_words_of_w_kernel<T, true> : lce_words_of_w_kernel<T, false>;
+        hipLaunchKernelGGL(kernel, dim3(nv < 16384 ? (nv + 3) / 4 : 4096), dim3(256), 0, s, at, p.ldw, nv, p.D, L.ld, to);
+        return {(const char*)to, L.ld * (long long)sizeof(T)};
     }
 };
 
 template <typename T>
 int fwd(const VcLceParams& p, hipStream_t s) {
-    const Plan L(p.N, p.D, p.V, sizeof(T), 0, chunks(p, sizeof(T)));
+    const Plan L(p.N, p.D, p.V, sizeof(T), 0, p.pack);
     char* ws = (char*)p.ws;
     float2* part = (float2*)(ws + L.part);
     float* zlab = (float*)(ws + L.zlab);
@@ -675,19 +745,19 @@ int fwd(const VcLceParams& p, hipStream_t s) {
     const Source<T> src(p, L, s);
     for (int v0 = 0; v0 < p.V; v0 += L.piece) {
         Gemm g = {};
-        g.nr = p.V - v0 < L.piece ? p.V - v0 : L.piece, g.ns_dev = p.rows + p.N, g.K = g.k_split = L.dp;
+        g.nr = p.V - v0 < L.piece ? p.V - v0 : L.piece, g.ns_dev = p.rows + p.N, g.K = L.kd;
         g.R = src.w(v0, g.nr), g.S = src.x;
         g.bias = p.bias, g.labels = p.labels, g.rows = p.rows, g.v0 = v0, g.part = part, g.part_ld = L.tiles, g.part0 = v0 / L.tile, g.zlab = zlab;
         gemm<T, EPI_STATS>(g, L.tile, p.N, 1, s);
     }
-    hipLaunchKernelGGL(lce_rows_kernel, dim3((p.N + 3) / 4), dim3(256), 0, s, part, L.tiles, zlab, p.labels, p.rows, p.N, p.V, p.lse,
+    hipLaunchKernelGGL(lce_rows_kernel, dim3((p.N + 15) / 16), dim3(1024), 0, s, part, L.tiles, zlab, p.labels, p.rows, p.N, p.V, p.lse,
                        loss_rows, p.reduction == 1, p.reduction != 0 ? p.loss : nullptr);
     return launched("linear_ce_fwd");
 }
 
 template <typename T>
 int bwd(const VcLceParams& p, hipStream_t s) {
-    const Plan L(p.N, p.D, p.V, sizeof(T), 1, chunks(p, sizeof(T)));
+    const Plan L(p.N, p.D, p.V, sizeof(T), 1, p.pack);
     char* ws = (char*)p.ws;
     float *acc = (float*)(ws + L.acc), *dbpart = (float*)(ws + L.dbpart);
     const int* count = p.rows + p.N;
@@ -700,7 +770,7 @@ int bwd(const VcLceParams& p, hipStream_t s) {
         const Operand w = src.w(v0, nv);
         Gemm g = {};
         g.R = w, g.S = src.x;
-        g.nr = nv, g.ns_dev = count, g.K = g.k_split = L.dp;
+        g.nr = nv, g.ns_dev = count, g.K = L.kd;
         g.bias = p.bias, g.labels = p.labels, g.rows = p.rows, g.v0 = v0;
         g.lse = p.lse, g.scale = p.reduction == 0 ? p.dloss : nullptr, g.P = ws + L.P, g.ldp = L.piece, g.dbpart = p.db != nullptr ? dbpart : nullptr;
         gemm<T, EPI_PROB>(g, L.tile, p.N, 1, s);
@@ -711,27 +781,30 @@ int bwd(const VcLceParams& p, hipStream_t s) {
             Gemm x = {};
             x.R = w, x.S = {ws + L.P, ldp};
             x.nr = p.D, x.ns_dev = count, x.K = nv, x.acc = acc, x.add = v0 > 0, x.acc_split = (long long)p.N * p.D;
-            x.k_split = ((nv + L.splits - 1) / L.splits + 127) / 128 * 128;
-            gemm<T, EPI_DX>(x, L.tile_dx, p.N, L.splits, s);
+            x.splits = L.dx;
+            gemm<T, EPI_DX>(x, L.tile_dx, p.N, L.dx.most, s);
         }
         if (p.dw != nullptr) {
             Gemm d = {};
             d.R = src.x, d.S = {ws + L.P, ldp};
-            d.nr = p.D, d.ns = nv, d.k_dev = count, d.k_split = 0x7fffffc0, d.out = (T*)p.dw + (long long)v0 * p.D, d.factor = factor;
+            d.nr = p.D, d.ns = nv, d.k_dev = count, d.out = (T*)p.dw + (long long)v0 * p.D, d.factor = factor;
             gemm<T, EPI_DW>(d, L.tile_dw, nv, 1, s);
         }
     }
     if (p.dx != nullptr)
-        hipLaunchKernelGGL((lce_dx_kernel<T>), dim3(p.N), dim3(256), 0, s, acc, L.splits, (long long)p.N * p.D, p.rows, factor, p.N, p.D, (T*)p.dx);
+        hipLaunchKernelGGL((lce_dx_kernel<T>), dim3(p.N), dim3(256), 0, s, acc, L.dx, (long long)p.N * p.D, p.rows, factor, p.N, p.D, (T*)p.dx);
     return launched("linear_ce_bwd");
 }
 
 }  // namespace
 
-size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, int op) {
+// Whether the products read a copy of w: where its rows are no whole 16-byte chunks or begin at none (or lie 4 GB apart).
+// (Rows that begin inside 128-byte lines are read as they are: the copies cost more than they gave, 778 against 813 us for 1777
+// x 1000 of 50257.)  w_align: the address of w, modulo 16.
+bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16) {
     const int elem = is_bf16 ? 2 : 4;
-    const size_t a = Plan(N, D, V, elem, op, true).bytes, b = Plan(N, D, V, elem, op, false).bytes;
-    return a > b ? a : b;
+    return (D * elem) % 16 != 0 || (ldw * elem) % 16 != 0 || w_align != 0 || ldw * elem >= (1ll << 32);
 }
+size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack).bytes; }
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? fwd<bf16>(p, s) : fwd<float>(p, s); }
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? bwd<bf16>(p, s) : bwd<float>(p, s); }

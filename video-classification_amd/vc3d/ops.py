@@ -741,7 +741,7 @@ def _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction):
         raise capi.Vc3dError("linear_ce: labels int64 [%d] expected, got %s %s" % (N, labels.dtype, tuple(labels.shape)))
     if bias is not None and tuple(bias.shape) != (V,):
         raise capi.Vc3dError("linear_ce: bias [%d] expected, got %s" % (V, tuple(bias.shape)))
-    return capi.LinearCeDesc(N, D, V, kind, reduction, 0, _ld(x), _ld(weight), ignore_index)
+    return capi.LinearCeDesc(N, D, V, kind, reduction, weight.data_ptr() & 15, _ld(x), _ld(weight), ignore_index)
 
 
 def linear_ce_fwd(x, weight, labels, bias=None, ignore_index=-100, reduction=1):
@@ -868,10 +868,11 @@ def gated_scan_step(gates, state):
     _chk(state, F32, B * H, "state")
     _same_device(gates, state=state)
     with _on(gates):
-        h = torch.empty(B, H, dtype=gates.dtype, device=gates.device)
+        h = torch.empty((B, H), dtype=gates.dtype, device=gates.device)
         if B:
-            check(lib.vc_gated_scan_step(ptr(gates), gates.stride(0), kind, ptr(state), ptr(h), B, H, cur_stream()), "vc_gated_scan_step")
-            torch.autograd.graph.increment_version(state)
+            check(lib.vc_gated_scan_step(gates.data_ptr(), gates.stride(0), kind, state.data_ptr(), h.data_ptr(), B, H, cur_stream()),
+                  "vc_gated_scan_step")
+            torch._C._increment_version([state])
     return h
 
 
@@ -945,7 +946,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, m_scale=None, v_scale=None, *
         check(lib.vc_adamw_step(table.buffer_info()[0], n, kind, 8 if eight else 32, hyper, ptr(scale_dev), cur_stream()), "vc_adamw_step")
     for ts in lists:
         if ts is not grads:
-            torch.autograd.graph.increment_version(ts)
+            torch._C._increment_version(ts)
 
 
 def ncthw_to_nthwc(x):

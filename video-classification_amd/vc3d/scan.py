@@ -66,8 +66,7 @@ def gated_scan(gates, h0=None, lengths=None, reverse=False):
     return _GatedScanFn.apply(gates, h0, lengths, bool(reverse))
 
 
-@torch.no_grad()
 def gated_scan_step(gates, state):
     """one step of gated_scan for each of B sequences, for serving: gates [B][2H], state [B][H] fp32, which is updated in place
     -> h [B][H] of gates' type.  No gradient."""
-    return ops.gated_scan_step(gates.detach(), state)
+    return ops.gated_scan_step(gates, state)
