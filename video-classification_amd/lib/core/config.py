@@ -46,6 +46,12 @@ config.MODEL.DTYPE = 'bf16'
 # the reference's recurrent head (lstm.py, model.py:18-25): backbone features -> LSTMCell -> action / class / critic heads.
 # Off by default: north_star's hot path is the 3D backbone with a plain classifier head.
 config.MODEL.USE_LSTM = False
+# the recurrent head's cell: 'lstm' (the reference's) or 'scan', a gated linear recurrence (models/recurrence.py), which also
+# takes whole sequences of features at once
+config.MODEL.RECURRENT_CELL = 'lstm'
+# training only: the class scores and their cross-entropy as one operator (vc3d.linear_cross_entropy): no logits are kept,
+# for class counts in the tens of thousands
+config.MODEL.FUSED_HEAD_LOSS = False
 # raw-frame input (uint8 N x Ts x Hs x Ws x 3 from a decoder): sampling / normalisation done on the GPU by
 # utils.ChooseInput -> vc_clip_pack_u8; mean / std in units of u8 / 255
 config.MODEL.FRAME_STEP = 1
@@ -58,6 +64,7 @@ config.TRAIN.LR = 0.001
 config.TRAIN.LR_DECAY_RATE = 1
 config.TRAIN.LR_MILESTONES = []
 config.TRAIN.OPTIMIZER = 'adam'
+config.TRAIN.STATE_BITS = 32  # of the moments of 'adamw': 32 or 8
 config.TRAIN.MOMENTUM = 0.9
 config.TRAIN.WD = 0.0001
 config.TRAIN.NESTEROV = False

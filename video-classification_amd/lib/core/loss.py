@@ -18,7 +18,9 @@ class Loss(torch.nn.Module):
         self.r_crt = config.TRAIN.R_CRT
 
     def forward(self, score, y, log_prob, advantages):
-        if (score.is_cuda and score.dim() == 2 and score.dtype == torch.float32 and y.dtype == torch.int64 and y.dim() == 1
+        if not torch.is_tensor(score):
+            total = score.cross_entropy(y)  # vc3d.HeadScores (MODEL.FUSED_HEAD_LOSS): scores and loss in one operator
+        elif (score.is_cuda and score.dim() == 2 and score.dtype == torch.float32 and y.dtype == torch.int64 and y.dim() == 1
                 and y.is_cuda and score.shape[1] <= 1024 and _FUSED_CE):
             # the same mean cross-entropy, value and gradient in one launch between the forward and the backward
             # instead of torch's six (vc_softmax_ce)

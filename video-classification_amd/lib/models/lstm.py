@@ -41,4 +41,10 @@ def getLSTM(config=None, in_dim=None):
     """reference lstm.py:32-40 (getLSTM() reads the global config); in_dim defaults to MODEL.LSTM_INDIM."""
     if config is None:
         from core.config import config
+    cell = config.MODEL.get("RECURRENT_CELL", "lstm")
+    if cell == "scan":
+        from models.recurrence import GatedScan
+        return GatedScan(in_dim or config.MODEL.LSTM_INDIM, config.MODEL.LSTM_OUTDIM)
+    if cell != "lstm":
+        raise ValueError("MODEL.RECURRENT_CELL is 'lstm' or 'scan', got %r" % (cell,))
     return LSTM(in_dim or config.MODEL.LSTM_INDIM, config.MODEL.LSTM_OUTDIM)

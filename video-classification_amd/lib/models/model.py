@@ -21,6 +21,7 @@ class VedioClfNet(nn.Module):
         super().__init__()
         self.backbone = getBackbone(config, is_train)
         self.use_lstm = bool(config.MODEL.get("USE_LSTM", False))
+        self.fused_head_loss = bool(config.MODEL.get("FUSED_HEAD_LOSS", False))
         if self.use_lstm:
             # the reference's recurrent head (model.py:18-25): LSTM -> act_head (Linear + Sigmoid), clf_haed, crit_head
             from models.lstm import getLSTM
@@ -35,6 +36,13 @@ class VedioClfNet(nn.Module):
     def features(self, x):
         return self.backbone(x)
 
+    def _scores(self, feat, eng=None):
+        """class logits; in training with MODEL.FUSED_HEAD_LOSS what Loss makes their cross-entropy of without them"""
+        head = self.clf_haed
+        if self.fused_head_loss and self.training:
+            return vc3d.HeadScores(feat, head.weight, head.bias, eng)
+        return vc3d.linear_apply(feat, head.weight, head.bias, eng)
+
     def forward(self, x):
         eng = self.backbone.engine
         if self.use_lstm:
@@ -43,16 +51,16 @@ class VedioClfNet(nn.Module):
             h = self.lstm(self.backbone(x))
             a0 = self.act_head[0]
             action = torch.sigmoid(vc3d.linear_apply(h, a0.weight, a0.bias))
-            score = vc3d.linear_apply(h, self.clf_haed.weight, self.clf_haed.bias)
+            score = self._scores(h)
             value = vc3d.linear_apply(h, self.crit_head.weight, self.crit_head.bias)
             return action, score, value
         eng.head_params = (self.clf_haed.weight, self.clf_haed.bias)
         feat = self.backbone(x)
-        score = vc3d.linear_apply(feat, self.clf_haed.weight, self.clf_haed.bias, eng)
+        score = self._scores(feat, eng)
         # (one constant tensor per batch size, not a fill launch per step between the head and the loss: nothing writes it)
-        key = (score.shape[0], score.dtype, score.device)
+        key = (feat.shape[0], feat.dtype, feat.device)
         if getattr(self, "_zeros_key", None) != key:
-            self._zeros_key, self._zeros = key, torch.zeros(score.shape[0], 1, dtype=score.dtype, device=score.device)
+            self._zeros_key, self._zeros = key, torch.zeros(feat.shape[0], 1, dtype=feat.dtype, device=feat.device)
         return self._zeros, score, self._zeros
 
     def init_weights(self):

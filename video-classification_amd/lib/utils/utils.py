@@ -7,7 +7,7 @@ import torch
 
 
 def create_optimizer(cfg, model):
-    """SGD(momentum, wd, nesterov) or Adam(lr); None for any other name (reference utils.py:13-36)."""
+    """SGD(momentum, wd, nesterov) or Adam(lr); None for any other name (reference utils.py:13-36).  Added: AdamW(lr, wd)."""
     name = cfg.TRAIN.OPTIMIZER
     params = [p for p in model.parameters()]
     if name == 'sgd' and _fusable(model):
@@ -22,6 +22,11 @@ def create_optimizer(cfg, model):
         return FlatAdam(model, lr=cfg.TRAIN.LR)
     if name == 'adam':
         return torch.optim.Adam(params, lr=cfg.TRAIN.LR)
+    if name == 'adamw' and all(p.is_cuda for p in params):
+        from vc3d.optim import AdamW  # any model, one launch per 60 tensors, moments in TRAIN.STATE_BITS (32 or 8) bits
+        return AdamW(params, lr=cfg.TRAIN.LR, weight_decay=cfg.TRAIN.WD, state_bits=cfg.TRAIN.STATE_BITS)
+    if name == 'adamw':
+        return torch.optim.AdamW(params, lr=cfg.TRAIN.LR, weight_decay=cfg.TRAIN.WD)
     return None
 
 

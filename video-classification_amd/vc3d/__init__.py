@@ -7,5 +7,5 @@ from . import capi  # noqa: F401  (loads the shared library, fails loudly)
 from . import ops  # noqa: F401
 from .engine import R3DEngine  # noqa: F401
 from .autograd import backbone_apply, linear_apply  # noqa: F401
-from .linear_ce import linear_cross_entropy  # noqa: F401
+from .linear_ce import HeadScores, linear_cross_entropy  # noqa: F401
 from .scan import gated_scan, gated_scan_step  # noqa: F401

@@ -10,22 +10,32 @@ _REDUCTION = {"none": 0, "mean": 1, "sum": 2}
 
 
 class _LinearCEFn(torch.autograd.Function):
+    """when ``engine`` is given, the gradients of weight and bias go to its flat buffer, as with autograd.linear_apply"""
+
     @staticmethod
-    def forward(ctx, x, weight, labels, bias, ignore_index, reduction):
+    def forward(ctx, x, weight, labels, bias, ignore_index, reduction, engine):
         d = ops._linear_ce_desc(x, weight, labels, bias, ignore_index, reduction)
         loss, lse, rows = ops._linear_ce_fwd(d, x, weight, labels, bias)
         if any(ctx.needs_input_grad):
             ctx.save_for_backward(x, weight, labels, bias, lse, rows)
-            ctx.desc = d
+            ctx.desc, ctx.engine, ctx.params = d, engine, (weight, bias)
         return loss if reduction == 0 else loss.view(())
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         x, weight, labels, bias, lse, rows = ctx.saved_tensors
-        want = ctx.needs_input_grad
+        want, eng = ctx.needs_input_grad, ctx.engine
         dx, dw, db = ops._linear_ce_bwd(ctx.desc, x, weight, labels, bias, lse, rows, dloss.contiguous(), (want[0], want[1], want[3]))
-        return dx, dw, None, db, None, None
+        wp, bp = ctx.params
+        if eng is not None and eng.flat_grad is not None and id(wp) in eng.grad_views:
+            eng._bind_grads()
+            for p, g in ((wp, dw), (bp, db)):
+                if g is not None:
+                    eng.gview(p).add_(g)
+            eng._ready(wp, *([bp] if bp is not None else []))
+            dw = db = None
+        return dx, dw, None, db, None, None, None
 
 
 def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduction="mean"):
@@ -44,5 +54,21 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     shape = labels.shape
     x2 = ops._rows(x.reshape(-1, x.shape[-1]))
     loss = _LinearCEFn.apply(x2, ops._rows(weight), labels.reshape(-1).contiguous(), None if bias is None else bias.contiguous(),
-                             int(ignore_index), _REDUCTION[reduction])
+                             int(ignore_index), _REDUCTION[reduction], None)
     return loss.view(shape) if reduction == "none" else loss
+
+
+class HeadScores:
+    """Class scores that are only wanted for their loss: the head's input and parameters, which a model in training hands to its
+    criterion in the place of logits (config MODEL.FUSED_HEAD_LOSS).  scores() computes them after all."""
+
+    def __init__(self, feat, weight, bias, engine=None):
+        self.feat, self.weight, self.bias, self.engine = feat, weight, bias, engine
+
+    def cross_entropy(self, y):
+        """mean cross-entropy against y (int64 [N]), differentiable in the features and the head's parameters"""
+        return _LinearCEFn.apply(self.feat.contiguous(), self.weight, y.contiguous(), self.bias, -100, _REDUCTION["mean"], self.engine)
+
+    def scores(self):
+        from .autograd import linear_apply
+        return linear_apply(self.feat, self.weight, self.bias, self.engine)

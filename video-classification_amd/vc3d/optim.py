@@ -6,7 +6,8 @@ launch (vc_pack_dgrad_batched) makes every conv's dgrad operand.  Replaces ~10 m
 launches plus one repack launch per conv per step.  Subclasses torch.optim.Optimizer, so
 ``zero_grad``, ``param_groups[0]['lr']`` and LR schedulers work as with the reference's optimizer
 (/root/reference/lib/utils/utils.py:22-29, lib/core/function.py:80-82).  FlatAdam is the same for
-torch.optim.Adam, the reference's default optimizer (config.py:43, utils.py:30-33): one vc_adam_step launch."""
+torch.optim.Adam, the reference's default optimizer (config.py:43, utils.py:30-33): one vc_adam_step launch.
+AdamW takes any list of parameters and can hold its moments in 8 bits (vc_adamw_step)."""
 import os
 
 import torch
@@ -283,3 +284,81 @@ class FlatSGD(_FlatOptimizer):
         super().load_state_dict(sd)
         dev = next(self.core.parameters()).device
         self.mom = None if mom is None else mom.detach().to(device=dev, dtype=torch.float32).clone()
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's arithmetic (decoupled weight decay, amsgrad off) over any list of fp32 or bf16 parameters, in one
+    launch for all that share a type, a device and a step count (vc_adamw_step; 60 tensors a launch): for models whose
+    parameters are in no flat buffer (the recurrent heads, classifiers of their own).  state_bits=8 holds both moments as e4m3
+    codes with an fp32 scale for every 256 elements: 2.03 bytes per parameter instead of 8.  The moments are fp32 or 8-bit
+    whatever the parameter's type; a parameter without a gradient is skipped, as torch does.  step() counts on the host and
+    refuses to be captured into a graph, where its count would stand still."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
+        if state_bits not in (8, 32):
+            raise Vc3dError("AdamW: moments are held in 32 or 8 bits (got %r)" % (state_bits,))
+        if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas)):
+            raise Vc3dError("AdamW: lr, eps and weight_decay are at least 0, the betas in [0, 1)")
+        self.state_bits = state_bits
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def _new_state(self, p):
+        if not p.is_cuda or p.dtype not in (torch.float32, torch.bfloat16):
+            raise Vc3dError("AdamW: fp32 and bf16 parameters on the GPU only (got %s on %s); torch.optim.AdamW takes others" % (p.dtype, p.device))
+        eight = self.state_bits == 8
+        st = {"step": 0}
+        for k in ("exp_avg", "exp_avg_sq"):
+            st[k] = torch.zeros_like(p, dtype=torch.float8_e4m3fn if eight else torch.float32, memory_format=torch.preserve_format)
+            if eight:
+                st[k + "_scale"] = torch.zeros((p.numel() + ops.ADAMW_BLOCK - 1) // ops.ADAMW_BLOCK, dtype=torch.float32, device=p.device)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale=None):
+        """grad_scale: a number or a one-element fp32 tensor on the device that the gradients are multiplied by (clipping
+        without a host synchronisation)"""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise Vc3dError("AdamW.step() counts on the host: it cannot be captured into a graph (ops.adamw_step with a step of your own can)")
+        for group in self.param_groups:
+            lists = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise Vc3dError("AdamW: sparse gradients are not supported")
+                st = self.state[p]
+                if not st:
+                    st.update(self._new_state(p))
+                st["step"] += 1
+                g = p.grad
+                if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+                    g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)  # into the parameter's order of memory
+                cols = lists.setdefault((p.dtype, p.device, st["step"]), tuple([] for _ in range(6)))
+                for col, t in zip(cols, (p, g, st["exp_avg"], st["exp_avg_sq"], st.get("exp_avg_scale"), st.get("exp_avg_sq_scale"))):
+                    col.append(t)
+            for (_, _, step), cols in lists.items():
+                ops.adamw_step(*cols[:4], *(cols[4:] if self.state_bits == 8 else (None, None)), lr=group["lr"], beta1=group["betas"][0],
+                               beta2=group["betas"][1], eps=group["eps"], weight_decay=group["weight_decay"], step=step, grad_scale=grad_scale)
+        return loss
+
+    def state_dict(self):
+        sd = super().state_dict()
+        sd["state_bits"] = self.state_bits
+        return sd
+
+    def load_state_dict(self, sd):
+        sd = dict(sd)
+        if sd.pop("state_bits", self.state_bits) != self.state_bits:
+            raise Vc3dError("AdamW: the saved moments are not held in %d bits" % self.state_bits)
+        saved = sd["state"]
+        super().load_state_dict(sd)
+        # torch casts what it loads to the parameter's type: the moments keep theirs
+        ids = [i for g in sd["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            for k, v in saved.get(i, {}).items():
+                if torch.is_tensor(v):
+                    self.state[p][k] = v.detach().to(p.device, copy=True)

@@ -70,3 +70,57 @@ def gated_scan_step(gates, state):
     """one step of gated_scan for each of B sequences, for serving: gates [B][2H], state [B][H] fp32, which is updated in place
     -> h [B][H] of gates' type.  No gradient."""
     return ops.gated_scan_step(gates, state)
+
+
+class PackedGateWeight:
+    """bf16 forward / weight-gradient operand of a gate projection and its data-gradient twin, rebuilt when the master changed"""
+
+    def __init__(self):
+        self.key = self.wf = self.wd = None
+
+    def get(self, weight):
+        key = (weight._version, weight.data_ptr(), weight.device)
+        if key != self.key:
+            co, ci = weight.shape
+            w5 = weight.detach().float().contiguous().view(co, 1, 1, 1, ci).permute(0, 4, 1, 2, 3)
+            self.wf, self.wd = ops.pack_weight(w5, want_dgrad=True)
+            self.key = key
+        return self.wf, self.wd
+
+
+class _GateProjectionFn(torch.autograd.Function):
+    """x [N][Fin] W^T -> bf16 [N][2H] as a 1x1x1 conv over N positions, like lstm.py's gates; gradients fp32"""
+
+    @staticmethod
+    def forward(ctx, x, weight, packed):
+        N, fin = x.shape
+        co = weight.shape[0]
+        wf, wd = packed.get(weight)
+        xb = x.detach().to(torch.bfloat16).contiguous()
+        d = ops.conv_desc(N, fin, 1, 1, 1, co, 1, 1, 0)
+        ctx.save_for_backward(xb)
+        ctx.d, ctx.wd = d, wd
+        return ops.conv3d_fwd(d, xb.view(N, 1, 1, 1, fin), wf).view(N, co)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dg):
+        xb, = ctx.saved_tensors
+        (N, fin), co = xb.shape, dg.shape[1]
+        dg5 = dg.contiguous().view(N, 1, 1, 1, co)
+        dx = ops.conv3d_dgrad(ctx.d, dg5, ctx.wd).view(N, fin).float() if ctx.needs_input_grad[0] else None
+        dw = torch.zeros(co, 1, 1, 1, fin, dtype=torch.float32, device=dg.device)
+        ops.conv3d_wgrad(ctx.d, xb.view(N, 1, 1, 1, fin), dg5, dw)
+        return dx, dw.view(co, fin), None
+
+
+def gate_projection(x, weight, bias, packed):
+    """gates [N][2H] in bf16 = x [N][Fin] W^T + b (the sum in fp32), from fp32 x, weight [2H][Fin] and bias [2H] (or None); Fin and 2H are multiples
+    of 64.  `packed`: a PackedGateWeight that keeps the bf16 operands from step to step."""
+    if not x.is_cuda:
+        raise Vc3dError("the vc3d gate projection runs on the GPU only (no CPU fallback)")
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or x.shape[1] % 64 or weight.shape[0] % 64:
+        raise Vc3dError("gate projection: x [N][Fin] and weight [2H][Fin] with Fin and 2H multiples of 64 expected, got %s and %s" %
+                        (tuple(x.shape), tuple(weight.shape)))
+    g = _GateProjectionFn.apply(x.float(), weight, packed)
+    return g if bias is None else (g.float() + bias).to(g.dtype)
