@@ -18,6 +18,9 @@
 #include "kernels.h"
 
 
+#ifndef DXT
+#define DXT 16
+#endif
 namespace {
 
 // ---------------------------------------------------------------- the list of rows
@@ -235,12 +238,15 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     // follow each other, so that the 32 workgroups of an XCD share 4 + 8 operand panels in its L2.  The shares are of the tiles
     // that there are: ns may be far below what the launch had to allow for (shares of all tiles of the launch: the XCDs with the
     // last tiles of s idle, 1777 rows of which 1244 count 221 us instead of 155).
-    const int stiles = (ns + BS - 1) / BS;
-    int r0, s0, st;
+    // A product with splits of k has its splits one after the other in that order: the tiles of a split share their panels.
+    const int stiles = (ns + BS - 1) / BS, z = EPI == EPI_DX ? g.splits.of(ns) : 1;
+    int r0, s0, st, split;
     {
-        const unsigned total = (unsigned)g.rtiles * stiles, lin = blockIdx.x, x = lin & 7u, base = total >> 3, rem = total & 7u;
+        const unsigned tiles = (unsigned)g.rtiles * stiles, total = tiles * z;
+        const unsigned lin = blockIdx.x, x = lin & 7u, base = total >> 3, rem = total & 7u;
         if (lin >= total) return;
-        const unsigned t = x * base + (x < rem ? x : rem) + (lin >> 3);
+        unsigned t = x * base + (x < rem ? x : rem) + (lin >> 3);
+        split = (int)(t / tiles), t -= split * tiles;
         const unsigned per = 4u * g.rtiles, grp = t / per, in = t - grp * per;
         const unsigned left = stiles - grp * 4u, w = left < 4u ? left : 4u;
         r0 = (int)(in / w) * BR, st = (int)(grp * 4u + in % w), s0 = st * BS;
@@ -255,9 +261,8 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
         for (int b = 0; b < NB; ++b) acc[a][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
     int kb = 0, ke = K;
     if constexpr (EPI == EPI_DX) {
-        const int z = g.splits.of(ns), each = ((K + z - 1) / z + 127) / 128 * 128;
-        if ((int)blockIdx.y >= z) return;
-        kb = blockIdx.y * each, ke = K < kb + each ? K : kb + each;
+        const int each = ((K + z - 1) / z + 127) / 128 * 128;
+        kb = split * each, ke = K < kb + each ? K : kb + each;
     }
     if (kb < ke) {
         TR tr;
@@ -484,7 +489,7 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
             for (int a = 0; a < NA; ++a) {
                 const int r = r0 + wr + a * 16 + lg * 4;
                 if constexpr (EPI == EPI_DX) {
-                    float* const q = g.acc + blockIdx.y * g.acc_split + (long long)s * g.nr + r;
+                    float* const q = g.acc + split * g.acc_split + (long long)s * g.nr + r;
                     if (vec && r < g.nr) *(f32x4*)q = g.add ? acc[a][b] + *(const f32x4*)q : acc[a][b];
                     else
 #pragma unroll
@@ -669,7 +674,7 @@ struct Plan {
         }
         // dx: smaller tiles need fewer splits of k, i.e. fewer sums to write and join (4000 x 256 of 2000 words: 182, 183 us; 500 x 256 of 100000: 349
         // us with 256, 286 with 128; 8192 x 2048 of 65536, 256 tiles of 256: 6.96 against 7.73 ms)
-        tile_dx = N > 128 && D > 128 && (N + 255ll) / 256 * ((D + 255) / 256) >= 128 ? 256 : N > 64 && D > 64 ? 128 : 64;
+        tile_dx = N > 128 && D > 128 && (N + 255ll) / 256 * ((D + 255) / 256) >= DXT ? 256 : N > 64 && D > 64 ? 128 : 64;
         tile_dw = pick_tile(piece < V ? piece : V, D);
         // up to 16 splits, 256 MB of sums
         dx = {tile_dx == 256 ? 256 : 512, 16, (D + tile_dx - 1) / tile_dx, tile_dx};
@@ -698,7 +703,7 @@ void gemm_tile(const Gemm& g, int tiles, int splits, hipStream_t s) {
     const auto kernel = lce_gemm<T, EPI, B, B, WR, WS>;
     static VcPerDeviceOnce once;
     once.run([&] { (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS); });
-    hipLaunchKernelGGL((lce_gemm<T, EPI, B, B, WR, WS>), dim3(tiles, splits), dim3(WR * WS * 64), LDS, s, g);
+    hipLaunchKernelGGL((lce_gemm<T, EPI, B, B, WR, WS>), dim3(tiles * splits), dim3(WR * WS * 64), LDS, s, g);
 }
 template <typename T, int EPI>
 void gemm(Gemm& g, int tile, int ns_most, int splits, hipStream_t s) {
