@@ -18,9 +18,6 @@
 #include "kernels.h"
 
 
-#ifndef DXT
-#define DXT 16
-#endif
 namespace {
 
 // ---------------------------------------------------------------- the list of rows
@@ -233,7 +230,8 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     typedef Tile<T, BS, SUBS, NTHR, SK> TS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int BUF = TR::BYTES + TS::BYTES;
-    const int ns = g.ns_dev != nullptr ? *g.ns_dev : g.ns, K = g.k_dev != nullptr ? *g.k_dev : g.K;
+    const int ns = __builtin_amdgcn_readfirstlane(g.ns_dev != nullptr ? *g.ns_dev : g.ns);
+    const int K = __builtin_amdgcn_readfirstlane(g.k_dev != nullptr ? *g.k_dev : g.K);
     // tile order: XCD x (workgroups go round the 8 XCDs) takes the x-th share of an order in which 4 tiles of s by all tiles of r
     // follow each other, so that the 32 workgroups of an XCD share 4 + 8 operand panels in its L2.  The shares are of the tiles
     // that there are: ns may be far below what the launch had to allow for (shares of all tiles of the launch: the XCDs with the
@@ -672,9 +670,9 @@ struct Plan {
             loss_rows = take((size_t)N * 4);
             return;
         }
-        // dx: smaller tiles need fewer splits of k, i.e. fewer sums to write and join (4000 x 256 of 2000 words: 182, 183 us; 500 x 256 of 100000: 349
-        // us with 256, 286 with 128; 8192 x 2048 of 65536, 256 tiles of 256: 6.96 against 7.73 ms)
-        tile_dx = N > 128 && D > 128 && (N + 255ll) / 256 * ((D + 255) / 256) >= DXT ? 256 : N > 64 && D > 64 ? 128 : 64;
+        // dx: smaller tiles need fewer splits of k, i.e. fewer sums to write and join (500 x 256 of 100000 words, 2 tiles of 256:
+        // 338 us with 256, 275 with 128; 1600 x 1000 of 50257, 28 tiles: 794 against 845; 8192 x 2048 of 65536: 6.96 against 7.73 ms)
+        tile_dx = N > 128 && D > 128 && (N + 255ll) / 256 * ((D + 255) / 256) >= 16 ? 256 : N > 64 && D > 64 ? 128 : 64;
         tile_dw = pick_tile(piece < V ? piece : V, D);
         // up to 16 splits, 256 MB of sums
         dx = {tile_dx == 256 ? 256 : 512, 16, (D + tile_dx - 1) / tile_dx, tile_dx};
