@@ -349,22 +349,24 @@ int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, flo
  *   z = x w^T + bias;  loss_n = logsumexp(z_n) - z[n][label_n]
  * x [N][D], w [V][D], bias [V] (nullable): all fp32 or all bf16; ldx, ldw = row strides in elements.  Rows whose label is
  * ignore_index take no part: loss 0, gradient 0, x not read.  Any other label outside [0, V) makes that row's loss NaN (as
- * vc_softmax_ce does).  reduction: 0 none (loss_rows [N]), 1 mean over the rows that count (0 if none does), 2 sum (loss [1]).
- * The forward writes lse [N] and rows (int32 [N + 4]: the rows that count, ascending; from the end those that do not; their
- * number), which the backward takes.  dloss: fp32 on the device, [1], or [N] with reduction 0.  dx [N][D], dw [V][D], db [V]
- * (each nullable) are contiguous and of x's type, and are written, not added to.  workspace (required):
- * vc_linear_ce_workspace_bytes(d, op), op 0 forward, 1 backward; it does not grow with N * V. */
+ * vc_softmax_ce does).  reduction: 0 none, 1 mean over the rows that count (0 if none does), 2 sum.
+ * loss: [1], or [N] with reduction 0.  saved (vc_linear_ce_saved_bytes, 256-byte aligned) is written by the forward and read by
+ * the backward of the same x, w, bias and labels: the rows' logsumexp, the list of rows that count, and, up to 32 MB, their
+ * copies.  dloss: fp32 on the device, [1], or [N] with reduction 0.  dx [N][D], dw [V][D], db [V] (each nullable) are contiguous
+ * and of x's type, and are written, not added to.  workspace (required, 256-byte aligned): vc_linear_ce_workspace_bytes(d, op),
+ * op 0 forward, 1 backward: of the N x V logits the forward keeps two floats for every 64 .. 256, the backward one block of up
+ * to 512 MB.  Results do not depend on the order in which workgroups run. */
 typedef struct vc_linear_ce_desc {
     int32_t N, D, V, is_bf16;
     int32_t reduction, w_align; /* w's address modulo 16: rows that are no whole 16-byte chunks are copied, piece by piece */
     int64_t ldx, ldw, ignore_index;
 } vc_linear_ce_desc;
 size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op);
+size_t vc_linear_ce_saved_bytes(const vc_linear_ce_desc* d);
 int vc_linear_ce_fwd(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels, float* loss,
-                     float* loss_rows, float* lse, int32_t* rows, void* workspace, size_t ws_bytes, void* stream);
+                     void* saved, void* workspace, size_t ws_bytes, void* stream);
 int vc_linear_ce_bwd(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels,
-                     const float* lse, const int32_t* rows, const float* dloss, void* dx, void* dw, void* db, void* workspace,
-                     size_t ws_bytes, void* stream);
+                     const void* saved, const float* dloss, void* dx, void* dw, void* db, void* workspace, size_t ws_bytes, void* stream);
 
 /* ---- Layout helpers at the API edge (NCTHW <-> NTHWC). */
 int vc_ncthw_to_nthwc(const void* in, int32_t in_is_bf16, void* out, int32_t N, int32_t C, int64_t S,

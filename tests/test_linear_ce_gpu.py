@@ -236,8 +236,8 @@ def test_captured_graphs_replay():
     one = torch.ones(1, device="cuda")
 
     def once(y):
-        loss, lse, rows = vc3d.ops.linear_ce_fwd(x, w, y, b)
-        return (loss,) + vc3d.ops.linear_ce_bwd(x, w, y, b, lse, rows, one)
+        loss, saved = vc3d.ops.linear_ce_fwd(x, w, y, b)
+        return (loss,) + vc3d.ops.linear_ce_bwd(x, w, y, b, saved, one)
     ins = [y.clone(), y.flip(0).contiguous()]
     s = torch.cuda.Stream()
     with torch.cuda.stream(s):

@@ -1305,42 +1305,45 @@ size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op) {
     if (lce_check(d) != 0) return 0;
     return vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, lce_pack(d), op);
 }
-static VcLceParams lce_params(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels, void* ws,
-                              size_t ws_bytes) {
+size_t vc_linear_ce_saved_bytes(const vc_linear_ce_desc* d) { return lce_check(d) != 0 ? 0 : vc_lce_saved(d->N, d->D, d->is_bf16 != 0); }
+// what both directions ask of their arguments
+static int lce_args(const char* name, const vc_linear_ce_desc* d, const void* x, const void* w, const int64_t* labels, const void* saved, const void* ws,
+                    size_t ws_bytes, int op) {
+    const int rc = lce_check(d);
+    if (rc) return rc;
+    VC_REQUIRE(x && w && labels && saved, "%s: null pointer", name);
+    VC_REQUIRE(((uintptr_t)saved & 255) == 0, "%s: saved is not 256-byte aligned", name);
+    VC_REQUIRE(((uintptr_t)w & 15) == (uintptr_t)d->w_align, "%s: w is at %d modulo 16, w_align says %d", name, (int)((uintptr_t)w & 15), d->w_align);
+    const size_t need = vc_linear_ce_workspace_bytes(d, op);
+    VC_REQUIRE(ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0, "%s: workspace of %zu bytes, %zu needed, 256-byte aligned", name, ws_bytes, need);
+    return 0;
+}
+static VcLceParams lce_params(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels, void* saved, void* ws) {
     VcLceParams p;
     memset(&p, 0, sizeof(p));
     p.N = d->N, p.D = d->D, p.V = d->V, p.ldx = d->ldx, p.ldw = d->ldw;
     p.x = x, p.w = w, p.bias = bias, p.labels = (const long long*)labels, p.ignore_index = d->ignore_index, p.reduction = d->reduction;
-    p.pack = lce_pack(d);
-    p.ws = ws, p.ws_bytes = ws_bytes;
+    p.pack = lce_pack(d), p.saved = saved, p.ws = ws;
     return p;
 }
 int vc_linear_ce_fwd(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels, float* loss,
-                     float* loss_rows, float* lse, int32_t* rows, void* workspace, size_t ws_bytes, void* stream) {
-    const int rc = lce_check(d);
+                     void* saved, void* workspace, size_t ws_bytes, void* stream) {
+    const int rc = lce_args("linear_ce_fwd", d, x, w, labels, saved, workspace, ws_bytes, 0);
     if (rc) return rc;
-    VC_REQUIRE(x && w && labels && lse && rows && (d->reduction == 0 ? loss_rows != nullptr : loss != nullptr), "linear_ce_fwd: null pointer");
-    VC_REQUIRE(((uintptr_t)w & 15) == (uintptr_t)d->w_align, "linear_ce_fwd: w is at %d modulo 16, w_align says %d", (int)((uintptr_t)w & 15),
-               d->w_align);
-    const size_t need = vc_linear_ce_workspace_bytes(d, 0);
-    VC_REQUIRE(workspace && ws_bytes >= need, "linear_ce_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
-    VcLceParams p = lce_params(d, x, w, bias, labels, workspace, ws_bytes);
-    p.loss = loss, p.loss_rows = loss_rows, p.lse = lse, p.rows = rows;
+    VC_REQUIRE(loss, "linear_ce_fwd: null pointer");
+    VcLceParams p = lce_params(d, x, w, bias, labels, saved, workspace);
+    if (d->reduction == 0) p.loss_rows = loss;
+    else p.loss = loss;
     return vc_lce_launch_fwd(p, d->is_bf16 != 0, S(stream));
 }
 int vc_linear_ce_bwd(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels,
-                     const float* lse, const int32_t* rows, const float* dloss, void* dx, void* dw, void* db, void* workspace,
-                     size_t ws_bytes, void* stream) {
-    const int rc = lce_check(d);
+                     const void* saved, const float* dloss, void* dx, void* dw, void* db, void* workspace, size_t ws_bytes, void* stream) {
+    const int rc = lce_args("linear_ce_bwd", d, x, w, labels, saved, workspace, ws_bytes, 1);
     if (rc) return rc;
-    VC_REQUIRE(x && w && labels && lse && rows && dloss, "linear_ce_bwd: null pointer");
+    VC_REQUIRE(dloss, "linear_ce_bwd: null pointer");
     VC_REQUIRE(db == nullptr || bias != nullptr, "linear_ce_bwd: a gradient of a bias that is not there");
-    VC_REQUIRE(((uintptr_t)w & 15) == (uintptr_t)d->w_align, "linear_ce_bwd: w is at %d modulo 16, w_align says %d", (int)((uintptr_t)w & 15),
-               d->w_align);
-    const size_t need = vc_linear_ce_workspace_bytes(d, 1);
-    VC_REQUIRE(workspace && ws_bytes >= need, "linear_ce_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
-    VcLceParams p = lce_params(d, x, w, bias, labels, workspace, ws_bytes);
-    p.lse = (float*)lse, p.rows = (int*)rows, p.dloss = dloss, p.dx = dx, p.dw = dw, p.db = db;
+    VcLceParams p = lce_params(d, x, w, bias, labels, (void*)saved, workspace);
+    p.dloss = dloss, p.dx = dx, p.dw = dw, p.db = db;
     return vc_lce_launch_bwd(p, d->is_bf16 != 0, S(stream));
 }
 

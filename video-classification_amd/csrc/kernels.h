@@ -236,8 +236,7 @@ struct VcLceParams {
     bool pack;      // the products read a copy of w
     float* loss;       // forward: [1], nullable with reduction 0
     float* loss_rows;  // forward: [N], nullable unless reduction is 0
-    float* lse;        // [N]
-    int* rows;         // [N + 4]: rows that count (in order), rows that do not, from the end; then their number
+    void* saved;       // what the forward leaves for the backward
     // backward
     const float* dloss;  // [1], or [N] with reduction 0
     void* dx;            // nullable
@@ -247,6 +246,7 @@ struct VcLceParams {
     size_t ws_bytes;
 };
 bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16);
+size_t vc_lce_saved(int N, int D, bool is_bf16);
 size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int op);
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s);
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s);

@@ -525,11 +525,38 @@ __global__ __launch_bounds__(256) void lce_words_of_w_kernel(const T* w, long lo
         copy_row<T, VEC>(w + v * ldw, out + (long long)v * ld, D, ld, threadIdx.x & 63, 64);
 }
 // the rows of x that count, one after the other (13 us of the 7 ms of 8192 x 2048 x 65536; the products then read x in order,
-// with k across too, and never a row that does not count)
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long long ldx, const int* rows, int N, int D, int ld, T* out) {
-    const int i = blockIdx.x;
-    if (i < rows[N]) copy_row<T, VEC>(x + rows[i] * ldx, out + (long long)i * ld, D, ld, threadIdx.x, 256);
+// with k across too, and never a row that does not count).  LIST: the list itself is made here too: every workgroup counts the
+// labels before its row (short batches: one launch instead of two)
+template <typename T, bool VEC, bool LIST>
+__global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long long ldx, int* rows, const long long* labels, long long ignore,
+                                                            int N, int D, int ld, T* out) {
+    int i = blockIdx.x, n;
+    if (LIST) {
+        __shared__ int before_sh[4], all_sh[4];
+        n = i;
+        int before = 0, all = 0;
+        for (int k = threadIdx.x; k < N; k += 256) {
+            const int keep = labels[k] != ignore ? 1 : 0;
+            all += keep;
+            before += k < n ? keep : 0;
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) before += __shfl_xor(before, o, 64), all += __shfl_xor(all, o, 64);
+        if ((threadIdx.x & 63) == 0) before_sh[threadIdx.x >> 6] = before, all_sh[threadIdx.x >> 6] = all;
+        __syncthreads();
+        before = before_sh[0] + before_sh[1] + before_sh[2] + before_sh[3];
+        const bool keep = labels[n] != ignore;
+        i = before;
+        if (threadIdx.x == 0) {
+            rows[keep ? before : N - 1 - (n - before)] = n;
+            if (n == 0) rows[N] = all_sh[0] + all_sh[1] + all_sh[2] + all_sh[3], rows[N + 1] = 0;
+        }
+        if (!keep) return;
+    } else {
+        if (i >= rows[N]) return;
+        n = rows[i];
+    }
+    copy_row<T, VEC>(x + n * ldx, out + (long long)i * ld, D, ld, threadIdx.x, 256);
 }
 
 // ---------------------------------------------------------------- the small launches around it
@@ -594,38 +621,49 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const float2* part, int 
         loss[0] = (float)(mean ? s / (double)(count > 0 ? count : 1) : s);
     }
 }
-// dx of the rows that count from their sums, zeros for the others
+// what is stored last: workgroup i < N the row i of the list of dx (its splits' sums; zeros for a row that does not count), the
+// others 256 words of db each (the sums of its row tiles)
+struct Last {
+    const float* acc;
+    Splits splits;
+    long long split;  // from split to split
+    const float* part;
+    long long ld;
+    int bs, words, nx;  // nx: workgroups for dx, N or 0
+    void *dx, *db;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void lce_dx_kernel(const float* acc, Splits splits_, long long split, const int* rows, Factor factor, int N, int D,
-                                                     T* dx) {
+__global__ __launch_bounds__(256) void lce_last_kernel(const Last q, const int* rows, Factor factor, int N, int D) {
     const float g = factor.get();
-    const int i = blockIdx.x, n = rows[i], count = rows[N], splits = splits_.of(count);
+    const int count = rows[N];
+    if ((int)blockIdx.x >= q.nx) {
+        const int r = (blockIdx.x - q.nx) * 256 + threadIdx.x;
+        if (r >= q.words) return;
+        const int tiles = (count + q.bs - 1) / q.bs;
+        float s = 0.f;
+        for (int t = 0; t < tiles; ++t) s += q.part[t * q.ld + r];
+        ((T*)q.db)[r] = (T)(s * g);
+        return;
+    }
+    const int i = blockIdx.x, n = rows[i], splits = q.splits.of(count);
     const bool keep = i < count;
+    const float* const from = q.acc + (long long)i * D;
+    T* const to = (T*)q.dx + (long long)n * D;
     if ((D & 3) == 0) {
         for (int d = threadIdx.x * 4; d < D; d += 1024) {
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < splits && keep; ++k) v += *(const f32x4*)(acc + k * split + (long long)i * D + d);
+            for (int k = 0; k < splits && keep; ++k) v += *(const f32x4*)(from + k * q.split + d);
             v = keep ? v * g : (f32x4){0.f, 0.f, 0.f, 0.f};
-            T* const q = dx + (long long)n * D + d;
-            if constexpr (sizeof(T) == 2) *(bf16x4*)q = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
-            else *(f32x4*)q = v;
+            if constexpr (sizeof(T) == 2) *(bf16x4*)(to + d) = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
+            else *(f32x4*)(to + d) = v;
         }
         return;
     }
     for (int d = threadIdx.x; d < D; d += 256) {
         float v = 0.f;
-        for (int k = 0; k < splits && keep; ++k) v += acc[k * split + (long long)i * D + d];
-        dx[(long long)n * D + d] = keep ? (T)(v * g) : (T)0.f;
+        for (int k = 0; k < splits && keep; ++k) v += from[k * q.split + d];
+        to[d] = keep ? (T)(v * g) : (T)0.f;
     }
-}
-template <typename T>
-__global__ __launch_bounds__(256) void lce_db_kernel(const float* part, long long ld, int bs, Factor factor, int nr, T* db) {
-    const int r = blockIdx.x * 256 + threadIdx.x;
-    if (r >= nr) return;
-    const int tiles = (*factor.count + bs - 1) / bs;
-    float s = 0.f;
-    for (int t = 0; t < tiles; ++t) s += part[t * ld + r];
-    db[r] = (T)(s * factor.get());
 }
 
 // ---------------------------------------------------------------- plan and workspace
@@ -651,10 +689,16 @@ struct Plan {
         bytes += (n + 255) & ~(size_t)255;
         return at;
     }
+    // row length of a copy: whole 128-byte lines; whether the copy of x is kept for the backward (up to 32 MB)
+    static int row(int D, int elem) { return (D * elem + 127) / 128 * 128 / elem; }
+    static bool saves_x(int N, int D, int elem) { return (long long)N * row(D, elem) * elem <= (32 << 20); }
+    // what the forward leaves for the backward: lse [N], the list [N + 4], the copy of x
+    static size_t list_at(int N) { return ((size_t)N * 4 + 255) & ~(size_t)255; }
+    static size_t x_at(int N) { return list_at(N) + ((((size_t)N + 4) * 4 + 255) & ~(size_t)255); }
+    static size_t saved(int N, int D, int elem) { return x_at(N) + (saves_x(N, D, elem) ? (size_t)N * row(D, elem) * elem : 0); }
     Plan(int N, int D, int V, int elem, int op, bool pack) {
-        const int per = 16 / elem;
-        kd = (D + per - 1) / per * per;
-        ld = (D + 8 * per - 1) / (8 * per) * 8 * per;
+        kd = (D * elem + 15) / 16 * 16 / elem;
+        ld = row(D, elem);
         const long long np = ((long long)N + 255) / 256 * 256, all = ((long long)V + 255) / 256 * 256;
         long long fit = (512ll << 20) / elem / np / 256 * 256;
         if (pack && op == 0) fit = (512ll << 20) / elem / ld / 256 * 256;  // (the forward holds a piece of w only)
@@ -662,7 +706,7 @@ struct Plan {
         piece = (int)(op == 0 && !pack ? all : fit < all ? fit : all);
         tile = pick_tile(N, piece < V ? piece : V);
         tiles = (int)(((long long)V + tile - 1) / tile);
-        xp = take((size_t)N * ld * elem);
+        if (!saves_x(N, D, elem)) xp = take((size_t)N * ld * elem);
         if (pack) wp = take((size_t)(piece < V ? piece : V) * ld * elem);
         if (op == 0) {
             part = take((size_t)N * tiles * sizeof(float2));
@@ -720,11 +764,20 @@ struct Source {
     hipStream_t s;
     Operand x;
     static bool chunks(const void* q, long long ld, int D) { return (((uintptr_t)q | (uintptr_t)(ld * sizeof(T)) | (uintptr_t)(D * sizeof(T))) & 15) == 0; }
-    Source(const VcLceParams& p, const Plan& L, hipStream_t s) : p(p), L(L), s(s) {
-        T* const to = (T*)((char*)p.ws + L.xp);
-        const auto kernel = chunks(p.x, p.ldx, p.D) ? lce_rows_of_x_kernel<T, true> : lce_rows_of_x_kernel<T, false>;
-        hipLaunchKernelGGL(kernel, dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, p.rows, p.N, p.D, L.ld, to);
+    float* lse;
+    int* rows;
+    Source(const VcLceParams& p, const Plan& L, hipStream_t s, bool forward) : p(p), L(L), s(s) {
+        char* const saved = (char*)p.saved;
+        const bool kept = Plan::saves_x(p.N, p.D, sizeof(T));
+        lse = (float*)saved, rows = (int*)(saved + Plan::list_at(p.N));
+        T* const to = (T*)(kept ? saved + Plan::x_at(p.N) : (char*)p.ws + L.xp);
         x = {(const char*)to, L.ld * (long long)sizeof(T)};
+        if (!forward && kept) return;
+        const bool list = forward && p.N <= 1024, vec = chunks(p.x, p.ldx, p.D);
+        if (forward && !list) hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, s, p.labels, p.ignore_index, p.N, rows);
+        const auto kernel = list ? (vec ? lce_rows_of_x_kernel<T, true, true> : lce_rows_of_x_kernel<T, false, true>)
+                                 : (vec ? lce_rows_of_x_kernel<T, true, false> : lce_rows_of_x_kernel<T, false, false>);
+        hipLaunchKernelGGL(kernel, dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, rows, p.labels, p.ignore_index, p.N, p.D, L.ld, to);
     }
     Operand w(int v0, int nv) const {
         const T* at = (const T*)p.w + v0 * p.ldw;
@@ -744,16 +797,15 @@ int fwd(const VcLceParams& p, hipStream_t s) {
     float* zlab = (float*)(ws + L.zlab);
     float* loss_rows = p.loss_rows != nullptr ? p.loss_rows : (float*)(ws + L.loss_rows);
     (void)hipGetLastError();
-    hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, s, p.labels, p.ignore_index, p.N, p.rows);
-    const Source<T> src(p, L, s);
+    const Source<T> src(p, L, s, true);
     for (int v0 = 0; v0 < p.V; v0 += L.piece) {
         Gemm g = {};
-        g.nr = p.V - v0 < L.piece ? p.V - v0 : L.piece, g.ns_dev = p.rows + p.N, g.K = L.kd;
+        g.nr = p.V - v0 < L.piece ? p.V - v0 : L.piece, g.ns_dev = src.rows + p.N, g.K = L.kd;
         g.R = src.w(v0, g.nr), g.S = src.x;
-        g.bias = p.bias, g.labels = p.labels, g.rows = p.rows, g.v0 = v0, g.part = part, g.part_ld = L.tiles, g.part0 = v0 / L.tile, g.zlab = zlab;
+        g.bias = p.bias, g.labels = p.labels, g.rows = src.rows, g.v0 = v0, g.part = part, g.part_ld = L.tiles, g.part0 = v0 / L.tile, g.zlab = zlab;
         gemm<T, EPI_STATS>(g, L.tile, p.N, 1, s);
     }
-    hipLaunchKernelGGL(lce_rows_kernel, dim3((p.N + 15) / 16), dim3(1024), 0, s, part, L.tiles, zlab, p.labels, p.rows, p.N, p.V, p.lse,
+    hipLaunchKernelGGL(lce_rows_kernel, dim3((p.N + 15) / 16), dim3(1024), 0, s, part, L.tiles, zlab, p.labels, src.rows, p.N, p.V, src.lse,
                        loss_rows, p.reduction == 1, p.reduction != 0 ? p.loss : nullptr);
     return launched("linear_ce_fwd");
 }
@@ -763,23 +815,20 @@ int bwd(const VcLceParams& p, hipStream_t s) {
     const Plan L(p.N, p.D, p.V, sizeof(T), 1, p.pack);
     char* ws = (char*)p.ws;
     float *acc = (float*)(ws + L.acc), *dbpart = (float*)(ws + L.dbpart);
-    const int* count = p.rows + p.N;
-    const Factor factor = {p.dloss, count, p.reduction};
     const long long ldp = (long long)L.piece * (int)sizeof(T);
     (void)hipGetLastError();
-    const Source<T> src(p, L, s);
+    const Source<T> src(p, L, s, false);
+    const int* count = src.rows + p.N;
+    const Factor factor = {p.dloss, count, p.reduction};
     for (int v0 = 0; v0 < p.V; v0 += L.piece) {
         const int nv = p.V - v0 < L.piece ? p.V - v0 : L.piece;
         const Operand w = src.w(v0, nv);
         Gemm g = {};
         g.R = w, g.S = src.x;
         g.nr = nv, g.ns_dev = count, g.K = L.kd;
-        g.bias = p.bias, g.labels = p.labels, g.rows = p.rows, g.v0 = v0;
-        g.lse = p.lse, g.scale = p.reduction == 0 ? p.dloss : nullptr, g.P = ws + L.P, g.ldp = L.piece, g.dbpart = p.db != nullptr ? dbpart : nullptr;
+        g.bias = p.bias, g.labels = p.labels, g.rows = src.rows, g.v0 = v0;
+        g.lse = src.lse, g.scale = p.reduction == 0 ? p.dloss : nullptr, g.P = ws + L.P, g.ldp = L.piece, g.dbpart = p.db != nullptr ? dbpart : nullptr;
         gemm<T, EPI_PROB>(g, L.tile, p.N, 1, s);
-        if (p.db != nullptr)
-            hipLaunchKernelGGL((lce_db_kernel<T>), dim3((nv + 255) / 256), dim3(256), 0, s, dbpart, (long long)L.piece, L.tile, factor, nv,
-                               (T*)p.db + v0);
         if (p.dx != nullptr) {
             Gemm x = {};
             x.R = w, x.S = {ws + L.P, ldp};
@@ -793,9 +842,11 @@ int bwd(const VcLceParams& p, hipStream_t s) {
             d.nr = p.D, d.ns = nv, d.k_dev = count, d.out = (T*)p.dw + (long long)v0 * p.D, d.factor = factor;
             gemm<T, EPI_DW>(d, L.tile_dw, nv, 1, s);
         }
+        const bool end = v0 + nv == p.V && p.dx != nullptr;
+        if (p.db == nullptr && !end) continue;
+        const Last q = {acc, L.dx, (long long)p.N * p.D, dbpart, L.piece, L.tile, nv, end ? p.N : 0, p.dx, p.db != nullptr ? (T*)p.db + v0 : nullptr};
+        hipLaunchKernelGGL((lce_last_kernel<T>), dim3(q.nx + (p.db != nullptr ? (nv + 255) / 256 : 0)), dim3(256), 0, s, q, src.rows, factor, p.N, p.D);
     }
-    if (p.dx != nullptr)
-        hipLaunchKernelGGL((lce_dx_kernel<T>), dim3(p.N), dim3(256), 0, s, acc, L.dx, (long long)p.N * p.D, p.rows, factor, p.N, p.D, (T*)p.dx);
     return launched("linear_ce_bwd");
 }
 
@@ -808,6 +859,7 @@ bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16) {
     const int elem = is_bf16 ? 2 : 4;
     return (D * elem) % 16 != 0 || (ldw * elem) % 16 != 0 || w_align != 0 || ldw * elem >= (1ll << 32);
 }
+size_t vc_lce_saved(int N, int D, bool is_bf16) { return Plan::saved(N, D, is_bf16 ? 2 : 4); }
 size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack).bytes; }
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? fwd<bf16>(p, s) : fwd<float>(p, s); }
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? bwd<bf16>(p, s) : bwd<float>(p, s); }

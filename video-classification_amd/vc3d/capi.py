@@ -150,8 +150,9 @@ PROTOTYPES = {
     "vc_gated_scan_bwd": [_SD, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P],
     "vc_gated_scan_step": [_P, _L, _I, _P, _P, _I, _I, _P],
     "vc_linear_ce_workspace_bytes": [_LD, _I],
-    "vc_linear_ce_fwd": [_LD] + [_P] * 9 + [C.c_size_t, _P],
-    "vc_linear_ce_bwd": [_LD] + [_P] * 11 + [C.c_size_t, _P],
+    "vc_linear_ce_saved_bytes": [_LD],
+    "vc_linear_ce_fwd": [_LD] + [_P] * 7 + [C.c_size_t, _P],
+    "vc_linear_ce_bwd": [_LD] + [_P] * 10 + [C.c_size_t, _P],
     "vc_ncthw_to_nthwc": [_P, _I, _P, _I, _I, _L, _P],
     "vc_nthwc_to_ncthw": [_P, _P, _I, _I, _I, _L, _P],
     "vc_replay": [C.POINTER(Cmd), _I, C.POINTER(C.c_void_p), _I, _I, _P, _P, _IP],
@@ -163,7 +164,8 @@ PROTOTYPES = {
 }
 _RESTYPE = {"vc_last_error": C.c_char_p, "vc_stem_packed_input_elems": C.c_size_t, "vc_static_scratch_bytes": C.c_size_t,
             "vc_conv3d_workspace_bytes": C.c_size_t, "vc_stem_wgrad_workspace_bytes": C.c_size_t,
-            "vc_gated_scan_workspace_bytes": C.c_size_t, "vc_linear_ce_workspace_bytes": C.c_size_t}
+            "vc_gated_scan_workspace_bytes": C.c_size_t, "vc_linear_ce_workspace_bytes": C.c_size_t,
+            "vc_linear_ce_saved_bytes": C.c_size_t}
 
 
 def _load():

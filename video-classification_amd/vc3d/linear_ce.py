@@ -15,18 +15,18 @@ class _LinearCEFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, labels, bias, ignore_index, reduction, engine):
         d = ops._linear_ce_desc(x, weight, labels, bias, ignore_index, reduction)
-        loss, lse, rows = ops._linear_ce_fwd(d, x, weight, labels, bias)
+        loss, saved = ops._linear_ce_fwd(d, x, weight, labels, bias)
         if any(ctx.needs_input_grad):
-            ctx.save_for_backward(x, weight, labels, bias, lse, rows)
+            ctx.save_for_backward(x, weight, labels, bias, saved)
             ctx.desc, ctx.engine, ctx.params = d, engine, (weight, bias)
         return loss if reduction == 0 else loss.view(())
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, weight, labels, bias, lse, rows = ctx.saved_tensors
+        x, weight, labels, bias, saved = ctx.saved_tensors
         want, eng = ctx.needs_input_grad, ctx.engine
-        dx, dw, db = ops._linear_ce_bwd(ctx.desc, x, weight, labels, bias, lse, rows, dloss.contiguous(), (want[0], want[1], want[3]))
+        dx, dw, db = ops._linear_ce_bwd(ctx.desc, x, weight, labels, bias, saved, dloss.contiguous(), (want[0], want[1], want[3]))
         wp, bp = ctx.params
         if eng is not None and eng.flat_grad is not None and id(wp) in eng.grad_views:
             eng._bind_grads()
@@ -52,8 +52,9 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
         raise Vc3dError("linear_cross_entropy: x [..., D], weight [V][D] and labels [...] expected, got %s, %s, %s" %
                         (tuple(x.shape), tuple(weight.shape), tuple(labels.shape)))
     shape = labels.shape
-    x2 = ops._rows(x.reshape(-1, x.shape[-1]))
-    loss = _LinearCEFn.apply(x2, ops._rows(weight), labels.reshape(-1).contiguous(), None if bias is None else bias.contiguous(),
+    if x.dim() != 2:
+        x, labels = x.reshape(-1, x.shape[-1]), labels.reshape(-1)
+    loss = _LinearCEFn.apply(ops._rows(x), ops._rows(weight), labels.contiguous(), None if bias is None else bias.contiguous(),
                              int(ignore_index), _REDUCTION[reduction], None)
     return loss.view(shape) if reduction == "none" else loss
 

@@ -718,7 +718,9 @@ def _same_device(ref, **others):
 
 def _rows(t):
     """a matrix whose last dimension is contiguous and whose rows do not overlap: as it is, or a copy"""
-    return t if (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+    if t.is_contiguous() or (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+        return t
+    return t.contiguous()
 
 
 def _ld(t):
@@ -746,40 +748,36 @@ def _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction):
 
 def linear_ce_fwd(x, weight, labels, bias=None, ignore_index=-100, reduction=1):
     """cross-entropy of x weight^T + bias against labels, the vocabulary in pieces (vc_linear_ce_fwd); reduction 0 none, 1 mean
-    over the rows that count, 2 sum -> (loss [1] or [N], lse [N], rows): lse and rows are what linear_ce_bwd takes.
-    x [N][D] and weight [V][D] have contiguous rows (_rows), bias and labels are contiguous."""
+    over the rows that count, 2 sum -> (loss [1] or [N], saved): saved (bytes) is what linear_ce_bwd of the same tensors takes.
+    x [N][D] and weight [V][D] have contiguous rows, bias and labels are contiguous."""
     return _linear_ce_fwd(_linear_ce_desc(x, weight, labels, bias, ignore_index, reduction), x, weight, labels, bias)
 
 
 def _linear_ce_fwd(d, x, weight, labels, bias):
-    N, red, dev = d.N, d.reduction, x.device
+    N, dev = d.N, x.device
     with _on(x):
-        loss = torch.empty(1 if red else N, dtype=F32, device=dev)
-        lse = torch.empty(N, dtype=F32, device=dev)
-        rows = torch.empty(N + 4, dtype=torch.int32, device=dev)
+        loss = torch.empty(1 if d.reduction else N, dtype=F32, device=dev)
         if N == 0:
-            return loss.zero_(), lse, rows
+            return loss.zero_(), torch.empty(0, dtype=torch.uint8, device=dev)
+        saved = torch.empty(lib.vc_linear_ce_saved_bytes(d), dtype=torch.uint8, device=dev)
         need = lib.vc_linear_ce_workspace_bytes(d, 0)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        at = loss.data_ptr()
-        check(lib.vc_linear_ce_fwd(d, x.data_ptr(), weight.data_ptr(), ptr(bias), labels.data_ptr(), at if red else None, None if red else at,
-                                   lse.data_ptr(), rows.data_ptr(), ws.data_ptr(), need, cur_stream()), "vc_linear_ce_fwd")
-    return loss, lse, rows
+        check(lib.vc_linear_ce_fwd(d, x.data_ptr(), weight.data_ptr(), ptr(bias), labels.data_ptr(), loss.data_ptr(), saved.data_ptr(),
+                                   ws.data_ptr(), need, cur_stream()), "vc_linear_ce_fwd")
+    return loss, saved
 
 
-def linear_ce_bwd(x, weight, labels, bias, lse, rows, dloss, ignore_index=-100, reduction=1, want=(True, True, True)):
+def linear_ce_bwd(x, weight, labels, bias, saved, dloss, ignore_index=-100, reduction=1, want=(True, True, True)):
     """gradients of linear_ce_fwd's loss with respect to (x, weight, bias), those that `want` names -> contiguous tensors of
     x's type, or None (vc_linear_ce_bwd)"""
     d = _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction)
-    N = x.shape[0]
-    _chk(lse, F32, N, "lse")
-    _chk(rows, torch.int32, N + 4, "rows")
-    _chk(dloss, F32, N if reduction == 0 else 1, "dloss")
-    _same_device(x, lse=lse, rows=rows, dloss=dloss)
-    return _linear_ce_bwd(d, x, weight, labels, bias, lse, rows, dloss, want)
+    _chk(saved, torch.uint8, lib.vc_linear_ce_saved_bytes(d) if d.N else 0, "saved")
+    _chk(dloss, F32, d.N if reduction == 0 else 1, "dloss")
+    _same_device(x, saved=saved, dloss=dloss)
+    return _linear_ce_bwd(d, x, weight, labels, bias, saved, dloss, want)
 
 
-def _linear_ce_bwd(d, x, weight, labels, bias, lse, rows, dloss, want):
+def _linear_ce_bwd(d, x, weight, labels, bias, saved, dloss, want):
     dt, dev = x.dtype, x.device
     with _on(x):
         dx = torch.empty((d.N, d.D), dtype=dt, device=dev) if want[0] else None
@@ -789,8 +787,8 @@ def _linear_ce_bwd(d, x, weight, labels, bias, lse, rows, dloss, want):
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
         need = lib.vc_linear_ce_workspace_bytes(d, 1)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        check(lib.vc_linear_ce_bwd(d, x.data_ptr(), weight.data_ptr(), ptr(bias), labels.data_ptr(), lse.data_ptr(), rows.data_ptr(),
-                                   dloss.data_ptr(), ptr(dx), ptr(dw), ptr(db), ws.data_ptr(), need, cur_stream()), "vc_linear_ce_bwd")
+        check(lib.vc_linear_ce_bwd(d, x.data_ptr(), weight.data_ptr(), ptr(bias), labels.data_ptr(), saved.data_ptr(), dloss.data_ptr(),
+                                   ptr(dx), ptr(dw), ptr(db), ws.data_ptr(), need, cur_stream()), "vc_linear_ce_bwd")
     return dx, dw, db
 
 
