@@ -351,8 +351,9 @@ int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, flo
  * ignore_index take no part: loss 0, gradient 0, x not read.  Any other label outside [0, V) makes that row's loss NaN (as
  * vc_softmax_ce does).  reduction: 0 none, 1 mean over the rows that count (0 if none does), 2 sum.
  * loss: [1], or [N] with reduction 0.  saved (vc_linear_ce_saved_bytes, 256-byte aligned) is written by the forward and read by
- * the backward of the same x, w, bias and labels: the rows' logsumexp, the list of rows that count, and, up to 32 MB, their
- * copies.  dloss: fp32 on the device, [1], or [N] with reduction 0.  dx [N][D], dw [V][D], db [V] (each nullable) are contiguous
+ * the backward of the same x, w, bias and labels: the rows' logsumexp, the list of rows that count, up to 32 MB of
+ * copies of them, and, where that is quicker than to compute the logits again and takes at most keep_bytes (-1: 2 GB), their N x V
+ * exponentials in x's type (keep_bytes 0: never; > 0: wherever they fit).  The backward may be called again.  dloss: fp32 on the device, [1], or [N] with reduction 0.  dx [N][D], dw [V][D], db [V] (each nullable) are contiguous
  * and of x's type, and are written, not added to.  workspace (required, 256-byte aligned): vc_linear_ce_workspace_bytes(d, op),
  * op 0 forward, 1 backward: of the N x V logits the forward keeps two floats for every 64 .. 256, the backward one block of up
  * to 512 MB.  Results do not depend on the order in which workgroups run. */
@@ -360,6 +361,7 @@ typedef struct vc_linear_ce_desc {
     int32_t N, D, V, is_bf16;
     int32_t reduction, w_align; /* w's address modulo 16: rows that are no whole 16-byte chunks are copied, piece by piece */
     int64_t ldx, ldw, ignore_index;
+    int64_t keep_bytes;
 } vc_linear_ce_desc;
 size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op);
 size_t vc_linear_ce_saved_bytes(const vc_linear_ce_desc* d);

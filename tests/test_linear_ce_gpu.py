@@ -6,6 +6,9 @@ exp, of the sum over V terms and of log: de = (64 + V / 16) 2^-24 (the sum runs 
 by 2 dz + de + |loss| 2^-24, and a probability relatively by 2 dz + de.  P is rounded to the operands' type (half a step: h)
 before the products dw = P^T x and dx = P w, whose sums run in fp32 over K terms: with Pa = |p| + onehot, a gradient is off by
   Pa^T |x| (2 dz + de + h + (K + 8) 2^-24) + h |gradient|      (h = 2^-8 for bf16, 2^-24 for fp32).
+Where the forward keeps exponentials for the backward (keep_bytes), P is rounded twice (2 h + h^2), and is a product of two
+exponentials, each off by its argument times 2^-24: below 64 each in these tests wherever p is not below 2^-90.  db then sums the
+kept ones, rounded once, where it otherwise sums what no rounding has touched: h + h^2 beside the rest.
 What underflows: exp and the matrix instructions take values below 2^-126 for 0, so a probability may be off by 2^-126 beside
 all that, a gradient by K 2^-126 max|x| and itself by 2^-126 (words of a probability of 1e-39 show it)."""
 import pytest
@@ -33,10 +36,21 @@ def check(got, want, tol, what):
         what, int(bad.sum()), float(err[bad].max()), float(tol.expand_as(err)[bad][err[bad].argmax()]))
 
 
-def run_and_check(x, w, b, y, reduction="mean", ignore=-100, dloss=None, f=None):
+ALL = 1 << 40
+
+
+def run_and_check(*args, keep=(0, ALL), **kw):
+    """without and with kept exponentials"""
+    for k in keep:
+        out = run_and_check_one(*args, keep_bytes=k, **kw)
+    return out
+
+
+def run_and_check_one(x, w, b, y, reduction="mean", ignore=-100, dloss=None, keep_bytes=0):
     import vc3d
     leaves = [t.detach().requires_grad_() for t in (x, w) + ((b,) if b is not None else ())]
-    loss = (f or vc3d.linear_cross_entropy)(leaves[0], leaves[1], y, leaves[2] if b is not None else None, ignore_index=ignore, reduction=reduction)
+    loss = vc3d.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2] if b is not None else None, ignore_index=ignore, reduction=reduction,
+                                     keep_bytes=keep_bytes)
     if dloss is None:
         dloss = torch.ones_like(loss)
     grads = torch.autograd.grad(loss, leaves, dloss)
@@ -66,13 +80,16 @@ def run_and_check(x, w, b, y, reduction="mean", ignore=-100, dloss=None, f=None)
     hot = torch.zeros_like(p).scatter_(1, at[:, None], 1.0)
     P, Pa, rel = (p - hot) * gn[:, None], (p + hot) * gn.abs()[:, None], (2 * dz + de + 4 * E)[:, None]
     h = HALF[x.dtype]
+    hp = h
+    if keep_bytes:
+        hp, rel = 2 * h + h * h, rel + 128 * E
     dx, dw = P @ W, P.t() @ X
-    check(grads[0], dx, (Pa * (rel + h + (V + 8) * E)) @ W.abs() + h * dx.abs() + UNDER * (1 + V * float(W.abs().max())), "dx")
-    check(grads[1], dw, (Pa * (rel + h + (N + 8) * E)).t() @ X.abs() + h * dw.abs() + UNDER * (1 + N * float(X.abs().max())), "dw")
+    check(grads[0], dx, (Pa * (rel + hp + (V + 8) * E)) @ W.abs() + h * dx.abs() + UNDER * (1 + V * float(W.abs().max())), "dx")
+    check(grads[1], dw, (Pa * (rel + hp + (N + 8) * E)).t() @ X.abs() + h * dw.abs() + UNDER * (1 + N * float(X.abs().max())), "dw")
     assert not bool(grads[0][~keep].any())
     if b is not None:
         db = P.sum(0)
-        check(grads[2], db, (Pa * (rel + (N + 8) * E)).sum(0) + h * db.abs() + UNDER * (1 + N), "db")
+        check(grads[2], db, (Pa * (rel + hp - h + (N + 8) * E)).sum(0) + h * db.abs() + UNDER * (1 + N), "db")
     return loss, grads
 
 
@@ -209,14 +226,76 @@ def test_gradient_against_differences():
     assert abs((value(eps) - value(-eps)) / (2 * eps) - slope) <= 2 * eps ** 2 + noise
 
 
-def test_streams_and_repeats_bit_for_bit():
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_kept_exponentials_that_do_not_fit_their_type(reduction, dtype):
+    """labels 44 nats and more behind another word, far enough that exp(z - z_label) overflows in one row: nothing of it is used"""
+    for far in (60.0, 300.0):
+        x, w, b, y = make(150, 64, 700, dtype, True, seed=20)
+        b[:] = torch.where(torch.arange(700, device="cuda") == 650, torch.tensor(far, dtype=dtype, device="cuda"), b)
+        y = torch.where(y == 650, y * 0, y)
+        run_and_check(x, w, b, y, reduction)
+        b[650] = 0
+        x[77], x[:, 0] = 0, 0
+        x[77, 0], w[650], w[650, 0], w[y[77], 0] = 8, 0, far / 8, 0  # one row alone
+        run_and_check(x, w, b, y, reduction)
+    y[3] = -100
+    y[4] = 5
+    b[5] = -float("inf")  # a label that is masked: loss inf, as torch has it
+    import vc3d
+    loss = vc3d.linear_cross_entropy(x.requires_grad_(), w, y, b, reduction="none", keep_bytes=ALL)
+    assert torch.equal(torch.isinf(loss), y == 5) and not bool(torch.isnan(loss).any())
+
+
+def test_bad_labels_and_values_with_kept_exponentials():
+    import vc3d
+    x, w, b, y = make(40, 64, 300, torch.bfloat16, False, seed=5)
+    y[3], y[5], y[7] = 300, -1, -100
+    x[9, 3], x[7] = float("inf"), float("nan")
+    got = []
+    for keep in (0, ALL):
+        leaves = [t.detach().clone().requires_grad_() for t in (x, w)]
+        loss = vc3d.linear_cross_entropy(leaves[0], leaves[1], y, reduction="none", keep_bytes=keep)
+        bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+        bad[3] = bad[5] = bad[9] = True
+        assert torch.equal(torch.isnan(loss), bad) and loss[7] == 0
+        dx, dw = torch.autograd.grad(loss.sum(), leaves)
+        assert torch.equal(torch.isnan(dx).any(1), bad) and not bool(dx[7].any())
+        got.append((loss, dx, dw))
+    assert torch.equal(torch.isnan(got[0][2]), torch.isnan(got[1][2]))
+
+
+def test_what_is_kept():
+    """the rule, the limit, nothing without a backward; a backward that is called twice"""
+    import vc3d
+    x, w, b, y = make(256, 512, 1 << 14, torch.bfloat16, False, seed=21)
+    size = [vc3d.ops.linear_ce_fwd(x, w, y, keep_bytes=k)[1].numel() for k in (0, -1, 1 << 23, (1 << 23) - 1)]
+    assert size[1] == size[2] == size[0] + (1 << 23) + 2 * 1024 and size[3] == size[0]
+    assert vc3d.ops.linear_ce_fwd(x[:, :256], w[:, :256], y)[1].numel() < 1 << 20  # short rows: quicker computed again
+    leaves = [t.requires_grad_() for t in (x, w)]
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        loss = vc3d.linear_cross_entropy(x, w, y)
+    torch.cuda.reset_peak_memory_stats()
+    with torch.no_grad():
+        loss = vc3d.linear_cross_entropy(x, w, y)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 22
+    loss = vc3d.linear_cross_entropy(x, w, y)
+    first = torch.autograd.grad(loss, leaves, retain_graph=True)
+    again = torch.autograd.grad(loss, leaves)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("keep", [0, ALL])
+def test_streams_and_repeats_bit_for_bit(keep):
     import vc3d
     x, w, b, y = make(700, 128, 3000, torch.bfloat16, True, seed=12)
     y[::7] = -100
     leaves = [t.requires_grad_() for t in (x, w, b)]
 
     def once():
-        loss = vc3d.linear_cross_entropy(x, w, y, b)
+        loss = vc3d.linear_cross_entropy(x, w, y, b, keep_bytes=keep)
         return (loss.detach(),) + torch.autograd.grad(loss, leaves)
     want = once()
     streams = [torch.cuda.Stream() for _ in range(3)]
@@ -230,14 +309,15 @@ def test_streams_and_repeats_bit_for_bit():
         assert all(torch.equal(a, b) for a, b in zip(want, g))
 
 
-def test_captured_graphs_replay():
+@pytest.mark.parametrize("keep", [0, ALL])
+def test_captured_graphs_replay(keep):
     import vc3d
     x, w, b, y = make(300, 128, 1500, torch.bfloat16, True, seed=13)
     one = torch.ones(1, device="cuda")
 
     def once(y):
-        loss, saved = vc3d.ops.linear_ce_fwd(x, w, y, b)
-        return (loss,) + vc3d.ops.linear_ce_bwd(x, w, y, b, saved, one)
+        loss, saved = vc3d.ops.linear_ce_fwd(x, w, y, b, keep_bytes=keep)
+        return (loss,) + vc3d.ops.linear_ce_bwd(x, w, y, b, saved, one, keep_bytes=keep)
     ins = [y.clone(), y.flip(0).contiguous()]
     s = torch.cuda.Stream()
     with torch.cuda.stream(s):

@@ -68,7 +68,7 @@ def test_c_entry_of_the_scan_refuses():
 
 def test_c_entry_of_the_linear_cross_entropy_refuses():
     c = _capi()
-    base = dict(N=100, D=64, V=1000, is_bf16=1, reduction=1, w_align=0, ldx=64, ldw=64, ignore_index=-100)
+    base = dict(N=100, D=64, V=1000, is_bf16=1, reduction=1, w_align=0, ldx=64, ldw=64, ignore_index=-100, keep_bytes=-1)
     ok = lambda **k: c.LinearCeDesc(**{**base, **k})  # noqa: E731
     need = c.lib.vc_linear_ce_workspace_bytes
     big = 1 << 30
@@ -77,14 +77,15 @@ def test_c_entry_of_the_linear_cross_entropy_refuses():
     bwd = lambda d, x=PTR, w=PTR, b=None, y=PTR, saved=PTR, g=PTR, db=None, ws=PTR, n=big: c.lib.vc_linear_ce_bwd(  # noqa: E731
         d, x, w, b, y, saved, g, PTR, PTR, db, ws, n, None)
     for bad in (None, ok(N=0), ok(D=0), ok(V=0), ok(N=(1 << 23) + 1), ok(V=(1 << 23) + 1), ok(ldx=63), ok(ldw=63), ok(reduction=3),
-                ok(reduction=-1), ok(w_align=16), ok(w_align=-1)):
+                ok(reduction=-1), ok(w_align=16), ok(w_align=-1), ok(keep_bytes=-2)):
         assert fwd(bad) == -2 and bwd(bad) == -2 and need(bad, 0) == 0 and c.lib.vc_linear_ce_saved_bytes(bad) == 0
     for bad in (dict(x=None), dict(w=None), dict(y=None), dict(saved=None), dict(saved=PTR + 16), dict(ws=None), dict(ws=PTR + 16), dict(n=16)):
         assert fwd(ok(), **bad) == -2 and bwd(ok(), **bad) == -2
     assert fwd(ok(), loss=None) == -2 and bwd(ok(), g=None) == -2 and bwd(ok(), db=PTR) == -2
     assert fwd(ok(), w=PTR + 2) == -2 and b"modulo 16" in c.lib.vc_last_error()  # the descriptor says that w is aligned
     # what is left for the backward: a few words a row, copies of x while they are small
-    assert c.lib.vc_linear_ce_saved_bytes(ok()) >= 100 * 8 + 100 * 128 and c.lib.vc_linear_ce_saved_bytes(ok(N=1 << 20, D=512, ldx=512, ldw=512)) < 16 << 20
+    assert c.lib.vc_linear_ce_saved_bytes(ok()) >= 100 * 8 + 100 * 128 and c.lib.vc_linear_ce_saved_bytes(ok(N=1 << 20, D=512, ldx=512, ldw=512, keep_bytes=0)) < 16 << 20
+    assert c.lib.vc_linear_ce_saved_bytes(ok(keep_bytes=1 << 20)) >= 256 * 1024 * 2
     # no N x V block: one piece's P, sums of dx, a pair for every row and tile
     n = need(ok(N=8192, D=2048, V=1 << 20, ldx=2048, ldw=2048), 1)
     assert n < 1.2e9 and n < 8192 * (1 << 20) * 2 / 10

@@ -1297,15 +1297,17 @@ static int lce_check(const vc_linear_ce_desc* d) {
     VC_REQUIRE(d->N <= (1 << 23) && d->V <= (1 << 23) && d->D <= (1 << 20), "linear_ce: at most 2^23 rows and classes, 2^20 features");
     VC_REQUIRE(d->ldx >= d->D && d->ldw >= d->D, "linear_ce: row strides %lld, %lld below D=%d", (long long)d->ldx, (long long)d->ldw, d->D);
     VC_REQUIRE(d->w_align >= 0 && d->w_align < 16, "linear_ce: w_align %d is no address modulo 16", d->w_align);
+    VC_REQUIRE(d->keep_bytes >= -1, "linear_ce: keep_bytes %lld", (long long)d->keep_bytes);
     VC_REQUIRE(d->reduction >= 0 && d->reduction <= 2, "linear_ce: reduction %d (0 none, 1 mean, 2 sum)", d->reduction);
     return 0;
 }
+static bool lce_keep(const vc_linear_ce_desc* d) { return vc_lce_keep(d->N, d->D, d->V, d->is_bf16 != 0, d->keep_bytes); }
 static bool lce_pack(const vc_linear_ce_desc* d) { return vc_lce_pack(d->D, d->ldw, d->w_align, d->is_bf16 != 0); }
 size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op) {
     if (lce_check(d) != 0) return 0;
     return vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, lce_pack(d), op);
 }
-size_t vc_linear_ce_saved_bytes(const vc_linear_ce_desc* d) { return lce_check(d) != 0 ? 0 : vc_lce_saved(d->N, d->D, d->is_bf16 != 0); }
+size_t vc_linear_ce_saved_bytes(const vc_linear_ce_desc* d) { return lce_check(d) != 0 ? 0 : vc_lce_saved(d->N, d->D, d->V, d->is_bf16 != 0, lce_keep(d)); }
 // what both directions ask of their arguments
 static int lce_args(const char* name, const vc_linear_ce_desc* d, const void* x, const void* w, const int64_t* labels, const void* saved, const void* ws,
                     size_t ws_bytes, int op) {
@@ -1323,7 +1325,7 @@ static VcLceParams lce_params(const vc_linear_ce_desc* d, const void* x, const v
     memset(&p, 0, sizeof(p));
     p.N = d->N, p.D = d->D, p.V = d->V, p.ldx = d->ldx, p.ldw = d->ldw;
     p.x = x, p.w = w, p.bias = bias, p.labels = (const long long*)labels, p.ignore_index = d->ignore_index, p.reduction = d->reduction;
-    p.pack = lce_pack(d), p.saved = saved, p.ws = ws;
+    p.pack = lce_pack(d), p.keep = lce_keep(d), p.saved = saved, p.ws = ws;
     return p;
 }
 int vc_linear_ce_fwd(const vc_linear_ce_desc* d, const void* x, const void* w, const void* bias, const int64_t* labels, float* loss,

@@ -234,6 +234,7 @@ struct VcLceParams {
     long long ignore_index;
     int reduction;  // 0 none, 1 mean, 2 sum
     bool pack;      // the products read a copy of w
+    bool keep;      // the forward keeps exponentials for the backward
     float* loss;       // forward: [1], nullable with reduction 0
     float* loss_rows;  // forward: [N], nullable unless reduction is 0
     void* saved;       // what the forward leaves for the backward
@@ -246,7 +247,8 @@ struct VcLceParams {
     size_t ws_bytes;
 };
 bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16);
-size_t vc_lce_saved(int N, int D, bool is_bf16);
+bool vc_lce_keep(int N, int D, int V, bool is_bf16, long long keep_bytes);
+size_t vc_lce_saved(int N, int D, int V, bool is_bf16, bool keep);
 size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int op);
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s);
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s);

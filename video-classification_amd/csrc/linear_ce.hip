@@ -41,7 +41,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(const long long* labels, lon
         __syncthreads();
         base = base_sh;
     }
-    if (tid == 0) rows[N] = base, rows[N + 1] = 0;  // (their number; workgroups of lce_rows_kernel that are done)
+    if (tid == 0) rows[N] = base, rows[N + 1] = 0, rows[N + 2] = 0;  // (their number; workgroups of lce_rows_kernel that are done; EPI_KEEP gave up)
 }
 
 // ---------------------------------------------------------------- matrix products
@@ -64,7 +64,7 @@ struct Operand {
     long long ld;  // bytes from row to row (k contiguous) or from k to k (k across), below 2^32
 };
 
-enum { EPI_STATS, EPI_PROB, EPI_DX, EPI_DW };
+enum { EPI_STATS, EPI_KEEP, EPI_PROB, EPI_DX, EPI_DW };
 
 // the factor common to all rows
 struct Factor {
@@ -96,7 +96,8 @@ struct Gemm {
     const int* k_dev;   // nullable: K is *k_dev
     int rtiles;
     Splits splits;  // EPI_DX
-    // EPI_STATS / EPI_PROB: r = word v0 + r, s = listed row
+    const int* when;  // nullable: nothing is done where *when is 0
+    // EPI_STATS / EPI_KEEP / EPI_PROB: r = word v0 + r, s = listed row
     const void* bias;
     const long long* labels;
     const int* rows;
@@ -104,6 +105,8 @@ struct Gemm {
     float2* part;  // [s][part_ld], this launch's tiles from part0 on
     int part_ld, part0;
     float* zlab;   // [s]: logit of the row's label
+    const float* ref;  // EPI_KEEP: [s], what a row's exponentials are taken relative to
+    int* gave_up;      // EPI_KEEP
     const float* lse;
     const float* scale;  // nullable: [N], each row's own factor
     void* P;
@@ -217,7 +220,7 @@ struct Tile {
 // fits; with k across four buffers of one fragment.
 template <int EPI, int B>
 struct Feed {
-    static constexpr bool ROWS_OF_K = EPI == EPI_STATS || EPI == EPI_PROB;
+    static constexpr bool ROWS_OF_K = EPI == EPI_STATS || EPI == EPI_KEEP || EPI == EPI_PROB;
     static constexpr int SUBS = ROWS_OF_K || B == 64 ? 2 : 1, RING = ROWS_OF_K && B > 64 ? 2 : 4;
 };
 
@@ -230,6 +233,7 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     typedef Tile<T, BS, SUBS, NTHR, SK> TS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int BUF = TR::BYTES + TS::BYTES;
+    if (g.when != nullptr && *g.when == 0) return;
     const int ns = __builtin_amdgcn_readfirstlane(g.ns_dev != nullptr ? *g.ns_dev : g.ns);
     const int K = __builtin_amdgcn_readfirstlane(g.k_dev != nullptr ? *g.k_dev : g.K);
     // tile order: XCD x (workgroups go round the 8 XCDs) takes the x-th share of an order in which 4 tiles of s by all tiles of r
@@ -343,7 +347,7 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
             }
     }
     // acc[a][b][j] = out[s = s0 + wsx + 16 b + l15][r = r0 + wr + 16 a + 4 lg + j]
-    if constexpr (EPI == EPI_STATS || EPI == EPI_PROB) {
+    if constexpr (EPI == EPI_STATS || EPI == EPI_KEEP || EPI == EPI_PROB) {
         const bool edge = r0 + BR > g.nr;
         if (g.bias != nullptr || edge)
 #pragma unroll
@@ -364,24 +368,55 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
         return __builtin_amdgcn_exp2f(direct ? __builtin_fmaf(z, LOG2E, -ref2) : (z - ref) * LOG2E);
     };
     auto direct = [&](float ref) { return sizeof(T) == 2 && __all(!(fabsf(ref) > 1e30f)); };
-    if constexpr (EPI == EPI_STATS) {
+    if constexpr (EPI == EPI_STATS || EPI == EPI_KEEP) {
         __syncthreads();  // (the tiles have been read)
         float2* const join = (float2*)smem;  // [WR][BS]
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const int s = s0 + wsx + b * 16 + l15;
             const long long label = s < ns ? g.labels[g.rows[s]] - g.v0 - r0 - wr : -1;
-            float m = acc[0][b][0], e = 0.f;
-#pragma unroll
-            for (int a = 0; a < NA; ++a)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) m = fmaxf(m, acc[a][b][j]);
+            float m, e = 0.f;
             if (__any(label >= 0 && label < BR / WR))  // (a wave in V / 128 has a row's label)
 #pragma unroll
                 for (int a = 0; a < NA; ++a)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (label == a * 16 + lg * 4 + j) g.zlab[s] = acc[a][b][j];
+            // EPI_KEEP: exponentials relative to the row's own label, stored; their sum is the tile's.  A row whose label is 44 nats
+            // or more behind some word (or no word, or not finite) has the pass over its logits made as if nothing were kept.
+            if constexpr (EPI == EPI_KEEP) {
+                m = s < ns ? g.ref[s] : 0.f;
+                bool ok = __all(fabsf(m) <= 1e30f);
+                if (ok) {
+                    const float ref2 = m * LOG2E;
+                    T* const row = (T*)g.P + (long long)s * g.ldp + r0 + wr + lg * 4;
+#pragma unroll
+                    for (int a = 0; a < NA; ++a) {
+                        f32x4 v;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = ex(acc[a][b][j], m, ref2, sizeof(T) == 2);
+                        e += (v[0] + v[1]) + (v[2] + v[3]);
+                        if (s < ns) {
+                            if constexpr (sizeof(T) == 2) *(bf16x4*)(row + a * 16) = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
+                            else *(f32x4*)(row + a * 16) = v;
+                        }
+                    }
+                    e += __shfl_xor(e, 16, 64);
+                    e += __shfl_xor(e, 32, 64);
+                    ok = __all(s >= ns || e < 0x1p64f);
+                }
+                if (ok) {
+                    if (lg == 0) join[(wave % WR) * BS + wsx + b * 16 + l15] = make_float2(m, e);
+                    continue;
+                }
+                if (lane == 0) __hip_atomic_store(g.gave_up, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                e = 0.f;
+            }
+            m = acc[0][b][0];
+#pragma unroll
+            for (int a = 0; a < NA; ++a)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) m = fmaxf(m, acc[a][b][j]);
             m = fmaxf(m, __shfl_xor(m, 16, 64));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
             const float ref = m == -INFINITY ? 0.f : m, ref2 = ref * LOG2E;
@@ -526,10 +561,18 @@ __global__ __launch_bounds__(256) void lce_words_of_w_kernel(const T* w, long lo
 }
 // the rows of x that count, one after the other (13 us of the 7 ms of 8192 x 2048 x 65536; the products then read x in order,
 // with k across too, and never a row that does not count).  LIST: the list itself is made here too: every workgroup counts the
-// labels before its row (short batches: one launch instead of two)
+// labels before its row (short batches: one launch instead of two).  With ref: ref[i] = the logit of the row's label, or inf where
+// that is no word or none that exponentials can be relative to.
+struct LabelLogit {
+    float* ref;  // nullable
+    const void* w;
+    long long ldw;
+    const void* bias;
+    int V;
+};
 template <typename T, bool VEC, bool LIST>
 __global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long long ldx, int* rows, const long long* labels, long long ignore,
-                                                            int N, int D, int ld, T* out) {
+                                                            int N, int D, int ld, T* out, LabelLogit q) {
     int i = blockIdx.x, n;
     if (LIST) {
         __shared__ int before_sh[4], all_sh[4];
@@ -549,7 +592,7 @@ __global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long lon
         i = before;
         if (threadIdx.x == 0) {
             rows[keep ? before : N - 1 - (n - before)] = n;
-            if (n == 0) rows[N] = all_sh[0] + all_sh[1] + all_sh[2] + all_sh[3], rows[N + 1] = 0;
+            if (n == 0) rows[N] = all_sh[0] + all_sh[1] + all_sh[2] + all_sh[3], rows[N + 1] = 0, rows[N + 2] = 0;
         }
         if (!keep) return;
     } else {
@@ -557,6 +600,21 @@ __global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long lon
         n = rows[i];
     }
     copy_row<T, VEC>(x + n * ldx, out + (long long)i * ld, D, ld, threadIdx.x, 256);
+    if (q.ref == nullptr) return;
+    __shared__ float sum_sh[4];
+    const long long y = labels[n];
+    const bool word = y >= 0 && y < q.V;
+    const T *const xr = x + n * ldx, *const wr = (const T*)q.w + (word ? y : 0) * q.ldw;
+    float s = 0.f;
+    for (int d = threadIdx.x; d < D; d += 256) s = __builtin_fmaf((float)xr[d], (float)wr[d], s);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) sum_sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = (sum_sh[0] + sum_sh[1]) + (sum_sh[2] + sum_sh[3]) + (q.bias != nullptr && word ? (float)((const T*)q.bias)[y] : 0.f);
+        q.ref[i] = word && fabsf(s) <= 1e30f ? s : INFINITY;
+    }
 }
 
 // ---------------------------------------------------------------- the small launches around it
@@ -564,7 +622,7 @@ __global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long lon
 // (It reads what the others wrote: their stores are device-scope atomics, complete before the workgroup counts itself done.)
 // 16 rows a workgroup: workgroups count themselves on one word, 15 ns each (4 rows: 34 us for 8192 rows, 16: 14 us)
 __global__ __launch_bounds__(1024) void lce_rows_kernel(const float2* part, int tiles, const float* zlab, const long long* labels,
-                                                       int* rows, int N, int V, float* lse, float* loss_rows, int mean, float* loss) {
+                                                       int* rows, int N, int V, float* lse, float* loss_rows, float* plab, int mean, float* loss) {
     __shared__ double sums[16];
     __shared__ int last;
     const int wave = threadIdx.x >> 6, i = blockIdx.x * 16 + wave, lane = threadIdx.x & 63, count = rows[N];
@@ -589,6 +647,7 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const float2* part, int 
             const bool ok = y >= 0 && y < V;
             l = ok ? m + logf(e) : NAN;  // (a label that is no word: NaN, as with vc_softmax_ce)
             loss_n = ok ? l - zlab[i] : NAN;
+            if (plab != nullptr && lane == 0) plab[i] = expm1f(-loss_n);  // P at the label: p - 1
         }
         if (lane == 0) {
             lse[n] = l;
@@ -619,6 +678,71 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const float2* part, int 
         s = 0.0;
         for (int w = 0; w < 16; ++w) s += sums[w];
         loss[0] = (float)(mean ? s / (double)(count > 0 ? count : 1) : s);
+    }
+}
+// P of a piece from what EPI_KEEP stored: E[s][v] exp(ref_s - lse_s), at the label its own value; db's partial sums.  A workgroup
+// takes a row tile by 64 chunks of 16 bytes, a wave a quarter of the rows.
+// (a second rounding of P, half a step of what the first left, for not computing the logits again)
+template <typename T>
+__global__ __launch_bounds__(256) void lce_kept_kernel(const T* E, long long lde, T* P, long long ldp, const int* rows, const float* lse, const float* ref,
+                                                       const float* plab, const long long* labels, const float* scale, int N, int v0, int nv, int tile,
+                                                       float* dbpart) {
+    constexpr int PER = 16 / (int)sizeof(T);
+    typedef T chunk_t __attribute__((ext_vector_type(PER)));
+    __shared__ float by[256], at[256];
+    __shared__ int label[256];
+    __shared__ float sums[4][64][PER + 1];
+    const int count = rows[N], s0 = blockIdx.y * tile, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    if (s0 >= count || rows[N + 2] != 0) return;
+    if (tid < tile) {
+        const int s = s0 + tid;
+        const bool in = s < count;
+        const int n = in ? rows[s] : 0;
+        const float f = scale != nullptr && in ? scale[n] : 1.f;
+        const long long y = in ? labels[n] - v0 : -1;
+        by[tid] = in ? __expf(ref[s] - lse[n]) * f : 0.f;
+        at[tid] = in ? plab[s] * f : 0.f;
+        label[tid] = y >= 0 && y < nv ? (int)y : -PER;
+    }
+    __syncthreads();
+    const int col = (blockIdx.x * 64 + lane) * PER;
+    float cs[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) cs[j] = 0.f;
+    if (col < nv) {
+        const T* const from = E + (long long)s0 * lde + v0 + col;
+        T* const to = P + (long long)s0 * ldp + col;
+        const int each = tile / 4;
+        for (int k0 = wave * each; k0 < (wave + 1) * each; k0 += 8) {
+            chunk_t v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = s0 + k0 + k < count ? *(const chunk_t*)(from + (k0 + k) * lde) : (chunk_t)(T)0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float c = by[k0 + k];
+                const int l = label[k0 + k] - col;
+                float f[PER];
+#pragma unroll
+                for (int j = 0; j < PER; ++j) f[j] = (float)v[k][j] * c;
+                if (l >= 0 && l < PER) {
+                    const float p = at[k0 + k];
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) f[j] = j == l ? p : f[j];
+                }
+                chunk_t o;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) cs[j] += f[j], o[j] = (T)f[j];
+                *(chunk_t*)(to + (k0 + k) * ldp) = o;
+            }
+        }
+    }
+    if (dbpart == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sums[wave][lane][j] = cs[j];
+    __syncthreads();
+    for (int c = tid; c < 64 * PER; c += 256) {
+        const int l = c / PER, j = c % PER, at_ = blockIdx.x * 64 * PER + c;
+        if (at_ < nv) dbpart[(long long)blockIdx.y * ldp + at_] = (sums[0][l][j] + sums[1][l][j]) + (sums[2][l][j] + sums[3][l][j]);
     }
 }
 // what is stored last: workgroup i < N the row i of the list of dx (its splits' sums; zeros for a row that does not count), the
@@ -684,6 +808,7 @@ struct Plan {
     int kd;                      // features, in whole 16-byte chunks
     int ld;                      // row length of copies of x, w: whole 128-byte lines
     size_t acc, P, dbpart, part, zlab, loss_rows, xp, wp;
+    long long lde;               // row length of what EPI_KEEP stores
     size_t take(size_t n) {
         const size_t at = bytes;
         bytes += (n + 255) & ~(size_t)255;
@@ -695,7 +820,12 @@ struct Plan {
     // what the forward leaves for the backward: lse [N], the list [N + 4], the copy of x
     static size_t list_at(int N) { return ((size_t)N * 4 + 255) & ~(size_t)255; }
     static size_t x_at(int N) { return list_at(N) + ((((size_t)N + 4) * 4 + 255) & ~(size_t)255); }
-    static size_t saved(int N, int D, int elem) { return x_at(N) + (saves_x(N, D, elem) ? (size_t)N * row(D, elem) * elem : 0); }
+    static size_t ref_at(int N, int D, int elem) { return x_at(N) + (((saves_x(N, D, elem) ? (size_t)N * row(D, elem) * elem : 0) + 255) & ~(size_t)255); }
+    // with `keep` also: ref [N], P at the label [N], the exponentials
+    static size_t plab_at(int N, int D, int elem) { return ref_at(N, D, elem) + list_at(N); }
+    static size_t exps_at(int N, int D, int elem) { return plab_at(N, D, elem) + list_at(N); }
+    static size_t exps(int N, int V, int elem) { return ((size_t)N + 255) / 256 * 256 * (((size_t)V + 255) / 256 * 256) * elem; }
+    static size_t saved(int N, int D, int V, int elem, bool keep) { return keep ? exps_at(N, D, elem) + exps(N, V, elem) : ref_at(N, D, elem); }
     Plan(int N, int D, int V, int elem, int op, bool pack) {
         kd = (D * elem + 15) / 16 * 16 / elem;
         ld = row(D, elem);
@@ -703,6 +833,7 @@ struct Plan {
         long long fit = (512ll << 20) / elem / np / 256 * 256;
         if (pack && op == 0) fit = (512ll << 20) / elem / ld / 256 * 256;  // (the forward holds a piece of w only)
         fit = fit < 256 ? 256 : fit;
+        lde = all;
         piece = (int)(op == 0 && !pack ? all : fit < all ? fit : all);
         tile = pick_tile(N, piece < V ? piece : V);
         tiles = (int)(((long long)V + tile - 1) / tile);
@@ -764,12 +895,16 @@ struct Source {
     hipStream_t s;
     Operand x;
     static bool chunks(const void* q, long long ld, int D) { return (((uintptr_t)q | (uintptr_t)(ld * sizeof(T)) | (uintptr_t)(D * sizeof(T))) & 15) == 0; }
-    float* lse;
+    float *lse, *ref, *plab;
     int* rows;
+    T* exps;
     Source(const VcLceParams& p, const Plan& L, hipStream_t s, bool forward) : p(p), L(L), s(s) {
         char* const saved = (char*)p.saved;
         const bool kept = Plan::saves_x(p.N, p.D, sizeof(T));
         lse = (float*)saved, rows = (int*)(saved + Plan::list_at(p.N));
+        ref = p.keep ? (float*)(saved + Plan::ref_at(p.N, p.D, sizeof(T))) : nullptr;
+        plab = p.keep ? (float*)(saved + Plan::plab_at(p.N, p.D, sizeof(T))) : nullptr;
+        exps = p.keep ? (T*)(saved + Plan::exps_at(p.N, p.D, sizeof(T))) : nullptr;
         T* const to = (T*)(kept ? saved + Plan::x_at(p.N) : (char*)p.ws + L.xp);
         x = {(const char*)to, L.ld * (long long)sizeof(T)};
         if (!forward && kept) return;
@@ -777,7 +912,8 @@ struct Source {
         if (forward && !list) hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, s, p.labels, p.ignore_index, p.N, rows);
         const auto kernel = list ? (vec ? lce_rows_of_x_kernel<T, true, true> : lce_rows_of_x_kernel<T, false, true>)
                                  : (vec ? lce_rows_of_x_kernel<T, true, false> : lce_rows_of_x_kernel<T, false, false>);
-        hipLaunchKernelGGL(kernel, dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, rows, p.labels, p.ignore_index, p.N, p.D, L.ld, to);
+        const LabelLogit q = {forward ? ref : nullptr, p.w, p.ldw, p.bias, p.V};
+        hipLaunchKernelGGL(kernel, dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, rows, p.labels, p.ignore_index, p.N, p.D, L.ld, to, q);
     }
     Operand w(int v0, int nv) const {
         const T* at = (const T*)p.w + v0 * p.ldw;
@@ -803,10 +939,14 @@ int fwd(const VcLceParams& p, hipStream_t s) {
         g.nr = p.V - v0 < L.piece ? p.V - v0 : L.piece, g.ns_dev = src.rows + p.N, g.K = L.kd;
         g.R = src.w(v0, g.nr), g.S = src.x;
         g.bias = p.bias, g.labels = p.labels, g.rows = src.rows, g.v0 = v0, g.part = part, g.part_ld = L.tiles, g.part0 = v0 / L.tile, g.zlab = zlab;
-        gemm<T, EPI_STATS>(g, L.tile, p.N, 1, s);
+        if (p.keep) {
+            g.ref = src.ref, g.gave_up = src.rows + p.N + 2, g.P = src.exps + v0, g.ldp = L.lde;
+            gemm<T, EPI_KEEP>(g, L.tile, p.N, 1, s);
+        } else
+            gemm<T, EPI_STATS>(g, L.tile, p.N, 1, s);
     }
     hipLaunchKernelGGL(lce_rows_kernel, dim3((p.N + 15) / 16), dim3(1024), 0, s, part, L.tiles, zlab, p.labels, src.rows, p.N, p.V, src.lse,
-                       loss_rows, p.reduction == 1, p.reduction != 0 ? p.loss : nullptr);
+                       loss_rows, src.plab, p.reduction == 1, p.reduction != 0 ? p.loss : nullptr);
     return launched("linear_ce_fwd");
 }
 
@@ -828,6 +968,11 @@ int bwd(const VcLceParams& p, hipStream_t s) {
         g.nr = nv, g.ns_dev = count, g.K = L.kd;
         g.bias = p.bias, g.labels = p.labels, g.rows = src.rows, g.v0 = v0;
         g.lse = src.lse, g.scale = p.reduction == 0 ? p.dloss : nullptr, g.P = ws + L.P, g.ldp = L.piece, g.dbpart = p.db != nullptr ? dbpart : nullptr;
+        if (p.keep) {
+            g.when = src.rows + p.N + 2;
+            hipLaunchKernelGGL((lce_kept_kernel<T>), dim3((nv * (int)sizeof(T) + 1023) / 1024, (p.N + L.tile - 1) / L.tile), dim3(256), 0, s, src.exps,
+                               L.lde, (T*)g.P, g.ldp, src.rows, src.lse, src.ref, src.plab, p.labels, g.scale, p.N, v0, nv, L.tile, g.dbpart);
+        }
         gemm<T, EPI_PROB>(g, L.tile, p.N, 1, s);
         if (p.dx != nullptr) {
             Gemm x = {};
@@ -859,7 +1004,12 @@ bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16) {
     const int elem = is_bf16 ? 2 : 4;
     return (D * elem) % 16 != 0 || (ldw * elem) % 16 != 0 || w_align != 0 || ldw * elem >= (1ll << 32);
 }
-size_t vc_lce_saved(int N, int D, bool is_bf16) { return Plan::saved(N, D, is_bf16 ? 2 : 4); }
+// Whether the forward keeps exp(z - ref) for the backward, which then need not compute the logits again.
+bool vc_lce_keep(int N, int D, int V, bool is_bf16, long long keep_bytes) {
+    const size_t bytes = Plan::exps(N, V, is_bf16 ? 2 : 4);
+    return keep_bytes >= 0 ? bytes <= (size_t)keep_bytes : bytes <= (size_t)2 << 30 && D >= 512 && (long long)N * V >= 1 << 22;
+}
+size_t vc_lce_saved(int N, int D, int V, bool is_bf16, bool keep) { return Plan::saved(N, D, V, is_bf16 ? 2 : 4, keep); }
 size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack).bytes; }
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? fwd<bf16>(p, s) : fwd<float>(p, s); }
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? bwd<bf16>(p, s) : bwd<float>(p, s); }

@@ -82,7 +82,7 @@ class ScanDesc(C.Structure):
 class LinearCeDesc(C.Structure):
     """vc_linear_ce_desc (include/vc3d.h)"""
     _fields_ = [(n, C.c_int32) for n in ("N", "D", "V", "is_bf16", "reduction", "w_align")] + \
-               [(n, C.c_int64) for n in ("ldx", "ldw", "ignore_index")]
+               [(n, C.c_int64) for n in ("ldx", "ldw", "ignore_index", "keep_bytes")]
 
 _CD = C.POINTER(ConvDesc)
 _PD = C.POINTER(PoolDesc)

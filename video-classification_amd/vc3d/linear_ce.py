@@ -13,8 +13,8 @@ class _LinearCEFn(torch.autograd.Function):
     """when ``engine`` is given, the gradients of weight and bias go to its flat buffer, as with autograd.linear_apply"""
 
     @staticmethod
-    def forward(ctx, x, weight, labels, bias, ignore_index, reduction, engine):
-        d = ops._linear_ce_desc(x, weight, labels, bias, ignore_index, reduction)
+    def forward(ctx, x, weight, labels, bias, ignore_index, reduction, engine, keep_bytes):
+        d = ops._linear_ce_desc(x, weight, labels, bias, ignore_index, reduction, keep_bytes)
         loss, saved = ops._linear_ce_fwd(d, x, weight, labels, bias)
         if any(ctx.needs_input_grad):
             ctx.save_for_backward(x, weight, labels, bias, saved)
@@ -35,15 +35,23 @@ class _LinearCEFn(torch.autograd.Function):
                     eng.gview(p).add_(g)
             eng._ready(wp, *([bp] if bp is not None else []))
             dw = db = None
-        return dx, dw, None, db, None, None, None
+        return dx, dw, None, db, None, None, None, None
 
 
-def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduction="mean"):
+def _apply(x, weight, labels, bias, ignore_index, reduction, engine, keep_bytes):
+    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad)):
+        keep_bytes = 0  # no backward will come
+    return _LinearCEFn.apply(x, weight, labels, bias, ignore_index, _REDUCTION[reduction], engine, keep_bytes)
+
+
+def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduction="mean", keep_bytes=-1):
     """F.cross_entropy(x @ weight.T + bias, labels) without the logits: x [..., D], weight [V][D], bias [V] or None, all fp32 or
     all bf16; labels int64 [...] on the GPU.  Logits, sums and the loss are fp32.  Rows whose label is ignore_index take no part
     (their x is not read and its gradient is 0); "mean" is over the others, and 0 where there is none (torch: NaN).  Any other
     label outside [0, V) gives a NaN.  reduction "none" returns labels' shape.  Differentiable in x, weight and bias; the
-    gradients are of the inputs' type."""
+    gradients are of the inputs' type.  keep_bytes: how much the forward may keep for the backward of the N x V exponentials
+    (of the inputs' type): 0 none, the backward computes the logits again; n: all, where they take at most n bytes; -1: all, where
+    that is quicker and takes at most 2 GB."""
     if not torch.is_tensor(x) or not x.is_cuda:
         raise Vc3dError("linear_cross_entropy runs on the GPU only (no CPU fallback)")
     if reduction not in _REDUCTION:
@@ -54,8 +62,8 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     shape = labels.shape
     if x.dim() != 2:
         x, labels = x.reshape(-1, x.shape[-1]), labels.reshape(-1)
-    loss = _LinearCEFn.apply(ops._rows(x), ops._rows(weight), labels.contiguous(), None if bias is None else bias.contiguous(),
-                             int(ignore_index), _REDUCTION[reduction], None)
+    loss = _apply(ops._rows(x), ops._rows(weight), labels.contiguous(), None if bias is None else bias.contiguous(),
+                  int(ignore_index), reduction, None, int(keep_bytes))
     return loss.view(shape) if reduction == "none" else loss
 
 
@@ -68,7 +76,7 @@ class HeadScores:
 
     def cross_entropy(self, y):
         """mean cross-entropy against y (int64 [N]), differentiable in the features and the head's parameters"""
-        return _LinearCEFn.apply(self.feat.contiguous(), self.weight, y.contiguous(), self.bias, -100, _REDUCTION["mean"], self.engine)
+        return _apply(self.feat.contiguous(), self.weight, y.contiguous(), self.bias, -100, "mean", self.engine, -1)
 
     def scores(self):
         from .autograd import linear_apply

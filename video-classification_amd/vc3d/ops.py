@@ -728,7 +728,7 @@ def _ld(t):
     return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
 
 
-def _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction):
+def _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction, keep_bytes):
     kind = _float_kind(x, "x")
     if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1]:
         raise capi.Vc3dError("linear_ce: x [N][D] and weight [V][D] expected, got %s and %s" % (tuple(x.shape), tuple(weight.shape)))
@@ -743,14 +743,15 @@ def _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction):
         raise capi.Vc3dError("linear_ce: labels int64 [%d] expected, got %s %s" % (N, labels.dtype, tuple(labels.shape)))
     if bias is not None and tuple(bias.shape) != (V,):
         raise capi.Vc3dError("linear_ce: bias [%d] expected, got %s" % (V, tuple(bias.shape)))
-    return capi.LinearCeDesc(N, D, V, kind, reduction, weight.data_ptr() & 15, _ld(x), _ld(weight), ignore_index)
+    return capi.LinearCeDesc(N, D, V, kind, reduction, weight.data_ptr() & 15, _ld(x), _ld(weight), ignore_index, keep_bytes)
 
 
-def linear_ce_fwd(x, weight, labels, bias=None, ignore_index=-100, reduction=1):
+def linear_ce_fwd(x, weight, labels, bias=None, ignore_index=-100, reduction=1, keep_bytes=-1):
     """cross-entropy of x weight^T + bias against labels, the vocabulary in pieces (vc_linear_ce_fwd); reduction 0 none, 1 mean
-    over the rows that count, 2 sum -> (loss [1] or [N], saved): saved (bytes) is what linear_ce_bwd of the same tensors takes.
-    x [N][D] and weight [V][D] have contiguous rows, bias and labels are contiguous."""
-    return _linear_ce_fwd(_linear_ce_desc(x, weight, labels, bias, ignore_index, reduction), x, weight, labels, bias)
+    over the rows that count, 2 sum -> (loss [1] or [N], saved): saved (bytes) is what linear_ce_bwd of the same tensors and
+    options takes.  x [N][D] and weight [V][D] have contiguous rows, bias and labels are contiguous.  keep_bytes: how much of
+    saved may be N x V exponentials (-1: up to 2 GB where that is quicker, 0: none)."""
+    return _linear_ce_fwd(_linear_ce_desc(x, weight, labels, bias, ignore_index, reduction, keep_bytes), x, weight, labels, bias)
 
 
 def _linear_ce_fwd(d, x, weight, labels, bias):
@@ -767,10 +768,10 @@ def _linear_ce_fwd(d, x, weight, labels, bias):
     return loss, saved
 
 
-def linear_ce_bwd(x, weight, labels, bias, saved, dloss, ignore_index=-100, reduction=1, want=(True, True, True)):
+def linear_ce_bwd(x, weight, labels, bias, saved, dloss, ignore_index=-100, reduction=1, want=(True, True, True), keep_bytes=-1):
     """gradients of linear_ce_fwd's loss with respect to (x, weight, bias), those that `want` names -> contiguous tensors of
     x's type, or None (vc_linear_ce_bwd)"""
-    d = _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction)
+    d = _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction, keep_bytes)
     _chk(saved, torch.uint8, lib.vc_linear_ce_saved_bytes(d) if d.N else 0, "saved")
     _chk(dloss, F32, d.N if reduction == 0 else 1, "dloss")
     _same_device(x, saved=saved, dloss=dloss)
