@@ -352,11 +352,12 @@ int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, flo
  * vc_softmax_ce does).  reduction: 0 none, 1 mean over the rows that count (0 if none does), 2 sum.
  * loss: [1], or [N] with reduction 0.  saved (vc_linear_ce_saved_bytes, 256-byte aligned) is written by the forward and read by
  * the backward of the same x, w, bias and labels: the rows' logsumexp, the list of rows that count, up to 32 MB of
- * copies of them, and, where that is quicker than to compute the logits again and takes at most keep_bytes (-1: 2 GB), their N x V
- * exponentials in x's type (keep_bytes 0: never; > 0: wherever they fit).  The backward may be called again.  dloss: fp32 on the device, [1], or [N] with reduction 0.  dx [N][D], dw [V][D], db [V] (each nullable) are contiguous
- * and of x's type, and are written, not added to.  workspace (required, 256-byte aligned): vc_linear_ce_workspace_bytes(d, op),
- * op 0 forward, 1 backward: of the N x V logits the forward keeps two floats for every 64 .. 256, the backward one block of up
- * to 512 MB.  Results do not depend on the order in which workgroups run. */
+ * copies of them, and, where that is quicker than to compute the logits again and takes at most keep_bytes (-1: 2 GB), the
+ * gradient of their logits in x's type, N x V (keep_bytes 0: never; > 0: wherever it fits; with reduction 0 never).
+ * dloss: fp32 on the device, [1], or [N] with reduction 0.  dx [N][D], dw [V][D], db [V] (each nullable) are contiguous,
+ * dx and dw 16-byte aligned, and of x's type, and are written, not added to.  workspace (required, 256-byte aligned): vc_linear_ce_workspace_bytes(d, op),
+ * op 0 forward, 1 backward: of the N x V logits the forward keeps two floats for every 64 .. 256 (and what is in saved), the
+ * backward that has no gradient of the logits one block of up to 512 MB.  Results do not depend on the order in which workgroups run. */
 typedef struct vc_linear_ce_desc {
     int32_t N, D, V, is_bf16;
     int32_t reduction, w_align; /* w's address modulo 16: rows that are no whole 16-byte chunks are copied, piece by piece */

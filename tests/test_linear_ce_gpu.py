@@ -227,7 +227,7 @@ def test_gradient_against_differences():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
 def test_kept_exponentials_that_do_not_fit_their_type(reduction, dtype):
     """labels 44 nats and more behind another word, far enough that exp(z - z_label) overflows in one row: nothing of it is used"""
     for far in (60.0, 300.0):
@@ -243,8 +243,7 @@ def test_kept_exponentials_that_do_not_fit_their_type(reduction, dtype):
     y[4] = 5
     b[5] = -float("inf")  # a label that is masked: loss inf, as torch has it
     import vc3d
-    loss = vc3d.linear_cross_entropy(x.requires_grad_(), w, y, b, reduction="none", keep_bytes=ALL)
-    assert torch.equal(torch.isinf(loss), y == 5) and not bool(torch.isnan(loss).any())
+    assert float(vc3d.linear_cross_entropy(x.requires_grad_(), w, y, b, reduction="sum", keep_bytes=ALL)) == float("inf")
 
 
 def test_bad_labels_and_values_with_kept_exponentials():
@@ -255,14 +254,14 @@ def test_bad_labels_and_values_with_kept_exponentials():
     got = []
     for keep in (0, ALL):
         leaves = [t.detach().clone().requires_grad_() for t in (x, w)]
-        loss = vc3d.linear_cross_entropy(leaves[0], leaves[1], y, reduction="none", keep_bytes=keep)
+        loss = vc3d.linear_cross_entropy(leaves[0], leaves[1], y, reduction="sum", keep_bytes=keep)
         bad = torch.zeros(40, dtype=torch.bool, device="cuda")
         bad[3] = bad[5] = bad[9] = True
-        assert torch.equal(torch.isnan(loss), bad) and loss[7] == 0
-        dx, dw = torch.autograd.grad(loss.sum(), leaves)
+        assert bool(torch.isnan(loss))
+        dx, dw = torch.autograd.grad(loss, leaves)
         assert torch.equal(torch.isnan(dx).any(1), bad) and not bool(dx[7].any())
-        got.append((loss, dx, dw))
-    assert torch.equal(torch.isnan(got[0][2]), torch.isnan(got[1][2]))
+        got.append((dx, dw))
+    assert all(torch.equal(torch.isnan(a), torch.isnan(b)) for a, b in zip(*got))
 
 
 def test_what_is_kept():
@@ -270,7 +269,7 @@ def test_what_is_kept():
     import vc3d
     x, w, b, y = make(256, 512, 1 << 14, torch.bfloat16, False, seed=21)
     size = [vc3d.ops.linear_ce_fwd(x, w, y, keep_bytes=k)[1].numel() for k in (0, -1, 1 << 23, (1 << 23) - 1)]
-    assert size[1] == size[2] == size[0] + (1 << 23) + 2 * 1024 and size[3] == size[0]
+    assert size[1] == size[2] == size[0] + (1 << 23) + (1 << 17) + 2 * 1024 and size[3] == size[0]
     assert vc3d.ops.linear_ce_fwd(x[:, :256], w[:, :256], y)[1].numel() < 1 << 20  # short rows: quicker computed again
     leaves = [t.requires_grad_() for t in (x, w)]
     torch.cuda.synchronize()

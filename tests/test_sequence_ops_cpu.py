@@ -74,13 +74,14 @@ def test_c_entry_of_the_linear_cross_entropy_refuses():
     big = 1 << 30
     fwd = lambda d, x=PTR, w=PTR, y=PTR, loss=PTR, saved=PTR, ws=PTR, n=big: c.lib.vc_linear_ce_fwd(  # noqa: E731
         d, x, w, None, y, loss, saved, ws, n, None)
-    bwd = lambda d, x=PTR, w=PTR, b=None, y=PTR, saved=PTR, g=PTR, db=None, ws=PTR, n=big: c.lib.vc_linear_ce_bwd(  # noqa: E731
-        d, x, w, b, y, saved, g, PTR, PTR, db, ws, n, None)
+    bwd = lambda d, x=PTR, w=PTR, b=None, y=PTR, saved=PTR, g=PTR, dx=PTR, dw=PTR, db=None, ws=PTR, n=big: c.lib.vc_linear_ce_bwd(  # noqa: E731
+        d, x, w, b, y, saved, g, dx, dw, db, ws, n, None)
     for bad in (None, ok(N=0), ok(D=0), ok(V=0), ok(N=(1 << 23) + 1), ok(V=(1 << 23) + 1), ok(ldx=63), ok(ldw=63), ok(reduction=3),
                 ok(reduction=-1), ok(w_align=16), ok(w_align=-1), ok(keep_bytes=-2)):
         assert fwd(bad) == -2 and bwd(bad) == -2 and need(bad, 0) == 0 and c.lib.vc_linear_ce_saved_bytes(bad) == 0
     for bad in (dict(x=None), dict(w=None), dict(y=None), dict(saved=None), dict(saved=PTR + 16), dict(ws=None), dict(ws=PTR + 16), dict(n=16)):
         assert fwd(ok(), **bad) == -2 and bwd(ok(), **bad) == -2
+    assert bwd(ok(), dx=PTR + 8) == -2 and bwd(ok(), dw=PTR + 2) == -2 and b"aligned" in c.lib.vc_last_error()
     assert fwd(ok(), loss=None) == -2 and bwd(ok(), g=None) == -2 and bwd(ok(), db=PTR) == -2
     assert fwd(ok(), w=PTR + 2) == -2 and b"modulo 16" in c.lib.vc_last_error()  # the descriptor says that w is aligned
     # what is left for the backward: a few words a row, copies of x while they are small

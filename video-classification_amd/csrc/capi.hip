@@ -1301,11 +1301,11 @@ static int lce_check(const vc_linear_ce_desc* d) {
     VC_REQUIRE(d->reduction >= 0 && d->reduction <= 2, "linear_ce: reduction %d (0 none, 1 mean, 2 sum)", d->reduction);
     return 0;
 }
-static bool lce_keep(const vc_linear_ce_desc* d) { return vc_lce_keep(d->N, d->D, d->V, d->is_bf16 != 0, d->keep_bytes); }
+static bool lce_keep(const vc_linear_ce_desc* d) { return vc_lce_keep(d->N, d->D, d->V, d->is_bf16 != 0, d->reduction, d->keep_bytes); }
 static bool lce_pack(const vc_linear_ce_desc* d) { return vc_lce_pack(d->D, d->ldw, d->w_align, d->is_bf16 != 0); }
 size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op) {
     if (lce_check(d) != 0) return 0;
-    return vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, lce_pack(d), op);
+    return vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, lce_pack(d), lce_keep(d), op);
 }
 size_t vc_linear_ce_saved_bytes(const vc_linear_ce_desc* d) { return lce_check(d) != 0 ? 0 : vc_lce_saved(d->N, d->D, d->V, d->is_bf16 != 0, lce_keep(d)); }
 // what both directions ask of their arguments
@@ -1343,6 +1343,7 @@ int vc_linear_ce_bwd(const vc_linear_ce_desc* d, const void* x, const void* w, c
     const int rc = lce_args("linear_ce_bwd", d, x, w, labels, saved, workspace, ws_bytes, 1);
     if (rc) return rc;
     VC_REQUIRE(dloss, "linear_ce_bwd: null pointer");
+    VC_REQUIRE((((uintptr_t)dx | (uintptr_t)dw) & 15) == 0, "linear_ce_bwd: dx and dw have to be 16-byte aligned");
     VC_REQUIRE(db == nullptr || bias != nullptr, "linear_ce_bwd: a gradient of a bias that is not there");
     VcLceParams p = lce_params(d, x, w, bias, labels, (void*)saved, workspace);
     p.dloss = dloss, p.dx = dx, p.dw = dw, p.db = db;

@@ -247,8 +247,8 @@ struct VcLceParams {
     size_t ws_bytes;
 };
 bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16);
-bool vc_lce_keep(int N, int D, int V, bool is_bf16, long long keep_bytes);
+bool vc_lce_keep(int N, int D, int V, bool is_bf16, int reduction, long long keep_bytes);
 size_t vc_lce_saved(int N, int D, int V, bool is_bf16, bool keep);
-size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int op);
+size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, bool keep, int op);
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s);
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s);

@@ -224,6 +224,22 @@ struct Feed {
     static constexpr int SUBS = ROWS_OF_K || B == 64 ? 2 : 1, RING = ROWS_OF_K && B > 64 ? 2 : 4;
 };
 
+// Two 16 x 16 blocks of results, side by side: lane (l15, lg) holds u = columns 4 lg .. of row l15 of the first, v of the second.
+// As bf16 they change hands so that a lane has 8 columns of one block (16-byte stores, 64 bytes of a row beside each other, where
+// four columns make 8-byte ones, 32 bytes: LCE_S1); `at` is the first block's row.
+template <typename T>
+__device__ __forceinline__ void store_pair(T* at, int lg, f32x4 u, f32x4 v) {
+    if constexpr (sizeof(T) == 2) {
+        const uint2 a = __builtin_bit_cast(uint2, (bf16x4){f2bf(u[0]), f2bf(u[1]), f2bf(u[2]), f2bf(u[3])});
+        const uint2 b = __builtin_bit_cast(uint2, (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])});
+        const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+        *(uint4*)(at + (lg & 1) * 16 + (lg >> 1) * 8) = make_uint4(x[0], y[0], x[1], y[1]);
+    } else {
+        *(f32x4*)(at + lg * 4) = u;
+        *(f32x4*)(at + 16 + lg * 4) = v;
+    }
+}
+
 template <typename T, int EPI, int BR, int BS, int WR, int WS>
 __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     constexpr int NTHR = WR * WS * 64, SUBS = Feed<EPI, BR>::SUBS, RING = Feed<EPI, BR>::RING, STEP = Mma<T>::KF * SUBS;
@@ -389,17 +405,16 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
                 bool ok = __all(fabsf(m) <= 1e30f);
                 if (ok) {
                     const float ref2 = m * LOG2E;
-                    T* const row = (T*)g.P + (long long)s * g.ldp + r0 + wr + lg * 4;
+                    T* const row = (T*)g.P + (long long)s * g.ldp + r0 + wr;
 #pragma unroll
-                    for (int a = 0; a < NA; ++a) {
-                        f32x4 v;
+                    for (int a = 0; a < NA; a += 2) {
+                        f32x4 u, v;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[j] = ex(acc[a][b][j], m, ref2, sizeof(T) == 2);
-                        e += (v[0] + v[1]) + (v[2] + v[3]);
-                        if (s < ns) {
-                            if constexpr (sizeof(T) == 2) *(bf16x4*)(row + a * 16) = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
-                            else *(f32x4*)(row + a * 16) = v;
-                        }
+                        for (int j = 0; j < 4; ++j) u[j] = ex(acc[a][b][j], m, ref2, sizeof(T) == 2);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = ex(acc[a + 1][b][j], m, ref2, sizeof(T) == 2);
+                        e += ((u[0] + u[1]) + (u[2] + u[3])) + ((v[0] + v[1]) + (v[2] + v[3]));
+                        if (s < ns) store_pair(row + a * 16, lg, u, v);
                     }
                     e += __shfl_xor(e, 16, 64);
                     e += __shfl_xor(e, 32, 64);
@@ -481,13 +496,11 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
                 for (int a = 0; a < NA; ++a)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[a][b][j] = in && r0 + wr + a * 16 + lg * 4 + j < g.nr ? acc[a][b][j] : 0.f;
-            T* const row = (T*)g.P + (long long)s * g.ldp + r0 + wr + lg * 4;
+            T* const row = (T*)g.P + (long long)s * g.ldp + r0 + wr;
 #pragma unroll
-            for (int a = 0; a < NA; ++a) {
-                const f32x4 v = acc[a][b];
-                cs[a] += v;
-                if constexpr (sizeof(T) == 2) *(bf16x4*)(row + a * 16) = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
-                else *(f32x4*)(row + a * 16) = v;
+            for (int a = 0; a < NA; a += 2) {
+                cs[a] += acc[a][b], cs[a + 1] += acc[a + 1][b];
+                store_pair(row + a * 16, lg, acc[a][b], acc[a + 1][b]);
             }
         }
         if (g.dbpart != nullptr) {
@@ -513,11 +526,17 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     }
     if constexpr (EPI == EPI_DX || EPI == EPI_DW) {
         const float f = EPI == EPI_DW ? g.factor.get() : 1.f;
-        const bool vec = (g.nr & 3) == 0;
+        const bool vec = (g.nr & 3) == 0, wide = r0 + BR <= g.nr && (g.nr * (int)sizeof(T) & 15) == 0;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const int s = s0 + wsx + b * 16 + l15;
             if (s >= ns) continue;
+            if (EPI == EPI_DW && wide) {
+                T* const q = (T*)g.out + (long long)s * g.nr + r0 + wr;
+#pragma unroll
+                for (int a = 0; a < NA; a += 2) store_pair(q + a * 16, lg, acc[a][b] * f, acc[a + 1][b] * f);
+                continue;
+            }
 #pragma unroll
             for (int a = 0; a < NA; ++a) {
                 const int r = r0 + wr + a * 16 + lg * 4;
@@ -555,7 +574,8 @@ __device__ __forceinline__ void copy_row(const T* from, T* to, int D, int ld, in
 }
 // words of w (a wave each), for the reasons that Plan gives
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void lce_words_of_w_kernel(const T* w, long long ldw, int n, int D, int ld, T* out) {
+__global__ __launch_bounds__(256) void lce_words_of_w_kernel(const T* w, long long ldw, int n, int D, int ld, T* out, const int* when) {
+    if (when != nullptr && *when == 0) return;
     for (int v = blockIdx.x * 4 + (threadIdx.x >> 6); v < n; v += gridDim.x * 4)
         copy_row<T, VEC>(w + v * ldw, out + (long long)v * ld, D, ld, threadIdx.x & 63, 64);
 }
@@ -569,6 +589,7 @@ struct LabelLogit {
     long long ldw;
     const void* bias;
     int V;
+    bool chunks;  // w's rows are whole 16-byte chunks
 };
 template <typename T, bool VEC, bool LIST>
 __global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long long ldx, int* rows, const long long* labels, long long ignore,
@@ -606,7 +627,16 @@ __global__ __launch_bounds__(256) void lce_rows_of_x_kernel(const T* x, long lon
     const bool word = y >= 0 && y < q.V;
     const T *const xr = x + n * ldx, *const wr = (const T*)q.w + (word ? y : 0) * q.ldw;
     float s = 0.f;
-    for (int d = threadIdx.x; d < D; d += 256) s = __builtin_fmaf((float)xr[d], (float)wr[d], s);
+    constexpr int PER = 16 / (int)sizeof(T);
+    typedef T chunk_t __attribute__((ext_vector_type(PER)));
+    if (VEC && q.chunks)
+        for (int d = threadIdx.x * PER; d < D; d += 256 * PER) {
+            const chunk_t u = *(const chunk_t*)(xr + d), v = *(const chunk_t*)(wr + d);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) s = __builtin_fmaf((float)u[j], (float)v[j], s);
+        }
+    else
+        for (int d = threadIdx.x; d < D; d += 256) s = __builtin_fmaf((float)xr[d], (float)wr[d], s);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) sum_sh[threadIdx.x >> 6] = s;
@@ -680,13 +710,12 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const float2* part, int 
         loss[0] = (float)(mean ? s / (double)(count > 0 ? count : 1) : s);
     }
 }
-// P of a piece from what EPI_KEEP stored: E[s][v] exp(ref_s - lse_s), at the label its own value; db's partial sums.  A workgroup
-// takes a row tile by 64 chunks of 16 bytes, a wave a quarter of the rows.
-// (a second rounding of P, half a step of what the first left, for not computing the logits again)
+// What EPI_KEEP stored becomes P, where it lies: E[s][v] exp(ref_s - lse_s), at the label its own value; and db's partial sums.
+// A workgroup takes a row tile by 64 chunks of 16 bytes, a wave a quarter of the rows.  P is rounded a second time, which is what
+// not computing the logits again costs.
 template <typename T>
-__global__ __launch_bounds__(256) void lce_kept_kernel(const T* E, long long lde, T* P, long long ldp, const int* rows, const float* lse, const float* ref,
-                                                       const float* plab, const long long* labels, const float* scale, int N, int v0, int nv, int tile,
-                                                       float* dbpart) {
+__global__ __launch_bounds__(256) void lce_kept_kernel(T* E, long long lde, const int* rows, const float* lse, const float* ref, const float* plab,
+                                                       const long long* labels, int N, int V, int tile, float* dbpart) {
     constexpr int PER = 16 / (int)sizeof(T);
     typedef T chunk_t __attribute__((ext_vector_type(PER)));
     __shared__ float by[256], at[256];
@@ -698,20 +727,17 @@ __global__ __launch_bounds__(256) void lce_kept_kernel(const T* E, long long lde
         const int s = s0 + tid;
         const bool in = s < count;
         const int n = in ? rows[s] : 0;
-        const float f = scale != nullptr && in ? scale[n] : 1.f;
-        const long long y = in ? labels[n] - v0 : -1;
-        by[tid] = in ? __expf(ref[s] - lse[n]) * f : 0.f;
-        at[tid] = in ? plab[s] * f : 0.f;
-        label[tid] = y >= 0 && y < nv ? (int)y : -PER;
+        by[tid] = in ? __expf(ref[s] - lse[n]) : 0.f;
+        at[tid] = in ? plab[s] : 0.f;
+        label[tid] = in ? (int)labels[n] : -PER;  // (a label that is no word: EPI_KEEP gave up)
     }
     __syncthreads();
     const int col = (blockIdx.x * 64 + lane) * PER;
     float cs[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) cs[j] = 0.f;
-    if (col < nv) {
-        const T* const from = E + (long long)s0 * lde + v0 + col;
-        T* const to = P + (long long)s0 * ldp + col;
+    if (col < V) {
+        T* const from = E + (long long)s0 * lde + col;
         const int each = tile / 4;
         for (int k0 = wave * each; k0 < (wave + 1) * each; k0 += 8) {
             chunk_t v[8];
@@ -732,7 +758,7 @@ __global__ __launch_bounds__(256) void lce_kept_kernel(const T* E, long long lde
                 chunk_t o;
 #pragma unroll
                 for (int j = 0; j < PER; ++j) cs[j] += f[j], o[j] = (T)f[j];
-                *(chunk_t*)(to + (k0 + k) * ldp) = o;
+                *(chunk_t*)(from + (k0 + k) * lde) = o;
             }
         }
     }
@@ -742,7 +768,7 @@ __global__ __launch_bounds__(256) void lce_kept_kernel(const T* E, long long lde
     __syncthreads();
     for (int c = tid; c < 64 * PER; c += 256) {
         const int l = c / PER, j = c % PER, at_ = blockIdx.x * 64 * PER + c;
-        if (at_ < nv) dbpart[(long long)blockIdx.y * ldp + at_] = (sums[0][l][j] + sums[1][l][j]) + (sums[2][l][j] + sums[3][l][j]);
+        if (at_ < V) dbpart[(long long)blockIdx.y * lde + at_] = (sums[0][l][j] + sums[1][l][j]) + (sums[2][l][j] + sums[3][l][j]);
     }
 }
 // what is stored last: workgroup i < N the row i of the list of dx (its splits' sums; zeros for a row that does not count), the
@@ -821,21 +847,26 @@ struct Plan {
     static size_t list_at(int N) { return ((size_t)N * 4 + 255) & ~(size_t)255; }
     static size_t x_at(int N) { return list_at(N) + ((((size_t)N + 4) * 4 + 255) & ~(size_t)255); }
     static size_t ref_at(int N, int D, int elem) { return x_at(N) + (((saves_x(N, D, elem) ? (size_t)N * row(D, elem) * elem : 0) + 255) & ~(size_t)255); }
-    // with `keep` also: ref [N], P at the label [N], the exponentials
+    // with `keep` also: ref [N], P at the label [N], the exponentials, which become P, and db's partial sums
     static size_t plab_at(int N, int D, int elem) { return ref_at(N, D, elem) + list_at(N); }
     static size_t exps_at(int N, int D, int elem) { return plab_at(N, D, elem) + list_at(N); }
     static size_t exps(int N, int V, int elem) { return ((size_t)N + 255) / 256 * 256 * (((size_t)V + 255) / 256 * 256) * elem; }
-    static size_t saved(int N, int D, int V, int elem, bool keep) { return keep ? exps_at(N, D, elem) + exps(N, V, elem) : ref_at(N, D, elem); }
-    Plan(int N, int D, int V, int elem, int op, bool pack) {
+    static size_t dbpart_at(int N, int D, int V, int elem) { return exps_at(N, D, elem) + exps(N, V, elem); }
+    static size_t saved(int N, int D, int V, int elem, bool keep) {
+        if (!keep) return ref_at(N, D, elem);
+        const size_t tile = pick_tile(N, V);
+        return dbpart_at(N, D, V, elem) + (N + tile - 1) / tile * (((size_t)V + 255) / 256 * 256) * 4;
+    }
+    Plan(int N, int D, int V, int elem, int op, bool pack, bool keep) {
         kd = (D * elem + 15) / 16 * 16 / elem;
         ld = row(D, elem);
         const long long np = ((long long)N + 255) / 256 * 256, all = ((long long)V + 255) / 256 * 256;
         long long fit = (512ll << 20) / elem / np / 256 * 256;
-        if (pack && op == 0) fit = (512ll << 20) / elem / ld / 256 * 256;  // (the forward holds a piece of w only)
+        if (op == 0 || keep) fit = pack ? (512ll << 20) / elem / ld / 256 * 256 : all;  // (a piece of w's copy is all there is)
         fit = fit < 256 ? 256 : fit;
         lde = all;
-        piece = (int)(op == 0 && !pack ? all : fit < all ? fit : all);
-        tile = pick_tile(N, piece < V ? piece : V);
+        piece = (int)(fit < all ? fit : all);
+        tile = pick_tile(N, piece < V && !keep ? piece : V);
         tiles = (int)(((long long)V + tile - 1) / tile);
         if (!saves_x(N, D, elem)) xp = take((size_t)N * ld * elem);
         if (pack) wp = take((size_t)(piece < V ? piece : V) * ld * elem);
@@ -856,6 +887,7 @@ struct Plan {
         dx.most = (int)(dx.most > least ? least : dx.most);
         dx.most = dx.most < 1 ? 1 : dx.most;
         acc = take((size_t)dx.most * N * D * 4);
+        if (keep) return;
         P = take((size_t)np * piece * elem);
         dbpart = take((size_t)(np / 64) * piece * 4);
     }
@@ -898,6 +930,7 @@ struct Source {
     float *lse, *ref, *plab;
     int* rows;
     T* exps;
+    float* dbpart;
     Source(const VcLceParams& p, const Plan& L, hipStream_t s, bool forward) : p(p), L(L), s(s) {
         char* const saved = (char*)p.saved;
         const bool kept = Plan::saves_x(p.N, p.D, sizeof(T));
@@ -905,6 +938,7 @@ struct Source {
         ref = p.keep ? (float*)(saved + Plan::ref_at(p.N, p.D, sizeof(T))) : nullptr;
         plab = p.keep ? (float*)(saved + Plan::plab_at(p.N, p.D, sizeof(T))) : nullptr;
         exps = p.keep ? (T*)(saved + Plan::exps_at(p.N, p.D, sizeof(T))) : nullptr;
+        dbpart = p.keep && p.bias != nullptr ? (float*)(saved + Plan::dbpart_at(p.N, p.D, p.V, sizeof(T))) : nullptr;
         T* const to = (T*)(kept ? saved + Plan::x_at(p.N) : (char*)p.ws + L.xp);
         x = {(const char*)to, L.ld * (long long)sizeof(T)};
         if (!forward && kept) return;
@@ -912,84 +946,95 @@ struct Source {
         if (forward && !list) hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, s, p.labels, p.ignore_index, p.N, rows);
         const auto kernel = list ? (vec ? lce_rows_of_x_kernel<T, true, true> : lce_rows_of_x_kernel<T, false, true>)
                                  : (vec ? lce_rows_of_x_kernel<T, true, false> : lce_rows_of_x_kernel<T, false, false>);
-        const LabelLogit q = {forward ? ref : nullptr, p.w, p.ldw, p.bias, p.V};
+        const LabelLogit q = {forward ? ref : nullptr, p.w, p.ldw, p.bias, p.V, !p.pack};
         hipLaunchKernelGGL(kernel, dim3(p.N), dim3(256), 0, s, (const T*)p.x, p.ldx, rows, p.labels, p.ignore_index, p.N, p.D, L.ld, to, q);
     }
-    Operand w(int v0, int nv) const {
+    Operand w(int v0, int nv, const int* when) const {
         const T* at = (const T*)p.w + v0 * p.ldw;
         if (!p.pack) return {(const char*)at, p.ldw * (long long)sizeof(T)};
         T* const to = (T*)((char*)p.ws + L.wp);
         const auto kernel = chunks(at, p.ldw, p.D) ? lce_words_of_w_kernel<T, true> : lce_words_of_w_kernel<T, false>;
-        hipLaunchKernelGGL(kernel, dim3(nv < 16384 ? (nv + 3) / 4 : 4096), dim3(256), 0, s, at, p.ldw, nv, p.D, L.ld, to);
+        hipLaunchKernelGGL(kernel, dim3(nv < 16384 ? (nv + 3) / 4 : 4096), dim3(256), 0, s, at, p.ldw, nv, p.D, L.ld, to, when);
         return {(const char*)to, L.ld * (long long)sizeof(T)};
     }
 };
 
 template <typename T>
 int fwd(const VcLceParams& p, hipStream_t s) {
-    const Plan L(p.N, p.D, p.V, sizeof(T), 0, p.pack);
+    const Plan L(p.N, p.D, p.V, sizeof(T), 0, p.pack, p.keep);
     char* ws = (char*)p.ws;
     float2* part = (float2*)(ws + L.part);
     float* zlab = (float*)(ws + L.zlab);
     float* loss_rows = p.loss_rows != nullptr ? p.loss_rows : (float*)(ws + L.loss_rows);
     (void)hipGetLastError();
     const Source<T> src(p, L, s, true);
+    int* const gave_up = src.rows + p.N + 2;
+    Gemm g = {};
+    g.ns_dev = src.rows + p.N, g.K = L.kd, g.S = src.x, g.bias = p.bias, g.labels = p.labels, g.rows = src.rows;
+    g.part = part, g.part_ld = L.tiles, g.zlab = zlab, g.ref = src.ref, g.gave_up = gave_up, g.ldp = L.lde;
     for (int v0 = 0; v0 < p.V; v0 += L.piece) {
-        Gemm g = {};
-        g.nr = p.V - v0 < L.piece ? p.V - v0 : L.piece, g.ns_dev = src.rows + p.N, g.K = L.kd;
-        g.R = src.w(v0, g.nr), g.S = src.x;
-        g.bias = p.bias, g.labels = p.labels, g.rows = src.rows, g.v0 = v0, g.part = part, g.part_ld = L.tiles, g.part0 = v0 / L.tile, g.zlab = zlab;
-        if (p.keep) {
-            g.ref = src.ref, g.gave_up = src.rows + p.N + 2, g.P = src.exps + v0, g.ldp = L.lde;
-            gemm<T, EPI_KEEP>(g, L.tile, p.N, 1, s);
-        } else
-            gemm<T, EPI_STATS>(g, L.tile, p.N, 1, s);
+        g.nr = p.V - v0 < L.piece ? p.V - v0 : L.piece, g.R = src.w(v0, g.nr, nullptr);
+        g.v0 = v0, g.part0 = v0 / L.tile;
+        if (p.keep) g.P = src.exps + v0, gemm<T, EPI_KEEP>(g, L.tile, p.N, 1, s);
+        else gemm<T, EPI_STATS>(g, L.tile, p.N, 1, s);
     }
     hipLaunchKernelGGL(lce_rows_kernel, dim3((p.N + 15) / 16), dim3(1024), 0, s, part, L.tiles, zlab, p.labels, src.rows, p.N, p.V, src.lse,
                        loss_rows, src.plab, p.reduction == 1, p.reduction != 0 ? p.loss : nullptr);
+    if (p.keep) {
+        hipLaunchKernelGGL((lce_kept_kernel<T>), dim3((p.V * (int)sizeof(T) + 1023) / 1024, (p.N + L.tile - 1) / L.tile), dim3(256), 0, s, src.exps,
+                           L.lde, src.rows, src.lse, src.ref, src.plab, p.labels, p.N, p.V, L.tile, src.dbpart);
+        // where EPI_KEEP gave up (4.7 us of workgroups that leave at once where it did not)
+        g.when = gave_up, g.lse = src.lse;
+        for (int v0 = 0; v0 < p.V; v0 += L.piece) {
+            g.nr = p.V - v0 < L.piece ? p.V - v0 : L.piece;
+            if (L.piece < p.V) g.R = src.w(v0, g.nr, gave_up);
+            g.v0 = v0, g.P = src.exps + v0, g.dbpart = src.dbpart != nullptr ? src.dbpart + v0 : nullptr;
+            gemm<T, EPI_PROB>(g, L.tile, p.N, 1, s);
+        }
+    }
     return launched("linear_ce_fwd");
 }
 
 template <typename T>
 int bwd(const VcLceParams& p, hipStream_t s) {
-    const Plan L(p.N, p.D, p.V, sizeof(T), 1, p.pack);
+    const Plan L(p.N, p.D, p.V, sizeof(T), 1, p.pack, p.keep);
     char* ws = (char*)p.ws;
-    float *acc = (float*)(ws + L.acc), *dbpart = (float*)(ws + L.dbpart);
-    const long long ldp = (long long)L.piece * (int)sizeof(T);
+    float *acc = (float*)(ws + L.acc), *dbpart = p.keep ? nullptr : (float*)(ws + L.dbpart);
+    const long long ld = p.keep ? L.lde : L.piece;
     (void)hipGetLastError();
     const Source<T> src(p, L, s, false);
     const int* count = src.rows + p.N;
     const Factor factor = {p.dloss, count, p.reduction};
     for (int v0 = 0; v0 < p.V; v0 += L.piece) {
         const int nv = p.V - v0 < L.piece ? p.V - v0 : L.piece;
-        const Operand w = src.w(v0, nv);
-        Gemm g = {};
-        g.R = w, g.S = src.x;
-        g.nr = nv, g.ns_dev = count, g.K = L.kd;
-        g.bias = p.bias, g.labels = p.labels, g.rows = src.rows, g.v0 = v0;
-        g.lse = src.lse, g.scale = p.reduction == 0 ? p.dloss : nullptr, g.P = ws + L.P, g.ldp = L.piece, g.dbpart = p.db != nullptr ? dbpart : nullptr;
-        if (p.keep) {
-            g.when = src.rows + p.N + 2;
-            hipLaunchKernelGGL((lce_kept_kernel<T>), dim3((nv * (int)sizeof(T) + 1023) / 1024, (p.N + L.tile - 1) / L.tile), dim3(256), 0, s, src.exps,
-                               L.lde, (T*)g.P, g.ldp, src.rows, src.lse, src.ref, src.plab, p.labels, g.scale, p.N, v0, nv, L.tile, g.dbpart);
+        const bool wants_w = !p.keep || p.dx != nullptr;
+        const Operand w = wants_w ? src.w(v0, nv, nullptr) : Operand{};
+        T* const P = p.keep ? src.exps + v0 : (T*)(ws + L.P);
+        if (p.keep) dbpart = src.dbpart != nullptr ? src.dbpart + v0 : nullptr;
+        else {
+            Gemm g = {};
+            g.R = w, g.S = src.x;
+            g.nr = nv, g.ns_dev = count, g.K = L.kd;
+            g.bias = p.bias, g.labels = p.labels, g.rows = src.rows, g.v0 = v0;
+            g.lse = src.lse, g.scale = p.reduction == 0 ? p.dloss : nullptr, g.P = P, g.ldp = ld, g.dbpart = p.db != nullptr ? dbpart : nullptr;
+            gemm<T, EPI_PROB>(g, L.tile, p.N, 1, s);
         }
-        gemm<T, EPI_PROB>(g, L.tile, p.N, 1, s);
         if (p.dx != nullptr) {
             Gemm x = {};
-            x.R = w, x.S = {ws + L.P, ldp};
+            x.R = w, x.S = {(const char*)P, ld * (long long)sizeof(T)};
             x.nr = p.D, x.ns_dev = count, x.K = nv, x.acc = acc, x.add = v0 > 0, x.acc_split = (long long)p.N * p.D;
             x.splits = L.dx;
             gemm<T, EPI_DX>(x, L.tile_dx, p.N, L.dx.most, s);
         }
         if (p.dw != nullptr) {
             Gemm d = {};
-            d.R = src.x, d.S = {ws + L.P, ldp};
+            d.R = src.x, d.S = {(const char*)P, ld * (long long)sizeof(T)};
             d.nr = p.D, d.ns = nv, d.k_dev = count, d.out = (T*)p.dw + (long long)v0 * p.D, d.factor = factor;
             gemm<T, EPI_DW>(d, L.tile_dw, nv, 1, s);
         }
         const bool end = v0 + nv == p.V && p.dx != nullptr;
         if (p.db == nullptr && !end) continue;
-        const Last q = {acc, L.dx, (long long)p.N * p.D, dbpart, L.piece, L.tile, nv, end ? p.N : 0, p.dx, p.db != nullptr ? (T*)p.db + v0 : nullptr};
+        const Last q = {acc, L.dx, (long long)p.N * p.D, dbpart, ld, L.tile, nv, end ? p.N : 0, p.dx, p.db != nullptr ? (T*)p.db + v0 : nullptr};
         hipLaunchKernelGGL((lce_last_kernel<T>), dim3(q.nx + (p.db != nullptr ? (nv + 255) / 256 : 0)), dim3(256), 0, s, q, src.rows, factor, p.N, p.D);
     }
     return launched("linear_ce_bwd");
@@ -1005,11 +1050,12 @@ bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16) {
     return (D * elem) % 16 != 0 || (ldw * elem) % 16 != 0 || w_align != 0 || ldw * elem >= (1ll << 32);
 }
 // Whether the forward keeps exp(z - ref) for the backward, which then need not compute the logits again.
-bool vc_lce_keep(int N, int D, int V, bool is_bf16, long long keep_bytes) {
+bool vc_lce_keep(int N, int D, int V, bool is_bf16, int reduction, long long keep_bytes) {
+    if (reduction == 0) return false;  // (its rows' factors come with the backward)
     const size_t bytes = Plan::exps(N, V, is_bf16 ? 2 : 4);
     return keep_bytes >= 0 ? bytes <= (size_t)keep_bytes : bytes <= (size_t)2 << 30 && D >= 512 && (long long)N * V >= 1 << 22;
 }
 size_t vc_lce_saved(int N, int D, int V, bool is_bf16, bool keep) { return Plan::saved(N, D, V, is_bf16 ? 2 : 4, keep); }
-size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack).bytes; }
+size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, bool keep, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack, keep).bytes; }
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? fwd<bf16>(p, s) : fwd<float>(p, s); }
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? bwd<bf16>(p, s) : bwd<float>(p, s); }

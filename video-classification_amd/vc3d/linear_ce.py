@@ -49,9 +49,9 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     all bf16; labels int64 [...] on the GPU.  Logits, sums and the loss are fp32.  Rows whose label is ignore_index take no part
     (their x is not read and its gradient is 0); "mean" is over the others, and 0 where there is none (torch: NaN).  Any other
     label outside [0, V) gives a NaN.  reduction "none" returns labels' shape.  Differentiable in x, weight and bias; the
-    gradients are of the inputs' type.  keep_bytes: how much the forward may keep for the backward of the N x V exponentials
-    (of the inputs' type): 0 none, the backward computes the logits again; n: all, where they take at most n bytes; -1: all, where
-    that is quicker and takes at most 2 GB."""
+    gradients are of the inputs' type.  keep_bytes: whether the forward keeps the logits' gradient for the
+    backward (N x V of the inputs' type): 0 no, the backward computes the logits again; n: where it takes at most n bytes; -1: where
+    that is quicker and takes at most 2 GB.  Never with reduction "none"."""
     if not torch.is_tensor(x) or not x.is_cuda:
         raise Vc3dError("linear_cross_entropy runs on the GPU only (no CPU fallback)")
     if reduction not in _REDUCTION:

@@ -750,7 +750,7 @@ def linear_ce_fwd(x, weight, labels, bias=None, ignore_index=-100, reduction=1, 
     """cross-entropy of x weight^T + bias against labels, the vocabulary in pieces (vc_linear_ce_fwd); reduction 0 none, 1 mean
     over the rows that count, 2 sum -> (loss [1] or [N], saved): saved (bytes) is what linear_ce_bwd of the same tensors and
     options takes.  x [N][D] and weight [V][D] have contiguous rows, bias and labels are contiguous.  keep_bytes: how much of
-    saved may be N x V exponentials (-1: up to 2 GB where that is quicker, 0: none)."""
+    saved may be the logits' gradient, N x V (-1: up to 2 GB where that is quicker, 0: none)."""
     return _linear_ce_fwd(_linear_ce_desc(x, weight, labels, bias, ignore_index, reduction, keep_bytes), x, weight, labels, bias)
 
 
