@@ -243,7 +243,7 @@ def test_kept_exponentials_that_do_not_fit_their_type(reduction, dtype):
     y[4] = 5
     b[5] = -float("inf")  # a label that is masked: loss inf, as torch has it
     import vc3d
-    assert float(vc3d.linear_cross_entropy(x.requires_grad_(), w, y, b, reduction="sum", keep_bytes=ALL)) == float("inf")
+    assert float(vc3d.linear_cross_entropy(x, w, y, b, reduction="sum", keep_bytes=ALL)) == float("inf")
 
 
 def test_bad_labels_and_values_with_kept_exponentials():
@@ -267,10 +267,10 @@ def test_bad_labels_and_values_with_kept_exponentials():
 def test_what_is_kept():
     """the rule, the limit, nothing without a backward; a backward that is called twice"""
     import vc3d
-    x, w, b, y = make(256, 512, 1 << 14, torch.bfloat16, False, seed=21)
-    size = [vc3d.ops.linear_ce_fwd(x, w, y, keep_bytes=k)[1].numel() for k in (0, -1, 1 << 23, (1 << 23) - 1)]
-    assert size[1] == size[2] == size[0] + (1 << 23) + (1 << 17) + 2 * 1024 and size[3] == size[0]
-    assert vc3d.ops.linear_ce_fwd(x[:, :256], w[:, :256], y)[1].numel() < 1 << 20  # short rows: quicker computed again
+    x, w, b, y = make(512, 512, 1 << 14, torch.bfloat16, False, seed=21)
+    size = [vc3d.ops.linear_ce_fwd(x, w, y, keep_bytes=k)[1].numel() for k in (0, -1, 1 << 24, (1 << 24) - 1)]
+    assert size[1] == size[2] == size[0] + (1 << 24) + (1 << 18) + 2 * 2048 and size[3] == size[0]
+    assert vc3d.ops.linear_ce_fwd(x[:, :128], w[:, :128], y)[1].numel() < 1 << 20  # short rows: quicker computed again
     leaves = [t.requires_grad_() for t in (x, w)]
     torch.cuda.synchronize()
     before = torch.cuda.memory_allocated()

@@ -80,7 +80,7 @@ struct Factor {
 
 // The product for dx has few tiles and a long k: k is split, each split into sums of its own, so that all tiles make one round on
 // the chip (`slots` workgroups at once).  The tiles that there are decide, not those that the launch allows for (1777 rows of
-// which 1244 count: 4 splits by the former, 6 by the latter, 232 against LCE_Z us).
+// which 1244 count: 4 splits by the former, 6 by the latter, 232 against 178 us).
 struct Splits {
     int slots, most, rtiles, bs;
     __device__ __forceinline__ int of(int ns) const {
@@ -226,7 +226,8 @@ struct Feed {
 
 // Two 16 x 16 blocks of results, side by side: lane (l15, lg) holds u = columns 4 lg .. of row l15 of the first, v of the second.
 // As bf16 they change hands so that a lane has 8 columns of one block (16-byte stores, 64 bytes of a row beside each other, where
-// four columns make 8-byte ones, 32 bytes: LCE_S1); `at` is the first block's row.
+// four columns make 8-byte ones, 32 bytes: the products of 2048 x 1024 of 32768 that store bf16 take 156 and 121 us instead of 167
+// and 127); `at` is the first block's row.
 template <typename T>
 __device__ __forceinline__ void store_pair(T* at, int lg, f32x4 u, f32x4 v) {
     if constexpr (sizeof(T) == 2) {
@@ -1049,11 +1050,17 @@ bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16) {
     const int elem = is_bf16 ? 2 : 4;
     return (D * elem) % 16 != 0 || (ldw * elem) % 16 != 0 || w_align != 0 || ldw * elem >= (1ll << 32);
 }
-// Whether the forward keeps exp(z - ref) for the backward, which then need not compute the logits again.
+// Whether the forward keeps the logits' gradient for the backward, which then need not compute the logits again: that saves a
+// product and costs storing, reading and storing N x V, and two launches.  By itself up to 2 GB (under 1 % of the memory) and
+// where there is enough to save.  Measured, again / kept in us, bf16: 2048 x 1024 of 32768 555 / 477, 8192 x 2048 of 65536
+// 7170 / 5900, 1000 x 512 of 20000 178 / 159, 4000 x 384 of 32000 553 / 535, 8192 x 256 of 60000 1660 / 1470, 64 x 2048 of 32000
+// 152 / 140; but 8192 x 128 of 60000 1200 / 1332, 512 x 512 of 8192 87 / 90.  fp32: 1000 x 1024 of 32000 2030 / 1590, 1000 x 64 of
+// 20000 214 / 190; but 4000 x 64 of 1000 172 / 171, 300 x 128 of 10000 148 / 152.
 bool vc_lce_keep(int N, int D, int V, bool is_bf16, int reduction, long long keep_bytes) {
     if (reduction == 0) return false;  // (its rows' factors come with the backward)
     const size_t bytes = Plan::exps(N, V, is_bf16 ? 2 : 4);
-    return keep_bytes >= 0 ? bytes <= (size_t)keep_bytes : bytes <= (size_t)2 << 30 && D >= 512 && (long long)N * V >= 1 << 22;
+    if (keep_bytes >= 0) return bytes <= (size_t)keep_bytes;
+    return bytes <= (size_t)2 << 30 && (double)N * V * D >= (is_bf16 ? 0x1p32 : 0x1p28) && (!is_bf16 || D >= 256);
 }
 size_t vc_lce_saved(int N, int D, int V, bool is_bf16, bool keep) { return Plan::saved(N, D, V, is_bf16 ? 2 : 4, keep); }
 size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, bool keep, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack, keep).bytes; }
