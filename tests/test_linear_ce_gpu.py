@@ -193,12 +193,30 @@ def test_layouts(dtype):
                  (big[:120:2, 4:100], big[110:200, 20:116]), (big[:1, :64].expand(60, 64), big[:90, :64])):
         run_and_check(x, w, None, y)
     x, w = big[:60, :128], big[60:150, :128]
-    for pick in range(2):  # gradients of one input alone
-        leaves = [t.detach().clone().requires_grad_(i == pick) for i, t in enumerate((x, w))]
-        both = [t.detach().clone().requires_grad_() for t in (x, w)]
-        got, = torch.autograd.grad(vc3d.linear_cross_entropy(leaves[0], leaves[1], y), leaves[pick])
-        want = torch.autograd.grad(vc3d.linear_cross_entropy(both[0], both[1], y), both)[pick]
-        assert torch.equal(got, want)
+    b = torch.randn(90, generator=g).to(dtype).cuda()
+    for keep in (0, ALL):
+        for pick in range(3):  # gradients of one input alone
+            leaves = [t.detach().clone().requires_grad_(i == pick) for i, t in enumerate((x, w, b))]
+            both = [t.detach().clone().requires_grad_() for t in (x, w, b)]
+            got, = torch.autograd.grad(vc3d.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], keep_bytes=keep), leaves[pick])
+            want = torch.autograd.grad(vc3d.linear_cross_entropy(both[0], both[1], y, both[2], keep_bytes=keep), both)[pick]
+            assert torch.equal(got, want)
+
+
+def test_the_plain_operators_refuse_layouts_that_they_cannot_read():
+    import vc3d
+    from vc3d.capi import Vc3dError
+    x, w, b, y = make(40, 64, 90, torch.float32, True, seed=22)
+    for bad in (dict(x=x.t()[:, :40].t()[:, ::2], w=w[:, :32]), dict(x=x[:1].expand(40, 64)), dict(w=w.t().contiguous().t()),
+                dict(y=torch.stack((y, y), 1)[:, 0]), dict(b=torch.stack((b, b), 1)[:, 0])):
+        a = {**dict(x=x, w=w, y=y, b=b), **bad}
+        with pytest.raises(Vc3dError):
+            vc3d.ops.linear_ce_fwd(a["x"], a["w"], a["y"], a["b"])
+    loss, saved = vc3d.ops.linear_ce_fwd(x, w, y, b)
+    for bad in (dict(saved=saved[:-1]), dict(dloss=loss.double()), dict(dloss=loss.cpu())):
+        a = {**dict(saved=saved, dloss=loss), **bad}
+        with pytest.raises(Vc3dError):
+            vc3d.ops.linear_ce_bwd(x, w, y, b, a["saved"], a["dloss"])
 
 
 def test_more_than_one_piece_of_the_vocabulary():

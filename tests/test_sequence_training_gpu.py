@@ -238,6 +238,35 @@ def test_adamw_state_survives_saving(bits, dtype, tmp_path):
         AdamW(three, state_bits=40 - bits).load_state_dict(ob.state_dict())
 
 
+def test_a_run_begun_with_torch_adamw_goes_on():
+    """torch.optim.AdamW's state is taken over (fp32 moments, its step count); one step on: torch's own, to its roundings"""
+    from vc3d.capi import Vc3dError
+    from vc3d.optim import AdamW
+    g = torch.Generator().manual_seed(17)
+    p = [torch.nn.Parameter(torch.randn(40, 7, generator=g).cuda()), torch.nn.Parameter(torch.randn(5, generator=g).cuda())]
+    theirs = torch.optim.AdamW(p, lr=1e-2)
+    for _ in range(3):
+        for q in p:
+            q.grad = torch.randn(q.shape, generator=g).cuda()
+        theirs.step()
+    mine_p = [torch.nn.Parameter(q.detach().clone()) for q in p]
+    mine = AdamW(mine_p, lr=1e-2)
+    mine.load_state_dict(theirs.state_dict())
+    assert all(mine.state[q]["step"] == 3 for q in mine_p)
+    for q, r in zip(p, mine_p):
+        q.grad = torch.randn(q.shape, generator=g).cuda()
+        r.grad = q.grad.clone()
+    theirs.step()
+    mine.step()
+    for q, r in zip(p, mine_p):
+        # both round each of some ten operations on values of at most |p| + 2 lr (|m'| <= 2 r at step 4)
+        assert bool(((q - r).abs() <= 10 * 2.0 ** -24 * (q.abs() + 0.02)).all())
+    with pytest.raises(Vc3dError):
+        AdamW(mine_p, lr=1e-2, state_bits=8).load_state_dict(theirs.state_dict())
+    with pytest.raises(Vc3dError):
+        mine.load_state_dict(torch.optim.AdamW(p, amsgrad=True).state_dict())
+
+
 def test_adamw_refuses_to_be_captured():
     from vc3d.capi import Vc3dError
     from vc3d.optim import AdamW

@@ -722,7 +722,8 @@ __global__ __launch_bounds__(256) void lce_kept_kernel(T* E, long long lde, cons
     __shared__ float by[256], at[256];
     __shared__ int label[256];
     __shared__ float sums[4][64][PER + 1];
-    const int count = rows[N], s0 = blockIdx.y * tile, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int cols = (V + 64 * PER - 1) / (64 * PER), st = blockIdx.x / cols;
+    const int count = rows[N], s0 = st * tile, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     if (s0 >= count || rows[N + 2] != 0) return;
     if (tid < tile) {
         const int s = s0 + tid;
@@ -733,7 +734,7 @@ __global__ __launch_bounds__(256) void lce_kept_kernel(T* E, long long lde, cons
         label[tid] = in ? (int)labels[n] : -PER;  // (a label that is no word: EPI_KEEP gave up)
     }
     __syncthreads();
-    const int col = (blockIdx.x * 64 + lane) * PER;
+    const int col0 = (blockIdx.x - st * cols) * 64 * PER, col = col0 + lane * PER;
     float cs[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) cs[j] = 0.f;
@@ -768,8 +769,8 @@ __global__ __launch_bounds__(256) void lce_kept_kernel(T* E, long long lde, cons
     for (int j = 0; j < PER; ++j) sums[wave][lane][j] = cs[j];
     __syncthreads();
     for (int c = tid; c < 64 * PER; c += 256) {
-        const int l = c / PER, j = c % PER, at_ = blockIdx.x * 64 * PER + c;
-        if (at_ < V) dbpart[(long long)blockIdx.y * lde + at_] = (sums[0][l][j] + sums[1][l][j]) + (sums[2][l][j] + sums[3][l][j]);
+        const int l = c / PER, j = c % PER;
+        if (col0 + c < V) dbpart[(long long)st * lde + col0 + c] = (sums[0][l][j] + sums[1][l][j]) + (sums[2][l][j] + sums[3][l][j]);
     }
 }
 // what is stored last: workgroup i < N the row i of the list of dx (its splits' sums; zeros for a row that does not count), the
@@ -851,12 +852,11 @@ struct Plan {
     // with `keep` also: ref [N], P at the label [N], the exponentials, which become P, and db's partial sums
     static size_t plab_at(int N, int D, int elem) { return ref_at(N, D, elem) + list_at(N); }
     static size_t exps_at(int N, int D, int elem) { return plab_at(N, D, elem) + list_at(N); }
-    static size_t exps(int N, int V, int elem) { return ((size_t)N + 255) / 256 * 256 * (((size_t)V + 255) / 256 * 256) * elem; }
+    static size_t row_tiles(int N, int V) { return ((size_t)N + pick_tile(N, V) - 1) / pick_tile(N, V); }
+    static size_t exps(int N, int V, int elem) { return row_tiles(N, V) * pick_tile(N, V) * (((size_t)V + 255) / 256 * 256) * elem; }
     static size_t dbpart_at(int N, int D, int V, int elem) { return exps_at(N, D, elem) + exps(N, V, elem); }
     static size_t saved(int N, int D, int V, int elem, bool keep) {
-        if (!keep) return ref_at(N, D, elem);
-        const size_t tile = pick_tile(N, V);
-        return dbpart_at(N, D, V, elem) + (N + tile - 1) / tile * (((size_t)V + 255) / 256 * 256) * 4;
+        return keep ? dbpart_at(N, D, V, elem) + row_tiles(N, V) * (((size_t)V + 255) / 256 * 256) * 4 : ref_at(N, D, elem);
     }
     Plan(int N, int D, int V, int elem, int op, bool pack, bool keep) {
         kd = (D * elem + 15) / 16 * 16 / elem;
@@ -982,8 +982,8 @@ int fwd(const VcLceParams& p, hipStream_t s) {
     hipLaunchKernelGGL(lce_rows_kernel, dim3((p.N + 15) / 16), dim3(1024), 0, s, part, L.tiles, zlab, p.labels, src.rows, p.N, p.V, src.lse,
                        loss_rows, src.plab, p.reduction == 1, p.reduction != 0 ? p.loss : nullptr);
     if (p.keep) {
-        hipLaunchKernelGGL((lce_kept_kernel<T>), dim3((p.V * (int)sizeof(T) + 1023) / 1024, (p.N + L.tile - 1) / L.tile), dim3(256), 0, s, src.exps,
-                           L.lde, src.rows, src.lse, src.ref, src.plab, p.labels, p.N, p.V, L.tile, src.dbpart);
+        hipLaunchKernelGGL((lce_kept_kernel<T>), dim3((p.V + 1024 / (int)sizeof(T) - 1) / (1024 / (int)sizeof(T)) * ((p.N + L.tile - 1) / L.tile)),
+                           dim3(256), 0, s, src.exps, L.lde, src.rows, src.lse, src.ref, src.plab, p.labels, p.N, p.V, L.tile, src.dbpart);
         // where EPI_KEEP gave up (4.7 us of workgroups that leave at once where it did not)
         g.when = gave_up, g.lse = src.lse;
         for (int v0 = 0; v0 < p.V; v0 += L.piece) {

@@ -716,11 +716,14 @@ def _same_device(ref, **others):
             raise capi.Vc3dError("%s is on %s, not on %s" % (name, t.device, ref.device))
 
 
+def _has_rows(t):
+    """whether a matrix's last dimension is contiguous and its rows do not overlap"""
+    return t.is_contiguous() or (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+
+
 def _rows(t):
-    """a matrix whose last dimension is contiguous and whose rows do not overlap: as it is, or a copy"""
-    if t.is_contiguous() or (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
-        return t
-    return t.contiguous()
+    """such a matrix: as it is, or a copy"""
+    return t if _has_rows(t) else t.contiguous()
 
 
 def _ld(t):
@@ -736,6 +739,11 @@ def _linear_ce_desc(x, weight, labels, bias, ignore_index, reduction, keep_bytes
     if V == 0 or D == 0:
         raise capi.Vc3dError("linear_ce: no classes or no features (weight %s)" % (tuple(weight.shape),))
     _same_device(x, weight=weight, labels=labels, bias=bias)
+    for name, t in (("x", x), ("weight", weight)):
+        if not _has_rows(t):
+            raise capi.Vc3dError("linear_ce: %s needs contiguous rows that do not overlap (strides %s)" % (name, tuple(t.stride())))
+    if not labels.is_contiguous() or bias is not None and not bias.is_contiguous():
+        raise capi.Vc3dError("linear_ce: labels and bias must be contiguous")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and t.dtype != x.dtype:
             raise capi.Vc3dError("linear_ce: %s is %s, x is %s" % (name, t.dtype, x.dtype))

@@ -352,13 +352,17 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, sd):
         sd = dict(sd)
-        if sd.pop("state_bits", self.state_bits) != self.state_bits:
+        if sd.pop("state_bits", 32) != self.state_bits:  # (torch.optim.AdamW's states name no bits: fp32 ones are taken over)
             raise Vc3dError("AdamW: the saved moments are not held in %d bits" % self.state_bits)
+        if any(g.get("amsgrad") or g.get("maximize") for g in sd["param_groups"]):
+            raise Vc3dError("AdamW: amsgrad and maximize are not supported")
         saved = sd["state"]
         super().load_state_dict(sd)
         # torch casts what it loads to the parameter's type: the moments keep theirs
         ids = [i for g in sd["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             for k, v in saved.get(i, {}).items():
-                if torch.is_tensor(v):
+                if k == "step":
+                    self.state[p][k] = int(v)
+                elif torch.is_tensor(v):
                     self.state[p][k] = v.detach().to(p.device, copy=True)

@@ -12,9 +12,8 @@ from .capi import Vc3dError
 
 class _GatedScanFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, gates, h0, lengths, reverse):
+    def forward(ctx, gates, h0, lengths, reverse, grad):
         ctx.set_materialize_grads(False)
-        grad = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
         d = ops._scan_desc(gates, lengths, reverse)
         if h0 is not None:
             ops._same_device(gates, h0=h0)
@@ -28,11 +27,11 @@ class _GatedScanFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast):
         if dy is None and dlast is None:
-            return None, None, None, None
+            return None, None, None, None, None
         gates, lengths, states = ctx.saved_tensors
         want = ctx.needs_input_grad
         dgates, dh0 = ops._gated_scan_bwd(ctx.desc, gates, lengths, states, _aligned(dy), None if dlast is None else dlast.contiguous(), want[1])
-        return dgates if want[0] else None, dh0, None, None
+        return dgates if want[0] else None, dh0, None, None, None
 
 
 def _aligned(t):
@@ -63,7 +62,8 @@ def gated_scan(gates, h0=None, lengths=None, reverse=False):
         lengths = lengths.contiguous() if lengths.dtype == torch.int32 else lengths.clamp(0, T).to(torch.int32)
     if gates.shape[2] and gates.stride(2) != 1:
         gates = gates.contiguous()
-    return _GatedScanFn.apply(gates, h0, lengths, bool(reverse))
+    grad = torch.is_grad_enabled() and (gates.requires_grad or h0 is not None and h0.requires_grad)  # whether a backward may come
+    return _GatedScanFn.apply(gates, h0, lengths, bool(reverse), grad)
 
 
 def gated_scan_step(gates, state):
@@ -73,7 +73,8 @@ def gated_scan_step(gates, state):
 
 
 class PackedGateWeight:
-    """bf16 forward / weight-gradient operand of a gate projection and its data-gradient twin, rebuilt when the master changed"""
+    """bf16 forward / weight-gradient operand of a gate projection and its data-gradient twin, rebuilt when the master changed (by
+    its version counter, as the engine's and the LSTM's operands: a write through ``weight.data`` is not seen)"""
 
     def __init__(self):
         self.key = self.wf = self.wd = None
