@@ -258,3 +258,25 @@ def test_a_captured_step_replays():
         ops.adamw_step(*tcols, step=4, **HYPER)
         torch.cuda.synchronize()
         assert all(same(a, b) for x, y in zip(dev, twin) for a, b in zip(x, y))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_2_31_elements(bits):
+    """the end of a long tensor moves as a short tensor of the same values does"""
+    import vc3d
+    n, tail = (1 << 31) + 300, 300  # (2^31 is whole blocks)
+    g = torch.Generator().manual_seed(61)
+    ends = [torch.randn(tail, generator=g).bfloat16().cuda() for _ in range(2)]
+    out = []
+    for size in (tail, n):
+        p, gr = (torch.zeros(size, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        p[-tail:], gr[-tail:] = ends[0], ends[1]
+        kind = torch.float32 if bits == 32 else torch.float8_e4m3fn
+        m, v = (torch.zeros(size, dtype=kind, device="cuda") for _ in range(2))
+        ms, vs = ([torch.zeros((size + 255) // 256, device="cuda")] if bits == 8 else None for _ in range(2))
+        for step in (1, 2):
+            vc3d.ops.adamw_step([p], [gr], [m], [v], ms, vs, lr=1e-2, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.1, step=step)
+        out.append([p[-tail:].clone(), m[-tail:].float(), v[-tail:].float()] + ([ms[0][-2:].clone(), vs[0][-2:].clone()] if bits == 8 else []))
+        assert not bool(p[:-tail].any())
+        del p, gr, m, v, ms, vs
+    assert all(torch.equal(a, b) for a, b in zip(*out))

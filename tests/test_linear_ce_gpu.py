@@ -355,3 +355,36 @@ def test_captured_graphs_replay(keep):
         torch.cuda.synchronize()
         for t, out in zip(ins, outs):
             assert all(torch.equal(a, b) for a, b in zip(once(t), out))
+
+
+@pytest.mark.parametrize("keep", [0, ALL])
+def test_more_than_2_31_logits(keep):
+    """33000 rows of 66000 words: offsets into the kept gradient of the logits pass 2^31 elements; the last rows and words"""
+    import vc3d
+    N, D, V, last = 33000, 64, 66000, 50
+    x, w, b, y = make(N, D, V, torch.bfloat16, True, seed=51, scale=1.0)
+    y[::9] = -100
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    loss = vc3d.linear_cross_entropy(x, w, y, b, keep_bytes=keep)
+    dx, dw, db = torch.autograd.grad(loss, leaves)
+    X, W, B = x.detach().double(), w.detach().double(), b.detach().double()
+    kept = y != -100
+    at = torch.where(kept, y, torch.zeros_like(y))
+    n = int(kept.sum())
+    lse = torch.cat([torch.logsumexp(X[i:i + 3000] @ W.t() + B, 1) for i in range(0, N, 3000)])
+    rows = torch.where(kept, lse - ((X * W[at]).sum(1) + B[at]), torch.zeros_like(lse))
+    S = float((X.abs().amax(0) * W.abs().amax(0)).sum() + B.abs().max())  # of |x| |w| + |b|, over all
+    rel = 2 * (D + 8) * E * S + (64 + V / 16) * E + 128 * E
+    check(loss, rows.sum() / n, torch.tensor(rel, device="cuda") + rows.abs().sum() / n * E, "loss")
+    h = HALF[torch.bfloat16]
+    hp = 2 * h + h * h
+    for what, got, r, v in (("dx", dx[-last:], slice(N - last, N), slice(0, V)), ("dw", dw[-last:], slice(0, N), slice(V - last, V))):
+        p = (X[r] @ W[v].t() + B[v] - lse[r, None]).exp()
+        hot = at[r, None] == torch.arange(V, device="cuda")[v]
+        P, Pa = [torch.where(kept[r, None], q / n, torch.zeros_like(p)) for q in (p - hot.double(), p + hot.double())]
+        want = P @ W[v] if what == "dx" else P.t() @ X[r]
+        size = Pa @ W[v].abs() if what == "dx" else Pa.t() @ X[r].abs()
+        check(got, want, size * (rel + hp + (max(N, V) + 8) * E) + h * want.abs() + UNDER * max(N, V) * 8, what)
+        if what == "dw":
+            want = P.sum(0)
+            check(db[-last:], want, Pa.sum(0) * (rel + hp + (N + 8) * E) + h * want.abs() + UNDER * N, "db")

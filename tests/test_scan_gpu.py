@@ -290,3 +290,30 @@ def test_two_captured_graphs_replay():
         torch.cuda.synchronize()
         for x, out in zip(ins, outs):
             assert all(torch.equal(a, b) for a, b in zip(once(x), out))
+
+
+def test_more_than_2_31_elements():
+    """one sequence whose gates pass 2^31 elements: its ends, against 400 steps around them (what lies further off is forgotten:
+    a product of 300 gates is below 2^-100)"""
+    import vc3d
+    T, H, near = 140000, 8192, 100
+    torch.manual_seed(41)
+    gates = torch.randn(1, T, 2 * H, dtype=torch.bfloat16, device="cuda")
+    gates[..., :H] += 1
+    dy = torch.randn(1, T, H, dtype=torch.bfloat16, device="cuda")
+    gates.requires_grad_()
+    h, last = vc3d.gated_scan(gates)
+    dgates, = torch.autograd.grad((h, last), gates, (dy, torch.ones_like(last)))
+    g = gates.detach()
+    M, z = 8.0, 8.0  # (normal values of 8 bits' mantissa: below)
+    half = HALF[torch.bfloat16]
+    for first in (True, False):
+        at = slice(0, 400) if first else slice(T - 400, T)
+        eh, el, eg, _, L = reference(g[:, at].clone(), None, None, False, dy[:, at], torch.zeros(1, H) if first else torch.ones(1, H))
+        part = slice(0, near) if first else slice(400 - near, 400)
+        C = 400 * 2 * (11 + z) * 2.0 ** -24
+        assert float(g[:, at].float().abs().max()) < M
+        check(h[:, at][:, part], eh[:, part], C * M, half, "h")
+        check(dgates[:, at][:, part, H:], eg[:, part, H:], C * L, half, "dv")
+        check(dgates[:, at][:, part, :H], eg[:, part, :H], C * 4 * M * L, half, "dz")
+    check(last, el, C * M, 2.0 ** -24, "last")

@@ -301,3 +301,44 @@ def test_clipping_by_a_scale_on_the_device():
         AdamW([p], lr=1e-2).step(grad_scale=scale if kind else float(scale))
         out.append(p.detach())
     assert torch.equal(out[0], out[1])
+
+
+@pytest.mark.parametrize("op", ["scan", "lce"])
+def test_public_entries_captured_with_their_backward(op):
+    """forward and backward through autograd in one graph, replayed with new inputs between eager work on other leaves.  (The
+    leaves' own eager graphs are gone when the capture begins.)"""
+    import vc3d
+    g = torch.Generator().manual_seed(31)
+    lengths = torch.tensor([500, 0, 700], dtype=torch.int32).cuda()
+    if op == "scan":
+        leaves = [torch.randn(3, 700, 160, generator=g).cuda(), torch.randn(3, 80, generator=g).cuda()]
+        up = torch.randn(3, 700, 80, generator=g).cuda()
+
+        def once(a, b):
+            h, last = vc3d.gated_scan(a, b, lengths=lengths)
+            return (h.detach(), last.detach()) + torch.autograd.grad((h, last), (a, b), (up, last.detach()))
+    else:
+        leaves = [torch.randn(600, 512, generator=g).bfloat16().cuda(), (torch.randn(16000, 512, generator=g) / 16).bfloat16().cuda()]
+        y = torch.randint(0, 16000, (600,), generator=g).cuda()
+
+        def once(a, b):
+            loss = vc3d.linear_cross_entropy(a, b, y)
+            return (loss.detach(),) + torch.autograd.grad(loss, (a, b))
+    leaves = [t.requires_grad_() for t in leaves]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            once(*leaves)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once(*leaves)
+    for rep in range(3):
+        with torch.no_grad():
+            for t in leaves:
+                t.copy_(torch.randn(t.shape, generator=g) * (0.5 + rep) / (1 if op == "scan" else 4))
+        want = once(*[t.detach().clone().requires_grad_() for t in leaves])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
