@@ -86,7 +86,7 @@ def test_c_entry_of_the_linear_cross_entropy_refuses():
     assert fwd(ok(), w=PTR + 2) == -2 and b"modulo 16" in c.lib.vc_last_error()  # the descriptor says that w is aligned
     # what is left for the backward: a few words a row, copies of x while they are small
     assert c.lib.vc_linear_ce_saved_bytes(ok()) >= 100 * 8 + 100 * 128 and c.lib.vc_linear_ce_saved_bytes(ok(N=1 << 20, D=512, ldx=512, ldw=512, keep_bytes=0)) < 16 << 20
-    assert c.lib.vc_linear_ce_saved_bytes(ok(keep_bytes=1 << 20)) >= 256 * 1024 * 2
+    assert c.lib.vc_linear_ce_saved_bytes(ok(keep_bytes=1 << 20)) >= 100 * 1000 * 2
     # no N x V block: one piece's P, sums of dx, a pair for every row and tile
     n = need(ok(N=8192, D=2048, V=1 << 20, ldx=2048, ldw=2048), 1)
     assert n < 1.2e9 and n < 8192 * (1 << 20) * 2 / 10

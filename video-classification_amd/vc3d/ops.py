@@ -4,7 +4,7 @@ Every wrapper checks device, dtype, contiguity and element counts on the host be
 launch: a kernel that reads past a buffer can take the whole GPU down.  torch is used for
 device memory and the current stream only.
 """
-import array
+import ctypes as C
 
 import torch
 
@@ -680,8 +680,12 @@ def linear_bwd(dlogits, feat, W, dW=None, db=None, want_dfeat=True):
 # current stream) and bring their own workspace from torch's allocator, per call: nothing is shared between calls, streams or
 # captured graphs.
 
-_E4M3 = torch.float8_e4m3fn
-_get_device, _numel, _data_ptr, _is_contiguous = (torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous)
+try:
+    from . import _tensors
+except ImportError as e:
+    raise capi.Vc3dError("vc3d/_tensors.so could not be loaded (%s): build it with `make -C video-classification_amd/csrc`" % e)
+
+_FLOAT_KIND = {F32: 0, BF16: 1}
 ADAMW_BLOCK = 256  # elements that share a scale of an 8-bit moment
 SCAN_STATE_STEPS = 64  # steps between two saved states
 
@@ -883,18 +887,6 @@ def gated_scan_step(gates, state):
     return h
 
 
-def _dense(t):
-    """whether a tensor's elements fill one stretch of memory, each once, in whatever order of dimensions"""
-    if t.is_contiguous():
-        return True
-    at = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
-        if stride != at:
-            return False
-        at *= size
-    return True
-
-
 def adamw_step(params, grads, exp_avg, exp_avg_sq, m_scale=None, v_scale=None, *, lr, beta1, beta2, eps, weight_decay, step,
                grad_scale=None):
     """one AdamW step, in place, over lists of tensors (vc_adamw_step).  params and grads are fp32 or bf16; exp_avg and
@@ -907,40 +899,13 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, m_scale=None, v_scale=None, *
     if eight != (v_scale is not None):
         raise capi.Vc3dError("adamw_step: 8-bit moments need m_scale and v_scale, 32-bit ones neither")
     lists = (params, grads, exp_avg, exp_avg_sq) + ((m_scale, v_scale) if eight else ())
-    if any(len(x) != n for x in lists):
-        raise capi.Vc3dError("adamw_step: the lists have %s entries" % ([len(x) for x in lists],))
+    # hundreds of small tensors are a step whose time is what is asked of each: that is done in one call (csrc/tensors.cpp)
+    table = bytearray(56 * n)  # vc_adamw_tensor [n]
+    wrong = _tensors.adamw_table(lists, table)
+    if wrong:
+        raise capi.Vc3dError("adamw_step: " + wrong)
     if n == 0:
         return
-    kind, dt = _float_kind(params[0], "params[0]"), params[0].dtype
-    # list by list: hundreds of small tensors are a step whose time is this
-    types = (dt, dt, _E4M3 if eight else F32, _E4M3 if eight else F32, F32, F32)
-    names = ("params", "grads", "exp_avg", "exp_avg_sq", "m_scale", "v_scale")
-    for name, want, ts in zip(names, types, lists):
-        if {t.dtype for t in ts} != {want}:
-            raise capi.Vc3dError("adamw_step: %s are %s; %s expected" % (name, {t.dtype for t in ts}, want))
-        if set(map(_get_device, ts)) != {params[0].get_device()}:
-            raise capi.Vc3dError("adamw_step: %s are not all on %s" % (name, params[0].device))
-    sizes = list(map(_numel, params))
-    if eight:
-        rows = [(k + ADAMW_BLOCK - 1) // ADAMW_BLOCK for k in sizes]
-        for name, ts in zip(names[4:], lists[4:]):
-            if list(map(_numel, ts)) != rows or not all(map(_is_contiguous, ts)):
-                raise capi.Vc3dError("adamw_step: %s hold ceil(numel / %d) contiguous values each" % (name, ADAMW_BLOCK))
-    shapes = [t.shape for t in params]
-    for name, ts in zip(names[1:4], lists[1:4]):
-        if [t.shape for t in ts] != shapes:
-            raise capi.Vc3dError("adamw_step: %s and params differ in shape" % name)
-    if not all(all(map(_is_contiguous, ts)) for ts in lists[:4]):
-        for i, (p, g, m, v) in enumerate(zip(*lists[:4])):
-            if not _dense(p) or sizes[i] > 1 and not g.stride() == m.stride() == v.stride() == p.stride():
-                raise capi.Vc3dError("adamw_step: tensor %d and its gradient and moments must lie in memory in one dense order" % i)
-    table = array.array("q", bytes(56 * n))
-    for k, ts in enumerate(lists):
-        table[k::7] = array.array("q", map(_data_ptr, ts))
-    table[6::7] = array.array("q", sizes)
-    starts = [q for q, k in zip(table[::7], sizes) if k]
-    if len(set(starts)) != len(starts):
-        raise capi.Vc3dError("adamw_step: a parameter is in the list twice")
     scale, scale_dev = 1.0, None
     if torch.is_tensor(grad_scale):
         _chk(grad_scale, F32, 1, "grad_scale")
@@ -949,11 +914,12 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, m_scale=None, v_scale=None, *
     elif grad_scale is not None:
         scale = float(grad_scale)
     hyper = capi.AdamwHyper(lr, beta1, beta2, eps, weight_decay, scale, step)
+    if capi.RECORDER is not None:
+        capi.RECORDER.failed = "adamw_step: its table of tensors lives for the call"
     with _on(params[0]):
-        check(lib.vc_adamw_step(table.buffer_info()[0], n, kind, 8 if eight else 32, hyper, ptr(scale_dev), cur_stream()), "vc_adamw_step")
-    for ts in lists:
-        if ts is not grads:
-            torch._C._increment_version(ts)
+        check(lib.vc_adamw_step(C.addressof(C.c_char.from_buffer(table)), n, _FLOAT_KIND[params[0].dtype], 8 if eight else 32, hyper,
+                                ptr(scale_dev), cur_stream()), "vc_adamw_step")
+    _tensors.written(params, *lists[2:])
 
 
 def ncthw_to_nthwc(x):
