@@ -9,6 +9,8 @@
 #include <string>
 #include <vector>
 
+#include "autograd.h"
+
 namespace {
 
 constexpr int64_t BLOCK = 256;  // VC_ADAMW_BLOCK
@@ -118,7 +120,13 @@ PyObject* written(PyObject*, PyObject* args) {
     Py_RETURN_NONE;
 }
 
-PyMethodDef METHODS[] = {{"adamw_table", adamw_table, METH_VARARGS, nullptr}, {"written", written, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+PyMethodDef METHODS[] = {{"adamw_table", adamw_table, METH_VARARGS, nullptr},
+                         {"written", written, METH_VARARGS, nullptr},
+                         {"bind", vc_bind, METH_VARARGS, nullptr},
+                         {"gated_scan", vc_gated_scan_py, METH_VARARGS, nullptr},
+                         {"gated_scan_step", vc_gated_scan_step_py, METH_VARARGS, nullptr},
+                         {"linear_cross_entropy", vc_linear_cross_entropy_py, METH_VARARGS, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, METHODS, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -9,39 +9,34 @@ from .capi import Vc3dError
 _REDUCTION = {"none": 0, "mean": 1, "sum": 2}
 
 
-class _LinearCEFn(torch.autograd.Function):
-    """when ``engine`` is given, the gradients of weight and bias go to its flat buffer, as with autograd.linear_apply"""
+class _EngineHeadFn(torch.autograd.Function):
+    """linear_cross_entropy of a head whose weight and bias live in an engine's flat buffers: their gradients go there, as with
+    autograd.linear_apply"""
 
     @staticmethod
-    def forward(ctx, x, weight, labels, bias, ignore_index, reduction, engine, keep_bytes):
-        d = ops._linear_ce_desc(x, weight, labels, bias, ignore_index, reduction, keep_bytes)
-        loss, saved = ops._linear_ce_fwd(d, x, weight, labels, bias)
-        if any(ctx.needs_input_grad):
+    def forward(ctx, x, weight, bias, labels, engine):
+        grad = any(ctx.needs_input_grad)
+        loss, saved = ops.linear_ce_fwd(x, weight, labels, bias, keep_bytes=-1 if grad else 0)
+        if grad:
             ctx.save_for_backward(x, weight, labels, bias, saved)
-            ctx.desc, ctx.engine, ctx.params = d, engine, (weight, bias)
-        return loss if reduction == 0 else loss.view(())
+            ctx.engine, ctx.params = engine, (weight, bias)
+        return loss.view(())
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         x, weight, labels, bias, saved = ctx.saved_tensors
         want, eng = ctx.needs_input_grad, ctx.engine
-        dx, dw, db = ops._linear_ce_bwd(ctx.desc, x, weight, labels, bias, saved, dloss.contiguous(), (want[0], want[1], want[3]))
+        dx, dw, db = ops.linear_ce_bwd(x, weight, labels, bias, saved, dloss.contiguous().view(1), want=want[:3])
         wp, bp = ctx.params
-        if eng is not None and eng.flat_grad is not None and id(wp) in eng.grad_views:
+        if eng.flat_grad is not None and id(wp) in eng.grad_views:
             eng._bind_grads()
             for p, g in ((wp, dw), (bp, db)):
                 if g is not None:
                     eng.gview(p).add_(g)
             eng._ready(wp, *([bp] if bp is not None else []))
             dw = db = None
-        return dx, dw, None, db, None, None, None, None
-
-
-def _apply(x, weight, labels, bias, ignore_index, reduction, engine, keep_bytes):
-    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad)):
-        keep_bytes = 0  # no backward will come
-    return _LinearCEFn.apply(x, weight, labels, bias, ignore_index, _REDUCTION[reduction], engine, keep_bytes)
+        return dx, dw, db, None, None
 
 
 def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduction="mean", keep_bytes=-1):
@@ -52,19 +47,9 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     gradients are of the inputs' type.  keep_bytes: whether the forward keeps the logits' gradient for the
     backward (N x V of the inputs' type): 0 no, the backward computes the logits again; n: where it takes at most n bytes; -1: where
     that is quicker and takes at most 2 GB.  Never with reduction "none"."""
-    if not torch.is_tensor(x) or not x.is_cuda:
-        raise Vc3dError("linear_cross_entropy runs on the GPU only (no CPU fallback)")
     if reduction not in _REDUCTION:
         raise Vc3dError("linear_cross_entropy: reduction 'none', 'mean' or 'sum', got %r" % (reduction,))
-    if x.dim() < 1 or x.shape[-1] == 0 or weight.dim() != 2 or tuple(labels.shape) != tuple(x.shape[:-1]):
-        raise Vc3dError("linear_cross_entropy: x [..., D], weight [V][D] and labels [...] expected, got %s, %s, %s" %
-                        (tuple(x.shape), tuple(weight.shape), tuple(labels.shape)))
-    shape = labels.shape
-    if x.dim() != 2:
-        x, labels = x.reshape(-1, x.shape[-1]), labels.reshape(-1)
-    loss = _apply(ops._rows(x), ops._rows(weight), labels.contiguous(), None if bias is None else bias.contiguous(),
-                  int(ignore_index), reduction, None, int(keep_bytes))
-    return loss.view(shape) if reduction == "none" else loss
+    return ops._tensors.linear_cross_entropy(x, weight, labels, bias, ignore_index, _REDUCTION[reduction], keep_bytes)
 
 
 class HeadScores:
@@ -76,7 +61,9 @@ class HeadScores:
 
     def cross_entropy(self, y):
         """mean cross-entropy against y (int64 [N]), differentiable in the features and the head's parameters"""
-        return _apply(self.feat.contiguous(), self.weight, y.contiguous(), self.bias, -100, "mean", self.engine, -1)
+        if self.engine is None:
+            return linear_cross_entropy(self.feat, self.weight, y, self.bias)
+        return _EngineHeadFn.apply(self.feat.contiguous(), self.weight, self.bias, y.contiguous(), self.engine)
 
     def scores(self):
         from .autograd import linear_apply

@@ -10,60 +10,12 @@ from . import ops
 from .capi import Vc3dError
 
 
-class _GatedScanFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gates, h0, lengths, reverse, grad):
-        ctx.set_materialize_grads(False)
-        d = ops._scan_desc(gates, lengths, reverse)
-        if h0 is not None:
-            ops._same_device(gates, h0=h0)
-        h, last, states = ops._gated_scan_fwd(d, gates, h0, lengths, grad)
-        if grad:
-            ctx.save_for_backward(gates, lengths, states)
-            ctx.desc = d
-        return h, last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dlast):
-        if dy is None and dlast is None:
-            return None, None, None, None, None
-        gates, lengths, states = ctx.saved_tensors
-        want = ctx.needs_input_grad
-        dgates, dh0 = ops._gated_scan_bwd(ctx.desc, gates, lengths, states, _aligned(dy), None if dlast is None else dlast.contiguous(), want[1])
-        return dgates if want[0] else None, dh0, None, None, None
-
-
-def _aligned(t):
-    """contiguous and at a multiple of two elements (a slice's storage may begin anywhere)"""
-    if t is None:
-        return None
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % (2 * t.element_size()) else t
-
-
 def gated_scan(gates, h0=None, lengths=None, reverse=False):
     """gates [B][T][2H] (fp32 or bf16; logits of the forget gate, then values; e.g. one GEMM's output), h0 [B][H] fp32 (zeros if
     None), lengths int32 or int64 [B] on the GPU (sequence b is its first lengths[b] steps; all T if None), reverse: from a
     sequence's last step to its first -> (h [B][T][H], last state [B][H] fp32).  h and the gradient of gates are 0 behind a
     sequence's end, whatever gates hold there; last is h0 where there is no step.  Differentiable in gates and h0."""
-    if not torch.is_tensor(gates) or not gates.is_cuda:
-        raise Vc3dError("gated_scan runs on the GPU only (no CPU fallback)")
-    if gates.dim() != 3:
-        raise Vc3dError("gated_scan: gates [B][T][2H] expected, got %s" % (tuple(gates.shape),))
-    B, T, H = gates.shape[0], gates.shape[1], gates.shape[2] // 2
-    if h0 is not None:
-        if h0.dtype != torch.float32 or tuple(h0.shape) != (B, H):
-            raise Vc3dError("gated_scan: h0 fp32 [%d][%d] expected, got %s %s" % (B, H, h0.dtype, tuple(h0.shape)))
-        h0 = h0.contiguous()
-    if lengths is not None:
-        if not torch.is_tensor(lengths) or lengths.dtype not in (torch.int32, torch.int64) or tuple(lengths.shape) != (B,):
-            raise Vc3dError("gated_scan: lengths int32 or int64 [%d] on the GPU expected" % B)
-        lengths = lengths.contiguous() if lengths.dtype == torch.int32 else lengths.clamp(0, T).to(torch.int32)
-    if gates.shape[2] and gates.stride(2) != 1:
-        gates = gates.contiguous()
-    grad = torch.is_grad_enabled() and (gates.requires_grad or h0 is not None and h0.requires_grad)  # whether a backward may come
-    return _GatedScanFn.apply(gates, h0, lengths, bool(reverse), grad)
+    return ops._tensors.gated_scan(gates, h0, lengths, reverse)
 
 
 def gated_scan_step(gates, state):
