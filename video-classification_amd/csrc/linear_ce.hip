@@ -8,7 +8,12 @@
 // rows; a second launch joins a row's pairs.  Backward: the vocabulary goes by in pieces; a piece's logits are computed
 // again, turned into P (rounded once, to the operands' type, for the two matrix products that read it) and multiplied into
 // dx and dw.  A factor g common to all rows stays out of P: P at the label is close to -1 in every row, and g times that would
-// round by the same amount in all of them, an error that adds up (measured: 3.5e-3 of dw instead of 2.3e-3 with bf16).  N x V is never held: the forward keeps N floats, the backward one N x piece block.
+// round by the same amount in all of them, an error that adds up (measured: 3.5e-3 of dw instead of 2.3e-3 with bf16).  N x V is
+// never held.
+// Where memory allows and it is quicker (vc_lce_keep), the forward keeps more: tiles store exp(z - ref) with ref = the logit of
+// the row's own label, which is known beforehand (EPI_KEEP); once the row's sum is known a pass over them makes P of them, where
+// they lie, and the backward is its two products.  ref is at most the row's maximum, so nothing of weight underflows; where some
+// exp(z - ref) passes 2^64 the forward computes P as the backward would have.
 //
 // Rows whose label is ignore_index take no part: the rows that count are listed first (rows_kernel) and all products run
 // over that list, so that an ignored row costs nothing and whatever it holds (NaN included) reaches nothing.
@@ -45,17 +50,24 @@ __global__ __launch_bounds__(1024) void rows_kernel(const long long* labels, lon
 }
 
 // ---------------------------------------------------------------- matrix products
-// out[s][r] = sum_k S(s, k) R(r, k).  A workgroup of WR x WS waves makes a BR x BS tile, a wave BR/WR x BS/WS of it, in steps
-// of 64 bytes of k (32 bf16, 16 fp32: one fragment).  The operands' tiles come in by DMA (global_load_lds, 16 bytes a lane)
-// into a ring of four buffers, three steps ahead of their use.  An operand lies in memory with k contiguous (rows of x, w; P
-// for dx) or with its rows contiguous and k across (w for dx; x and P for dw: nothing is transposed in memory):
-//   k contiguous: LDS rows of 64 bytes; a fragment is one ds_read_b128.  The 16-byte chunk c of row r lies at slot
-//     c ^ turn(r / 4 % 4), turn = 0 2 3 1: of the sixteen lanes that one cycle pair serves, whether they are rows 0-15 of one
+// out[s][r] = sum_k S(s, k) R(r, k).  A workgroup of WR x WS waves makes a BR x BS tile (256, 128 or 64 square), a wave BR/WR x
+// BS/WS of it, in steps of one or two fragments of k (a fragment: 32 bf16 or 16 fp32, 64 bytes; Feed says which).  The operands'
+// tiles come in by DMA (global_load_lds, 16 bytes a lane) into a ring of two or four buffers, one or three steps ahead of their
+// use.  An operand lies in memory with k contiguous (rows of x, w; P for dx) or with its rows contiguous and k across (w for dx;
+// x and P for dw: nothing is transposed in memory):
+//   k contiguous: LDS rows of 64 or 128 bytes; a fragment is one ds_read_b128.  The 16-byte chunk c of row r lies at slot
+//     c ^ turn(r): of the sixteen lanes that one cycle pair serves, whether they are rows 0-15 of one
 //     chunk or rows 0-3, 12-15 of one and 4-11 of the next, no two meet in a bank (measured: 0 conflicts).
 //   k across: LDS rows of one k each.  bf16: fragments come through ds_read_b64_tr_b16, which hands lane i of 16 the i-th
 //     column of four rows; a lane group reads four rows x 32 bytes, so the 32-byte unit u of row k lies at u ^ f(k) with f
 //     different for the eight rows that half a wave reads at once.  fp32: one ds_read_b32 a value, units of 64 bytes at u ^ (k / 4 % 4).
 // The swizzles act on the DMA's source address: what a lane fetches, not where it lands.
+// Bound by the matrix cores' issue: the loops of 256 x 256 tiles run at some 1.25 PFLOP/s (59 % of the cycles issue a matrix
+// instruction, at 2.1 GHz), near what a large library product reaches here (1.33).  1843 rows x 1024 of 32768, us: EPI_STATS 133,
+// EPI_KEEP 156, EPI_PROB 156, EPI_DX 133, EPI_DW 120 (123.7 GFLOP each); 7373 x 2048 of 65536: 1555, 1791, 1898, 1734, 1573 (1979
+// GFLOP each).  The difference of the first three is the epilogue's stores.  What did not help: fragments read four slots ahead
+// or raised wave priority (within 1 %), rows of 64 bytes of k for the forward (+15 %), touching the next lines early (+10 %),
+// workgroups that stay and fetch their next tile during the epilogue (+33 %: registers spill).
 // Nothing is read outside the operands: rows and columns behind the end are read from a row or column inside (what they make
 // is not stored), k behind the end from a page of zeros (k contiguous) or, with k across, from a k inside, where the other
 // operand, P, is 0 (EPI_PROB writes whole tiles of P, zeros behind the last row and the last word).
@@ -881,9 +893,9 @@ struct Plan {
         // 338 us with 256, 275 with 128; 1600 x 1000 of 50257, 28 tiles: 794 against 845; 8192 x 2048 of 65536: 6.96 against 7.73 ms)
         tile_dx = N > 128 && D > 128 && (N + 255ll) / 256 * ((D + 255) / 256) >= 16 ? 256 : N > 64 && D > 64 ? 128 : 64;
         tile_dw = pick_tile(piece < V ? piece : V, D);
-        // up to 16 splits, 256 MB of sums
+        // up to 16 splits, 256 MB of sums, 128 words a split (512: 64 x 512 of 400 classes 66 us instead of 61)
         dx = {tile_dx == 256 ? 256 : 512, 16, (D + tile_dx - 1) / tile_dx, tile_dx};
-        const long long room = (256ll << 20) / ((long long)N * D * 4), least = piece / 512;
+        const long long room = (256ll << 20) / ((long long)N * D * 4), least = piece / 128;
         dx.most = (int)(dx.most > room ? room : dx.most);
         dx.most = (int)(dx.most > least ? least : dx.most);
         dx.most = dx.most < 1 ? 1 : dx.most;
@@ -1052,15 +1064,17 @@ bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16) {
 }
 // Whether the forward keeps the logits' gradient for the backward, which then need not compute the logits again: that saves a
 // product and costs storing, reading and storing N x V, and two launches.  By itself up to 2 GB (under 1 % of the memory) and
-// where there is enough to save.  Measured, again / kept in us, bf16: 2048 x 1024 of 32768 555 / 477, 8192 x 2048 of 65536
-// 7170 / 5900, 1000 x 512 of 20000 178 / 159, 4000 x 384 of 32000 553 / 535, 8192 x 256 of 60000 1660 / 1470, 64 x 2048 of 32000
-// 152 / 140; but 8192 x 128 of 60000 1200 / 1332, 512 x 512 of 8192 87 / 90.  fp32: 1000 x 1024 of 32000 2030 / 1590, 1000 x 64 of
-// 20000 214 / 190; but 4000 x 64 of 1000 172 / 171, 300 x 128 of 10000 148 / 152.
+// where there is enough to save: a long sum, or a large product.  Kernels of a step, again / kept in us, bf16: 2048 x 1024 of
+// 32768 555 / 477, 8192 x 2048 of 65536 7170 / 5900, 4000 x 384 of 32000 553 / 535, 8192 x 256 of 60000 1660 / 1470, 512 x 512 of
+// 8192 80 / 74, 30 x 1024 of 1000 45.3 / 43.8, 1 x 2048 of 32000 125 / 110; but 8192 x 128 of 60000 1200 / 1332, 200 x 512 of
+// 8000 59.6 / 61.7.  fp32: 1000 x 1024 of 32000 2030 / 1590, 1000 x 64 of 20000 214 / 190, 64 x 512 of 400 61 / 52; but 300 x 128 of
+// 10000 121.5 / 122.4.
 bool vc_lce_keep(int N, int D, int V, bool is_bf16, int reduction, long long keep_bytes) {
     if (reduction == 0) return false;  // (its rows' factors come with the backward)
     const size_t bytes = Plan::exps(N, V, is_bf16 ? 2 : 4);
     if (keep_bytes >= 0) return bytes <= (size_t)keep_bytes;
-    return bytes <= (size_t)2 << 30 && (double)N * V * D >= (is_bf16 ? 0x1p32 : 0x1p28) && (!is_bf16 || D >= 256);
+    const double work = (double)N * V * D;
+    return bytes <= (size_t)2 << 30 && (is_bf16 ? D >= 1024 || (D >= 256 && work >= 0x1p31) : D >= 512 || work >= 0x1p29);
 }
 size_t vc_lce_saved(int N, int D, int V, bool is_bf16, bool keep) { return Plan::saved(N, D, V, is_bf16 ? 2 : 4, keep); }
 size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, bool keep, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack, keep).bytes; }
