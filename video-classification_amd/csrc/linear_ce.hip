@@ -9,7 +9,7 @@
 // again, turned into P (rounded once, to the operands' type, for the two matrix products that read it) and multiplied into
 // dx and dw.  A factor g common to all rows stays out of P: P at the label is close to -1 in every row, and g times that would
 // round by the same amount in all of them, an error that adds up (measured: 3.5e-3 of dw instead of 2.3e-3 with bf16).  N x V is
-// never held.
+// not held.
 // Where memory allows and it is quicker (vc_lce_keep), the forward keeps more: tiles store exp(z - ref) with ref = the logit of
 // the row's own label, which is known beforehand (EPI_KEEP); once the row's sum is known a pass over them makes P of them, where
 // they lie, and the backward is its two products.  ref is at most the row's maximum, so nothing of weight underflows; where some

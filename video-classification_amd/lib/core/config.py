@@ -49,8 +49,8 @@ config.MODEL.USE_LSTM = False
 # the recurrent head's cell: 'lstm' (the reference's) or 'scan', a gated linear recurrence (models/recurrence.py), which also
 # takes whole sequences of features at once
 config.MODEL.RECURRENT_CELL = 'lstm'
-# training only: the class scores and their cross-entropy as one operator (vc3d.linear_cross_entropy): no logits are kept,
-# for class counts in the tens of thousands
+# training only: the class scores and their cross-entropy as one operator (vc3d.linear_cross_entropy), for
+# class counts in the tens of thousands
 config.MODEL.FUSED_HEAD_LOSS = False
 # raw-frame input (uint8 N x Ts x Hs x Ws x 3 from a decoder): sampling / normalisation done on the GPU by
 # utils.ChooseInput -> vc_clip_pack_u8; mean / std in units of u8 / 255
