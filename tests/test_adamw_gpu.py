@@ -219,14 +219,14 @@ def test_dense_orders_and_refusals():
     ops.adamw_step(*[[t] for t in dev], step=1, **HYPER)
     want = plain_step(p.permute(0, 2, 3, 4, 1), gr.permute(0, 2, 3, 4, 1), m.permute(0, 2, 3, 4, 1), v.permute(0, 2, 3, 4, 1), None, None, 1, **HYPER)
     assert same(dev[0].permute(0, 2, 3, 4, 1).contiguous(), want[0])
-    x = [torch.zeros(8, 8, device="cuda") for _ in range(4)]
+    x = [torch.zeros(8, 8, device="cuda") for _ in range(7)]
     call = lambda *a, **k: ops.adamw_step(*a, **{"step": 1, **HYPER, **k})  # noqa: E731
-    ok = [[t] for t in x]
+    ok = [[t] for t in x[:4]]
     half = torch.zeros(8, 8, device="cuda", dtype=torch.float16)
     for bad in ([[x[0]], [x[1].t()], [x[2]], [x[3]]], [[x[0][:, :4]], [x[1][:, :4]], [x[2][:, :4]], [x[3][:, :4]]],
                 [[x[0], x[0]], [x[1], x[1]], [x[2], x[2]], [x[3], x[3]]], [[x[0]], [x[1].cpu()], [x[2]], [x[3]]],
                 [[x[0]], [x[1].bfloat16()], [x[2]], [x[3]]], [[half], [half], [x[2]], [x[3]]], [[x[0]], [x[1][0]], [x[2]], [x[3]]],
-                [[x[0]], [], [x[2]], [x[3]]]):
+                [[x[0]], [], [x[2]], [x[3]]], [x[:2], x[2:4], [x[4], x[4]], [x[5], x[6]]], [[x[0]], [x[1]], [x[2]], [x[2]]]):
         with pytest.raises(Vc3dError):
             call(*bad)
     for k in (dict(step=0), dict(beta1=1.0), dict(lr=-1.0), dict(eps=-1e-9), dict(weight_decay=-0.1)):

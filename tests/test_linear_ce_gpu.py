@@ -122,6 +122,8 @@ def test_another_ignore_index_and_leading_dimensions():
     want = vc3d.linear_cross_entropy(x, w, y, reduction="none")
     got = vc3d.linear_cross_entropy(x.view(4, 15, 32), w, y.view(4, 15), reduction="none")
     assert got.shape == (4, 15) and torch.equal(got.view(-1), want)
+    one = vc3d.linear_cross_entropy(x[1], w, y[1], reduction="none")  # a row by itself
+    assert one.shape == () and abs(float(one) - float(want[1])) <= 64 * E * (1 + abs(float(want[1])))
 
 
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])

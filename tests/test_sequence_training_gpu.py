@@ -342,3 +342,40 @@ def test_public_entries_captured_with_their_backward(op):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("op", ["scan", "lce"])
+def test_a_gradient_of_a_gradient_is_refused(op):
+    import vc3d
+    x = torch.randn(4, 6, 8, device="cuda", requires_grad=True)
+    if op == "scan":
+        out = vc3d.gated_scan(x)[0].sum()
+    else:
+        out = vc3d.linear_cross_entropy(x, torch.randn(10, 8, device="cuda"), torch.zeros(4, 6, dtype=torch.int64, device="cuda"))
+    first, = torch.autograd.grad(out, x, create_graph=True)
+    assert bool(torch.isfinite(first).all())
+    with pytest.raises(RuntimeError, match="once"):
+        first.sum().backward(retain_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), x)
+
+
+def test_errors_reach_the_caller_as_this_package_s():
+    import vc3d
+    from vc3d.capi import Vc3dError
+    g = torch.zeros(2, 3, 8, device="cuda")
+    x, w, y = torch.zeros(4, 8, device="cuda"), torch.zeros(10, 8, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    for call in (lambda: vc3d.gated_scan(g.half()), lambda: vc3d.gated_scan(g[0]), lambda: vc3d.gated_scan(g[..., :7]),
+                 lambda: vc3d.gated_scan(g, torch.zeros(2, 3, device="cuda")), lambda: vc3d.gated_scan(g, torch.zeros(2, 4)),
+                 lambda: vc3d.gated_scan(g, torch.zeros(2, 4, device="cuda").bfloat16()), lambda: vc3d.gated_scan(g, lengths=[1, 2]),
+                 lambda: vc3d.gated_scan(g, lengths=torch.zeros(3, dtype=torch.int32, device="cuda")),
+                 lambda: vc3d.gated_scan(g, lengths=torch.zeros(2, dtype=torch.int32)), lambda: vc3d.gated_scan(3),
+                 lambda: vc3d.gated_scan_step(g[0], torch.zeros(3, 3, device="cuda")), lambda: vc3d.gated_scan_step(g[0].t(), torch.zeros(8, 1, device="cuda")),
+                 lambda: vc3d.gated_scan_step(g[0], torch.zeros(3, 8, device="cuda")[:, ::2]),
+                 lambda: vc3d.linear_cross_entropy(x, w.bfloat16(), y), lambda: vc3d.linear_cross_entropy(x, w[:, :4], y),
+                 lambda: vc3d.linear_cross_entropy(x, w, y[:3]), lambda: vc3d.linear_cross_entropy(x, w, y.int()),
+                 lambda: vc3d.linear_cross_entropy(x, w, y.cpu()), lambda: vc3d.linear_cross_entropy(x, w[:0], y),
+                 lambda: vc3d.linear_cross_entropy(x, w, y, torch.zeros(9, device="cuda")), lambda: vc3d.linear_cross_entropy(x, w, y, reduction="avg"),
+                 lambda: vc3d.linear_cross_entropy(x.requires_grad_(), w, y, keep_bytes=-2), lambda: vc3d.linear_cross_entropy(x.half(), w.half(), y)):
+        with pytest.raises(Vc3dError):
+            call()

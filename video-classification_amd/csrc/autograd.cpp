@@ -67,6 +67,8 @@ void same_device(const Tensor& ref, const Maybe& t, const char* name) {
 // gradients of gradients are not there: whoever asks for them is told so, not given none
 torch::autograd::variable_list once(torch::autograd::variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor& g : grads)
+        if (g.defined()) g = g.detach().set_requires_grad(true);
     torch::autograd::DelayedError error("this operator of vc3d is differentiable once only", (int64_t)grads.size());
     return error.apply(std::move(grads));
 }

@@ -4,7 +4,6 @@
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <algorithm>
 #include <cstdint>
 #include <string>
 #include <vector>
@@ -26,13 +25,30 @@ struct Sequence {
     ~Sequence() { Py_XDECREF(o); }
 };
 
+// addresses of what a launch writes: each may be there once (two workgroups would otherwise write one element)
+struct Once {
+    std::vector<uint64_t> slots;
+    size_t mask;
+    explicit Once(size_t most) {
+        size_t n = 64;
+        while (n < 2 * most) n *= 2;
+        slots.assign(n, 0), mask = n - 1;
+    }
+    bool add(uint64_t a) {
+        size_t i = (a * 0x9E3779B97F4A7C15ull >> 20) & mask;
+        for (; slots[i] != 0; i = (i + 1) & mask)
+            if (slots[i] == a) return false;
+        slots[i] = a;
+        return true;
+    }
+};
+
 // fills `rows`; what is wrong, or "" (an exception is set where the lists hold something else than tensors)
 std::string fill(Sequence* lists, int columns, Py_ssize_t n, Row* rows) {
     const bool eight = columns == 6;
     const at::Tensor* first = nullptr;
     at::ScalarType type{};
-    std::vector<uint64_t> starts;
-    starts.reserve(n);
+    Once written((size_t)n * (columns - 1));
     for (Py_ssize_t i = 0; i < n; ++i) {
         const at::Tensor* t[6];
         for (int c = 0; c < columns; ++c) {
@@ -67,10 +83,10 @@ std::string fill(Sequence* lists, int columns, Py_ssize_t n, Row* rows) {
         }
         auto at = [](const at::Tensor& x) { return (uint64_t)(uintptr_t)x.mutable_data_ptr(); };
         rows[i] = {at(p), (uint64_t)(uintptr_t)t[1]->const_data_ptr(), at(*t[2]), at(*t[3]), eight ? at(*t[4]) : 0, eight ? at(*t[5]) : 0, numel};
-        if (numel > 0) starts.push_back(rows[i].p);
+        if (numel > 0 && !(written.add(rows[i].p) && written.add(rows[i].m) && written.add(rows[i].v) &&
+                           (!eight || (written.add(rows[i].m_scale) && written.add(rows[i].v_scale)))))
+            return "tensor " + std::to_string(i) + ", or one of its moments, is in the lists twice";
     }
-    std::sort(starts.begin(), starts.end());
-    if (std::adjacent_find(starts.begin(), starts.end()) != starts.end()) return "a parameter is in the list twice";
     return "";
 }
 
