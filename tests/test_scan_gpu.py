@@ -101,6 +101,16 @@ def test_matches_the_recurrence(B, T, H, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,lengths,reverse", [(1, [4500, 0, 2049], False), (2, [1, 2048, 4097], True), (5, [2047, 16, 3000], False), (16, [4200, 129, 2048], False),
+                                               (15, [1025, 1023, 17], True), (17, [2100, 8, 1024], False), (32, [1024, 1040, 2050], True), (31, [7, 2000, 513], False),
+                                               (33, [1300, 512, 0], False), (63, [511, 513, 1024], True), (64, [1100, 256, 255], False), (65, [300, 257, 1], True)])
+def test_few_channels_share_a_wave_with_later_steps(H, lengths, reverse, dtype):
+    """the borders of groups, waves and tiles for every number of lanes that hold channels, odd numbers of channels"""
+    gates, h0, dy, dlast = make(3, max(lengths) + 3, H, dtype, seed=H)
+    run_and_check(gates, h0, lengths, reverse, dy, dlast)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("reverse", [False, True])
 def test_lengths_direction_and_what_lies_behind_the_end(dtype, reverse):
     lengths = [0, 1, 300, 63, 64, 65, 129, 299]

@@ -1256,7 +1256,7 @@ static VcScanParams scan_params(const vc_scan_desc* d, const void* gates, const 
 }
 static bool pair_aligned(const void* q, int32_t is_bf16) { return ((uintptr_t)q & (is_bf16 ? 3 : 7)) == 0; }
 size_t vc_gated_scan_workspace_bytes(const vc_scan_desc* d, int32_t op) {
-    return scan_check(d) != 0 ? 0 : vc_scan_workspace(d->B, d->T, d->H, op);
+    return scan_check(d) != 0 ? 0 : vc_scan_workspace(d->B, d->T, d->H, d->is_bf16 != 0, op);
 }
 int vc_gated_scan_fwd(const vc_scan_desc* d, const void* gates, const float* h0, const int32_t* lengths, void* h, float* last,
                       float* states, void* workspace, size_t ws_bytes, void* stream) {
@@ -1264,7 +1264,7 @@ int vc_gated_scan_fwd(const vc_scan_desc* d, const void* gates, const float* h0,
     if (rc) return rc;
     VC_REQUIRE(gates && h && last, "gated_scan_fwd: null pointer");
     VC_REQUIRE(pair_aligned(h, d->is_bf16), "gated_scan_fwd: h is not aligned to two elements");
-    const size_t need = vc_scan_workspace(d->B, d->T, d->H, 0);
+    const size_t need = vc_scan_workspace(d->B, d->T, d->H, d->is_bf16 != 0, 0);
     VC_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                "gated_scan_fwd: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, need);
     VcScanParams p = scan_params(d, gates, lengths);
@@ -1277,7 +1277,7 @@ int vc_gated_scan_bwd(const vc_scan_desc* d, const void* gates, const int32_t* l
     if (rc) return rc;
     VC_REQUIRE(gates && states && dgates, "gated_scan_bwd: null pointer");
     VC_REQUIRE(pair_aligned(dgates, d->is_bf16) && pair_aligned(dy, d->is_bf16), "gated_scan_bwd: dy or dgates is not aligned to two elements");
-    const size_t need = vc_scan_workspace(d->B, d->T, d->H, 1);
+    const size_t need = vc_scan_workspace(d->B, d->T, d->H, d->is_bf16 != 0, 1);
     VC_REQUIRE(need == 0 || (workspace && ws_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                "gated_scan_bwd: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, need);
     VcScanParams p = scan_params(d, gates, lengths);

@@ -6,8 +6,8 @@
 //   dh0 = mu in front of the first step.
 //
 // A step is an affine map of the state, h -> a h + b, and maps compose: (a2, b2) o (a1, b1) = (a2 a1, a2 b1 + b2).  So a
-// workgroup takes a tile of steps x 128 channels at once: each wave composes the maps of its own SUB steps (two channels per
-// lane, held in registers), the waves exchange their compositions through LDS, and with the state in front of its first step
+// workgroup takes a tile of steps x 128 channels at once (64, 32 or 16 where there are no more, and more steps): each wave composes
+// the maps of its own SUB steps (two channels per lane, held in registers), the waves exchange their compositions through LDS, and with the state in front of its first step
 // each wave runs its steps again and writes them.  gates are read from memory once, h is written once.  The backward pass
 // needs h_(t-1) and does not read h: it recomputes the states from the gates, which it has to read anyway, starting at the
 // fp32 states that the forward saved every VC_SCAN_CHUNK steps (4 bytes per 64 steps and channel against 2-4 bytes per step,
@@ -21,7 +21,7 @@
 // their number from a counter, earlier steps first, so a tile only ever waits for tiles that run already, and every wait ends.
 //
 // Measured (copies on this card reach 5.14 TB/s): 8 x 2048 x 2048 bf16 forward 44 us = 4.6 TB/s, backward 82 us = 4.1; one
-// sequence of 131072 x 1024 193 us = 4.2 TB/s.
+// sequence of 131072 x 1024 181 us = 4.45 TB/s.
 //
 // All arithmetic and the state are fp32; h and dgates round once, to their type.  1 - f is computed as its own quotient
 // (sigmoid(-z)), so that a gate near 1 keeps its relative precision.
@@ -29,6 +29,9 @@
 
 #include "common.h"
 #include "kernels.h"
+
+// every product and sum as written: the paths below (whole waves or not, dy there or not) give the same bits
+#pragma clang fp contract(off)
 
 namespace {
 
@@ -44,66 +47,55 @@ __device__ __forceinline__ void gate(float z, float& f, float& q) {
 struct f2 {
     float x, y;
 };
+// a b + c
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { return {__builtin_fmaf(a.x, b.x, c.x), __builtin_fmaf(a.y, b.y, c.y)}; }
 
-// two neighbouring channels as they lie in memory.  VEC: at a multiple of their size; otherwise one by one (d: elements from
-// the first to the second, 0 where there is no second).
+// Two neighbouring channels as they lie in memory, one load or store for both, at any multiple of an element (the hardware takes
+// addresses of any alignment; one by one, 8 x 2048 x 2047 bf16, forward and backward, took 250 us instead of 177).  What a lane of the last
+// column does with H odd: it loads the channel in front of its own beside it, so that nothing behind the row is read, and stores
+// one value.  H = 1 has none in front: values one by one.
+enum Channels { EVEN, ODD, ONE };
 template <typename T>
 struct Raw;
 template <>
 struct Raw<bf16> {
+    typedef unsigned any_t __attribute__((aligned(2)));
     unsigned w;
-    template <bool VEC>
+    template <Channels C>
     __device__ __forceinline__ void load(const bf16* p, int d) {
-        if (VEC) w = *(const unsigned*)p;
-        else w = (unsigned)*(const unsigned short*)p | (unsigned)*(const unsigned short*)(p + d) << 16;
+        if (C == EVEN) w = *(const any_t*)p;
+        else if (C == ODD) {
+            w = *(const any_t*)(p - 1 + d);
+            w = d ? w : w >> 16;
+        } else
+            w = *(const unsigned short*)p;
     }
     __device__ __forceinline__ f2 get() const { return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}; }
 };
 template <>
 struct Raw<float> {
     float a, b;
-    template <bool VEC>
+    template <Channels C>
     __device__ __forceinline__ void load(const float* p, int d) {
-        if (VEC) {
-            const float2 v = *(const float2*)p;
-            a = v.x, b = v.y;
-        } else
-            a = p[0], b = p[d];
+        if (C == ONE) a = b = p[0];
+        else {
+            float v[2];
+            __builtin_memcpy(v, C == ODD ? p - 1 + d : p, 8);
+            a = C == ODD && !d ? v[1] : v[0], b = v[1];
+        }
     }
     __device__ __forceinline__ f2 get() const { return {a, b}; }
 };
-// two neighbouring values as they lie in memory
-template <typename T>
-struct Pair;
-template <>
-struct Pair<float> {
-    typedef float2 type;
-    static __device__ __forceinline__ type make(f2 v) { return make_float2(v.x, v.y); }
-};
-template <>
-struct Pair<bf16> {
-    typedef __attribute__((ext_vector_type(2))) __bf16 type;
-    static __device__ __forceinline__ type make(f2 v) { return (type){f2bf(v.x), f2bf(v.y)}; }
-};
-template <typename T>
-__device__ __forceinline__ typename Pair<T>::type pair(f2 v) {
-    return Pair<T>::make(v);
+__device__ __forceinline__ void put2(float* p, f2 v) { __builtin_memcpy(p, &v, 8); }
+__device__ __forceinline__ void put2(bf16* p, f2 v) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    *(Raw<bf16>::any_t*)p = __builtin_bit_cast(unsigned, (bf16x2){f2bf(v.x), f2bf(v.y)});
 }
-template <bool VEC>
-__device__ __forceinline__ void store2(float* p, f2 v, int n) {
-    if (VEC && n == 2) *(float2*)p = pair<float>(v);
-    else {
-        if (n > 0) p[0] = v.x;
-        if (n > 1) p[1] = v.y;
-    }
-}
-template <bool VEC>
-__device__ __forceinline__ void store2(bf16* p, f2 v, int n) {
-    if (VEC && n == 2) *(Pair<bf16>::type*)p = pair<bf16>(v);
-    else {
-        if (n > 0) p[0] = f2bf(v.x);
-        if (n > 1) p[1] = f2bf(v.y);
-    }
+// n: 0, 1 or 2 channels
+template <typename T>
+__device__ __forceinline__ void store2(T* p, f2 v, int n) {
+    if (n == 2) put2(p, v);
+    else if (n == 1) p[0] = (T)v.x;
 }
 
 // ---------------------------------------------------------------- states between tiles
@@ -156,8 +148,8 @@ struct Between {
 #pragma unroll
             for (int i = 0; i < W; ++i)
                 if (k + i < tile)
-                    h = {__uint_as_float((unsigned)(x[i] >> 32) & 0x7fffffffu) * h.x + low(x[i]),
-                         __uint_as_float((unsigned)(y[i] >> 32) & 0x7fffffffu) * h.y + low(y[i])};
+                    h = fma2({__uint_as_float((unsigned)(x[i] >> 32) & 0x7fffffffu), __uint_as_float((unsigned)(y[i] >> 32) & 0x7fffffffu)}, h,
+                             {low(x[i]), low(y[i])});
         }
         return h;
     }
@@ -177,13 +169,44 @@ __global__ __launch_bounds__(256) void scan_clear_kernel(uint4* p, long long n) 
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = make_uint4(0, 0, 0, 0);
 }
 
+// (a later map behind an earlier one)
+struct Map {
+    f2 a, b;
+};
+__device__ __forceinline__ Map after(Map later, Map earlier) {
+    return {{later.a.x * earlier.a.x, later.a.y * earlier.a.y}, fma2(later.a, earlier.b, later.b)};
+}
+__device__ __forceinline__ f2 apply(Map m, f2 h) { return fma2(m.a, h, m.b); }
+// Few channels: LANES of a wave's lanes hold the channels (two each), the next LANES the following steps, and so on.
+// Compositions over a wave's groups of lanes: `m` becomes that of all groups up to and with the own (DOWN: from the own on, in
+// the backward's order); returns that of the groups in front of the own.
+template <int LANES, bool DOWN>
+__device__ __forceinline__ Map over_groups(Map& m, int lane) {
+    Map e = {{1.f, 1.f}, {0.f, 0.f}};
+    if constexpr (LANES < 64) {
+        auto from = [&](Map v, int by) {
+            const int src = DOWN ? lane + by : lane - by;
+            return Map{{__shfl(v.a.x, src, 64), __shfl(v.a.y, src, 64)}, {__shfl(v.b.x, src, 64), __shfl(v.b.y, src, 64)}};
+        };
+        auto has = [&](int by) { return DOWN ? lane + by < 64 : lane >= by; };
+#pragma unroll
+        for (int by = LANES; by < 64; by *= 2) {
+            const Map o = from(m, by);
+            if (has(by)) m = after(m, o);
+        }
+        const Map o = from(m, LANES);
+        if (has(LANES)) e = o;
+    }
+    return e;
+}
+
 // what a workgroup and a lane of it work on
-template <typename T>
+template <typename T, int LANES>
 struct Place {
     int tile, ntiles, c, n, d, b, len;  // c: first of the lane's n (0, 1, 2) channels (0 if it has none); d: to its second
     Between between;
     __device__ Place(const VcScanParams& p, int steps, int lane, int* shared) {
-        const int cols = (p.H + 127) >> 7;
+        const int cols = (p.H + 2 * LANES - 1) / (2 * LANES);
         ntiles = (p.T + steps - 1) / steps;
         int id = blockIdx.x;
         if (ntiles > 1) {
@@ -195,7 +218,7 @@ struct Place {
         tile = id / per;
         id -= tile * per;
         b = id / cols;
-        c = (id - b * cols) * 128 + lane * 2;
+        c = (id - b * cols) * (2 * LANES) + (lane & (LANES - 1)) * 2;
         n = p.H - c >= 2 ? 2 : p.H - c > 0 ? p.H - c : 0;
         c = n > 0 ? c : 0;
         d = c + 1 < p.H ? 1 : 0;
@@ -208,18 +231,18 @@ struct Place {
     }
 };
 
-template <typename T, int WAVES, int SUB, bool VEC>
+template <typename T, int WAVES, int SUB, Channels C, int LANES>
 __global__ __launch_bounds__(WAVES * 64, 4) void scan_fwd_kernel(const VcScanParams p) {
-    constexpr int TILE = WAVES * SUB;
+    constexpr int GROUPS = 64 / LANES, TILE = WAVES * GROUPS * SUB;
     static_assert(TILE % VC_SCAN_CHUNK == 0 && VC_SCAN_CHUNK % SUB == 0, "saved states sit where a wave starts");
-    __shared__ float4 agg[WAVES][64];
-    __shared__ f2 carry[64];
+    __shared__ float4 agg[WAVES][LANES];
+    __shared__ f2 carry[LANES];
     __shared__ int shared;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    typedef typename Pair<T>::type P2;
-    const Place<T> L(p, TILE, lane, &shared);
+    const int cl = lane & (LANES - 1), group = LANES < 64 ? lane / LANES : 0;
+    const Place<T, LANES> L(p, TILE, lane, &shared);
     T* const out = (T*)p.h + (long long)L.b * p.T * p.H + L.c;
-    const int w0 = L.tile * TILE + wave * SUB;  // the wave's first step
+    const int w0 = L.tile * TILE + (wave * GROUPS + group) * SUB;  // the lane's first step (the wave's, with one group)
     const int left = L.len - w0;                // steps that are there from it on
     // step w0 + j is at time t0 + j dt
     const int dt = p.reverse ? -1 : 1;
@@ -233,15 +256,15 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_fwd_kernel(const VcScanPar
             if (left >= SUB) {
 #pragma unroll
                 for (int j = 0; j < SUB; ++j) {
-                    z[j].template load<VEC>(g + j * st, L.d);
-                    v[j].template load<VEC>(g + j * st + p.H, L.d);
+                    z[j].template load<C>(g + j * st, L.d);
+                    v[j].template load<C>(g + j * st + p.H, L.d);
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < SUB; ++j) {
                     const long long at = (j < left ? j : left - 1) * st;  // (read again, not used)
-                    z[j].template load<VEC>(g + at, L.d);
-                    v[j].template load<VEC>(g + at + p.H, L.d);
+                    z[j].template load<C>(g + at, L.d);
+                    v[j].template load<C>(g + at + p.H, L.d);
                 }
             }
         }
@@ -258,76 +281,80 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_fwd_kernel(const VcScanPar
                     u[j] = {q.x * vv.x, q.y * vv.y};
                 }
                 a = {a.x * f[j].x, a.y * f[j].y};
-                b = {f[j].x * b.x + u[j].x, f[j].y * b.y + u[j].y};
+                b = fma2(f[j], b, u[j]);
             }
         };
-        if (left >= SUB) compose(std::true_type());
+        if (LANES == 64 ? left >= SUB : __all(left >= SUB)) compose(std::true_type());
         else compose(std::false_type());
-        agg[wave][lane] = make_float4(a.x, a.y, b.x, b.y);
+        Map own = {a, b};
+        const Map front = over_groups<LANES, false>(own, lane);
+        if (group == GROUPS - 1) agg[wave][cl] = make_float4(own.a.x, own.a.y, own.b.x, own.b.y);
         __syncthreads();
         if (wave == 0) {
+            const int n = group == 0 ? L.n : 0;
             f2 h;
             if (L.tile == 0) h = p.h0 != nullptr ? f2{p.h0[sc], p.h0[sc + L.d]} : f2{0.f, 0.f};
             a = {1.f, 1.f}, b = {0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float4 m = agg[w][lane];
+                const float4 m = agg[w][cl];
                 a = {a.x * m.x, a.y * m.y};
-                b = {m.x * b.x + m.z, m.y * b.y + m.w};
+                b = fma2({m.x, m.y}, b, {m.z, m.w});
             }
             const bool more = (L.tile + 1) * TILE < L.len;
             if (L.tile > 0) {
-                if (more) L.between.put_map(L.tile, a, b, L.n);
+                if (more) L.between.put_map(L.tile, a, b, n);
                 h = L.between.before(L.tile);
             }
-            carry[lane] = h;
-            h = {a.x * h.x + b.x, a.y * h.y + b.y};
-            if (more) L.between.put_state(L.tile, h, L.n);
-            else store2<false>(p.last + sc, h, L.n);
+            if (group == 0) carry[cl] = h;
+            h = fma2(a, h, b);
+            if (more) L.between.put_state(L.tile, h, n);
+            else store2(p.last + sc, h, n);
         }
         __syncthreads();
-        f2 h = carry[lane];
+        f2 h = carry[cl];
         for (int w = 0; w < wave; ++w) {
-            const float4 m = agg[w][lane];
-            h = {m.x * h.x + m.z, m.y * h.y + m.w};
+            const float4 m = agg[w][cl];
+            h = fma2({m.x, m.y}, h, {m.z, m.w});
         }
+        if (LANES < 64) h = apply(front, h);
         if (p.states != nullptr && w0 % VC_SCAN_CHUNK == 0 && left > 0) {
             const long long chunks = (p.T + VC_SCAN_CHUNK - 1) / VC_SCAN_CHUNK;
-            store2<false>(p.states + (L.b * chunks + w0 / VC_SCAN_CHUNK) * p.H + L.c, h, L.n);
+            store2(p.states + (L.b * chunks + w0 / VC_SCAN_CHUNK) * p.H + L.c, h, L.n);
         }
         T* const o = out + t0 * p.H;
         const long long so = (long long)p.H * dt;
         auto write = [&](auto whole) {
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
-                h = {f[j].x * h.x + u[j].x, f[j].y * h.y + u[j].y};
-                if (decltype(whole)::value) *(P2*)(o + j * so) = pair<T>(h);
-                else if (j < left) store2<VEC>(o + j * so, h, L.n);
+                h = fma2(f[j], h, u[j]);
+                if (decltype(whole)::value) put2(o + j * so, h);
+                else if (j < left) store2(o + j * so, h, L.n);
             }
         };
-        if (VEC && left >= SUB && __all(L.n == 2)) write(std::true_type());
+        if (C == EVEN && __all(left >= SUB && L.n == 2)) write(std::true_type());
         else write(std::false_type());
     } else if (L.len == 0 && L.tile == 0 && wave == 0)
-        store2<false>(p.last + sc, p.h0 != nullptr ? f2{p.h0[sc], p.h0[sc + L.d]} : f2{0.f, 0.f}, L.n);
+        store2(p.last + sc, p.h0 != nullptr ? f2{p.h0[sc], p.h0[sc + L.d]} : f2{0.f, 0.f}, L.n);
     if (left < SUB)  // behind the end: zeros
-        for (int t = left > 0 ? L.len : w0; t < w0 + SUB && t < p.T; ++t) store2<VEC>(out + (long long)t * p.H, {0.f, 0.f}, L.n);
+        for (int t = left > 0 ? L.len : w0; t < w0 + SUB && t < p.T; ++t) store2(out + (long long)t * p.H, {0.f, 0.f}, L.n);
 }
 
-template <typename T, int WAVES, int SUB, bool VEC>
+template <typename T, int WAVES, int SUB, Channels C, int LANES>
 __global__ __launch_bounds__(WAVES * 64, 4) void scan_bwd_kernel(const VcScanParams p) {
-    constexpr int TILE = WAVES * SUB;
+    constexpr int GROUPS = 64 / LANES, TILE = WAVES * GROUPS * SUB;
     static_assert(TILE % VC_SCAN_CHUNK == 0, "a tile starts at a saved state");
-    __shared__ float4 agg[WAVES][64];  // forward maps
-    __shared__ f2 back[WAVES][64];     // constant part of the backward maps (their factor is the forward's)
-    __shared__ f2 carry[64];
+    __shared__ float4 agg[WAVES][LANES];  // forward maps
+    __shared__ f2 back[WAVES][LANES];     // constant part of the backward maps (their factor is the forward's)
+    __shared__ f2 carry[LANES];
     __shared__ int shared;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    typedef typename Pair<T>::type P2;
-    const Place<T> L(p, TILE, lane, &shared);
+    const int cl = lane & (LANES - 1), group = LANES < 64 ? lane / LANES : 0;
+    const Place<T, LANES> L(p, TILE, lane, &shared);
     const int tile = L.ntiles - 1 - L.tile;                  // the last steps come first
     const int first = (L.len + TILE - 1) / TILE - 1 - tile;  // tiles of this sequence that come before
     T* const out = (T*)p.dgates + (long long)L.b * p.T * 2 * p.H + L.c;
-    const int w0 = tile * TILE + wave * SUB, left = L.len - w0;
+    const int w0 = tile * TILE + (wave * GROUPS + group) * SUB, left = L.len - w0;
     const int dt = p.reverse ? -1 : 1;
     const long long t0 = p.reverse ? L.len - 1 - w0 : w0;
     const long long sc = (long long)L.b * p.H + L.c;
@@ -339,14 +366,14 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_bwd_kernel(const VcScanPar
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
                 const long long at = (j < left ? j : left - 1) * st;  // (behind the end: read again, not used)
-                z[j].template load<VEC>(g + at, L.d);
-                v[j].template load<VEC>(g + at + p.H, L.d);
+                z[j].template load<C>(g + at, L.d);
+                v[j].template load<C>(g + at + p.H, L.d);
             }
             if (p.dy != nullptr) {
                 const T* const y = (const T*)p.dy + ((long long)L.b * p.T + t0) * p.H + L.c;
                 const long long so = (long long)p.H * dt;
 #pragma unroll
-                for (int j = 0; j < SUB; ++j) d[j].template load<VEC>(y + (j < left ? j : left - 1) * so, L.d);
+                for (int j = 0; j < SUB; ++j) d[j].template load<C>(y + (j < left ? j : left - 1) * so, L.d);
             }
         }
         f2 f[SUB], q[SUB], a = {1.f, 1.f}, b = {0.f, 0.f}, c = {0.f, 0.f};
@@ -361,7 +388,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_bwd_kernel(const VcScanPar
                     gate(zz.x, f[j].x, q[j].x);
                     gate(zz.y, f[j].y, q[j].y);
                     const f2 vv = v[j].get();
-                    b = {f[j].x * b.x + q[j].x * vv.x, f[j].y * b.y + q[j].y * vv.y};
+                    b = fma2(f[j], b, {q[j].x * vv.x, q[j].y * vv.y});
                 }
                 a = {a.x * f[j].x, a.y * f[j].y};
             }
@@ -371,45 +398,50 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_bwd_kernel(const VcScanPar
                 c = {f[j].x * (e.x + c.x), f[j].y * (e.y + c.y)};
             }
         };
-        if (left >= SUB && has_dy) compose(std::true_type());
+        if (has_dy && (LANES == 64 ? left >= SUB : __all(left >= SUB))) compose(std::true_type());
         else compose(std::false_type());
-        agg[wave][lane] = make_float4(a.x, a.y, b.x, b.y);
-        back[wave][lane] = c;
+        Map own = {a, b}, future = {a, c};
+        const Map front = over_groups<LANES, false>(own, lane), behind = over_groups<LANES, true>(future, lane);
+        if (group == GROUPS - 1) agg[wave][cl] = make_float4(own.a.x, own.a.y, own.b.x, own.b.y);
+        if (group == 0) back[wave][cl] = future.b;
         __syncthreads();
         if (wave == 0) {
+            const int n = group == 0 ? L.n : 0;
             f2 mu;
             if (first == 0) mu = p.dlast != nullptr ? f2{p.dlast[sc], p.dlast[sc + L.d]} : f2{0.f, 0.f};
             a = {1.f, 1.f}, c = {0.f, 0.f};
 #pragma unroll
             for (int w = WAVES - 1; w >= 0; --w) {
-                const float4 m = agg[w][lane];
-                const f2 n = back[w][lane];
+                const float4 m = agg[w][cl];
+                const f2 k = back[w][cl];
                 a = {a.x * m.x, a.y * m.y};
-                c = {m.x * c.x + n.x, m.y * c.y + n.y};
+                c = fma2({m.x, m.y}, c, k);
             }
             if (first > 0) {
-                if (tile > 0) L.between.put_map(first, a, c, L.n);
+                if (tile > 0) L.between.put_map(first, a, c, n);
                 mu = L.between.before(first);
             }
-            carry[lane] = mu;
-            mu = {a.x * mu.x + c.x, a.y * mu.y + c.y};
-            if (tile > 0) L.between.put_state(first, mu, L.n);
-            else if (p.dh0 != nullptr) store2<false>(p.dh0 + sc, mu, L.n);
+            if (group == 0) carry[cl] = mu;
+            mu = fma2(a, mu, c);
+            if (tile > 0) L.between.put_state(first, mu, n);
+            else if (p.dh0 != nullptr) store2(p.dh0 + sc, mu, n);
         }
         const long long chunks = (p.T + VC_SCAN_CHUNK - 1) / VC_SCAN_CHUNK;
         const float* st = p.states + (L.b * chunks + tile * (TILE / VC_SCAN_CHUNK)) * p.H + L.c;
         f2 h = {st[0], st[L.d]};
         for (int w = 0; w < wave; ++w) {
-            const float4 m = agg[w][lane];
-            h = {m.x * h.x + m.z, m.y * h.y + m.w};
+            const float4 m = agg[w][cl];
+            h = fma2({m.x, m.y}, h, {m.z, m.w});
         }
+        if (LANES < 64) h = apply(front, h);
         __syncthreads();
-        f2 mu = carry[lane];
+        f2 mu = carry[cl];
         for (int w = WAVES - 1; w > wave; --w) {
-            const float4 m = agg[w][lane];
-            const f2 n = back[w][lane];
-            mu = {m.x * mu.x + n.x, m.y * mu.y + n.y};
+            const float4 m = agg[w][cl];
+            const f2 k = back[w][cl];
+            mu = fma2({m.x, m.y}, mu, k);
         }
+        if (LANES < 64) mu = apply(behind, mu);
         f2 before[SUB];
         T* const o = out + t0 * 2 * p.H;
         const long long so = 2ll * p.H * dt;
@@ -418,7 +450,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_bwd_kernel(const VcScanPar
             for (int j = 0; j < SUB; ++j) {
                 const f2 vv = v[j].get();
                 before[j] = h;
-                if (decltype(whole)::value || j < left) h = {f[j].x * h.x + q[j].x * vv.x, f[j].y * h.y + q[j].y * vv.y};
+                if (decltype(whole)::value || j < left) h = fma2(f[j], h, {q[j].x * vv.x, q[j].y * vv.y});
             }
 #pragma unroll
             for (int j = SUB - 1; j >= 0; --j) {
@@ -427,22 +459,22 @@ __global__ __launch_bounds__(WAVES * 64, 4) void scan_bwd_kernel(const VcScanPar
                 const f2 dv = {q[j].x * lam.x, q[j].y * lam.y};
                 const f2 dz = {mu.x * q[j].x * (before[j].x - vv.x), mu.y * q[j].y * (before[j].y - vv.y)};
                 if (decltype(whole)::value) {
-                    *(P2*)(o + j * so) = pair<T>(dz);
-                    *(P2*)(o + j * so + p.H) = pair<T>(dv);
+                    put2(o + j * so, dz);
+                    put2(o + j * so + p.H, dv);
                 } else if (j < left) {
-                    store2<VEC>(o + j * so, dz, L.n);
-                    store2<VEC>(o + j * so + p.H, dv, L.n);
+                    store2(o + j * so, dz, L.n);
+                    store2(o + j * so + p.H, dv, L.n);
                 }
             }
         };
-        if (VEC && has_dy && left >= SUB && __all(L.n == 2)) write(std::true_type());
+        if (C == EVEN && has_dy && __all(left >= SUB && L.n == 2)) write(std::true_type());
         else write(std::false_type());
     } else if (L.len == 0 && tile == 0 && wave == 0 && p.dh0 != nullptr)
-        store2<false>(p.dh0 + sc, p.dlast != nullptr ? f2{p.dlast[sc], p.dlast[sc + L.d]} : f2{0.f, 0.f}, L.n);
+        store2(p.dh0 + sc, p.dlast != nullptr ? f2{p.dlast[sc], p.dlast[sc + L.d]} : f2{0.f, 0.f}, L.n);
     if (left < SUB)  // behind the end: zeros
         for (int t = left > 0 ? L.len : w0; t < w0 + SUB && t < p.T; ++t) {
-            store2<VEC>(out + (long long)t * 2 * p.H, {0.f, 0.f}, L.n);
-            store2<VEC>(out + (long long)t * 2 * p.H + p.H, {0.f, 0.f}, L.n);
+            store2(out + (long long)t * 2 * p.H, {0.f, 0.f}, L.n);
+            store2(out + (long long)t * 2 * p.H + p.H, {0.f, 0.f}, L.n);
         }
 }
 
@@ -456,7 +488,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* gates, long lon
         const size_t e = (size_t)b * H + c;
         float f, q;
         gate((float)row[0], f, q);
-        const float n = f * state[e] + q * (float)row[H];
+        const float n = __builtin_fmaf(f, state[e], q * (float)row[H]);
         state[e] = n;
         h[e] = (T)n;
     }
@@ -475,54 +507,70 @@ int launched(const char* what) {
 
 namespace {
 
-// Forward: 16 waves of 16 steps, one workgroup a CU.  Half as many waves or steps: 8 .. 30 % slower (a sequence is more tiles,
-// whose states wait for each other, and a wave has fewer loads in flight); 32 steps spill.  Backward: its three inputs and h
-// in registers leave room for 8 steps; 16 waves against 8: one sequence of 131072 x 512 320 against 433 us, 32 sequences
+// Forward, bf16: 16 waves of 16 steps, one workgroup a CU.  Half as many waves or steps: 8 .. 30 % slower (a sequence is more
+// tiles, whose states wait for each other, and a wave has fewer loads in flight); 32 steps spill.  fp32: 8 steps (its 16 spill: 8 x
+// 2048 x 2048 forward and backward 240 against 228 us, 32 x 23 x 3686 forward 22.7 against 15.2).  Backward: its three inputs and
+// h in registers leave room for 8 steps; 16 waves against 8: one sequence of 131072 x 512 320 against 433 us, 32 sequences
 // of 2048 x 1024 262 against 258.  Workgroups that stay and ask for their next tile's gates while they finish one measured 20 %
 // slower in both directions (more registers, fewer loads in flight).
-constexpr int FWD_WAVES = 16, FWD_SUB = 16, BWD_WAVES = 16, BWD_SUB = 8;
+constexpr int WAVES = 16, BWD_SUB = 8;
+constexpr int fwd_sub(bool is_bf16) { return is_bf16 ? 16 : 8; }
 
-// whether every pair of channels begins at a multiple of two elements
-bool pairs(const VcScanParams& p, int elem) {
-    return ((p.H | p.sb | p.st) & 1) == 0 && ((uintptr_t)p.gates & (2 * elem - 1)) == 0;
-}
+// lanes of a wave that hold channels: the fewest that hold all of them (bf16, forward and backward: 45 x 8291 x 32 147 us
+// with 64, 76 with 16; 1 x 131072 x 16 205 with 64, 78 with 8)
+int lanes(int H) { return H > 64 ? 64 : H > 32 ? 32 : H > 16 ? 16 : 8; }
+int tile_steps(int H, bool is_bf16, int op) { return WAVES * (op == 0 ? fwd_sub(is_bf16) : BWD_SUB) * (64 / lanes(H)); }
 // the workgroups of a launch; clears what they exchange their states through
-unsigned begin(const VcScanParams& p, int steps, size_t bytes, hipStream_t s) {
-    const long long tiles = (p.T + steps - 1) / steps;
-    if (bytes > 0) {
-        const long long n = (long long)bytes / 16, blocks = (n + 255) / 256;
-        hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)p.ws, n);
-    }
-    return (unsigned)(tiles * ((p.H + 127) / 128) * p.B);
+unsigned begin(const VcScanParams& p, bool is_bf16, int op, hipStream_t s) {
+    const int steps = tile_steps(p.H, is_bf16, op), channels = 2 * lanes(p.H);
+    const long long tiles = (p.T + (long long)steps - 1) / steps, n = (long long)vc_scan_workspace(p.B, p.T, p.H, is_bf16, op) / 16, blocks = (n + 255) / 256;
+    if (n > 0) hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)p.ws, n);
+    return (unsigned)(tiles * ((p.H + channels - 1) / channels) * p.B);
 }
 
-template <typename T>
-int fwd(const VcScanParams& p, hipStream_t s) {
-    (void)hipGetLastError();
-    const dim3 grid(begin(p, FWD_WAVES * FWD_SUB, vc_scan_workspace(p.B, p.T, p.H, 0), s)), block(FWD_WAVES * 64);
-    if (pairs(p, sizeof(T))) hipLaunchKernelGGL((scan_fwd_kernel<T, FWD_WAVES, FWD_SUB, true>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((scan_fwd_kernel<T, FWD_WAVES, FWD_SUB, false>), grid, block, 0, s, p);
-    return launched("gated_scan_fwd");
+template <typename T, Channels C, int LANES>
+void launch(const VcScanParams& p, int op, hipStream_t s) {
+    constexpr bool is_bf16 = sizeof(T) == 2;
+    const dim3 grid(begin(p, is_bf16, op, s)), block(WAVES * 64);
+    if (op == 0) hipLaunchKernelGGL((scan_fwd_kernel<T, WAVES, fwd_sub(is_bf16), C, LANES>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((scan_bwd_kernel<T, WAVES, BWD_SUB, C, LANES>), grid, block, 0, s, p);
+}
+template <typename T, Channels C>
+void launch(const VcScanParams& p, int op, hipStream_t s) {
+    switch (lanes(p.H)) {
+        case 64: return launch<T, C, 64>(p, op, s);
+        case 32: return launch<T, C, 32>(p, op, s);
+        case 16: return launch<T, C, 16>(p, op, s);
+        default: return launch<T, C, 8>(p, op, s);
+    }
 }
 template <typename T>
-int bwd(const VcScanParams& p, hipStream_t s) {
-    (void)hipGetLastError();
-    const dim3 grid(begin(p, BWD_WAVES * BWD_SUB, vc_scan_workspace(p.B, p.T, p.H, 1), s)), block(BWD_WAVES * 64);
-    if (pairs(p, sizeof(T))) hipLaunchKernelGGL((scan_bwd_kernel<T, BWD_WAVES, BWD_SUB, true>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((scan_bwd_kernel<T, BWD_WAVES, BWD_SUB, false>), grid, block, 0, s, p);
-    return launched("gated_scan_bwd");
+void launch(const VcScanParams& p, int op, hipStream_t s) {
+    if (p.H % 2 == 0) launch<T, EVEN>(p, op, s);
+    else if (p.H > 1) launch<T, ODD>(p, op, s);
+    else launch<T, ONE, 8>(p, op, s);
 }
 
 }  // namespace
 
 // what the tiles of a sequence exchange: 0 where a sequence is one tile
-size_t vc_scan_workspace(int B, int T, int H, int op) {
-    const int steps = op == 0 ? FWD_WAVES * FWD_SUB : BWD_WAVES * BWD_SUB;
+size_t vc_scan_workspace(int B, int T, int H, bool is_bf16, int op) {
+    const int steps = tile_steps(H, is_bf16, op);
     const long long tiles = ((long long)T + steps - 1) / steps;
     return tiles > 1 ? (size_t)(256 + 2 * 8 * tiles * B * H) : 0;
 }
-int vc_scan_launch_fwd(const VcScanParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? fwd<bf16>(p, s) : fwd<float>(p, s); }
-int vc_scan_launch_bwd(const VcScanParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? bwd<bf16>(p, s) : bwd<float>(p, s); }
+int vc_scan_launch_fwd(const VcScanParams& p, bool is_bf16, hipStream_t s) {
+    (void)hipGetLastError();
+    if (is_bf16) launch<bf16>(p, 0, s);
+    else launch<float>(p, 0, s);
+    return launched("gated_scan_fwd");
+}
+int vc_scan_launch_bwd(const VcScanParams& p, bool is_bf16, hipStream_t s) {
+    (void)hipGetLastError();
+    if (is_bf16) launch<bf16>(p, 1, s);
+    else launch<float>(p, 1, s);
+    return launched("gated_scan_bwd");
+}
 int vc_scan_launch_step(const void* gates, long long sb, float* state, void* h, int B, int H, bool is_bf16, hipStream_t s) {
     const dim3 grid((H + 255) / 256, B < 4096 ? B : 4096);
     (void)hipGetLastError();
