@@ -246,10 +246,11 @@ __device__ __forceinline__ void store_pair(T* at, int lg, f32x4 u, f32x4 v) {
         const uint2 a = __builtin_bit_cast(uint2, (bf16x4){f2bf(u[0]), f2bf(u[1]), f2bf(u[2]), f2bf(u[3])});
         const uint2 b = __builtin_bit_cast(uint2, (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])});
         const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
-        *(uint4*)(at + (lg & 1) * 16 + (lg >> 1) * 8) = make_uint4(x[0], y[0], x[1], y[1]);
+        const uint4 q = make_uint4(x[0], y[0], x[1], y[1]);
+        __builtin_memcpy(at + (lg & 1) * 16 + (lg >> 1) * 8, &q, 16);
     } else {
-        *(f32x4*)(at + lg * 4) = u;
-        *(f32x4*)(at + 16 + lg * 4) = v;
+        __builtin_memcpy(at + lg * 4, &u, 16);
+        __builtin_memcpy(at + 16 + lg * 4, &v, 16);
     }
 }
 
@@ -539,7 +540,7 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
     }
     if constexpr (EPI == EPI_DX || EPI == EPI_DW) {
         const float f = EPI == EPI_DW ? g.factor.get() : 1.f;
-        const bool vec = (g.nr & 3) == 0, wide = r0 + BR <= g.nr && (g.nr * (int)sizeof(T) & 15) == 0;
+        const bool wide = r0 + BR <= g.nr;  // (rows begin anywhere: the stores take any address)
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const int s = s0 + wsx + b * 16 + l15;
@@ -555,17 +556,24 @@ __global__ __launch_bounds__(WR* WS * 64, 2) void lce_gemm(const Gemm g) {
                 const int r = r0 + wr + a * 16 + lg * 4;
                 if constexpr (EPI == EPI_DX) {
                     float* const q = g.acc + split * g.acc_split + (long long)s * g.nr + r;
-                    if (vec && r < g.nr) *(f32x4*)q = g.add ? acc[a][b] + *(const f32x4*)q : acc[a][b];
-                    else
+                    if (r + 4 <= g.nr) {
+                        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                        if (g.add) __builtin_memcpy(&v, q, 16);
+                        v += acc[a][b];
+                        __builtin_memcpy(q, &v, 16);
+                    } else
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
                             if (r + j < g.nr) q[j] = acc[a][b][j] + (g.add ? q[j] : 0.f);
                 } else {
                     T* const q = (T*)g.out + (long long)s * g.nr + r;
                     const f32x4 v = acc[a][b] * f;
-                    if (vec && r < g.nr) {
-                        if constexpr (sizeof(T) == 2) *(bf16x4*)q = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
-                        else *(f32x4*)q = v;
+                    if (r + 4 <= g.nr) {
+                        if constexpr (sizeof(T) == 2) {
+                            const bf16x4 o = {f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
+                            __builtin_memcpy(q, &o, 8);
+                        } else
+                            __builtin_memcpy(q, &v, 16);
                     } else
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
@@ -674,10 +682,17 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const float2* part, int 
         const int n = rows[i];
         float m = -INFINITY, e = 0.f, l = 0.f, loss_n = 0.f;
         if (i < count) {
-            for (int t = lane; t < tiles; t += 64) {
-                const float2 p = part[(size_t)i * tiles + t];
-                const float k = fmaxf(m, p.x), ref = k == -INFINITY ? 0.f : k;
-                e = e * __expf(m - ref) + p.y * __expf(p.x - ref);
+            for (int t0 = lane; t0 < tiles; t0 += 256) {  // (four pairs under way)
+                float2 p[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[j] = t0 + j * 64 < tiles ? part[(size_t)i * tiles + t0 + j * 64] : make_float2(-INFINITY, 0.f);
+                float k = m;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) k = fmaxf(k, p[j].x);
+                const float ref = k == -INFINITY ? 0.f : k;
+                e *= __expf(m - ref);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) e += p[j].y * __expf(p[j].x - ref);
                 m = k;
             }
 #pragma unroll
@@ -814,20 +829,33 @@ __global__ __launch_bounds__(256) void lce_last_kernel(const Last q, const int* 
     const bool keep = i < count;
     const float* const from = q.acc + (long long)i * D;
     T* const to = (T*)q.dx + (long long)n * D;
-    if ((D & 3) == 0) {
-        for (int d = threadIdx.x * 4; d < D; d += 1024) {
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < splits && keep; ++k) v += *(const f32x4*)(from + k * q.split + d);
-            v = keep ? v * g : (f32x4){0.f, 0.f, 0.f, 0.f};
-            if constexpr (sizeof(T) == 2) *(bf16x4*)(to + d) = (bf16x4){f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
-            else *(f32x4*)(to + d) = v;
-        }
-        return;
-    }
-    for (int d = threadIdx.x; d < D; d += 256) {
-        float v = 0.f;
-        for (int k = 0; k < splits && keep; ++k) v += from[k * q.split + d];
-        to[d] = keep ? (T)(v * g) : (T)0.f;
+    for (int d0 = threadIdx.x * 4; d0 < D; d0 += 1024) {
+        const int d = d0 + 4 > D && D >= 4 ? D - 4 : d0, left = D - d;  // (the last four once more, in part: the same values)
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (keep && left >= 4)
+            for (int k0 = 0; k0 < splits; k0 += 8) {  // (eight sums under way)
+                f32x4 t[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) __builtin_memcpy(&t[k], from + (k0 + k < splits ? k0 + k : splits - 1) * q.split + d, 16);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v += k0 + k < splits ? t[k] : (f32x4){0.f, 0.f, 0.f, 0.f};
+            }
+        else if (keep)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                for (int k = 0; k < splits && j < left; ++k) v[j] += from[k * q.split + d + j];
+        v *= g;
+        if (!keep) v = (f32x4){0.f, 0.f, 0.f, 0.f};  // (g may be no number)
+        if (left >= 4) {
+            if constexpr (sizeof(T) == 2) {
+                const bf16x4 o = {f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
+                __builtin_memcpy(to + d, &o, 8);
+            } else
+                __builtin_memcpy(to + d, &v, 16);
+        } else
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < left) to[d + j] = (T)v[j];
     }
 }
 
@@ -894,8 +922,9 @@ struct Plan {
         // 338 us with 256, 275 with 128; 1600 x 1000 of 50257, 28 tiles: 794 against 845; 8192 x 2048 of 65536: 6.96 against 7.73 ms)
         tile_dx = N > 128 && D > 128 && (N + 255ll) / 256 * ((D + 255) / 256) >= 16 ? 256 : N > 64 && D > 64 ? 128 : 64;
         tile_dw = pick_tile(piece < V ? piece : V, D);
-        // up to 16 splits, 256 MB of sums, 128 words a split (512: 64 x 512 of 400 classes 66 us instead of 61)
-        dx = {tile_dx == 256 ? 256 : 512, 16, (D + tile_dx - 1) / tile_dx, tile_dx};
+        // up to 64 splits (16: the product of 224 rows x 768 of 75745 words 57 us instead of 30), 256 MB of sums, 128 words a split
+        // (512: 64 x 512 of 400 classes 66 us instead of 61)
+        dx = {tile_dx == 256 ? 256 : 512, 64, (D + tile_dx - 1) / tile_dx, tile_dx};
         const long long room = (256ll << 20) / ((long long)N * D * 4), least = piece / 128;
         dx.most = (int)(dx.most > room ? room : dx.most);
         dx.most = (int)(dx.most > least ? least : dx.most);
