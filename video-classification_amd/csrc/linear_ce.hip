@@ -1094,17 +1094,20 @@ bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16) {
 }
 // Whether the forward keeps the logits' gradient for the backward, which then need not compute the logits again: that saves a
 // product and costs storing, reading and storing N x V, and two launches.  By itself up to 2 GB (under 1 % of the memory) and
-// where there is enough to save: a long sum, or a large product.  Kernels of a step, again / kept in us, bf16: 2048 x 1024 of
+// where there is enough to save: a long sum, a large product, or a large w that few rows would read again.  Kernels of a step, again / kept in us, bf16: 2048 x 1024 of
 // 32768 555 / 477, 8192 x 2048 of 65536 7170 / 5900, 4000 x 384 of 32000 553 / 535, 8192 x 256 of 60000 1660 / 1470, 512 x 512 of
 // 8192 80 / 74, 30 x 1024 of 1000 45.3 / 43.8, 1 x 2048 of 32000 125 / 110; but 8192 x 128 of 60000 1200 / 1332, 200 x 512 of
 // 8000 59.6 / 61.7.  fp32: 1000 x 1024 of 32000 2030 / 1590, 1000 x 64 of 20000 214 / 190, 64 x 512 of 400 61 / 52; but 300 x 128 of
-// 10000 121.5 / 122.4.
+// 10000 121.5 / 122.4.  Few rows: bf16 16 x 256 of 130000 108 / 92, 100 x 128 of 130000 115 / 108, fp32 6 x 415 of 85803 362 / 316;
+// but 16 x 512 of 8000 46.3 / 46.2.
 bool vc_lce_keep(int N, int D, int V, bool is_bf16, int reduction, long long keep_bytes) {
     if (reduction == 0) return false;  // (its rows' factors come with the backward)
     const size_t bytes = Plan::exps(N, V, is_bf16 ? 2 : 4);
     if (keep_bytes >= 0) return bytes <= (size_t)keep_bytes;
     const double work = (double)N * V * D;
-    return bytes <= (size_t)2 << 30 && (is_bf16 ? D >= 1024 || (D >= 256 && work >= 0x1p31) : D >= 512 || work >= 0x1p29);
+    if (bytes > (size_t)2 << 30) return false;
+    if (N <= D && (double)D * V >= 0x1p23) return true;
+    return is_bf16 ? D >= 1024 || (D >= 256 && work >= 0x1p31) : D >= 512 || work >= 0x1p29;
 }
 size_t vc_lce_saved(int N, int D, int V, bool is_bf16, bool keep) { return Plan::saved(N, D, V, is_bf16 ? 2 : 4, keep); }
 size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, bool keep, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack, keep).bytes; }
