@@ -291,6 +291,14 @@ def test_what_is_kept():
     size = [vc3d.ops.linear_ce_fwd(x, w, y, keep_bytes=k)[1].numel() for k in (0, -1, 1 << 24, (1 << 24) - 1)]
     assert size[1] == size[2] == size[0] + (1 << 24) + (1 << 18) + 2 * 2048 and size[3] == size[0]
     assert vc3d.ops.linear_ce_fwd(x[:, :128], w[:, :128], y)[1].numel() < 1 << 20  # short rows: quicker computed again
+    # rows that are no whole chunks: w is copied, and the copy kept where there is room for it too
+    xo, wo = x[:, :511].contiguous(), w[:, :511].contiguous()
+    one = torch.ones(1, device="cuda")
+    got = []
+    for k in (1 << 24, ALL):
+        loss, saved = vc3d.ops.linear_ce_fwd(xo, wo, y, keep_bytes=k)
+        got.append((saved.numel(), loss) + vc3d.ops.linear_ce_bwd(xo, wo, y, None, saved, one, keep_bytes=k))
+    assert got[1][0] == got[0][0] + (1 << 14) * 1024 and all(torch.equal(a, b) for a, b in zip(got[0][1:4], got[1][1:4]))
     leaves = [t.requires_grad_() for t in (x, w)]
     torch.cuda.synchronize()
     before = torch.cuda.memory_allocated()

@@ -44,7 +44,7 @@ def test_c_entry_of_the_scan_refuses():
     c = _capi()
     ok = lambda **k: c.ScanDesc(**{**dict(B=2, T=100, H=8, is_bf16=1, reverse=0, pad_=0, stride_b=1600, stride_t=16), **k})  # noqa: E731
     need = c.lib.vc_gated_scan_workspace_bytes
-    assert need(ok(), 0) == 0 and need(ok(T=100000), 0) > 0 and need(ok(T=100000), 1) > need(ok(T=1000), 1) > 0
+    assert need(ok(), 0) == 0 and need(ok(T=100000), 0) > 0 and need(ok(T=100000), 1) > need(ok(T=10000), 1) > 0
     assert need(None, 0) == 0 and need(ok(H=0), 0) == 0
     fwd = lambda d, g=PTR, h=PTR, last=PTR, ws=None, n=0: c.lib.vc_gated_scan_fwd(d, g, None, None, h, last, None, ws, n, None)  # noqa: E731
     bwd = lambda d, g=PTR, st=PTR, dy=PTR, dg=PTR, ws=None, n=0: c.lib.vc_gated_scan_bwd(d, g, None, st, dy, None, dg, None, ws, n, None)  # noqa: E731

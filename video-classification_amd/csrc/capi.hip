@@ -1301,8 +1301,8 @@ static int lce_check(const vc_linear_ce_desc* d) {
     VC_REQUIRE(d->reduction >= 0 && d->reduction <= 2, "linear_ce: reduction %d (0 none, 1 mean, 2 sum)", d->reduction);
     return 0;
 }
-static bool lce_keep(const vc_linear_ce_desc* d) { return vc_lce_keep(d->N, d->D, d->V, d->is_bf16 != 0, d->reduction, d->keep_bytes); }
 static bool lce_pack(const vc_linear_ce_desc* d) { return vc_lce_pack(d->D, d->ldw, d->w_align, d->is_bf16 != 0); }
+static int lce_keep(const vc_linear_ce_desc* d) { return vc_lce_keep(d->N, d->D, d->V, d->is_bf16 != 0, lce_pack(d), d->reduction, d->keep_bytes); }
 size_t vc_linear_ce_workspace_bytes(const vc_linear_ce_desc* d, int32_t op) {
     if (lce_check(d) != 0) return 0;
     return vc_lce_workspace(d->N, d->D, d->V, d->is_bf16 != 0, lce_pack(d), lce_keep(d), op);

@@ -234,7 +234,7 @@ struct VcLceParams {
     long long ignore_index;
     int reduction;  // 0 none, 1 mean, 2 sum
     bool pack;      // the products read a copy of w
-    bool keep;      // the forward keeps exponentials for the backward
+    int keep;       // 1: the forward keeps the gradient of the logits for the backward, 2: and its copy of w
     float* loss;       // forward: [1], nullable with reduction 0
     float* loss_rows;  // forward: [N], nullable unless reduction is 0
     void* saved;       // what the forward leaves for the backward
@@ -247,8 +247,8 @@ struct VcLceParams {
     size_t ws_bytes;
 };
 bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16);
-bool vc_lce_keep(int N, int D, int V, bool is_bf16, int reduction, long long keep_bytes);
-size_t vc_lce_saved(int N, int D, int V, bool is_bf16, bool keep);
-size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, bool keep, int op);
+int vc_lce_keep(int N, int D, int V, bool is_bf16, bool pack, int reduction, long long keep_bytes);
+size_t vc_lce_saved(int N, int D, int V, bool is_bf16, int keep);
+size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int keep, int op);
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s);
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s);

@@ -56,8 +56,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(const long long* labels, lon
 // use.  An operand lies in memory with k contiguous (rows of x, w; P for dx) or with its rows contiguous and k across (w for dx;
 // x and P for dw: nothing is transposed in memory):
 //   k contiguous: LDS rows of 64 or 128 bytes; a fragment is one ds_read_b128.  The 16-byte chunk c of row r lies at slot
-//     c ^ turn(r): of the sixteen lanes that one cycle pair serves, whether they are rows 0-15 of one
-//     chunk or rows 0-3, 12-15 of one and 4-11 of the next, no two meet in a bank (measured: 0 conflicts).
+//     c ^ turn(r): of the sixteen lanes that one cycle pair serves, whether they are rows 0-15 of one chunk or rows 0-3, 12-15 of one and 4-11 of the next, no two meet in a bank (measured: 0 conflicts).
 //   k across: LDS rows of one k each.  bf16: fragments come through ds_read_b64_tr_b16, which hands lane i of 16 the i-th
 //     column of four rows; a lane group reads four rows x 32 bytes, so the 32-byte unit u of row k lies at u ^ f(k) with f
 //     different for the eight rows that half a wave reads at once.  fp32: one ds_read_b32 a value, units of 64 bytes at u ^ (k / 4 % 4).
@@ -890,28 +889,29 @@ struct Plan {
     static size_t list_at(int N) { return ((size_t)N * 4 + 255) & ~(size_t)255; }
     static size_t x_at(int N) { return list_at(N) + ((((size_t)N + 4) * 4 + 255) & ~(size_t)255); }
     static size_t ref_at(int N, int D, int elem) { return x_at(N) + (((saves_x(N, D, elem) ? (size_t)N * row(D, elem) * elem : 0) + 255) & ~(size_t)255); }
-    // with `keep` also: ref [N], P at the label [N], the exponentials, which become P, and db's partial sums
+    // with `keep` also: ref [N], P at the label [N], the exponentials, which become P, and db's partial sums; with 2 the copy of w
     static size_t plab_at(int N, int D, int elem) { return ref_at(N, D, elem) + list_at(N); }
     static size_t exps_at(int N, int D, int elem) { return plab_at(N, D, elem) + list_at(N); }
     static size_t row_tiles(int N, int V) { return ((size_t)N + pick_tile(N, V) - 1) / pick_tile(N, V); }
     static size_t exps(int N, int V, int elem) { return row_tiles(N, V) * pick_tile(N, V) * (((size_t)V + 255) / 256 * 256) * elem; }
     static size_t dbpart_at(int N, int D, int V, int elem) { return exps_at(N, D, elem) + exps(N, V, elem); }
-    static size_t saved(int N, int D, int V, int elem, bool keep) {
-        return keep ? dbpart_at(N, D, V, elem) + row_tiles(N, V) * (((size_t)V + 255) / 256 * 256) * 4 : ref_at(N, D, elem);
+    static size_t w_at(int N, int D, int V, int elem) { return dbpart_at(N, D, V, elem) + row_tiles(N, V) * (((size_t)V + 255) / 256 * 256) * 4; }
+    static size_t saved(int N, int D, int V, int elem, int keep) {
+        return keep ? w_at(N, D, V, elem) + (keep == 2 ? (size_t)V * row(D, elem) * elem : 0) : ref_at(N, D, elem);
     }
-    Plan(int N, int D, int V, int elem, int op, bool pack, bool keep) {
+    Plan(int N, int D, int V, int elem, int op, bool pack, int keep) {
         kd = (D * elem + 15) / 16 * 16 / elem;
         ld = row(D, elem);
         const long long np = ((long long)N + 255) / 256 * 256, all = ((long long)V + 255) / 256 * 256;
         long long fit = (512ll << 20) / elem / np / 256 * 256;
-        if (op == 0 || keep) fit = pack ? (512ll << 20) / elem / ld / 256 * 256 : all;  // (a piece of w's copy is all there is)
+        if (op == 0 || keep) fit = pack && keep < 2 ? (512ll << 20) / elem / ld / 256 * 256 : all;  // (a piece of w's copy is all there is)
         fit = fit < 256 ? 256 : fit;
         lde = all;
         piece = (int)(fit < all ? fit : all);
         tile = pick_tile(N, piece < V && !keep ? piece : V);
         tiles = (int)(((long long)V + tile - 1) / tile);
         if (!saves_x(N, D, elem)) xp = take((size_t)N * ld * elem);
-        if (pack) wp = take((size_t)(piece < V ? piece : V) * ld * elem);
+        if (pack && keep < 2) wp = take((size_t)(piece < V ? piece : V) * ld * elem);
         if (op == 0) {
             part = take((size_t)N * tiles * sizeof(float2));
             zlab = take((size_t)N * 4);
@@ -974,7 +974,9 @@ struct Source {
     int* rows;
     T* exps;
     float* dbpart;
-    Source(const VcLceParams& p, const Plan& L, hipStream_t s, bool forward) : p(p), L(L), s(s) {
+    T* kept_w;
+    bool forward;
+    Source(const VcLceParams& p, const Plan& L, hipStream_t s, bool forward) : p(p), L(L), s(s), forward(forward) {
         char* const saved = (char*)p.saved;
         const bool kept = Plan::saves_x(p.N, p.D, sizeof(T));
         lse = (float*)saved, rows = (int*)(saved + Plan::list_at(p.N));
@@ -982,6 +984,7 @@ struct Source {
         plab = p.keep ? (float*)(saved + Plan::plab_at(p.N, p.D, sizeof(T))) : nullptr;
         exps = p.keep ? (T*)(saved + Plan::exps_at(p.N, p.D, sizeof(T))) : nullptr;
         dbpart = p.keep && p.bias != nullptr ? (float*)(saved + Plan::dbpart_at(p.N, p.D, p.V, sizeof(T))) : nullptr;
+        kept_w = p.keep == 2 ? (T*)(saved + Plan::w_at(p.N, p.D, p.V, sizeof(T))) : nullptr;
         T* const to = (T*)(kept ? saved + Plan::x_at(p.N) : (char*)p.ws + L.xp);
         x = {(const char*)to, L.ld * (long long)sizeof(T)};
         if (!forward && kept) return;
@@ -995,7 +998,8 @@ struct Source {
     Operand w(int v0, int nv, const int* when) const {
         const T* at = (const T*)p.w + v0 * p.ldw;
         if (!p.pack) return {(const char*)at, p.ldw * (long long)sizeof(T)};
-        T* const to = (T*)((char*)p.ws + L.wp);
+        T* const to = kept_w != nullptr ? kept_w + (long long)v0 * L.ld : (T*)((char*)p.ws + L.wp);
+        if (kept_w != nullptr && !forward) return {(const char*)to, L.ld * (long long)sizeof(T)};
         const auto kernel = chunks(at, p.ldw, p.D) ? lce_words_of_w_kernel<T, true> : lce_words_of_w_kernel<T, false>;
         hipLaunchKernelGGL(kernel, dim3(nv < 16384 ? (nv + 3) / 4 : 4096), dim3(256), 0, s, at, p.ldw, nv, p.D, L.ld, to, when);
         return {(const char*)to, L.ld * (long long)sizeof(T)};
@@ -1094,22 +1098,23 @@ bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16) {
 }
 // Whether the forward keeps the logits' gradient for the backward, which then need not compute the logits again: that saves a
 // product and costs storing, reading and storing N x V, and two launches.  By itself up to 2 GB (under 1 % of the memory) and
-// where there is enough to save: a long sum, a large product, or a large w that few rows would read again.  Kernels of a step, again / kept in us, bf16: 2048 x 1024 of
-// 32768 555 / 477, 8192 x 2048 of 65536 7170 / 5900, 4000 x 384 of 32000 553 / 535, 8192 x 256 of 60000 1660 / 1470, 512 x 512 of
-// 8192 80 / 74, 30 x 1024 of 1000 45.3 / 43.8, 1 x 2048 of 32000 125 / 110; but 8192 x 128 of 60000 1200 / 1332, 200 x 512 of
-// 8000 59.6 / 61.7.  fp32: 1000 x 1024 of 32000 2030 / 1590, 1000 x 64 of 20000 214 / 190, 64 x 512 of 400 61 / 52; but 300 x 128 of
-// 10000 121.5 / 122.4.  Few rows: bf16 16 x 256 of 130000 108 / 92, 100 x 128 of 130000 115 / 108, fp32 6 x 415 of 85803 362 / 316;
-// but 16 x 512 of 8000 46.3 / 46.2.
-bool vc_lce_keep(int N, int D, int V, bool is_bf16, int reduction, long long keep_bytes) {
-    if (reduction == 0) return false;  // (its rows' factors come with the backward)
-    const size_t bytes = Plan::exps(N, V, is_bf16 ? 2 : 4);
-    if (keep_bytes >= 0) return bytes <= (size_t)keep_bytes;
+// where there is enough to save: a long sum, a large product, or a large w that few rows would read again.  Kernels of a step,
+// again / kept in us, bf16: 2048 x 1024 of 32768 555 / 477, 8192 x 2048 of 65536 7170 / 5900, 4000 x 384 of 32000 553 / 535, 8192 x
+// 256 of 60000 1660 / 1470, 512 x 512 of 8192 80 / 74, 30 x 1024 of 1000 45.3 / 43.8, 1 x 2048 of 32000 125 / 110; but 8192 x 128
+// of 60000 1200 / 1332, 200 x 512 of 8000 59.6 / 61.7.  fp32: 1000 x 1024 of 32000 2030 / 1590, 1000 x 64 of 20000 214 / 190, 64 x
+// 512 of 400 61 / 52; but 300 x 128 of 10000 121.5 / 122.4.  Few rows: bf16 16 x 256 of 130000 108 / 92, 100 x 128 of 130000
+// 115 / 108, fp32 6 x 415 of 85803 362 / 316; but 16 x 512 of 8000 46.3 / 46.2.
+// 2: and the copy of w, where the products read one and there is room.
+int vc_lce_keep(int N, int D, int V, bool is_bf16, bool pack, int reduction, long long keep_bytes) {
+    if (reduction == 0) return 0;  // (its rows' factors come with the backward)
+    const int elem = is_bf16 ? 2 : 4;
+    const size_t bytes = Plan::exps(N, V, elem), limit = keep_bytes >= 0 ? (size_t)keep_bytes : (size_t)2 << 30;
     const double work = (double)N * V * D;
-    if (bytes > (size_t)2 << 30) return false;
-    if (N <= D && (double)D * V >= 0x1p23) return true;
-    return is_bf16 ? D >= 1024 || (D >= 256 && work >= 0x1p31) : D >= 512 || work >= 0x1p29;
+    const bool pays = (N <= D && (double)D * V >= 0x1p23) || (is_bf16 ? D >= 1024 || (D >= 256 && work >= 0x1p31) : D >= 512 || work >= 0x1p29);
+    if (bytes > limit || (keep_bytes < 0 && !pays)) return 0;
+    return pack && bytes + (size_t)V * Plan::row(D, elem) * elem <= limit ? 2 : 1;
 }
-size_t vc_lce_saved(int N, int D, int V, bool is_bf16, bool keep) { return Plan::saved(N, D, V, is_bf16 ? 2 : 4, keep); }
-size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, bool keep, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack, keep).bytes; }
+size_t vc_lce_saved(int N, int D, int V, bool is_bf16, int keep) { return Plan::saved(N, D, V, is_bf16 ? 2 : 4, keep); }
+size_t vc_lce_workspace(int N, int D, int V, bool is_bf16, bool pack, int keep, int op) { return Plan(N, D, V, is_bf16 ? 2 : 4, op, pack, keep).bytes; }
 int vc_lce_launch_fwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? fwd<bf16>(p, s) : fwd<float>(p, s); }
 int vc_lce_launch_bwd(const VcLceParams& p, bool is_bf16, hipStream_t s) { return is_bf16 ? bwd<bf16>(p, s) : bwd<float>(p, s); }
