@@ -56,7 +56,8 @@ __global__ __launch_bounds__(1024) void rows_kernel(const long long* labels, lon
 // use.  An operand lies in memory with k contiguous (rows of x, w; P for dx) or with its rows contiguous and k across (w for dx;
 // x and P for dw: nothing is transposed in memory):
 //   k contiguous: LDS rows of 64 or 128 bytes; a fragment is one ds_read_b128.  The 16-byte chunk c of row r lies at slot
-//     c ^ turn(r): of the sixteen lanes that one cycle pair serves, whether they are rows 0-15 of one chunk or rows 0-3, 12-15 of one and 4-11 of the next, no two meet in a bank (measured: 0 conflicts).
+//     c ^ turn(r): of the sixteen lanes that one cycle pair serves, whether they are rows 0-15 of one chunk or rows 0-3,
+//     12-15 of one and 4-11 of the next, no two meet in a bank (measured: 0 conflicts).
 //   k across: LDS rows of one k each.  bf16: fragments come through ds_read_b64_tr_b16, which hands lane i of 16 the i-th
 //     column of four rows; a lane group reads four rows x 32 bytes, so the 32-byte unit u of row k lies at u ^ f(k) with f
 //     different for the eight rows that half a wave reads at once.  fp32: one ds_read_b32 a value, units of 64 bytes at u ^ (k / 4 % 4).
@@ -65,8 +66,8 @@ __global__ __launch_bounds__(1024) void rows_kernel(const long long* labels, lon
 // instruction, at 2.1 GHz), near what a large library product reaches here (1.33).  1843 rows x 1024 of 32768, us: EPI_STATS 133,
 // EPI_KEEP 156, EPI_PROB 156, EPI_DX 133, EPI_DW 120 (123.7 GFLOP each); 7373 x 2048 of 65536: 1555, 1791, 1898, 1734, 1573 (1979
 // GFLOP each).  The difference of the first three is the epilogue's stores.  What did not help: fragments read four slots ahead
-// or raised wave priority (within 1 %), tiles of 256 x 128 in three buffers, two workgroups a CU (+2 .. +20 %), rows of 64 bytes of k for the forward (+15 %), touching the next lines early (+10 %),
-// workgroups that stay and fetch their next tile during the epilogue (+33 %: registers spill).
+// or raised wave priority (within 1 %), tiles of 256 x 128 in three buffers, two workgroups a CU (+2 .. +20 %), rows of 64 bytes
+// of k for the forward (+15 %), touching the next lines early (+10 %), workgroups that stay and fetch their next tile during the epilogue (+33 %: registers spill).
 // Nothing is read outside the operands: rows and columns behind the end are read from a row or column inside (what they make
 // is not stored), k behind the end from a page of zeros (k contiguous) or, with k across, from a k inside, where the other
 // operand, P, is 0 (EPI_PROB writes whole tiles of P, zeros behind the last row and the last word).

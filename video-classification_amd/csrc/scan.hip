@@ -7,8 +7,8 @@
 //
 // A step is an affine map of the state, h -> a h + b, and maps compose: (a2, b2) o (a1, b1) = (a2 a1, a2 b1 + b2).  So a
 // workgroup takes a tile of steps x 128 channels at once (64, 32 or 16 where there are no more, and more steps): each wave composes
-// the maps of its own SUB steps (two channels per lane, held in registers), the waves exchange their compositions through LDS, and with the state in front of its first step
-// each wave runs its steps again and writes them.  gates are read from memory once, h is written once.  The backward pass
+// the maps of its own SUB steps (two channels per lane, held in registers), the waves exchange their compositions through LDS,
+// and with the state in front of its first step each wave runs its steps again and writes them.  gates are read from memory once, h is written once.  The backward pass
 // needs h_(t-1) and does not read h: it recomputes the states from the gates, which it has to read anyway, starting at the
 // fp32 states that the forward saved every VC_SCAN_CHUNK steps (4 bytes per 64 steps and channel against 2-4 bytes per step,
 // and without the rounding of a 16-bit h inside h_(t-1) - v_t).

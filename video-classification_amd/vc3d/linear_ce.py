@@ -45,7 +45,7 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     (their x is not read and its gradient is 0); "mean" is over the others, and 0 where there is none (torch: NaN).  Any other
     label outside [0, V) gives a NaN.  reduction "none" returns labels' shape.  Differentiable in x, weight and bias; the
     gradients are of the inputs' type.  keep_bytes: whether the forward keeps the logits' gradient for the
-    backward (N x V of the inputs' type): 0 no, the backward computes the logits again; n: where it takes at most n bytes; -1: where
+    backward (N x V of the inputs' type; and, while there is room, the copy of a weight whose rows are no whole 16 bytes): 0 no, the backward computes the logits again; n: where it takes at most n bytes; -1: where
     that is quicker and takes at most 2 GB.  Never with reduction "none"."""
     if reduction not in _REDUCTION:
         raise Vc3dError("linear_cross_entropy: reduction 'none', 'mean' or 'sum', got %r" % (reduction,))
