@@ -244,7 +244,6 @@ struct VcLceParams {
     void* dw;            // nullable
     void* db;            // nullable
     void* ws;
-    size_t ws_bytes;
 };
 bool vc_lce_pack(int D, long long ldw, int w_align, bool is_bf16);
 int vc_lce_keep(int N, int D, int V, bool is_bf16, bool pack, int reduction, long long keep_bytes);

@@ -130,7 +130,11 @@ PyObject* written(PyObject*, PyObject* args) {
             PyObject* const o = PySequence_Fast_GET_ITEM(list.o, i);
             if (!THPVariable_Check(o)) return PyErr_Format(PyExc_TypeError, "tensors expected"), nullptr;
             const at::Tensor& t = THPVariable_Unpack(o);
-            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+            try {
+                if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+            } catch (const std::exception& e) {
+                return PyErr_SetString(PyExc_RuntimeError, e.what()), nullptr;
+            }
         }
     }
     Py_RETURN_NONE;
