@@ -8,6 +8,7 @@ import torch
 
 from . import ops
 from .capi import Vc3dError
+from .packed import PackedOperand
 
 
 def gated_scan(gates, h0=None, lengths=None, reverse=False):
@@ -24,21 +25,8 @@ def gated_scan_step(gates, state):
     return ops.gated_scan_step(gates, state)
 
 
-class PackedGateWeight:
-    """bf16 forward / weight-gradient operand of a gate projection and its data-gradient twin, rebuilt when the master changed (by
-    its version counter, as the engine's and the LSTM's operands: a write through ``weight.data`` is not seen)"""
-
-    def __init__(self):
-        self.key = self.wf = self.wd = None
-
-    def get(self, weight):
-        key = (weight._version, weight.data_ptr(), weight.device)
-        if key != self.key:
-            co, ci = weight.shape
-            w5 = weight.detach().float().contiguous().view(co, 1, 1, 1, ci).permute(0, 4, 1, 2, 3)
-            self.wf, self.wd = ops.pack_weight(w5, want_dgrad=True)
-            self.key = key
-        return self.wf, self.wd
+class PackedGateWeight(PackedOperand):
+    """bf16 operands of a gate projection's weight, kept from call to call"""
 
 
 class _GateProjectionFn(torch.autograd.Function):
