@@ -47,8 +47,9 @@ def world(monkeypatch):
 
 
 def operands():
+    from vc3d.lstm import _PackedLSTMWeights
     from vc3d.scan import PackedGateWeight
-    return [(PackedGateWeight, 1)]
+    return [(PackedGateWeight, 1), (_PackedLSTMWeights, 2)]
 
 
 def weights_at(memory, count):

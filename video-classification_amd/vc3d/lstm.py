@@ -9,26 +9,16 @@ import torch
 
 from . import ops
 from .capi import Vc3dError, check, cur_stream, lib, ptr
+from .packed import PackedOperand
 
 F32, BF16 = torch.float32, torch.bfloat16
 
 
-class _PackedLSTMWeights:
-    """bf16 [4H][Fin+H] forward / wgrad operand and its [Fin+H][4H] dgrad twin, rebuilt when a master weight changed."""
+class _PackedLSTMWeights(PackedOperand):
+    """bf16 [4H][Fin+H] forward / wgrad operand and its [Fin+H][4H] dgrad twin, kept from call to call"""
 
-    def __init__(self):
-        self.key = None
-        self.wf = self.wd = None
-
-    def get(self, w_ih, w_hh):
-        key = (w_ih._version, w_hh._version, w_ih.data_ptr(), w_hh.data_ptr(), w_ih.device)
-        if key != self.key:
-            wcat = torch.cat([w_ih.detach(), w_hh.detach()], 1).float().contiguous()
-            co, ci = wcat.shape
-            w5 = wcat.view(co, 1, 1, 1, ci).permute(0, 4, 1, 2, 3)  # [Co][Ci][1][1][1] in channels_last_3d storage
-            self.wf, self.wd = ops.pack_weight(w5, want_dgrad=True)
-            self.key = key
-        return self.wf, self.wd
+    def matrix(self, w_ih, w_hh):
+        return torch.cat([w_ih.detach(), w_hh.detach()], 1).float().contiguous()
 
 
 class _LSTMCellFn(torch.autograd.Function):
