@@ -125,14 +125,25 @@ _WS = {}  # device -> split-K workspace (grown on demand; reuse is safe: launche
 USE_WORKSPACE = True
 
 
+class _Address(int):
+    """an address that keeps the tensor alive which lies there"""
+
+
 def _workspace(d, op, device, need=None):
-    """(ptr, bytes) of a workspace large enough for conv `d`, op 0/1/2; (None, 0) if none is needed."""
+    """(ptr, bytes) of a workspace large enough for conv `d`, op 0/1/2; (None, 0) if none is needed.  A call that is captured into
+    a graph gets one of its own, in the graph's memory: a shared one would be written by two graphs that run at the same time,
+    and would be freed under the graph when a later call needs a larger one."""
     if not USE_WORKSPACE:
         return None, 0
     if need is None:
         need = int(lib.vc_conv3d_workspace_bytes(d, op))
     if need == 0:
         return None, 0
+    if torch.cuda.is_current_stream_capturing():
+        buf = torch.empty(need, dtype=torch.uint8, device=device)
+        at = _Address(buf.data_ptr())
+        at.tensor = buf
+        return at, need
     key = (device.type, device.index, torch.cuda.current_stream().cuda_stream)
     buf = _WS.get(key)
     if buf is None or buf.numel() < need:
