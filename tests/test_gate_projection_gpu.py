@@ -73,3 +73,56 @@ def test_a_captured_sequence_follows_the_weights(warm):
                 junk = [torch.full((256, 128), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(64)]
                 torch.cuda.synchronize()
                 del junk
+
+
+def operands(N, F, C, seed):
+    """bf16-exact x and weight, a bias that takes each column's first product away again: what is left is small beside both"""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(1, F, generator=g) + 2.0 ** -6 * torch.randn(N, F, generator=g)).bfloat16().float()
+    w = (torch.randn(C, F, generator=g) * 4.0).bfloat16().float()
+    b = -(x[0].double() @ w.double().t()).float()
+    return x, w, b
+
+
+@pytest.mark.parametrize("N,F,C", [(1, 64, 64), (5, 64, 128), (64, 512, 1024), (64, 2048, 1024), (33, 2048, 2048), (1000, 192, 320)])
+def test_gates_are_rounded_once(N, F, C):
+    """gates = bf16(x W^T + b): operands are exact, the sum of F + 3 products runs in fp32, and one rounding (half a step: 2^-8)
+    follows it"""
+    from vc3d.scan import PackedGateWeight, gate_projection
+    x, w, b = operands(N, F, C, N + F)
+    got = gate_projection(x.cuda(), w.cuda(), b.cuda(), PackedGateWeight())
+    assert got.dtype == torch.bfloat16
+    want = x.double() @ w.double().t() + b.double()
+    off = (F + 8) * 2.0 ** -24 * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+    assert bool(((got.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + (1 + 2.0 ** -8) * off).all())
+
+
+def test_gradients_of_a_projection_with_a_bias():
+    """dx = dg W, dW = dg^T x, db = sum dg: fp32 sums of exact products (dx rounds to bf16, 2^-8)"""
+    from vc3d.scan import PackedGateWeight, gate_projection
+    N, F, C = 300, 128, 192
+    x, w, b = operands(N, F, C, 9)
+    dg = torch.randn(N, C, generator=torch.Generator().manual_seed(10)).bfloat16()
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    gate_projection(*leaves, PackedGateWeight()).backward(dg.cuda())
+    d, e = dg.double(), 2.0 ** -24
+    want = [d @ w.double(), d.t() @ x.double(), d.sum(0)]
+    size = [d.abs() @ w.double().abs(), d.abs().t() @ x.double().abs(), d.abs().sum(0)]
+    for t, v, s, terms, half in zip(leaves, want, size, (C, N, N), (2.0 ** -8, e, e)):
+        off = (terms + 8) * e * s
+        assert t.grad.shape == t.shape and t.grad.dtype == torch.float32
+        assert bool(((t.grad.cpu().double() - v).abs() <= half * v.abs() + (1 + half) * off).all())
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), 3.3895e38, 1e-39, 0.0])
+def test_a_bias_at_the_ends_of_its_range(value):
+    """a gate that is held open or shut by its bias; the other columns do not see it"""
+    from vc3d.scan import PackedGateWeight, gate_projection
+    x, w, b = operands(7, 64, 64, 11)
+    plain = gate_projection(x.cuda(), w.cuda(), b.cuda(), PackedGateWeight()).cpu()
+    b[5] = value
+    got = gate_projection(x.cuda(), w.cuda(), b.cuda(), PackedGateWeight()).cpu()
+    others = torch.arange(64) != 5
+    assert torch.equal(got[:, others], plain[:, others]) and not bool(got.isnan().any())
+    if abs(value) > 1e38:
+        assert bool((got[:, 5].double() * (1 if value > 0 else -1) >= 3.3e38).all())

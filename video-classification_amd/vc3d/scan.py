@@ -26,42 +26,73 @@ def gated_scan_step(gates, state):
 
 
 class PackedGateWeight(PackedOperand):
-    """bf16 operands of a gate projection's weight, kept from call to call"""
+    """bf16 operands of a gate projection's weight and bias, kept from call to call: [W | b0 b1 b2 0 ...], where the bias lies in 64
+    more columns as the three bf16 numbers whose sum it is (8 bits each of its 24)"""
+
+    def matrix(self, weight, bias=None):
+        if bias is None:
+            return weight.detach().float().contiguous()
+        co, fin = weight.shape
+        m = torch.zeros(co, fin + 64, dtype=torch.float32, device=weight.device)
+        m[:, :fin] = weight.detach()
+        rest = bias.detach().float()
+        for k in range(3):
+            part = rest.bfloat16().float()
+            m[:, fin + k] = part
+            rest = torch.where(part.isfinite(), rest - part, 0.0)
+        return m
 
 
 class _GateProjectionFn(torch.autograd.Function):
-    """x [N][Fin] W^T -> bf16 [N][2H] as a 1x1x1 conv over N positions, like lstm.py's gates; gradients fp32"""
+    """x [N][Fin] W^T + b -> bf16 [N][2H] as a 1x1x1 conv over N positions, like lstm.py's gates; gradients fp32.  With a bias x gets
+    64 more columns, ones and zeros: the bias is a part of the product, is added in its fp32 sums and rounded with them, once;
+    and its gradient is a column of the weight's."""
 
     @staticmethod
-    def forward(ctx, x, weight, packed):
+    def forward(ctx, x, weight, bias, packed):
         N, fin = x.shape
         co = weight.shape[0]
-        wf, wd = packed.get(weight)
-        xb = x.detach().to(torch.bfloat16).contiguous()
-        d = ops.conv_desc(N, fin, 1, 1, 1, co, 1, 1, 0)
+        wf, wd = packed.get(weight, bias)
+        if bias is None:
+            width, xb = fin, x.detach().to(torch.bfloat16).contiguous()
+        else:
+            width = fin + 64
+            xb = torch.empty(N, width, dtype=torch.bfloat16, device=x.device)
+            xb[:, :fin] = x.detach()
+            xb[:, fin:fin + 3] = 1.0
+            xb[:, fin + 3:] = 0.0
+        d = ops.conv_desc(N, width, 1, 1, 1, co, 1, 1, 0)
         ctx.save_for_backward(xb)
-        ctx.d, ctx.wd = d, wd
-        return ops.conv3d_fwd(d, xb.view(N, 1, 1, 1, fin), wf).view(N, co)
+        ctx.d, ctx.wd, ctx.fin = d, wd, fin
+        return ops.conv3d_fwd(d, xb.view(N, 1, 1, 1, width), wf).view(N, co)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dg):
         xb, = ctx.saved_tensors
-        (N, fin), co = xb.shape, dg.shape[1]
+        (N, width), co, fin, want = xb.shape, dg.shape[1], ctx.fin, ctx.needs_input_grad
         dg5 = dg.contiguous().view(N, 1, 1, 1, co)
-        dx = ops.conv3d_dgrad(ctx.d, dg5, ctx.wd).view(N, fin).float() if ctx.needs_input_grad[0] else None
-        dw = torch.zeros(co, 1, 1, 1, fin, dtype=torch.float32, device=dg.device)
-        ops.conv3d_wgrad(ctx.d, xb.view(N, 1, 1, 1, fin), dg5, dw)
-        return dx, dw.view(co, fin), None
+        dx = dw = db = None
+        if want[0]:
+            dx = ops.conv3d_dgrad(ctx.d, dg5, ctx.wd).view(N, width)[:, :fin].float()
+        if want[1] or want[2]:
+            both = torch.zeros(co, 1, 1, 1, width, dtype=torch.float32, device=dg.device)
+            ops.conv3d_wgrad(ctx.d, xb.view(N, 1, 1, 1, width), dg5, both)
+            both = both.view(co, width)
+            dw = both[:, :fin].contiguous() if want[1] else None
+            db = both[:, fin].contiguous() if want[2] else None
+        return dx, dw, db, None
 
 
 def gate_projection(x, weight, bias, packed):
-    """gates [N][2H] in bf16 = x [N][Fin] W^T + b (the sum in fp32), from fp32 x, weight [2H][Fin] and bias [2H] (or None); Fin and 2H are multiples
-    of 64.  `packed`: a PackedGateWeight that keeps the bf16 operands from step to step."""
+    """gates [N][2H] in bf16 = x [N][Fin] W^T + b, from fp32 x, weight [2H][Fin] and bias [2H] (or None); Fin and 2H are multiples of
+    64.  x and W are rounded to bf16, the bias is not; the sums are fp32 and round once, to the gates.  `packed`: a PackedGateWeight
+    that keeps the bf16 operands from step to step."""
     if not x.is_cuda:
         raise Vc3dError("the vc3d gate projection runs on the GPU only (no CPU fallback)")
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or x.shape[1] % 64 or weight.shape[0] % 64:
         raise Vc3dError("gate projection: x [N][Fin] and weight [2H][Fin] with Fin and 2H multiples of 64 expected, got %s and %s" %
                         (tuple(x.shape), tuple(weight.shape)))
-    g = _GateProjectionFn.apply(x.float(), weight, packed)
-    return g if bias is None else (g.float() + bias).to(g.dtype)
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise Vc3dError("gate projection: bias [%d] expected, got %s" % (weight.shape[0], tuple(bias.shape)))
+    return _GateProjectionFn.apply(x.float(), weight, bias, packed)
