@@ -126,3 +126,25 @@ def test_a_bias_at_the_ends_of_its_range(value):
     assert torch.equal(got[:, others], plain[:, others]) and not bool(got.isnan().any())
     if abs(value) > 1e38:
         assert bool((got[:, 5].double() * (1 if value > 0 else -1) >= 3.3e38).all())
+
+
+@pytest.mark.parametrize("B,T", [(0, 7), (3, 0), (0, 0)])
+@pytest.mark.parametrize("h0", [False, True])
+def test_an_empty_sequence(B, T, h0):
+    """no sequences, or none with a step: empty h, the state as it was, gradients of zero"""
+    cell, g = cell_of(64, 64, 12), torch.Generator().manual_seed(13)
+    x = torch.randn(B, T, 64, generator=g).cuda().requires_grad_()
+    start = torch.randn(B, 64, generator=g).cuda().requires_grad_() if h0 else None
+    h, last = cell.sequence(x, h0=start)
+    assert h.shape == (B, T, 64) and torch.equal(last, torch.zeros(B, 64, device="cuda") if start is None else start)
+    (h.sum() + (2.0 * last).sum()).backward()
+    assert not x.grad.any() and not cell.gates.weight.grad.any() and not cell.gates.bias.grad.any()
+    assert start is None or bool((start.grad == 2.0).all())
+
+
+def test_a_step_of_no_sequences():
+    cell = cell_of(64, 64, 14)
+    x = torch.zeros(0, 64, device="cuda")
+    assert cell(x).shape == (0, 64)
+    with torch.no_grad():
+        assert cell(x).shape == (0, 64)

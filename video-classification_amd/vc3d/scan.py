@@ -64,6 +64,8 @@ class _GateProjectionFn(torch.autograd.Function):
         d = ops.conv_desc(N, width, 1, 1, 1, co, 1, 1, 0)
         ctx.save_for_backward(xb)
         ctx.d, ctx.wd, ctx.fin = d, wd, fin
+        if N == 0:
+            return torch.empty(0, co, dtype=torch.bfloat16, device=x.device)
         return ops.conv3d_fwd(d, xb.view(N, 1, 1, 1, width), wf).view(N, co)
 
     @staticmethod
@@ -74,10 +76,11 @@ class _GateProjectionFn(torch.autograd.Function):
         dg5 = dg.contiguous().view(N, 1, 1, 1, co)
         dx = dw = db = None
         if want[0]:
-            dx = ops.conv3d_dgrad(ctx.d, dg5, ctx.wd).view(N, width)[:, :fin].float()
+            dx = ops.conv3d_dgrad(ctx.d, dg5, ctx.wd).view(N, width)[:, :fin].float() if N > 0 else torch.empty(0, fin, device=dg.device)
         if want[1] or want[2]:
             both = torch.zeros(co, 1, 1, 1, width, dtype=torch.float32, device=dg.device)
-            ops.conv3d_wgrad(ctx.d, xb.view(N, 1, 1, 1, width), dg5, both)
+            if N > 0:
+                ops.conv3d_wgrad(ctx.d, xb.view(N, 1, 1, 1, width), dg5, both)
             both = both.view(co, width)
             dw = both[:, :fin].contiguous() if want[1] else None
             db = both[:, fin].contiguous() if want[2] else None
