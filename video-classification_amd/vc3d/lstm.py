@@ -66,4 +66,6 @@ class _LSTMCellFn(torch.autograd.Function):
 
 
 def lstm_cell(x, h_prev, c_prev, w_ih, w_hh, b_ih, b_hh, packed):
-    return _LSTMCellFn.apply(x.float(), h_prev, c_prev, w_ih, w_hh, b_ih, b_hh, packed)
+    ops._same_device(x, h_prev=h_prev, c_prev=c_prev, w_ih=w_ih, w_hh=w_hh, b_ih=b_ih, b_hh=b_hh)
+    with ops._on(x):  # (the launches go to the current device's stream)
+        return _LSTMCellFn.apply(x.float(), h_prev, c_prev, w_ih, w_hh, b_ih, b_hh, packed)

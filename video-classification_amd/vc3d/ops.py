@@ -706,7 +706,7 @@ class _on:
     """the current device set to a tensor's, where it is another one"""
 
     def __init__(self, t):
-        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+        self.guard = torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else None
 
     def __enter__(self):
         if self.guard is not None:

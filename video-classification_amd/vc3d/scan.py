@@ -98,4 +98,6 @@ def gate_projection(x, weight, bias, packed):
                         (tuple(x.shape), tuple(weight.shape)))
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise Vc3dError("gate projection: bias [%d] expected, got %s" % (weight.shape[0], tuple(bias.shape)))
-    return _GateProjectionFn.apply(x.float(), weight, bias, packed)
+    ops._same_device(x, weight=weight, bias=bias)
+    with ops._on(x):  # (the conv's launches go to the current device's stream)
+        return _GateProjectionFn.apply(x.float(), weight, bias, packed)
