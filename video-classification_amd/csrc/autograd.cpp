@@ -164,9 +164,11 @@ Tensor gated_scan_step(const Tensor& gates, const Tensor& state) {
         refuse("gated_scan_step: gates [B][2H] with contiguous rows expected, got ", gates.sizes());
     const int64_t B = gates.size(0), H = gates.size(1) / 2;
     if (B > INT32_MAX || H > INT32_MAX) refuse("gated_scan_step: gates ", gates.sizes(), " are too large");
-    if (state.scalar_type() != at::kFloat || state.numel() != B * H || !state.is_contiguous())
+    if (state.scalar_type() != at::kFloat || state.sizes() != at::IntArrayRef({B, H}) || !state.is_contiguous())
         refuse("gated_scan_step: state fp32 [", B, "][", H, "], contiguous, expected, got ", state.scalar_type(), " ", state.sizes());
     same_device(gates, state, "state");
+    if (at::GradMode::is_enabled() && (gates.requires_grad() || state.requires_grad()))
+        refuse("gated_scan_step has no gradient, and gates or state want one: torch.no_grad() around it, or gated_scan over one step");
     const c10::DeviceGuard guard(gates.device());
     const Tensor h = at::empty({B, H}, gates.options());
     if (B > 0) {

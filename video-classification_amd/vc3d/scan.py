@@ -21,7 +21,7 @@ def gated_scan(gates, h0=None, lengths=None, reverse=False):
 
 def gated_scan_step(gates, state):
     """one step of gated_scan for each of B sequences, for serving: gates [B][2H], state [B][H] fp32, which is updated in place
-    -> h [B][H] of gates' type.  No gradient."""
+    -> h [B][H] of gates' type.  No gradient: refused where one is wanted (torch.no_grad() around it serves)."""
     return ops.gated_scan_step(gates, state)
 
 
