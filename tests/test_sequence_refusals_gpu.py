@@ -31,3 +31,47 @@ def test_a_state_of_another_shape_is_refused():
     for shape in ((8, 3), (24,), (3, 1, 8), (1, 3, 8), (3, 7)):
         with pytest.raises(Vc3dError):
             vc3d.gated_scan_step(gates, torch.zeros(shape, device="cuda"))
+
+
+class limited:
+    """torch's allocator may hold `more` bytes beside what it holds now"""
+
+    def __init__(self, more):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        self.total = torch.cuda.get_device_properties(0).total_memory
+        self.most = torch.cuda.memory_reserved() + more
+
+    def __enter__(self):
+        torch.cuda.set_per_process_memory_fraction(self.most / self.total)
+
+    def __exit__(self, *exc):
+        torch.cuda.set_per_process_memory_fraction(1.0)
+
+
+def test_memory_that_runs_out_is_torchs_error():
+    """callers that catch torch.OutOfMemoryError, to free memory or take a smaller batch, see it"""
+    import vc3d
+    gates = torch.zeros(64, 1024, 2048, device="cuda")  # 512 MB; h: 256
+    x, w, y = torch.zeros(65536, 8, device="cuda"), torch.zeros(8192, 8, device="cuda"), torch.zeros(65536, dtype=torch.int64, device="cuda")
+    for call in (lambda: vc3d.gated_scan(gates), lambda: vc3d.linear_cross_entropy(x.requires_grad_(), w, y, keep_bytes=4 << 30)):
+        with limited(32 << 20):
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+    assert not vc3d.gated_scan(gates)[0].any()
+
+
+def test_what_a_hook_raises_reaches_the_caller():
+    import vc3d
+
+    class Mine(Exception):
+        pass
+
+    def pack(t):
+        raise Mine("from the hook")
+    gates = torch.zeros(2, 3, 8, device="cuda", requires_grad=True)
+    x, w, y = torch.zeros(4, 8, device="cuda", requires_grad=True), torch.zeros(10, 8, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    for call in (lambda: vc3d.gated_scan(gates), lambda: vc3d.linear_cross_entropy(x, w, y)):
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            with pytest.raises(Mine, match="from the hook"):
+                call()

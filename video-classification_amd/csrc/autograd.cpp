@@ -3,6 +3,7 @@
 // us for some 55 us of kernels, a scan of 3 x 1531 x 1000 135; here 61 and 69.
 #include <Python.h>
 #include <dlfcn.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -270,16 +271,18 @@ Tensor linear_cross_entropy(Tensor x, Tensor w, Tensor labels, Maybe bias, int64
 }
 
 // ---------------------------------------------------------------- Python
+// what this module refuses comes as its own exception, everything else as torch's operators would let it through (memory that runs
+// out, what a caller's hooks raise)
 template <typename F>
 PyObject* guarded(F f) {
+    HANDLE_TH_ERRORS
     try {
         return f();
     } catch (const Error& e) {
         PyErr_SetString(error_class, e.what());
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
     }
-    return nullptr;
+    END_HANDLE_TH_ERRORS
 }
 Tensor tensor(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) refuse(name, " is no tensor");

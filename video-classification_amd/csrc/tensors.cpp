@@ -2,6 +2,7 @@
 // device, sizes, strides and address cost 40-70 ns each through Python; for AdamW over 100 tensors with 8-bit moments that was
 // 140 of a step's 180 us (its kernels: 15).
 #include <Python.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -110,18 +111,20 @@ PyObject* adamw_table(PyObject*, PyObject* args) {
     if (PyObject_GetBuffer(buffer, &view, PyBUF_WRITABLE) != 0) return nullptr;
     PyObject* out = nullptr;
     if (view.len != (Py_ssize_t)(n * sizeof(Row))) PyErr_Format(PyExc_ValueError, "a table of %zd bytes expected", n * sizeof(Row));
-    else try {
+    else
+        out = [&]() -> PyObject* {
+            HANDLE_TH_ERRORS
             const std::string wrong = fill(lists, (int)columns, n, (Row*)view.buf);
-            out = wrong.empty() ? Py_NewRef(Py_None) : PyUnicode_FromStringAndSize(wrong.data(), (Py_ssize_t)wrong.size());
-        } catch (const std::exception& e) {
-            PyErr_SetString(PyExc_RuntimeError, e.what());
-        }
+            return wrong.empty() ? Py_NewRef(Py_None) : PyUnicode_FromStringAndSize(wrong.data(), (Py_ssize_t)wrong.size());
+            END_HANDLE_TH_ERRORS
+        }();
     PyBuffer_Release(&view);
     return out;
 }
 
 // written(list, ...): counts a write in place for each tensor, as torch's own operators do
 PyObject* written(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
     for (Py_ssize_t c = 0; c < PyTuple_GET_SIZE(args); ++c) {
         Sequence list;
         list.o = PySequence_Fast(PyTuple_GET_ITEM(args, c), "lists of tensors expected");
@@ -130,14 +133,11 @@ PyObject* written(PyObject*, PyObject* args) {
             PyObject* const o = PySequence_Fast_GET_ITEM(list.o, i);
             if (!THPVariable_Check(o)) return PyErr_Format(PyExc_TypeError, "tensors expected"), nullptr;
             const at::Tensor& t = THPVariable_Unpack(o);
-            try {
-                if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-            } catch (const std::exception& e) {
-                return PyErr_SetString(PyExc_RuntimeError, e.what()), nullptr;
-            }
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
         }
     }
     Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef METHODS[] = {{"adamw_table", adamw_table, METH_VARARGS, nullptr},
