@@ -75,3 +75,28 @@ def test_what_a_hook_raises_reaches_the_caller():
         with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
             with pytest.raises(Mine, match="from the hook"):
                 call()
+
+
+@pytest.mark.parametrize("engine", [False, True])
+def test_nothing_is_kept_where_there_is_no_room(engine):
+    """8192 x 65536 bf16 logits are 1 GB: with less the step runs as with keep_bytes=0, to the same bits; what the caller asked to be
+    kept is not dropped"""
+    import vc3d
+    from vc3d.linear_ce import _EngineHeadFn
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(8192, 1024, device="cuda", generator=g).bfloat16().requires_grad_()
+    w = (torch.randn(65536, 1024, device="cuda", generator=g) / 32).bfloat16().requires_grad_()
+    y = torch.randint(0, 65536, (8192,), device="cuda", generator=g)
+
+    def step(keep):
+        if engine and keep == -1:
+            loss = _EngineHeadFn.apply(x, w, None, y, type("Engine", (), dict(flat_grad=None)))
+        else:
+            loss = vc3d.linear_cross_entropy(x, w, y, keep_bytes=keep)
+        return (loss.detach(),) + torch.autograd.grad(loss, (x, w))
+    want = step(0)
+    with limited(1000 << 20):
+        got = step(-1)
+        with pytest.raises(torch.OutOfMemoryError):
+            step(2 << 30)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

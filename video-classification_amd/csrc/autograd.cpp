@@ -198,16 +198,24 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& labels, const Maybe& bias, int64_t ignore,
                           int64_t reduction, int64_t keep, bool grad) {
         const c10::DeviceGuard guard(x.device());
-        const vc_linear_ce_desc d = lce_desc(x, w, ignore, reduction, keep);
+        vc_linear_ce_desc d = lce_desc(x, w, ignore, reduction, keep);
         const auto f32 = x.options().dtype(at::kFloat);
         Tensor loss = reduction == 0 ? at::empty({d.N}, f32) : at::empty({}, f32), saved;
         if (d.N == 0) {
             loss.zero_();
             saved = bytes(0, x);
         } else {
-            saved = bytes(lib.lce_saved(&d), x);
-            const size_t need = lib.lce_workspace(&d, 0);
-            const Tensor ws = bytes(need, x);
+            size_t need = 0;
+            Tensor ws;
+            auto allocate = [&] { saved = bytes(lib.lce_saved(&d), x), need = lib.lce_workspace(&d, 0), ws = bytes(need, x); };
+            try {
+                allocate();
+            } catch (const c10::OutOfMemoryError&) {  // what is kept by itself is kept where there is room for it
+                if (keep != -1) throw;
+                saved = ws = Tensor();
+                d.keep_bytes = keep = 0;
+                allocate();
+            }
             check(lib.lce_fwd(&d, x.data_ptr(), w.data_ptr(), ptr(bias), (const int64_t*)labels.data_ptr(), (float*)loss.data_ptr(), saved.data_ptr(),
                               ws.data_ptr(), need, stream(x)),
                   "vc_linear_ce_fwd");

@@ -16,7 +16,12 @@ class _EngineHeadFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, labels, engine):
         grad = any(ctx.needs_input_grad)
-        loss, saved = ops.linear_ce_fwd(x, weight, labels, bias, keep_bytes=-1 if grad else 0)
+        ctx.keep = -1 if grad else 0
+        try:
+            loss, saved = ops.linear_ce_fwd(x, weight, labels, bias, keep_bytes=ctx.keep)
+        except torch.OutOfMemoryError:
+            ctx.keep = 0
+            loss, saved = ops.linear_ce_fwd(x, weight, labels, bias, keep_bytes=0)
         if grad:
             ctx.save_for_backward(x, weight, labels, bias, saved)
             ctx.engine, ctx.params = engine, (weight, bias)
@@ -27,7 +32,7 @@ class _EngineHeadFn(torch.autograd.Function):
     def backward(ctx, dloss):
         x, weight, labels, bias, saved = ctx.saved_tensors
         want, eng = ctx.needs_input_grad, ctx.engine
-        dx, dw, db = ops.linear_ce_bwd(x, weight, labels, bias, saved, dloss.contiguous().view(1), want=want[:3])
+        dx, dw, db = ops.linear_ce_bwd(x, weight, labels, bias, saved, dloss.contiguous().view(1), want=want[:3], keep_bytes=ctx.keep)
         wp, bp = ctx.params
         if eng.flat_grad is not None and id(wp) in eng.grad_views:
             eng._bind_grads()
@@ -44,9 +49,10 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     all bf16; labels int64 [...] on the GPU.  Logits, sums and the loss are fp32.  Rows whose label is ignore_index take no part
     (their x is not read and its gradient is 0); "mean" is over the others, and 0 where there is none (torch: NaN).  Any other
     label outside [0, V) gives a NaN.  reduction "none" returns labels' shape.  Differentiable in x, weight and bias; the
-    gradients are of the inputs' type.  keep_bytes: whether the forward keeps the logits' gradient for the
-    backward (N x V of the inputs' type; and, while there is room, the copy of a weight whose rows are no whole 16 bytes): 0 no, the backward computes the logits again; n: where it takes at most n bytes; -1: where
-    that is quicker and takes at most 2 GB.  Never with reduction "none"."""
+    gradients are of the inputs' type.  keep_bytes: whether the forward keeps the logits' gradient for the backward (N x V of the
+    inputs' type; and, while there is room, the copy of a weight whose rows are no whole 16 bytes): 0 no, the backward computes the
+    logits again; n: where it takes at most n bytes; -1: where that is quicker, takes at most 2 GB and there is memory for it.
+    Never with reduction "none"."""
     if reduction not in _REDUCTION:
         raise Vc3dError("linear_cross_entropy: reduction 'none', 'mean' or 'sum', got %r" % (reduction,))
     return ops._tensors.linear_cross_entropy(x, weight, labels, bias, ignore_index, _REDUCTION[reduction], keep_bytes)
