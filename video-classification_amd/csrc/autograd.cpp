@@ -65,6 +65,17 @@ bool is_bf16(const Tensor& t, const char* name) {
 void same_device(const Tensor& ref, const Maybe& t, const char* name) {
     if (t && t->device() != ref.device()) refuse(name, " is on ", t->device(), ", not on ", ref.device());
 }
+// What autograd hands back may have passed through a caller's hooks (kept elsewhere and loaded again, at another address, with other
+// strides): the backward asks of it again what its launches rely on.
+std::vector<int64_t> shape_of(const Tensor& t) {
+    std::vector<int64_t> v = t.sizes().vec();
+    v.insert(v.end(), {(int64_t)t.scalar_type(), (int64_t)t.device().index()});
+    return v;
+}
+void as_saved(const Tensor& t, const char* name, at::IntArrayRef sizes, at::ScalarType type, const Tensor& where) {
+    if (!t.is_cuda() || t.layout() != at::kStrided || t.device() != where.device() || t.scalar_type() != type || t.sizes() != sizes)
+        refuse(name, " came back from the saved tensors' hooks as another tensor: ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+}
 // gradients of gradients are not there: whoever asks for them is told so, not given none
 torch::autograd::variable_list once(torch::autograd::variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -105,14 +116,24 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
             ctx->save_for_backward({gates, defined(lengths), states});
             ctx->saved_data["reverse"] = reverse;
             ctx->saved_data["h0"] = h0.has_value();
+            ctx->saved_data["shape"] = shape_of(gates);
         }
         return {h, last};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list up) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &gates = saved[0], &lengths = saved[1], &states = saved[2];
+        Tensor gates = saved[0], lengths = saved[1], states = saved[2];
         Tensor dy = up[0], dlast = up[1], dgates, dh0;
         if (!dy.defined() && !dlast.defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        {
+            const auto v = ctx->saved_data["shape"].toIntVector();  // B, T, 2H, type, device
+            const Tensor& up = dy.defined() ? dy : dlast;
+            as_saved(gates, "gates", at::IntArrayRef(v).slice(0, 3), (at::ScalarType)v[3], up);
+            if (lengths.defined()) as_saved(lengths, "lengths", {v[0]}, at::kInt, up), lengths = lengths.contiguous();
+            as_saved(states, "states", {v[0], (v[1] + VC_SCAN_STATE_STEPS - 1) / VC_SCAN_STATE_STEPS, v[2] / 2}, at::kFloat, up);
+            if (gates.stride(2) != 1) gates = gates.contiguous();
+            states = states.contiguous();
+        }
         const c10::DeviceGuard guard(gates.device());
         const vc_scan_desc d = scan_desc(gates, ctx->saved_data["reverse"].toBool());
         if (dy.defined()) {  // contiguous, at a multiple of two elements (a slice's storage may begin anywhere)
@@ -225,15 +246,30 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
             ctx->saved_data["ignore"] = ignore;
             ctx->saved_data["reduction"] = reduction;
             ctx->saved_data["keep"] = keep;
+            ctx->saved_data["shape"] = std::vector<int64_t>{d.N, d.D, d.V, (int64_t)x.scalar_type(), saved.numel()};
         }
         return loss;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list up) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &labels = saved[2], &bias = saved[3];
+        Tensor x = saved[0], w = saved[1], labels = saved[2], bias = saved[3], kept = saved[4];
+        {
+            const auto v = ctx->saved_data["shape"].toIntVector();  // N, D, V, type, bytes saved
+            const auto type = (at::ScalarType)v[3];
+            as_saved(x, "x", {v[0], v[1]}, type, up[0]), as_saved(w, "weight", {v[2], v[1]}, type, up[0]);
+            as_saved(labels, "labels", {v[0]}, at::kLong, up[0]), as_saved(kept, "what the forward saved", {v[4]}, at::kByte, up[0]);
+            if (bias.defined()) as_saved(bias, "bias", {v[2]}, type, up[0]), bias = bias.contiguous();
+            x = rows(x), w = rows(w), labels = labels.contiguous(), kept = kept.contiguous();
+            if ((uintptr_t)kept.data_ptr() % 256 != 0) kept = kept.clone();
+        }
         const c10::DeviceGuard guard(x.device());
-        const vc_linear_ce_desc d =
-            lce_desc(x, w, ctx->saved_data["ignore"].toInt(), ctx->saved_data["reduction"].toInt(), ctx->saved_data["keep"].toInt());
+        auto desc = [&] {
+            return lce_desc(x, w, ctx->saved_data["ignore"].toInt(), ctx->saved_data["reduction"].toInt(), ctx->saved_data["keep"].toInt());
+        };
+        vc_linear_ce_desc d = desc();
+        // whether the forward left a copy of w goes by where w lay then: one that would need the copy now is laid as it was
+        if (d.N > 0 && lib.lce_saved(&d) > (size_t)kept.numel()) w = w.clone(at::MemoryFormat::Contiguous), d = desc();
+        if (d.N > 0 && lib.lce_saved(&d) > (size_t)kept.numel()) refuse("linear_cross_entropy: the weight came back in another layout");
         const Tensor dloss = up[0].contiguous();
         Tensor dx, dw, db;
         if (ctx->needs_input_grad(0)) dx = at::empty({d.N, d.D}, x.options());
@@ -245,7 +281,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         } else {
             const size_t need = lib.lce_workspace(&d, 1);
             const Tensor ws = bytes(need, x);
-            check(lib.lce_bwd(&d, x.data_ptr(), w.data_ptr(), ptr(bias), (const int64_t*)labels.data_ptr(), saved[4].data_ptr(),
+            check(lib.lce_bwd(&d, x.data_ptr(), w.data_ptr(), ptr(bias), (const int64_t*)labels.data_ptr(), kept.data_ptr(),
                               (const float*)dloss.data_ptr(), ptr(dx), ptr(dw), ptr(db), ws.data_ptr(), need, stream(x)),
                   "vc_linear_ce_bwd");
         }
