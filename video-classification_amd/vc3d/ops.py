@@ -691,11 +691,23 @@ def linear_bwd(dlogits, feat, W, dW=None, db=None, want_dfeat=True):
 # current stream) and bring their own workspace from torch's allocator, per call: nothing is shared between calls, streams or
 # captured graphs.
 
+class _Missing:
+    """in the place of _tensors.so where it cannot be loaded (it is bound to one build of torch, libvc3d.so is not): the operators
+    that need it fail, the video path does without"""
+
+    def __init__(self, why):
+        self._why = why
+
+    def __getattr__(self, name):
+        raise capi.Vc3dError("%s needs vc3d/_tensors.so, which could not be loaded (%s): build it with `make -C video-classification_amd/csrc`" %
+                             (name, self._why))
+
+
 try:
     from . import _tensors
+    _tensors.bind(capi.LIB_PATH, capi.Vc3dError)
 except ImportError as e:
-    raise capi.Vc3dError("vc3d/_tensors.so could not be loaded (%s): build it with `make -C video-classification_amd/csrc`" % e)
-_tensors.bind(capi.LIB_PATH, capi.Vc3dError)
+    _tensors = _Missing(e)
 
 _FLOAT_KIND = {F32: 0, BF16: 1}
 ADAMW_BLOCK = 256  # elements that share a scale of an 8-bit moment
