@@ -326,7 +326,8 @@ int vc_adamw_step(const vc_adamw_tensor* tensors, int32_t count, int32_t is_bf16
  * gates and dy hold there is not read.  reverse: the recurrence runs from the last step to the first.  h0 (nullable: zeros), last, dlast
  * (nullable), dh0 (nullable) are fp32 [B][H]; last = the state behind the last step, h0 for a sequence without steps.  The
  * state is fp32 throughout; h, dgates are of gates' type, contiguous [B][T][H] and [B][T][2H], as is dy (nullable) and all of
- * them aligned to two elements.  gates has any strides over B and T.  states (fp32 [B][ceil(T / 64)][H]; forward: nullable)
+ * them aligned to two elements.  gates has any strides over B and T.  At most 65535 sequences, H <= 2^24, T <= 2^30, and one sequence
+ * of fewer than some 4 million tiles (of 128 steps x 128 channels or more).  states (fp32 [B][ceil(T / 64)][H]; forward: nullable)
  * carries the forward's states to the backward.  workspace: vc_gated_scan_workspace_bytes(d, op), op 0 forward, 1 backward
  * (0: none needed); its content is not kept.  Results do not depend on the order in which workgroups run. */
 #define VC_SCAN_STATE_STEPS 64
@@ -358,7 +359,7 @@ int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, flo
  * dloss: fp32 on the device, [1], or [N] with reduction 0.  dx [N][D], dw [V][D], db [V] (each nullable) are contiguous,
  * dx and dw 16-byte aligned, and of x's type, and are written, not added to.  workspace (required, 256-byte aligned): vc_linear_ce_workspace_bytes(d, op),
  * op 0 forward, 1 backward: of the N x V logits the forward keeps two floats for every 64 .. 256 (and what is in saved), the
- * backward that has no gradient of the logits one block of up to 512 MB.  Results do not depend on the order in which workgroups run. */
+ * backward that has no gradient of the logits one block of up to 512 MB.  N, V <= 2^23, D <= 2^20, N D and V D <= 2^37.  Results do not depend on the order in which workgroups run. */
 typedef struct vc_linear_ce_desc {
     int32_t N, D, V, is_bf16;
     int32_t reduction, w_align; /* w's address modulo 16: rows that are no whole 16-byte chunks are copied, piece by piece */

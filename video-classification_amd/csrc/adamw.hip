@@ -313,11 +313,11 @@ int vc_adamw_launch(const VcAdamwTensor* t, int count, bool is_bf16, int bits, V
     for (int i = 0; i < count;) {
         a.count = 0;
         unsigned blocks = 0;
-        // a launch takes up to VC_ADAMW_MAX_TENSORS tensors and 2^30 workgroups
+        // a launch takes up to VC_ADAMW_MAX_TENSORS tensors and fewer than 2^32 lanes (HIP's limit): 2^24 - 1 workgroups
         for (; i < count && a.count < VC_ADAMW_MAX_TENSORS; ++i) {
             if (t[i].n == 0) continue;
             const long long need = (t[i].n + CHUNK - 1) / CHUNK;
-            if (a.count > 0 && blocks + need > (1ll << 30)) break;
+            if (a.count > 0 && blocks + need >= (1ll << 24)) break;
             a.t[a.count] = t[i];
             a.first[a.count++] = blocks;
             blocks += (unsigned)need;

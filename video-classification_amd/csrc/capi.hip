@@ -1220,7 +1220,7 @@ int vc_adamw_step(const vc_adamw_tensor* tensors, int32_t count, int32_t is_bf16
                "adamw_step: lr, eps and weight_decay are at least 0, the betas in [0, 1)");
     for (int32_t i = 0; i < count; ++i) {
         const vc_adamw_tensor& t = tensors[i];
-        VC_REQUIRE(t.n >= 0 && t.n < (1ll << 42), "adamw_step: tensor %d has %lld elements", i, (long long)t.n);
+        VC_REQUIRE(t.n >= 0 && t.n <= (1ll << 36) - 4096, "adamw_step: tensor %d has %lld elements", i, (long long)t.n);
         if (t.n == 0) continue;
         VC_REQUIRE(t.p && t.g && t.m && t.v, "adamw_step: null pointer in tensor %d", i);
         VC_REQUIRE(state_bits == 32 || (t.m_scale && t.v_scale), "adamw_step: tensor %d has no scales for its 8-bit moments", i);
@@ -1243,8 +1243,7 @@ static int scan_check(const vc_scan_desc* d) {
     VC_REQUIRE(d->B > 0 && d->T > 0 && d->H > 0, "gated_scan: bad sizes B=%d T=%d H=%d", d->B, d->T, d->H);
     VC_REQUIRE(d->B <= 65535, "gated_scan: at most 65535 sequences (got %d)", d->B);
     VC_REQUIRE(d->T <= (1 << 30) && d->H <= (1 << 24), "gated_scan: T=%d or H=%d too large", d->T, d->H);
-    VC_REQUIRE(((long long)d->T + 63) / 64 * d->B * ((d->H + 127) / 128) < (1ll << 31), "gated_scan: B=%d T=%d H=%d are too many tiles", d->B,
-               d->T, d->H);
+    VC_REQUIRE(vc_scan_fits(d->T, d->H, d->is_bf16 != 0), "gated_scan: T=%d H=%d are too many tiles", d->T, d->H);
     return 0;
 }
 static VcScanParams scan_params(const vc_scan_desc* d, const void* gates, const int32_t* lengths) {
@@ -1286,7 +1285,7 @@ int vc_gated_scan_bwd(const vc_scan_desc* d, const void* gates, const int32_t* l
     return vc_scan_launch_bwd(p, d->is_bf16 != 0, S(stream));
 }
 int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, float* state, void* h, int32_t B, int32_t H, void* stream) {
-    VC_REQUIRE(gates && state && h && B > 0 && H > 0, "gated_scan_step: bad arguments");
+    VC_REQUIRE(gates && state && h && B > 0 && H > 0 && H <= (1 << 30), "gated_scan_step: bad arguments");
     return vc_scan_launch_step(gates, stride_b, state, h, B, H, is_bf16 != 0, S(stream));
 }
 
@@ -1295,6 +1294,7 @@ static int lce_check(const vc_linear_ce_desc* d) {
     VC_REQUIRE(d != nullptr, "null descriptor");
     VC_REQUIRE(d->N > 0 && d->D > 0 && d->V > 0, "linear_ce: bad sizes N=%d D=%d V=%d", d->N, d->D, d->V);
     VC_REQUIRE(d->N <= (1 << 23) && d->V <= (1 << 23) && d->D <= (1 << 20), "linear_ce: at most 2^23 rows and classes, 2^20 features");
+    VC_REQUIRE((long long)d->N * d->D <= (1ll << 37) && (long long)d->V * d->D <= (1ll << 37), "linear_ce: x or w has more than 2^37 elements");
     VC_REQUIRE(d->ldx >= d->D && d->ldw >= d->D, "linear_ce: row strides %lld, %lld below D=%d", (long long)d->ldx, (long long)d->ldw, d->D);
     VC_REQUIRE(d->w_align >= 0 && d->w_align < 16, "linear_ce: w_align %d is no address modulo 16", d->w_align);
     VC_REQUIRE(d->keep_bytes >= -1, "linear_ce: keep_bytes %lld", (long long)d->keep_bytes);

@@ -218,6 +218,7 @@ struct VcScanParams {
     float* dh0;          // nullable [B][H]
     char* ws;
 };
+bool vc_scan_fits(int T, int H, bool is_bf16);  // whether a launch has room for one sequence
 size_t vc_scan_workspace(int B, int T, int H, bool is_bf16, int op);
 int vc_scan_launch_fwd(const VcScanParams& p, bool is_bf16, hipStream_t s);
 int vc_scan_launch_bwd(const VcScanParams& p, bool is_bf16, hipStream_t s);

@@ -922,6 +922,10 @@ struct Plan {
         const long long np = ((long long)N + 255) / 256 * 256, all = ((long long)V + 255) / 256 * 256;
         long long fit = (512ll << 20) / elem / np / 256 * 256;
         if (op == 0 || keep) fit = pack && keep < 2 ? (512ll << 20) / elem / ld / 256 * 256 : all;  // (a piece of w's copy is all there is)
+        if (op == 0 || keep) {  // a launch has fewer than 2^32 lanes (HIP's limit), 512 for a tile of 256 x 256
+            const long long most = ((1ll << 23) - 1) / (np / 256) * 256;
+            fit = fit < most ? fit : most;
+        }
         fit = fit < 256 ? 256 : fit;
         lde = all;
         piece = (int)(fit < all ? fit : all);

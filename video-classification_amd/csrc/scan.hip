@@ -520,20 +520,42 @@ constexpr int fwd_sub(bool is_bf16) { return is_bf16 ? 16 : 8; }
 // with 64, 76 with 16; 1 x 131072 x 16 205 with 64, 78 with 8)
 int lanes(int H) { return H > 64 ? 64 : H > 32 ? 32 : H > 16 ? 16 : 8; }
 int tile_steps(int H, bool is_bf16, int op) { return WAVES * (op == 0 ? fwd_sub(is_bf16) : BWD_SUB) * (64 / lanes(H)); }
-// the workgroups of a launch; clears what they exchange their states through
-unsigned begin(const VcScanParams& p, bool is_bf16, int op, hipStream_t s) {
-    const int steps = tile_steps(p.H, is_bf16, op), channels = 2 * lanes(p.H);
-    const long long tiles = (p.T + (long long)steps - 1) / steps, n = (long long)vc_scan_workspace(p.B, p.T, p.H, is_bf16, op) / 16, blocks = (n + 255) / 256;
-    if (n > 0) hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)p.ws, n);
-    return (unsigned)(tiles * ((p.H + channels - 1) / channels) * p.B);
+// the workgroups of one sequence
+long long workgroups(int T, int H, bool is_bf16, int op) {
+    const int steps = tile_steps(H, is_bf16, op), channels = 2 * lanes(H);
+    return ((long long)T + steps - 1) / steps * ((H + channels - 1) / channels);
+}
+// a launch has fewer than 2^32 lanes (HIP's limit for a dimension of the grid)
+constexpr long long MOST_WORKGROUPS = ((1ll << 32) - 1) / (WAVES * 64);
+
+// the sequences from b on, n of them
+VcScanParams part(const VcScanParams& p, bool is_bf16, int b, int n) {
+    const long long elem = is_bf16 ? 2 : 4, row = (long long)b * p.H, steps = row * p.T;
+    const auto at = [](const void* q, long long bytes) { return q != nullptr ? (char*)q + bytes : nullptr; };
+    VcScanParams q = p;
+    q.B = n;
+    q.gates = at(p.gates, b * p.sb * elem);
+    q.lengths = (const int*)at(p.lengths, b * 4ll);
+    q.h0 = (const float*)at(p.h0, row * 4), q.last = (float*)at(p.last, row * 4);
+    q.dlast = (const float*)at(p.dlast, row * 4), q.dh0 = (float*)at(p.dh0, row * 4);
+    q.states = (float*)at(p.states, row * ((p.T + VC_SCAN_CHUNK - 1) / VC_SCAN_CHUNK) * 4);
+    q.h = at(p.h, steps * elem), q.dy = at(p.dy, steps * elem), q.dgates = at(p.dgates, 2 * steps * elem);
+    return q;
 }
 
 template <typename T, Channels C, int LANES>
-void launch(const VcScanParams& p, int op, hipStream_t s) {
+void launch(const VcScanParams& all, int op, hipStream_t s) {
     constexpr bool is_bf16 = sizeof(T) == 2;
-    const dim3 grid(begin(p, is_bf16, op, s)), block(WAVES * 64);
-    if (op == 0) hipLaunchKernelGGL((scan_fwd_kernel<T, WAVES, fwd_sub(is_bf16), C, LANES>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((scan_bwd_kernel<T, WAVES, BWD_SUB, C, LANES>), grid, block, 0, s, p);
+    const long long each = workgroups(all.T, all.H, is_bf16, op), most = MOST_WORKGROUPS / each;
+    for (long long b = 0; b < all.B; b += most) {  // (all sequences in one launch up to some 4 million workgroups)
+        const VcScanParams p = part(all, is_bf16, (int)b, (int)(all.B - b < most ? all.B - b : most));
+        // what the tiles exchange their states through
+        const long long n = (long long)vc_scan_workspace(p.B, p.T, p.H, is_bf16, op) / 16, blocks = (n + 255) / 256;
+        if (n > 0) hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, (uint4*)p.ws, n);
+        const dim3 grid((unsigned)(each * p.B)), block(WAVES * 64);
+        if (op == 0) hipLaunchKernelGGL((scan_fwd_kernel<T, WAVES, fwd_sub(is_bf16), C, LANES>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((scan_bwd_kernel<T, WAVES, BWD_SUB, C, LANES>), grid, block, 0, s, p);
+    }
 }
 template <typename T, Channels C>
 void launch(const VcScanParams& p, int op, hipStream_t s) {
@@ -553,6 +575,7 @@ void launch(const VcScanParams& p, int op, hipStream_t s) {
 
 }  // namespace
 
+bool vc_scan_fits(int T, int H, bool is_bf16) { return workgroups(T, H, is_bf16, 0) <= MOST_WORKGROUPS && workgroups(T, H, is_bf16, 1) <= MOST_WORKGROUPS; }
 // what the tiles of a sequence exchange: 0 where a sequence is one tile
 size_t vc_scan_workspace(int B, int T, int H, bool is_bf16, int op) {
     const int steps = tile_steps(H, is_bf16, op);
