@@ -333,16 +333,17 @@ class AdamW(torch.optim.Optimizer):
                 st = self.state[p]
                 if not st:
                     st.update(self._new_state(p))
-                st["step"] += 1
                 g = p.grad
                 if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
                     g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)  # into the parameter's order of memory
-                cols = lists.setdefault((p.dtype, p.device, st["step"]), tuple([] for _ in range(6)))
-                for col, t in zip(cols, (p, g, st["exp_avg"], st["exp_avg_sq"], st.get("exp_avg_scale"), st.get("exp_avg_sq_scale"))):
+                cols = lists.setdefault((p.dtype, p.device, st["step"] + 1), tuple([] for _ in range(7)))
+                for col, t in zip(cols, (p, g, st["exp_avg"], st["exp_avg_sq"], st.get("exp_avg_scale"), st.get("exp_avg_sq_scale"), st)):
                     col.append(t)
-            for (_, _, step), cols in lists.items():
+            for (_, _, step), (*cols, states) in lists.items():
                 ops.adamw_step(*cols[:4], *(cols[4:] if self.state_bits == 8 else (None, None)), lr=group["lr"], beta1=group["betas"][0],
                                beta2=group["betas"][1], eps=group["eps"], weight_decay=group["weight_decay"], step=step, grad_scale=grad_scale)
+                for st in states:  # (a step that is refused does not count)
+                    st["step"] = step
         return loss
 
     def state_dict(self):
