@@ -44,3 +44,15 @@ def test_a_refused_step_does_not_count(adamw):
     ps[0].grad = None
     opt.step()
     assert counts(opt, ps) == [2, 3, 2] and [c[1] for c in calls[-2:]] == [3, 2]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_copy_holds_its_moments_in_as_many_bits(bits):
+    import copy
+    import pickle
+
+    from vc3d.optim import AdamW
+    opt = AdamW([torch.nn.Parameter(torch.zeros(3))], lr=0.5, state_bits=bits)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.state_bits == bits and other.param_groups[0]["lr"] == 0.5
+        assert other.state_dict()["state_bits"] == bits

@@ -346,6 +346,9 @@ class AdamW(torch.optim.Optimizer):
                     st["step"] = step
         return loss
 
+    def __getstate__(self):  # (torch's holds what it knows of)
+        return {**super().__getstate__(), "state_bits": self.state_bits}
+
     def state_dict(self):
         sd = super().state_dict()
         sd["state_bits"] = self.state_bits
