@@ -56,3 +56,19 @@ def test_a_copy_holds_its_moments_in_as_many_bits(bits):
     for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
         assert other.state_bits == bits and other.param_groups[0]["lr"] == 0.5
         assert other.state_dict()["state_bits"] == bits
+
+
+def test_moments_that_torch_held_in_the_parameters_type_are_widened():
+    """torch.optim.AdamW holds the moments of a bf16 parameter in bf16; here they are fp32 whatever the parameter's type"""
+    from vc3d.optim import AdamW
+    p = torch.nn.Parameter(torch.randn(40).bfloat16())
+    theirs = torch.optim.AdamW([p], lr=1e-2)
+    for _ in range(2):
+        p.grad = torch.randn(40).bfloat16()
+        theirs.step()
+    mine = AdamW([p], lr=1e-2)
+    mine.load_state_dict(theirs.state_dict())
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert theirs.state[p][k].dtype == torch.bfloat16 and mine.state[p][k].dtype == torch.float32
+        assert torch.equal(mine.state[p][k], theirs.state[p][k].float())
+    assert mine.state[p]["step"] == 2

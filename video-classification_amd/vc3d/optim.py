@@ -356,7 +356,7 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, sd):
         sd = dict(sd)
-        if sd.pop("state_bits", 32) != self.state_bits:  # (torch.optim.AdamW's states name no bits: fp32 ones are taken over)
+        if sd.pop("state_bits", 32) != self.state_bits:  # (torch.optim.AdamW's states name no bits: they are taken over as fp32)
             raise Vc3dError("AdamW: the saved moments are not held in %d bits" % self.state_bits)
         if any(g.get("amsgrad") or g.get("maximize") for g in sd["param_groups"]):
             raise Vc3dError("AdamW: amsgrad and maximize are not supported")
@@ -369,4 +369,5 @@ class AdamW(torch.optim.Optimizer):
                 if k == "step":
                     self.state[p][k] = int(v)
                 elif torch.is_tensor(v):
-                    self.state[p][k] = v.detach().to(p.device, copy=True)
+                    widen = self.state_bits == 32 and v.is_floating_point()  # (torch's moments of a bf16 parameter are bf16)
+                    self.state[p][k] = v.detach().to(p.device, torch.float32 if widen else v.dtype, copy=True)
