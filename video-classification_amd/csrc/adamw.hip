@@ -26,10 +26,13 @@
 // launch, so a captured step replays.
 //
 // Root and quotient are correctly rounded.  The compiler's sequences for that (33 issue slots together) cover every input; a
-// wave whose values all lie in the middle of the range (v and |m'| in [2^-90, 2^20]) uses shorter ones (20): with y = the
-// reciprocal (root) from the hardware's estimate by one Newton step, q' = q + (a - b q) y is correctly rounded (P. Markstein,
-// Computation of elementary functions on the IBM RISC System/6000 processor, 1990); tests/test_adamw_gpu.py compares the
-// root's for all mantissas.
+// wave whose values all lie in the middle of the range (v and |m'| in [2^-90, 2^20]) uses shorter ones (20).  With y = the correctly
+// rounded reciprocal (root), q' = q + (a - b q) y is correctly rounded (P. Markstein, Computation of elementary functions on the IBM
+// RISC System/6000 processor, 1990; a divisor whose mantissa is all ones is left out there).  That one Newton step makes such a y of
+// the hardware's estimate does not follow: by arithmetic, an estimate one unit above the rounded reciprocal would miss it for 32
+// mantissas, and one unit beside it for all ones.  It holds for this hardware's estimates (gfx950: off by one unit for 897 675 of the
+// 2^23 mantissas): y compared for all 2^23, the root for all 2^24 of two octaves, the quotients by an all-ones divisor for all 2^23
+// numerators.  tests/test_adamw_mantissas_gpu.py repeats the last two.
 #include "common.h"
 #include "kernels.h"
 
