@@ -72,3 +72,12 @@ def test_moments_that_torch_held_in_the_parameters_type_are_widened():
         assert theirs.state[p][k].dtype == torch.bfloat16 and mine.state[p][k].dtype == torch.float32
         assert torch.equal(mine.state[p][k], theirs.state[p][k].float())
     assert mine.state[p]["step"] == 2
+
+
+def test_eight_bits_that_there_are_not_are_refused():
+    """without a GPU 'adamw' is torch's, whose moments have no other width"""
+    from helpers import make_config
+    from utils.utils import create_optimizer
+    cfg = make_config(18, 10, OPTIMIZER="adamw", STATE_BITS=8)
+    with pytest.raises(ValueError, match="STATE_BITS"):
+        create_optimizer(cfg, torch.nn.Linear(4, 2))

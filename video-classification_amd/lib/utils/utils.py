@@ -26,6 +26,9 @@ def create_optimizer(cfg, model):
         from vc3d.optim import AdamW  # any model, one launch per 60 tensors, moments in TRAIN.STATE_BITS (32 or 8) bits
         return AdamW(params, lr=cfg.TRAIN.LR, weight_decay=cfg.TRAIN.WD, state_bits=cfg.TRAIN.STATE_BITS)
     if name == 'adamw':
+        if cfg.TRAIN.STATE_BITS != 32:
+            raise ValueError("TRAIN.STATE_BITS is %r and the model is not on the GPU: moments in fewer than 32 bits are held there only" %
+                             (cfg.TRAIN.STATE_BITS,))
         return torch.optim.AdamW(params, lr=cfg.TRAIN.LR, weight_decay=cfg.TRAIN.WD)
     return None
 
