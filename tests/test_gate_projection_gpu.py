@@ -148,3 +148,30 @@ def test_a_step_of_no_sequences():
     assert cell(x).shape == (0, 64)
     with torch.no_grad():
         assert cell(x).shape == (0, 64)
+
+
+def test_a_captured_sequence_with_its_backward():
+    """forward and backward in one graph, replayed with new inputs and new weights between eager work on a copy of the module"""
+    cell, g = cell_of(128, 192, 15), torch.Generator().manual_seed(16)
+    x = torch.randn(6, 150, 128, generator=g).cuda().requires_grad_()
+    up = torch.randn(6, 150, 192, generator=g).cuda()
+
+    def once(c, x):
+        h, last = c.sequence(x)
+        return (h.detach(), last.detach()) + torch.autograd.grad((h, last), (x, c.gates.weight, c.gates.bias), (up, last.detach()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once(cell, x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once(cell, x)
+    for rep in range(4):
+        with torch.no_grad():
+            for t in (x, cell.gates.weight, cell.gates.bias):
+                t.copy_(torch.randn(t.shape, generator=g) * (0.5 + rep) / 8)
+        want = once(copy.deepcopy(cell), x.detach().clone().requires_grad_())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert equal(out, want), rep
