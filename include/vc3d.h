@@ -344,6 +344,11 @@ int vc_gated_scan_bwd(const vc_scan_desc* d, const void* gates, const int32_t* l
 /* one step for each of B sequences (serving): state [B][H] fp32 is updated in place, h [B][H] is of gates' type; gates row b
  * is at gates + b * stride_b */
 int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, float* state, void* h, int32_t B, int32_t H, void* stream);
+/* operands of a product (vc_conv3d_fwd, 1x1x1) that adds a bias inside its fp32 sums, for the gates of the recurrences above (the
+ * reference's cell adds its bias to the products: lib/models/lstm.py:16): in [rows][D] -> out [rows][D + 64], where behind each row
+ * stand, bias null: 1 1 1 0 ... 0 (rows of x); bias [rows]: three numbers of 8 bits whose sum it is, and zeros (rows of the weight).
+ * D is a multiple of 4; out is bf16 or fp32. */
+int vc_bias_columns(const float* in, const float* bias, void* out, int32_t out_is_bf16, int64_t rows, int32_t D, void* stream);
 
 /* ---- Linear classifier + cross-entropy in one operator, the vocabulary in pieces: the reference's clf_haed and
  * CrossEntropyLoss (lib/models/model.py:24,38, lib/core/loss.py:10,25) for class counts whose logits are not worth keeping.

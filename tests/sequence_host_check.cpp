@@ -1,5 +1,5 @@
 // Host-side check of the operators of long sequences and large vocabularies (include/vc3d.h: vc_gated_scan_*, vc_linear_ce_*,
-// vc_adamw_step) under AddressSanitizer + UndefinedBehaviorSanitizer, no GPU needed.  The HIP calls that a launch makes are defined
+// vc_adamw_step, vc_bias_columns) under AddressSanitizer + UndefinedBehaviorSanitizer, no GPU needed.  The HIP calls that a launch makes are defined
 // here: they write the launch down and succeed, so the planners, workspace layouts and loops over pieces run to their end, for
 // small, odd and the largest sizes, with addresses that are never read.  What is checked of every launch: fewer than 2^32 lanes in a
 // dimension, no empty grid; of sequences that take several launches, where each part begins.
@@ -113,6 +113,8 @@ static void adamw(const std::vector<int64_t>& sizes, bool bf16, int bits) {
 
 int main() {
     for (bool bf16 : {false, true}) {
+        for (int64_t rows : {(int64_t)1, (int64_t)5, (int64_t)262143, (int64_t)1 << 40})
+            for (int D : {4, 64, 1 << 24}) run("bias columns", rows, D, 0, [&] { return vc_bias_columns((float*)P, D == 64 ? (float*)P : nullptr, P, bf16, rows, D, nullptr); });
         for (int B : {1, 3, 64, 65535})
             for (int T : {1, 2, 63, 64, 65, 129, 1531, 8192})
                 for (int H : {1, 2, 15, 16, 17, 33, 127, 128, 129, 1000, 4096}) scan(B, T, H, bf16);

@@ -175,3 +175,33 @@ def test_a_captured_sequence_with_its_backward():
         graph.replay()
         torch.cuda.synchronize()
         assert equal(out, want), rep
+
+
+@pytest.mark.parametrize("rows,D", [(1, 4), (3, 64), (5, 60), (1000, 512), (300000, 64)])
+def test_bias_columns(rows, D):
+    """x and W with the columns of a bias, exactly: the bias's three parts are bf16 numbers and sum to it"""
+    from vc3d import ops
+    g = torch.Generator().manual_seed(rows)
+    big = torch.randn(rows * D + 1, generator=g).cuda()
+    for t in (big[:-1].view(rows, D), big[1:].view(rows, D)):  # (any alignment)
+        b = (torch.randn(rows, generator=g) * 10.0 ** torch.randint(-20, 20, (rows,), generator=g)).cuda()
+        b[0] = 0.0
+        ones = ops.bias_columns(t)
+        assert ones.dtype == torch.bfloat16 and torch.equal(ones[:, :D], t.bfloat16())
+        assert bool((ones[:, D:D + 3] == 1).all()) and not ones[:, D + 3:].any()
+        for dtype in (torch.float32, torch.bfloat16):
+            out = ops.bias_columns(t, b, dtype)
+            parts = out[:, D:D + 3]
+            assert out.dtype == dtype and torch.equal(out[:, :D], t.to(dtype)) and not out[:, D + 3:].any()
+            assert torch.equal(parts.bfloat16().to(dtype), parts) and torch.equal(parts.double().sum(1), b.double())
+
+
+def test_bias_columns_refuses():
+    from vc3d import ops
+    from vc3d.capi import Vc3dError
+    t = torch.zeros(4, 64, device="cuda")
+    for args in ((t.cpu(),), (t.bfloat16(),), (t[:, :62],), (t[:, :32],), (t[0],), (t, t[0]), (t, t[:, 0].double()), (t, t[:, 0].cpu()),
+                 (t, None, torch.float64)):
+        with pytest.raises(Vc3dError):
+            ops.bias_columns(*args)
+    assert ops.bias_columns(t[:0]).shape == (0, 128)

@@ -1288,6 +1288,10 @@ int vc_gated_scan_step(const void* gates, int64_t stride_b, int32_t is_bf16, flo
     VC_REQUIRE(gates && state && h && B > 0 && H > 0 && H <= (1 << 30), "gated_scan_step: bad arguments");
     return vc_scan_launch_step(gates, stride_b, state, h, B, H, is_bf16 != 0, S(stream));
 }
+int vc_bias_columns(const float* in, const float* bias, void* out, int32_t out_is_bf16, int64_t rows, int32_t D, void* stream) {
+    VC_REQUIRE(in && out && rows > 0 && D > 0 && D % 4 == 0 && D <= (1 << 24), "bias_columns: bad arguments");
+    return vc_bias_columns_launch(in, bias, out, out_is_bf16 != 0, rows, D, S(stream));
+}
 
 /* ------------------------------------------------------------------ linear classifier + cross-entropy */
 static int lce_check(const vc_linear_ce_desc* d) {

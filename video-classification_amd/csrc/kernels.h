@@ -223,6 +223,7 @@ size_t vc_scan_workspace(int B, int T, int H, bool is_bf16, int op);
 int vc_scan_launch_fwd(const VcScanParams& p, bool is_bf16, hipStream_t s);
 int vc_scan_launch_bwd(const VcScanParams& p, bool is_bf16, hipStream_t s);
 int vc_scan_launch_step(const void* gates, long long sb, float* state, void* h, int B, int H, bool is_bf16, hipStream_t s);
+int vc_bias_columns_launch(const float* in, const float* bias, void* out, bool to_bf16, long long rows, int D, hipStream_t s);
 
 // linear_ce.hip: linear classifier + cross-entropy in pieces of the vocabulary
 struct VcLceParams {

@@ -149,6 +149,7 @@ PROTOTYPES = {
     "vc_gated_scan_fwd": [_SD, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P],
     "vc_gated_scan_bwd": [_SD, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P],
     "vc_gated_scan_step": [_P, _L, _I, _P, _P, _I, _I, _P],
+    "vc_bias_columns": [_P, _P, _P, _I, _L, _I, _P],
     "vc_linear_ce_workspace_bytes": [_LD, _I],
     "vc_linear_ce_saved_bytes": [_LD],
     "vc_linear_ce_fwd": [_LD] + [_P] * 7 + [C.c_size_t, _P],

@@ -873,6 +873,22 @@ def gated_scan_bwd(gates, lengths, states, dy, dlast, reverse=False, want_dh0=Tr
     return dgates, dh0
 
 
+def bias_columns(t, bias=None, dtype=BF16):
+    """fp32 [rows][D] -> [rows][D + 64] of `dtype` (bf16 or fp32) for a product that adds a bias in its sums (vc_bias_columns): behind
+    the rows of x (no bias) 1 1 1 0 ..., behind those of a weight the bias [rows] as three bf16 numbers"""
+    _chk(t, F32, name="rows")
+    if t.dim() != 2 or t.shape[1] == 0 or t.shape[1] % 4 or dtype not in _FLOAT_KIND:
+        raise capi.Vc3dError("bias_columns: fp32 [rows][D], D a multiple of 4, to bf16 or fp32, got %s to %s" % (tuple(t.shape), dtype))
+    _chk(bias, F32, t.shape[0], "bias")
+    _same_device(t, bias=bias)
+    with _on(t):
+        out = torch.empty(t.shape[0], t.shape[1] + 64, dtype=dtype, device=t.device)
+        if t.shape[0] > 0:
+            check(lib.vc_bias_columns(t.data_ptr(), ptr(bias), out.data_ptr(), _FLOAT_KIND[dtype], t.shape[0], t.shape[1], cur_stream()),
+                  "vc_bias_columns")
+    return out
+
+
 def gated_scan_step(gates, state):
     """one step for each of B sequences: gates [B][2H] (rows of any stride), state [B][H] fp32 updated in place -> h [B][H] of
     gates' type (vc_gated_scan_step)"""

@@ -41,7 +41,9 @@ class PackedOperand:
                     t.record_stream(here)
             return kept[5]
         operands = _matrix_pack(self.matrix(*weights))
-        packed = torch.cuda.Event()
+        # (an event is made for a stream once: to destroy one for every change of weights took 20 us)
+        same = kept is not None and kept[3] == stream and kept[1][0][-1] == key[0][-1]
+        packed = kept[4] if same else torch.cuda.Event()
         packed.record()
         self.kept = (tuple(None if w is None else weakref.ref(w) for w in weights), key, tuple(None if w is None else w.detach() for w in weights),
                      stream, packed, operands)

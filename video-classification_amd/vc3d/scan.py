@@ -30,17 +30,8 @@ class PackedGateWeight(PackedOperand):
     more columns as the three bf16 numbers whose sum it is (8 bits each of its 24)"""
 
     def matrix(self, weight, bias=None):
-        if bias is None:
-            return weight.detach().float().contiguous()
-        co, fin = weight.shape
-        m = torch.zeros(co, fin + 64, dtype=torch.float32, device=weight.device)
-        m[:, :fin] = weight.detach()
-        rest = bias.detach().float()
-        for k in range(3):
-            part = rest.bfloat16().float()
-            m[:, fin + k] = part
-            rest = torch.where(part.isfinite(), rest - part, 0.0)
-        return m
+        w = weight.detach().float().contiguous()
+        return w if bias is None else ops.bias_columns(w, bias.detach().float().contiguous(), torch.float32)
 
 
 class _GateProjectionFn(torch.autograd.Function):
@@ -53,14 +44,9 @@ class _GateProjectionFn(torch.autograd.Function):
         N, fin = x.shape
         co = weight.shape[0]
         wf, wd = packed.get(weight, bias)
-        if bias is None:
-            width, xb = fin, x.detach().to(torch.bfloat16).contiguous()
-        else:
-            width = fin + 64
-            xb = torch.empty(N, width, dtype=torch.bfloat16, device=x.device)
-            xb[:, :fin] = x.detach()
-            xb[:, fin:fin + 3] = 1.0
-            xb[:, fin + 3:] = 0.0
+        x = x.detach().contiguous()
+        xb = x.to(torch.bfloat16) if bias is None else ops.bias_columns(x)
+        width = xb.shape[1]
         d = ops.conv_desc(N, width, 1, 1, 1, co, 1, 1, 0)
         ctx.save_for_backward(xb)
         ctx.d, ctx.wd, ctx.fin = d, wd, fin
