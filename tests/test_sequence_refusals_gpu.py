@@ -34,19 +34,30 @@ def test_a_state_of_another_shape_is_refused():
 
 
 class limited:
-    """torch's allocator may hold `more` bytes beside what it holds now"""
+    """torch's allocator may hold `more` bytes beside what it holds now; the holes in that (other tests' work leaves some, of any size) are
+    filled"""
 
     def __init__(self, more):
-        torch.cuda.synchronize()
-        torch.cuda.empty_cache()
-        self.total = torch.cuda.get_device_properties(0).total_memory
-        self.most = torch.cuda.memory_reserved() + more
+        self.more, self.total = more, torch.cuda.get_device_properties(0).total_memory
+
+    def most(self, n):
+        torch.cuda.set_per_process_memory_fraction(n / self.total)
 
     def __enter__(self):
-        torch.cuda.set_per_process_memory_fraction(self.most / self.total)
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        self.most(torch.cuda.memory_reserved())
+        self.holes, size = [], 1 << 32
+        while size >= 4 << 20:
+            try:
+                self.holes.append(torch.empty(size, dtype=torch.uint8, device="cuda"))
+            except torch.OutOfMemoryError:
+                size //= 2
+        self.most(torch.cuda.memory_reserved() + self.more)
 
     def __exit__(self, *exc):
-        torch.cuda.set_per_process_memory_fraction(1.0)
+        self.most(self.total)
+        del self.holes
 
 
 def test_memory_that_runs_out_is_torchs_error():
