@@ -42,32 +42,52 @@ __device__ __forceinline__ float vc_stat_load(const float* p) {
 // several channels) are in flight at once.  With the mode test inside, the compiler cannot hoist the loads across it
 // and the last workgroup's tail becomes a chain of dependent round trips below the L2 (R3D-50's 2048-channel
 // downsample conv: 42 -> 206 us) -- so the callers test the mode ONCE and take this path or the deterministic one.
-template <bool AGENT>
+// AHEAD: replicas whose loads are issued before the first of them is added (0: the compiler's choice).  Without packed fp32
+// instructions the compiler's choice in the separate finalize kernels and in the stem's tail is one load at a time, 64 round trips
+// (5.4 -> 18.5 us a launch, seven of them in an R3D-18 step, and +17 us of the stem); the others keep theirs, as their registers are
+// set by what is around this.
+template <bool AGENT, int AHEAD = 0>
 __device__ __forceinline__ void vc_stat_sum_f(const float* stats, int C, int c, float& s, float& q) {
     s = 0.f, q = 0.f;
+    if constexpr (AHEAD > 0) {
+        static_assert(VC_STAT_REPLICAS % AHEAD == 0, "");
+#pragma unroll
+        for (int r0 = 0; r0 < VC_STAT_REPLICAS; r0 += AHEAD) {
+            float u[AHEAD], v[AHEAD];
+#pragma unroll
+            for (int r = 0; r < AHEAD; ++r) {
+                u[r] = vc_stat_load<AGENT>(stats + (size_t)(r0 + r) * 2 * C + c);
+                v[r] = vc_stat_load<AGENT>(stats + (size_t)(r0 + r) * 2 * C + C + c);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int r = 0; r < AHEAD; ++r) s += u[r], q += v[r];
+        }
+        return;
+    }
 #pragma unroll
     for (int r = 0; r < VC_STAT_REPLICAS; ++r) {
         s += vc_stat_load<AGENT>(stats + (size_t)r * 2 * C + c);
         q += vc_stat_load<AGENT>(stats + (size_t)r * 2 * C + C + c);
     }
 }
-template <bool AGENT>
+template <bool AGENT, int AHEAD = 0>
 __device__ __forceinline__ void vc_stat_sum(const float* stats, int C, int c, float& s, float& q) {
     if (vc_stat_is_det(stats)) {
         s = vc_stat_total_det(stats, C, c, AGENT);
         q = vc_stat_total_det(stats, C, C + c, AGENT);
     } else {
-        vc_stat_sum_f<AGENT>(stats, C, c, s, q);
+        vc_stat_sum_f<AGENT, AHEAD>(stats, C, c, s, q);
     }
 }
 
-template <bool AGENT>
+template <bool AGENT, int AHEAD = 0>
 __device__ __forceinline__ void vc_bn_finalize_channel(const float* stats, int C, int c, float count, const float* gamma,
                                                        const float* beta, float* running_mean, float* running_var,
                                                        float momentum, float eps, float* params,
                                                        const float* shift = nullptr, float* shift_out = nullptr) {
     float s, q;
-    vc_stat_sum<AGENT>(stats, C, c, s, q);
+    vc_stat_sum<AGENT, AHEAD>(stats, C, c, s, q);
     const float m1 = s / count;  // mean of (y - shift)
     const float mean = (shift != nullptr ? shift[c] : 0.f) + m1;
     float var = q / count - m1 * m1;
@@ -86,11 +106,11 @@ __device__ __forceinline__ void vc_bn_finalize_channel(const float* stats, int C
     }
 }
 
-template <bool AGENT>
+template <bool AGENT, int AHEAD = 0>
 __device__ __forceinline__ void vc_bn_bwd_finalize_channel(const float* sums, int C, int c, float count, float* coef,
                                                            float* dgamma, float* dbeta) {
     float s, q;
-    vc_stat_sum<AGENT>(sums, C, c, s, q);
+    vc_stat_sum<AGENT, AHEAD>(sums, C, c, s, q);
     coef[c] = s / count;
     coef[C + c] = q / count;
     if (dgamma != nullptr) dgamma[c] += q;
@@ -147,13 +167,13 @@ __device__ __forceinline__ bool vc_last_workgroup(unsigned* ticket) {
 // channel: the GEMM kernels (register budget set by their accumulators) take four channels, the bandwidth kernels,
 // whose occupancy hangs on staying within 64 VGPRs, take VC_FIN_BATCH = 1 (they finalize at most a few hundred channels
 // per thread block anyway).
-template <int VC_FIN_BATCH = 1>
+template <int VC_FIN_BATCH = 1, int AHEAD = 0>
 __device__ __forceinline__ void vc_bn_fin_last(const VcBnFin& f, const float* stats, int C) {
     if (f.ticket == nullptr || stats == nullptr) return;
     if (!vc_last_workgroup(f.ticket)) return;
     if (VC_FIN_BATCH == 1) {
         for (int c = threadIdx.x; c < C; c += blockDim.x)
-            vc_bn_finalize_channel<true>(stats, C, c, f.count, f.gamma, f.beta, f.running_mean, f.running_var, f.momentum,
+            vc_bn_finalize_channel<true, AHEAD>(stats, C, c, f.count, f.gamma, f.beta, f.running_mean, f.running_var, f.momentum,
                                          f.eps, f.params, f.shift, f.shift_out);
         return;
     }

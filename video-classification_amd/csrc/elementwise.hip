@@ -27,7 +27,7 @@ __global__ void bn_finalize_kernel(const float* __restrict__ stats, int C, float
                                    float eps, float* params, const float* shift, float* shift_out) {
     const int c = blockIdx.x * blockDim.x + threadIdx.x;
     if (c >= C) return;
-    vc_bn_finalize_channel<false>(stats, C, c, count, gamma, beta, running_mean, running_var, momentum, eps, params, shift,
+    vc_bn_finalize_channel<false, VC_STAT_REPLICAS>(stats, C, c, count, gamma, beta, running_mean, running_var, momentum, eps, params, shift,
                                   shift_out);
 }
 
@@ -377,7 +377,7 @@ __global__ void bn_bwd_finalize_kernel(const float* __restrict__ sums, int C, fl
                                        float* dbeta) {
     const int c = blockIdx.x * blockDim.x + threadIdx.x;
     if (c >= C) return;
-    vc_bn_bwd_finalize_channel<false>(sums, C, c, count, coef, dgamma, dbeta);
+    vc_bn_bwd_finalize_channel<false, VC_STAT_REPLICAS>(sums, C, c, count, coef, dgamma, dbeta);
 }
 
 // BN backward apply: dy = scale * (g - c1 - xhat*c2); optionally writes g (the masked

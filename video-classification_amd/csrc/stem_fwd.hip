@@ -322,7 +322,7 @@ __global__ __launch_bounds__(NWAVE * 64) __attribute__((amdgpu_waves_per_eu(NWAV
             vc_stat_add(p.stats, blockIdx.x, 64, (tid < 64 ? 0 : 64) + (tid & 63), s);
         }
     }
-    vc_bn_fin_last(p.fin, p.stats, 64);
+    vc_bn_fin_last<1, VC_STAT_REPLICAS>(p.fin, p.stats, 64);
 }
 
 }  // namespace
