@@ -65,7 +65,6 @@ __global__ __launch_bounds__(256, WPE) void pw_kernel(const VcPwParams p) {
     const gptr_t zero = (gptr_t)vc_pw_zero_page;
     // byte offsets from the (uniform) tensor bases, 32 bits each: scalar base + vector offset addressing keeps the
     // loader's state at one register per piece (a tensor stays below 2^31 elements, the C ABI splits the batch above)
-    const unsigned woff = (unsigned)((co0 + lrow) * p.K + lslot * 8) * 2u;  // + j * 32 * K * 2 per piece
     const char* const wbase = (const char*)p.wgt;
     const char* const xbase = (const char*)p.src;
 
@@ -81,9 +80,11 @@ __global__ __launch_bounds__(256, WPE) void pw_kernel(const VcPwParams p) {
 
     for (int tile = (int)bx; tile < ntiles; tile += gridDim.x) {
         const int m0 = tile * BM;
-        unsigned woff_t = woff;  // (opaque per tile: hoisted out of the tile loop, the pieces' 64-bit addresses were spills)
+        // (opaque per tile: hoisted out of the tile loop, the pieces' 64-bit addresses were spills, and the offset itself, carried
+        // through it, was one without packed fp32 instructions)
         int lrow_t = lrow;
-        asm volatile("" : "+v"(woff_t), "+v"(lrow_t));
+        asm volatile("" : "+v"(lrow_t));
+        const unsigned woff_t = (unsigned)((co0 + lrow_t) * p.K + lslot * 8) * 2u;  // + j * 32 * K * 2 per piece
         auto issue_chunk = [&](int c, int buf) {
             char* bW = smem + buf * Cfg::BUF_BYTES + wave * (8 * ROWB);
             char* bX = bW + BCO * ROWB;
