@@ -359,7 +359,7 @@ int vc_bias_columns(const float* in, const float* bias, void* out, int32_t out_i
  * loss: [1], or [N] with reduction 0.  saved (vc_linear_ce_saved_bytes, 256-byte aligned) is written by the forward and read by
  * the backward of the same x, w, bias and labels: the rows' logsumexp, the list of rows that count, up to 32 MB of
  * copies of them, and, where that is quicker than to compute the logits again and takes at most keep_bytes (-1: 2 GB), the
- * gradient of their logits in x's type, N x V, and where w is copied and there is room its copy (keep_bytes 0: never; > 0: wherever
+ * gradient of their logits in x's type (rounded twice then, once where the backward computes it), N x V, and where w is copied and there is room its copy (keep_bytes 0: never; > 0: wherever
  * it fits; with reduction 0 never).
  * dloss: fp32 on the device, [1], or [N] with reduction 0.  dx [N][D], dw [V][D], db [V] (each nullable) are contiguous,
  * dx and dw 16-byte aligned, and of x's type, and are written, not added to.  workspace (required, 256-byte aligned): vc_linear_ce_workspace_bytes(d, op),

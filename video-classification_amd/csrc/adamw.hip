@@ -21,7 +21,7 @@
 // lane's elements lie in pieces of 16 bytes of p and g, neighbouring lanes' pieces beside each other.
 // With 32-bit moments a lane has four elements of each of UNROLL stretches.
 // Measured (copies reach 5.14 TB/s): 33.4 M fp32 parameters, 32-bit moments, 182 us = 5.14 TB/s; 357 M bf16 parameters, 8-bit
-// moments, 660 us = 5.4 TB/s; 100 tensors of 42 thousand elements in all 18 us, the host's time.
+// moments, 664 us = 5.4 TB/s; 100 tensors of 42 thousand elements in all 21 us: two launches of 8 us, one behind the other, and the host.
 // The tensors' addresses travel as kernel arguments (60 per launch): nothing on the device has to be written before the
 // launch, so a captured step replays.
 //

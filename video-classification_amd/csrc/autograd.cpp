@@ -1,6 +1,6 @@
 // Module vc3d._tensors, second part (host only): the gated scan and the linear cross-entropy with their gradients, as autograd
 // nodes around libvc3d.so's entry points.  In C++ because a short call's time is this: 64 x 512 of 400 classes in Python took 144
-// us for some 55 us of kernels, a scan of 3 x 1531 x 1000 135; here 61 and 69.
+// us for some 50 us of kernels, a scan of 3 x 1531 x 1000 135; here 61 to 92 (as the autograd engine's thread is placed) and 69 to 74.
 #include <Python.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>

@@ -44,7 +44,7 @@ __device__ __forceinline__ float vc_stat_load(const float* p) {
 // downsample conv: 42 -> 206 us) -- so the callers test the mode ONCE and take this path or the deterministic one.
 // AHEAD: replicas whose loads are issued before the first of them is added (0: the compiler's choice).  Without packed fp32
 // instructions the compiler's choice in the separate finalize kernels and in the stem's tail is one load at a time, 64 round trips
-// (5.4 -> 18.5 us a launch, seven of them in an R3D-18 step, and +17 us of the stem); the others keep theirs, as their registers are
+// (5.4 -> 18.7 us a launch, seven of them in an R3D-18 step, and 535 -> 545 us for the stem); the others keep theirs, as their registers are
 // set by what is around this.
 template <bool AGENT, int AHEAD = 0>
 __device__ __forceinline__ void vc_stat_sum_f(const float* stats, int C, int c, float& s, float& q) {

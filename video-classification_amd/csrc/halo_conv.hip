@@ -587,7 +587,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         }
     }
     if (p.stats != nullptr) {
-        // four channels at a time (packed fp32), without the per-element slot test when every slot of the wave is a real
+        // four channels at a time, without the per-element slot test when every slot of the wave is a real
         // position (wave-uniform): this accumulation is exposed -- it cost a layer1 forward 15 us of 134
         bool anybad = false;
 #pragma unroll

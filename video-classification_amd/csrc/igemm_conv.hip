@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void igemm_kernel(const VcIgemmParams p) {
             }
         }
         if (p.stats != nullptr) {
-            // four channels at a time (packed fp32 adds and fmas): this accumulation sits on the tile's critical path
+            // four channels at a time: this accumulation sits on the tile's critical path
             if (m0 + BM <= M) {  // whole tile inside the tensor (uniform): no row tests
 #pragma unroll
                 for (int a = 0; a < 4; ++a)
