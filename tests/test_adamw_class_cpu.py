@@ -81,3 +81,20 @@ def test_eight_bits_that_there_are_not_are_refused():
     cfg = make_config(18, 10, OPTIMIZER="adamw", STATE_BITS=8)
     with pytest.raises(ValueError, match="STATE_BITS"):
         create_optimizer(cfg, torch.nn.Linear(4, 2))
+
+
+def test_a_parameter_that_is_listed_twice_is_stepped_twice(monkeypatch):
+    """as torch does (with a warning): two steps, one after the other, each with its own count"""
+    import warnings
+
+    from vc3d import ops, optim
+    calls = []
+    monkeypatch.setattr(ops, "adamw_step", lambda params, *a, **k: calls.append((len(params), k["step"])))
+    monkeypatch.setattr(optim.AdamW, "_new_state", lambda self, p: {"step": 0, "exp_avg": torch.zeros_like(p), "exp_avg_sq": torch.zeros_like(p)})
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(2))
+    p.grad, q.grad = torch.ones(3), torch.ones(2)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        opt = optim.AdamW([p, q, p])
+    opt.step()
+    assert calls == [(2, 1), (1, 2)] and opt.state[p]["step"] == 2 and opt.state[q]["step"] == 1

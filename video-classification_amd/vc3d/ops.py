@@ -901,7 +901,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, m_scale=None, v_scale=None, *
     exp_avg_sq are fp32, or, with m_scale and v_scale, float8_e4m3fn codes with one fp32 scale per 256 elements
     (ceil(numel / 256) of them; exp_avg_sq's codes then hold the ROOT of the second moment).  A parameter may lie in memory in any
     dense order of its dimensions (channels_last ...); its gradient and moments lie in the same one.  `step` counts from 1.
-    grad_scale: a number, or a one-element fp32 tensor on the device, that gradients are multiplied by."""
+    No two of the tensors may share memory.  grad_scale: a number, or a one-element fp32 tensor on the device, that gradients are
+    multiplied by."""
     n = len(params)
     eight = m_scale is not None
     if eight != (v_scale is not None):

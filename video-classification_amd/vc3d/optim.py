@@ -324,7 +324,7 @@ class AdamW(torch.optim.Optimizer):
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise Vc3dError("AdamW.step() counts on the host: it cannot be captured into a graph (ops.adamw_step with a step of your own can)")
         for group in self.param_groups:
-            lists = {}
+            lists, counts = {}, {}
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -336,7 +336,8 @@ class AdamW(torch.optim.Optimizer):
                 g = p.grad
                 if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
                     g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)  # into the parameter's order of memory
-                cols = lists.setdefault((p.dtype, p.device, st["step"] + 1), tuple([] for _ in range(7)))
+                counts[p] = counts.get(p, st["step"]) + 1  # (a parameter that is listed twice takes two steps)
+                cols = lists.setdefault((p.dtype, p.device, counts[p]), tuple([] for _ in range(7)))
                 for col, t in zip(cols, (p, g, st["exp_avg"], st["exp_avg_sq"], st.get("exp_avg_scale"), st.get("exp_avg_sq_scale"), st)):
                     col.append(t)
             for (_, _, step), (*cols, states) in lists.items():
